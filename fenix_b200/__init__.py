@@ -31,6 +31,8 @@ STATUS_NAMES = {
 }
 PREC_BF16, PREC_FP8, PREC_F16 = 0, 1, 2
 PRECISIONS = {"bf16": PREC_BF16, "fp8": PREC_FP8, "f16": PREC_F16}
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}  # fx_dtype
+SCALE_MODES = {None: 0, "tensor": 1, "row": 2}  # fx_scale
 
 
 class FxError(RuntimeError):
@@ -201,6 +203,11 @@ def lib():
     _sig(L, "fx_fxvol_encode_tiles", i32, [vp, vp, i64, C.c_float, C.c_float, C.c_float, i32, vp, C.c_uint64, u64p,
                                            u32p])
     _sig(L, "fx_predict_fxvol", i32, [vp, C.c_char_p, C.c_char_p, C.POINTER(InferOpts), C.c_float])
+    _sig(L, "fx_rms_norm", i32, [vp, i32, i64, i64, i64, vp, i32, i64, vp, i64, vp, i32, C.c_float, vp, i32, i64, vp,
+                                 i32, vp])
+    _sig(L, "fx_w4_linear", i32, [vp, i32, i64, i64, vp, i32, vp, vp, i32, vp, i64, i64, i64, vp, vp, i32, i64, vp])
+    _sig(L, "fx_w4_quantize", i32, [vp, i32, i64, i64, i64, i64, vp, vp, i32, vp, vp])
+    _sig(L, "fx_w4_dequantize", i32, [vp, vp, i32, vp, i64, i64, i64, vp, i32, i64, vp])
     _lib = L
     return L
 
@@ -301,6 +308,47 @@ def tc_rate(precision: str = "fp8", n_cols: int = 256, ms_per_run: float = 50.0,
 
 def device_count() -> int:
     return lib().fx_device_count()
+
+
+# ---- token rows: norm, 4-bit linear layers (device pointers) --------------------------------
+def rms_norm_dev(x_ptr: int, y_ptr: int, rows: int, cols: int, x_type: str = "bf16", y_type: str = "bf16",
+                 weight_ptr: int | None = None, weight_type: str = "bf16", eps: float = 1e-6, x_stride: int = 0,
+                 y_stride: int = 0, residual_ptr: int | None = None, residual_type: str = "bf16",
+                 residual_stride: int = 0, sum_ptr: int | None = None, sum_stride: int = 0,
+                 scale_ptr: int | None = None, scale_mode: str | None = None, stream: int | None = None) -> None:
+    """fx_rms_norm: y = RMS norm of x + residual, the sum stored at ``sum_ptr``. Types are "f32", "f16" or
+    "bf16"; ``y_type`` "e4m3" with ``scale_mode`` "row" (scales written to ``scale_ptr`` [rows]) or
+    "tensor" (one scale read there). Strides are in elements, 0 for packed rows."""
+    check(lib().fx_rms_norm(x_ptr, DTYPES[x_type], rows, cols, x_stride, residual_ptr, DTYPES[residual_type],
+                            residual_stride, sum_ptr, sum_stride, weight_ptr, DTYPES[weight_type], eps, y_ptr,
+                            DTYPES[y_type], y_stride, scale_ptr, SCALE_MODES[scale_mode], stream))
+
+
+def w4_linear_dev(x_ptr: int, y_ptr: int, rows: int, n: int, k: int, group: int, codes_ptr: int, scales_ptr: int,
+                  zeros_ptr: int | None = None, x_type: str = "bf16", y_type: str = "bf16", scale_type: str = "f16",
+                  x_stride: int = 0, y_stride: int = 0, x_scale_ptr: int | None = None,
+                  x_scale_mode: str | None = None, bias_ptr: int | None = None, stream: int | None = None) -> None:
+    """fx_w4_linear: y [rows][n] = x [rows][k] times the 4-bit weights, plus bias (f32). ``x_type`` "e4m3" takes
+    its scales as rms_norm_dev writes them."""
+    check(lib().fx_w4_linear(x_ptr, DTYPES[x_type], rows, x_stride, x_scale_ptr, SCALE_MODES[x_scale_mode], codes_ptr,
+                             scales_ptr, DTYPES[scale_type], zeros_ptr, n, k, group, bias_ptr, y_ptr, DTYPES[y_type],
+                             y_stride, stream))
+
+
+def w4_quantize_dev(w_ptr: int, n: int, k: int, group: int, codes_ptr: int, scales_ptr: int,
+                    zeros_ptr: int | None = None, w_type: str = "f32", scale_type: str = "f16", w_stride: int = 0,
+                    stream: int | None = None) -> None:
+    """fx_w4_quantize: weights [n][k] to 4-bit codes and group scales; with ``zeros_ptr``, zero points too."""
+    check(lib().fx_w4_quantize(w_ptr, DTYPES[w_type], n, k, w_stride, group, codes_ptr, scales_ptr, DTYPES[scale_type],
+                               zeros_ptr, stream))
+
+
+def w4_dequantize_dev(codes_ptr: int, scales_ptr: int, n: int, k: int, group: int, w_ptr: int,
+                      zeros_ptr: int | None = None, w_type: str = "f32", scale_type: str = "f16", w_stride: int = 0,
+                      stream: int | None = None) -> None:
+    """fx_w4_dequantize: the values that 4-bit codes, scales and zero points stand for."""
+    check(lib().fx_w4_dequantize(codes_ptr, scales_ptr, DTYPES[scale_type], zeros_ptr, n, k, group, w_ptr,
+                                 DTYPES[w_type], w_stride, stream))
 
 
 # ---- nets ----------------------------------------------------------------------------------

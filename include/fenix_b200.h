@@ -394,6 +394,65 @@ fx_status fx_accum_finalize(const float* dev_acc, int64_t dz, int64_t dy, int64_
                             const float* dev_wz, const float* dev_wy, const float* dev_wx, float* dev_prob,
                             uint8_t* dev_u8, void* stream);
 
+/* ---- token rows: norm, 4-bit linear layers (device pointers) ----
+ * A token model's step between two attention or mixing layers: normalise the rows (with the residual's
+ * addition, to 8 bits with scales or to 16 / 32), multiply them by a linear layer held in 4 bits. No
+ * reference counterpart (its token models run through libtorch, src/ml/nets/dinovol.hpp).
+ * Common to these calls: matrices are row-major with their rows `*_stride` elements apart (at least the
+ * row's length; 0: packed) and their elements at least element-aligned. Every pointer of a call is device
+ * memory of one device, which need not be the current one; `stream` (NULL: that device's default stream)
+ * belongs to that device. The calls enqueue one kernel, allocate nothing, keep nothing between calls and
+ * do not synchronise, so any number may run at once and be captured into graphs. Extents and strides are
+ * below 2^30. No row (rows or n = 0) is not an error: nothing is done. */
+typedef enum fx_dtype { FX_F32 = 0, FX_F16 = 1, FX_BF16 = 2, FX_E4M3 = 3 } fx_dtype;
+/* Scale of 8-bit rows (value = e4m3 * scale): none, one for the tensor, or one per row. */
+typedef enum fx_scale { FX_SCALE_NONE = 0, FX_SCALE_TENSOR = 1, FX_SCALE_ROW = 2 } fx_scale;
+
+/* Root-mean-square norm of rows, with the residual's addition before it and quantisation after it:
+ *   h = x + residual,  v = h / sqrt(mean(h^2) + eps) * weight
+ * per row of `cols` values, in f32. dev_residual may be NULL (h = x); dev_sum (may be NULL) receives h
+ * rounded to residual_type (the norm is of the unrounded h); dev_weight may be NULL (ones).
+ * x, residual / sum and weight are f32, f16 or bf16 each. y_type f32, f16, bf16: y = v rounded, no scale.
+ * y_type e4m3: y = v / scale rounded to nearest and saturated to +-448, with
+ *   FX_SCALE_ROW     scale[row] = max(max |v|, 1e-30) / 448, written to dev_scale [rows]
+ *   FX_SCALE_TENSOR  scale = dev_scale[0], read (a calibrated activation scale)
+ * A row that holds a NaN or infinity follows the formula: its values (and a row scale) come out NaN, save
+ * the finite values of a row of infinities under a tensor scale and in 16 / 32 bits, which become zero.
+ * In place: dev_sum may be dev_residual or dev_x, and dev_y may be dev_x, at equal types and strides; no
+ * other overlap. 1 <= cols <= 32768, eps > 0. Extents that are multiples of 8 with 16-byte aligned rows
+ * take 16-byte accesses. */
+fx_status fx_rms_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                      const void* dev_residual, fx_dtype residual_type, int64_t residual_stride, void* dev_sum,
+                      int64_t sum_stride, const void* dev_weight, fx_dtype weight_type, float eps, void* dev_y,
+                      fx_dtype y_type, int64_t y_stride, float* dev_scale, fx_scale scale_mode, void* stream);
+
+/* Linear layer with 4-bit weights: y = x W^T + bias for `rows` rows of k values and n outputs, where
+ *   W[o][i] = scales[o][i / group] * (code[o][i] - zeros[o][i / group])
+ * with 4-bit codes packed two to a byte, the even input in the low half (dev_codes [n][k / 2], 16-byte
+ * aligned), scales [n][k / group] of scale_type (f32, f16, bf16) and zero points [n][k / group] of 0..15
+ * (NULL: 8 everywhere). group is a multiple of 32 that divides k; rows and n are any numbers. x is f16,
+ * bf16, or e4m3 with x_scale (f32: FX_SCALE_TENSOR one value, FX_SCALE_ROW [rows]); y is f16 or bf16,
+ * rounded once; bias is f32 [n] or NULL. Sums are held in f32. y overlaps no input. */
+fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t x_stride, const float* dev_x_scale,
+                       fx_scale x_scale_mode, const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
+                       const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, const float* dev_bias,
+                       void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream);
+
+/* The 4-bit form of weights [n][k] (f32, f16, bf16) in fx_w4_linear's layout, one scale (and zero point) per
+ * `group` inputs, each quotient rounded to nearest, ties to even:
+ *   dev_zeros NULL  scale = max |w| / 7 rounded to scale_type, code = clamp(round(w / scale) + 8, 0, 15)
+ *   else            lo = min(w, 0), hi = max(w, 0) over the group, scale = (hi - lo) / 15 rounded to
+ *                   scale_type, zero = clamp(round(-lo / scale), 0, 15),
+ *                   code = clamp(round(w / scale) + zero, 0, 15)
+ * A scale past scale_type's range becomes its largest finite value; a group whose scale is 0 gets
+ * code = zero (8; 0 with zero points); a NaN is left out of the extremes and gets code = zero. */
+fx_status fx_w4_quantize(const void* dev_w, fx_dtype w_type, int64_t n, int64_t k, int64_t w_stride, int64_t group,
+                         uint8_t* dev_codes, void* dev_scales, fx_dtype scale_type, uint8_t* dev_zeros, void* stream);
+/* The values such weights stand for: w = scale * (code - zero), rounded once to w_type (f32, f16, bf16). */
+fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
+                           const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, void* dev_w,
+                           fx_dtype w_type, int64_t w_stride, void* stream);
+
 /* ---- .fxvol archives and the chunk codec ---------------------------------------------------
  * A 64^3 chunk is one tile of 4^3 DCT-16 blocks whose magnitude categories share up to 8 clustered
  * rANS tables. Payloads and files are bit-compatible with the reference's codec and container. */
