@@ -18,6 +18,7 @@ fx_status abi_exception();
 namespace {
 
 constexpr int64_t kMaxExtent = int64_t{1} << 30;  // rows, columns and strides: byte offsets stay below 2^62
+constexpr int64_t kMaxInner = int64_t{1} << 24;   // k of a 4-bit layer: 32-bit offsets inside 128 of its rows
 
 fx_status bad(const char* fn, const char* what) {
     return fxh::abi_error(FX_INVALID_ARGUMENT, std::string(fn) + ": " + what);
@@ -95,7 +96,7 @@ fx_status guarded(F&& f) {
 fx_status check_w4(const char* fn, const uint8_t* codes, const void* scales, int scale_type, int64_t n, int64_t k,
                    int64_t group) {
     if (!is_float(scale_type)) return bad(fn, "scales are f32, f16 or bf16");
-    if (n < 0 || n >= kMaxExtent || k < 1 || k >= kMaxExtent) return bad(fn, "n or k out of range");
+    if (n < 0 || n >= kMaxExtent || k < 1 || k >= kMaxInner) return bad(fn, "n or k out of range");
     if (group < 32 || group % 32 || k % group) return bad(fn, "group must be a multiple of 32 that divides k");
     if (n == 0) return FX_OK;
     if (!codes || !scales) return bad(fn, "null codes or scales");

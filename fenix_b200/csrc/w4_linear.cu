@@ -1,57 +1,481 @@
 // w4_linear.cu — linear layer with 4-bit weights and group scales.
 #include "counters.hpp"
+#include "ptx.cuh"
+#include "tmap.hpp"
 #include "token.cuh"
+
+#include <atomic>
 
 namespace fxk {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRowsAtOnce = 8;
+// ---- few rows ----------------------------------------------------------------------------------
+// With few token rows the time is the weights' way from memory: 4.5 bits a weight, each used once per
+// row, and the bound close behind is the instructions that make operands of the codes. One block per SM
+// walks over tiles of 16 MT outputs: a producer warp keeps a ring of bulk copies ahead of the consumer
+// warps, across tiles, so that memory never waits for a tile's end; each consumer takes 128 inputs of a
+// stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs, B: inputs x 8 rows); the rows lie in
+// shared memory for the whole walk, converted once and in the MMA's order.
+// Codes become exact 16-bit integers: in f16 code - zero, in bf16 128 + code, whose offset leaves in f32
+// with one more MMA of ones, shared by the m-tiles, that sums the inputs of a group:
+//   sum (code - zero) x = sum (128 + code) x - (128 + zero) sum x
+// (the difference loses 5 of f32's 24 bits). Scales are applied in f32 to a group's sum: no weight is
+// rounded. The consumers' partial sums meet in shared memory.
 
-// One warp per output and eight rows; lanes over k.
-__global__ void __launch_bounds__(kThreads) w4_linear_kernel(const W4LinearArgs a) {
-    const int lane = threadIdx.x % 32;
-    const int o = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-    if (o >= a.w.n) return;
-    const int64_t per_row = a.w.k / a.w.group;
-    for (int64_t r0 = static_cast<int64_t>(blockIdx.y) * kRowsAtOnce; r0 < a.rows;
-         r0 += static_cast<int64_t>(gridDim.y) * kRowsAtOnce) {
-        float acc[kRowsAtOnce] = {};
-        for (int i = 2 * lane; i < a.w.k; i += 64) {
-            const int64_t g = o * per_row + i / a.w.group;
-            const int c = a.w.codes[(static_cast<int64_t>(o) * a.w.k + i) / 2];
-            const int z = a.w.zeros ? a.w.zeros[g] : 8;
-            const float s = tok_load(a.w.scales, g, a.w.scale_type);
-            const float w0 = s * static_cast<float>((c & 15) - z), w1 = s * static_cast<float>((c >> 4) - z);
+constexpr int kBlockK = 128;  // inputs of a consumer warp in a stage
+constexpr int kMaxConsumers = 16;
+
+// Bounded wait for a phase: gives up after some seconds' worth of tries (each may sleep for a while in hardware), or
+// when another role of the block has. No clock is read, so that a wait which has to sleep costs no more than that.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile int* abort) {
+    for (int it = 0; it < 1 << 24; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (it % 256 == 255 && abort && *abort) return false;
+    }
+    return false;
+}
+
+// Set by a kernel whose bounded wait gave up; read and cleared by w4_device_status.
+__device__ uint32_t g_w4_status;
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if (BF)
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Nibbles (i, i + 4) of a word of eight codes as two 16-bit floats, by or'ing them into the mantissa of a
+// power of two. bf16: 128 + code (three shifts for a word's four pairs). f16: 1024 + code or 1024 + 16 code
+// (one shift), from which one fused multiply-add makes code - zero; z = {1024 + zero, -(64 + zero)}.
+// (w & mask) | bits
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, const uint32_t (&z)[2]) {
+    if (BF) return and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+    const uint32_t h = and_or(i >= 2 ? w >> 8 : w, i & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+    uint32_t r;
+    if (i & 1)
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(h), "r"(0x2c002c00u), "r"(z[1]));
+    else
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(z[0]));
+    return r;
+}
+
+// Eight inputs of one row, given as they lie in memory, as 16-bit pairs (i, i + 4), i = 0..3: code_pair's order.
+__device__ __forceinline__ uint4 paired(const uint8_t* p, int x_type, bool vec) {
+    uint32_t v[4];
+    if (x_type == kTokE4M3) {
+        if (vec) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            v[0] = u.x, v[1] = u.y;
+        } else {
 #pragma unroll
-            for (int r = 0; r < kRowsAtOnce; ++r) {
-                if (r0 + r >= a.rows) break;
-                const int64_t at = (r0 + r) * a.x_stride + i;
-                acc[r] += w0 * tok_load(a.x, at, a.x_type) + w1 * tok_load(a.x, at + 1, a.x_type);
+            for (int e = 0; e < 2; ++e)
+                v[e] = __ldg(p + 4 * e) | __ldg(p + 4 * e + 1) << 8 | __ldg(p + 4 * e + 2) << 16 | __ldg(p + 4 * e + 3) << 24;
+        }
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
+                static_cast<__nv_fp8x2_storage_t>((v[0] >> (8 * i) & 0xff) | (v[1] >> (8 * i) & 0xff) << 8), __NV_E4M3);
+            r[i] = reinterpret_cast<const uint32_t&>(h);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    if (vec) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+    } else {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __ldg(q + 2 * e) | static_cast<uint32_t>(__ldg(q + 2 * e + 1)) << 16;
+    }
+    return make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
+                      __byte_perm(v[1], v[3], 0x7632));
+}
+
+// How the few-rows kernel walks and where its parts lie in shared memory; made by the host.
+struct FewPlan {
+    int consumers;   // warps, even; a stage is 128 inputs for each
+    int stages;      // of the ring
+    int seg_blocks;  // blocks of 128 inputs whose rows and scales are in shared memory at once, a multiple of consumers
+    int wide;        // tiles of 32 outputs, all blocks having as many; the outputs after them go in tiles of 16
+    int tiles;
+    int x_pitch;     // of a row's inputs: 64 modulo 128, so that 2 rows x 4 lanes of 16 bytes hit all banks once
+    int s_pitch, z_pitch;  // of an output's scales and zero points: 16 modulo 128, so that 8 outputs hit different banks
+    int red_bufs;
+    int x, scale, accum, red, ring, bytes;  // offsets; accum: the sums of earlier segments, by tile of this block
+    bool x_vec;
+};
+
+constexpr int kM = 32;  // outputs of a wide tile
+constexpr int kMaxStages = 6;
+
+__device__ __forceinline__ void consumers_sync(int warps) { asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory"); }
+
+// Bytes [0, bytes) of each of `rows` rows, `src_pitch` apart, to shared memory rows `dst_pitch` apart by one warp,
+// asynchronously in pieces of UNIT bytes where the addresses allow it (the caller's mbarrier arrival follows them).
+template <int UNIT>
+__device__ __forceinline__ void rows_async(uint32_t dst, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
+    const int lane = threadIdx.x % 32;
+    for (int r = lane / 4; r < rows; r += 8)
+        for (int at = lane % 4 * UNIT; at < bytes; at += 4 * UNIT) {
+            if constexpr (UNIT == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + r * dst_pitch + at), "l"(src + r * src_pitch + at) : "memory");
+            else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + r * dst_pitch + at), "l"(src + r * src_pitch + at) : "memory");
+        }
+}
+__device__ __forceinline__ void rows_to_shared(uint8_t* to, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
+    const int64_t all = static_cast<int64_t>(reinterpret_cast<uintptr_t>(src)) | src_pitch;
+    if (all % 16 == 0 && bytes % 16 == 0) {
+        rows_async<16>(smem_u32(to), dst_pitch, src, src_pitch, rows, bytes);
+    } else if (all % 4 == 0 && bytes % 4 == 0) {
+        rows_async<4>(smem_u32(to), dst_pitch, src, src_pitch, rows, bytes);
+    } else {
+        const int lane = threadIdx.x % 32;
+        for (int r = lane / 4; r < rows; r += 8)
+#pragma unroll 8
+            for (int at = lane % 4; at < bytes; at += 4) to[r * dst_pitch + at] = __ldg(src + r * src_pitch + at);
+        __threadfence_block();
+    }
+}
+
+// CPF chunks of 32 inputs times MT m-tiles of 16 outputs into acc, under one scale per output. The codes of output
+// m 16 + h 8 (+ this lane's g, in `codes`) lie 128 bytes apart, 16-byte cell c of them at cell c ^ g (cell: of the first
+// chunk); `x`: this lane's rows; scales and zero points as they are stored.
+template <bool BF, int CPF, bool Z, int MT>
+__device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_t x_at, int cell, uint32_t s_at, int s_pitch,
+                                     int scale_type, uint32_t z_at, int z_pitch) {
+    uint32_t x[CPF][4], w[MT][2][CPF], z[MT][2][2], zero[MT][2];
+    float scale[MT][2], part[MT][4] = {}, xs[4] = {};
+#pragma unroll
+    for (int c = 0; c < CPF; ++c) {
+        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(x[c][0]), "=r"(x[c][1]), "=r"(x[c][2]), "=r"(x[c][3])
+                     : "r"(x_at + c * 64));
+        const uint32_t at = codes + (cell ^ c) * 16;  // the first chunk's cell is a multiple of CPF before the swizzle
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[m][h][c]) : "r"(at + (m * 16 + h * 8) * 128));
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t at = s_at + (m * 16 + h * 8) * s_pitch;
+            if (scale_type == kTokF32) {
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale[m][h]) : "r"(at));
+            } else {
+                unsigned short raw;
+                asm volatile("ld.shared.b16 %0, [%1];" : "=h"(raw) : "r"(at));
+                scale[m][h] = scale_type == kTokF16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float(static_cast<uint32_t>(raw) << 16);
+            }
+            zero[m][h] = 8;
+            if (Z) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(zero[m][h]) : "r"(z_at + (m * 16 + h * 8) * z_pitch));
+            z[m][h][0] = 0x64006400u + 0x00010001u * zero[m][h];  // f16 pairs of 1024 + zero
+            z[m][h][1] = 0xd400d400u + 0x00100010u * zero[m][h];  // and -(64 + zero)
+        }
+#pragma unroll
+    for (int c = 0; c < CPF; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            if (BF) mma16816<BF>(xs, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, x[c][i], x[c][i + 1]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const uint32_t f0 = code_pair<BF>(w[m][0][c], i, z[m][0]), f1 = code_pair<BF>(w[m][1][c], i, z[m][1]);
+                const uint32_t f2 = code_pair<BF>(w[m][0][c], i + 1, z[m][0]), f3 = code_pair<BF>(w[m][1][c], i + 1, z[m][1]);
+                mma16816<BF>(part[m], f0, f1, f2, f3, x[c][i], x[c][i + 1]);
             }
         }
 #pragma unroll
-        for (int r = 0; r < kRowsAtOnce; ++r) {
-            if (r0 + r >= a.rows) break;
-            float v = acc[r];
-            for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-            if (lane == 0) {
-                if (a.x_scale) v *= a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
-                if (a.bias) v += a.bias[o];
-                tok_store(a.y, (r0 + r) * a.y_stride + o, a.y_type, v);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p = BF ? fmaf(-128.f - static_cast<float>(zero[m][e / 2]), xs[e % 2], part[m][e]) : part[m][e];
+            acc[m][e] = fmaf(scale[m][e / 2], p, acc[m][e]);
+        }
+}
+
+// CPF: the scale changes every CPF chunks of 32 inputs at most (4: groups are multiples of 128, 2: of 64, 1: of 32);
+// such a unit is summed in the MMAs before its scale is applied. Lane t of a quad takes inputs 8 t .. 8 t + 7 of a
+// chunk, as code words and rows lie. Besides the consumers: a warp that issues the codes' TMA loads, 128 bytes x 16
+// outputs each, and one that brings a tile's scales (and zero points: Z) to shared memory a tile ahead.
+template <bool BF, int CPF, bool Z>
+__global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
+    w4_few_kernel(const __grid_constant__ W4LinearArgs a, const int row0, const __grid_constant__ FewPlan plan,
+                  const __grid_constant__ CUtensorMap map_wide, const __grid_constant__ CUtensorMap map_narrow) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4];  // ring full, ring empty, scales full, scales empty
+    __shared__ volatile int abort_flag;
+    constexpr int kUnits = 4 / CPF;
+    const int warps = plan.consumers, warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const int n = a.w.n, k = a.w.k, group = a.w.group;
+    const int blocks = (k + kBlockK - 1) / kBlockK;
+    const int rows = min(a.rows - row0, 8);
+    const int stage_bytes = warps / 2 * kM * 128, s_bytes = kM * (plan.s_pitch + (Z ? plan.z_pitch : 0));
+    const uint32_t ring = smem_u32(smem + plan.ring), full = smem_u32(bars), empty = full + 8 * kMaxStages;
+    const uint32_t s_full = full + 16 * kMaxStages, s_empty = s_full + 16;
+    auto tile_row = [&](int tile) { return tile < plan.wide ? tile * kM : plan.wide * kM + (tile - plan.wide) * 16; };
+    auto gave_up = [&](uint32_t code) {
+        abort_flag = 1;
+        set_status(&g_w4_status, code);
+    };
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < plan.stages; ++i) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, warps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 32);
+            mbar_init(s_empty + 8 * i, warps);
+        }
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    __syncthreads();
+    int slot = 0, s_slot = 0;
+    uint32_t phase = 0, s_phase = 0;
+
+    if (warp == warps) {  // codes
+        if (lane) return;
+        int issued = 0;
+        for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
+            const int seg_end = min(seg + plan.seg_blocks, blocks);
+            for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x) {
+                const bool wide = tile < plan.wide;
+                const CUtensorMap* const map = wide ? &map_wide : &map_narrow;
+                const int o0 = tile_row(tile), box_bytes = (wide ? kM : 16) * 128;
+                for (int blk = seg; blk < seg_end; blk += warps) {
+                    const int boxes = (min(warps, seg_end - blk) + 1) / 2;  // of 256 inputs; past the end they read as zeros
+                    if (!wait_phase(empty + 8 * slot, phase ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                    if (abort_flag) break;
+                    mbar_arrive_expect_tx(full + 8 * slot, boxes * box_bytes);
+                    for (int i = 0; i < boxes; ++i)
+                        tma_load_2d(ring + slot * stage_bytes + i * kM * 128, map, (blk / 2 + i) * 16, o0, full + 8 * slot);
+                    ++issued;
+                    if (++slot == plan.stages) slot = 0, phase ^= 1;
+                }
             }
+        }
+        if (abort_flag)  // the consumers no longer wait for the copies still on their way
+            for (int i = min(issued, plan.stages); i > 0; --i) {
+                if (slot-- == 0) slot = plan.stages - 1, phase ^= 1;
+                wait_phase(full + 8 * slot, phase, nullptr);
+            }
+        return;
+    }
+    const int sb = a.w.scale_type == kTokF32 ? 4 : 2;
+    if (warp == warps + 1) {  // scales, as they are stored
+        const int groups = k / group;
+        for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
+            const int seg_end = min(seg + plan.seg_blocks, blocks);
+            const int g0 = seg * kBlockK / group, gn = (min(seg_end * kBlockK, k) - 1) / group + 1 - g0;
+            for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x) {
+                if (!wait_phase(s_empty + 8 * s_slot, s_phase ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                uint8_t* const to = smem + plan.scale + s_slot * s_bytes;
+                const int o0 = tile_row(tile), per = min(tile < plan.wide ? kM : 16, n - o0);
+                const int64_t at = static_cast<int64_t>(o0) * groups + g0;
+                rows_to_shared(to, plan.s_pitch, static_cast<const uint8_t*>(a.w.scales) + at * sb, static_cast<int64_t>(groups) * sb, per, gn * sb);
+                if (Z) rows_to_shared(to + kM * plan.s_pitch, plan.z_pitch, a.w.zeros + at, groups, per, gn);
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(s_full + 8 * s_slot) : "memory");
+                if (++s_slot == 2) s_slot = 0, s_phase ^= 1;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+    }
+
+    const uint32_t x_lane = smem_u32(smem + plan.x) + min(g, rows - 1) * plan.x_pitch + t * 16;  // rows past the last: nothing reads their sums
+    const float inv_group = 1.f / static_cast<float>(group);
+    int red_buf = 0;
+    for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
+        const int seg_end = min(seg + plan.seg_blocks, blocks), g0 = seg * kBlockK / group;
+        if (seg) consumers_sync(warps);  // the last segment's rows are read
+        {  // the rows' inputs of this segment
+            const int kxb = a.x_type == kTokE4M3 ? 1 : 2, eights = min((seg_end - seg) * kBlockK, k - seg * kBlockK) / 8;
+            for (int r = 0; r < rows; ++r) {
+                const uint8_t* const p = static_cast<const uint8_t*>(a.x) + (static_cast<int64_t>(row0 + r) * a.x_stride + seg * kBlockK) * kxb;
+                for (int i = threadIdx.x; i < eights; i += warps * 32)
+                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = paired(p + i * 8 * kxb, a.x_type, plan.x_vec);
+            }
+        }
+        consumers_sync(warps);
+        int turn = 0;
+        for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x, ++turn) {
+            const bool wide = tile < plan.wide;
+            const int per = wide ? kM : 16;
+            float acc[2][4] = {};
+            if (!wait_phase(s_full + 8 * s_slot, s_phase, &abort_flag))
+                gave_up(kStatusTimeoutFull);
+            const uint32_t s_at = smem_u32(smem + plan.scale + s_slot * s_bytes) + g * plan.s_pitch;
+            const uint32_t z_at = smem_u32(smem + plan.scale + s_slot * s_bytes) + kM * plan.s_pitch + g * plan.z_pitch;
+            for (int blk0 = seg; blk0 < seg_end; blk0 += warps) {
+                const int blk = blk0 + warp, k0 = blk * kBlockK;
+                if (!wait_phase(full + 8 * slot, phase, &abort_flag))
+                    gave_up(kStatusTimeoutFull);
+                if (blk < seg_end) {
+                    const uint32_t cw = ring + slot * stage_bytes + warp / 2 * kM * 128 + g * 128 + t * 4;
+                    const uint32_t xw = x_lane + (k0 - seg * kBlockK) * 2;
+#pragma unroll
+                    for (int u = 0; u < kUnits; ++u) {
+                        const int kc = k0 + u * 32 * CPF;
+                        if (CPF < 4 && kc >= k) break;
+                        // (kc + 1/2) / group truncated: exact while k < 2^21
+                        const int gi = (k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group) - g0;
+                        if (wide)
+                            unit<BF, CPF, Z, 2>(acc, cw, xw + u * CPF * 64, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
+                                                a.w.scale_type, z_at + gi, plan.z_pitch);
+                        else
+                            unit<BF, CPF, Z, 1>(acc, cw, xw + u * CPF * 64, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
+                                                a.w.scale_type, z_at + gi, plan.z_pitch);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty + 8 * slot);
+                if (++slot == plan.stages) slot = 0, phase ^= 1;
+            }
+            if (lane == 0) mbar_arrive(s_empty + 8 * s_slot);
+            if (++s_slot == 2) s_slot = 0, s_phase ^= 1;
+            // partial sums [warp][row][output]; with two buffers the next tile's go to the other one, and its barrier
+            // comes after every thread's reads of this one
+            float* const red = reinterpret_cast<float*>(smem + plan.red) + red_buf * warps * rows * kM;
+            if (plan.red_bufs == 2) red_buf ^= 1;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (2 * t + (e & 1) < rows) red[(warp * rows + 2 * t + (e & 1)) * kM + m * 16 + (e / 2) * 8 + g] = acc[m][e];
+            consumers_sync(warps);
+            for (int i = threadIdx.x; i < rows * kM; i += warps * 32) {
+                const int r = i / kM, o = tile_row(tile) + i % kM;
+                if (i % kM >= per || o >= n) continue;
+                float v = 0.f;
+                for (int w = 0; w < warps; ++w) v += red[w * rows * kM + i];
+                float* const kept = reinterpret_cast<float*>(smem + plan.accum) + turn * rows * kM + i;
+                if (seg) v += *kept;
+                if (seg_end < blocks) {
+                    *kept = v;
+                } else {
+                    if (a.x_scale) v *= a.x_scale[a.x_scale_mode == kScaleRow ? row0 + r : 0];
+                    if (a.bias) v += a.bias[o];
+                    tok_store(a.y, static_cast<int64_t>(row0 + r) * a.y_stride + o, a.y_type, v);
+                }
+            }
+            if (plan.red_bufs == 1) consumers_sync(warps);
         }
     }
+}
+
+int sm_count() {
+    static std::atomic<int> count[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int c = dev < 64 ? count[dev].load(std::memory_order_relaxed) : 0;
+    if (!c) {
+        cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
+        if (dev < 64) count[dev].store(c, std::memory_order_relaxed);
+    }
+    return c;
+}
+
+constexpr int kFewSmem = 226 * 1024;  // a block's shared memory, less the barriers
+
+int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
+    constexpr int kXRoom = 80 * 1024, kScaleRoom = 24 * 1024;  // for the rows, and one tile's scales, at most
+    FewPlan p{};
+    const int blocks = (a.w.k + kBlockK - 1) / kBlockK;
+    // as many consumers as leave the fewest idle in a tile's last stage
+    const int turns = (blocks + kMaxConsumers - 1) / kMaxConsumers;
+    p.consumers = round_up((blocks + turns - 1) / turns, 2);
+    const int x_fit = kXRoom / rows / (p.consumers * kBlockK * 2 + 64);
+    const int sb = a.w.scale_type == kTokF32 ? 4 : 2;
+    const int64_t s_fit = static_cast<int64_t>((kScaleRoom / kM - 2 * 128) / (a.w.zeros ? sb + 1 : sb) - 1) * a.w.group / (p.consumers * kBlockK);
+    int fit = x_fit < s_fit ? x_fit : static_cast<int>(s_fit);
+    if (fit < 1) fit = 1;
+    const int segs = (turns + fit - 1) / fit;
+    p.seg_blocks = (turns + segs - 1) / segs * p.consumers;
+    p.x_pitch = round_up(p.seg_blocks * kBlockK * 2, 128) + 64;
+    const int seg_k = p.seg_blocks < blocks ? p.seg_blocks * kBlockK : a.w.k;
+    const int seg_groups = (seg_k + a.w.group - 1) / a.w.group + 1;  // a segment may begin inside a group
+    p.s_pitch = round_up(seg_groups * sb, 128) + 16;
+    p.z_pitch = round_up(seg_groups, 128) + 16;
+    *grid = sms;
+    p.wide = a.w.n / kM / sms * sms;
+    p.tiles = p.wide + (a.w.n - p.wide * kM + 15) / 16;
+    if (p.tiles < sms) *grid = p.tiles;
+    p.red_bufs = rows <= 4 ? 2 : 1;
+    p.x = 0;
+    p.scale = round_up(rows * p.x_pitch, 128);
+    p.accum = p.scale + round_up(2 * kM * (p.s_pitch + (a.w.zeros ? p.z_pitch : 0)), 128);
+    p.red = p.accum;
+    if (p.seg_blocks < blocks) {  // room for the sums of a block's tiles between segments
+        const int per = 16 * 1024 / (rows * kM * 4);
+        if ((p.tiles + *grid - 1) / *grid > per) *grid = (p.tiles + per - 1) / per;
+        p.red += round_up((p.tiles + *grid - 1) / *grid * rows * kM * 4, 128);
+    }
+    p.ring = round_up(p.red + p.red_bufs * p.consumers * rows * kM * 4, 1024);
+    const int stage = p.consumers / 2 * kM * 128;
+    p.stages = (kFewSmem - p.ring) / stage;
+    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    p.bytes = p.ring + p.stages * stage;
+    return p;
+}
+
+template <bool BF, int CPF, bool Z>
+cudaError_t launch_few(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t s) {
+    auto* kern = w4_few_kernel<BF, CPF, Z>;
+    int grid;
+    FewPlan p = few_plan(a, a.rows - row0 < 8 ? a.rows - row0 : 8, sm_count(), &grid);
+    p.x_vec = x_vec;
+    CUtensorMap wide, narrow;
+    cudaError_t e = tmap_rows(&wide, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kM);
+    if (e == cudaSuccess) e = tmap_rows(&narrow, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, 16);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
+    if (e != cudaSuccess) return e;
+    count_launch();
+    kern<<<grid, (p.consumers + 2) * 32, p.bytes, s>>>(a, row0, p, wide, narrow);
+    return cudaGetLastError();
+}
+template <bool BF, bool Z>
+cudaError_t launch_few_cpf(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t s) {
+    if (a.w.group % 128 == 0) return launch_few<BF, 4, Z>(a, row0, x_vec, s);
+    if (a.w.group % 64 == 0) return launch_few<BF, 2, Z>(a, row0, x_vec, s);
+    return launch_few<BF, 1, Z>(a, row0, x_vec, s);
+}
+cudaError_t launch_few_typed(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t s) {
+    if (a.x_type == kTokBF16) return a.w.zeros ? launch_few_cpf<true, true>(a, row0, x_vec, s) : launch_few_cpf<true, false>(a, row0, x_vec, s);
+    return a.w.zeros ? launch_few_cpf<false, true>(a, row0, x_vec, s) : launch_few_cpf<false, false>(a, row0, x_vec, s);
 }
 
 }  // namespace
 
 cudaError_t launch_w4_linear(const W4LinearArgs& a, cudaStream_t s) {
-    const int64_t tiles = (static_cast<int64_t>(a.rows) + kRowsAtOnce - 1) / kRowsAtOnce;
-    dim3 grid((a.w.n + kThreads / 32 - 1) / (kThreads / 32), static_cast<unsigned>(tiles < 65535 ? tiles : 65535));
-    count_launch();
-    w4_linear_kernel<<<grid, kThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
+    const bool x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
+    for (int row0 = 0; row0 < a.rows; row0 += 8) {
+        const cudaError_t e = launch_few_typed(a, row0, x_vec, s);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace fxk

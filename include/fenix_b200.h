@@ -430,7 +430,7 @@ fx_status fx_rms_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t 
  *   W[o][i] = scales[o][i / group] * (code[o][i] - zeros[o][i / group])
  * with 4-bit codes packed two to a byte, the even input in the low half (dev_codes [n][k / 2], 16-byte
  * aligned), scales [n][k / group] of scale_type (f32, f16, bf16) and zero points [n][k / group] of 0..15
- * (NULL: 8 everywhere). group is a multiple of 32 that divides k; rows and n are any numbers. x is f16,
+ * (NULL: 8 everywhere). group is a multiple of 32 that divides k < 2^24; rows and n are any numbers. x is f16,
  * bf16, or e4m3 with x_scale (f32: FX_SCALE_TENSOR one value, FX_SCALE_ROW [rows]); y is f16 or bf16,
  * rounded once; bias is f32 [n] or NULL. Sums are held in f32. y overlaps no input. */
 fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t x_stride, const float* dev_x_scale,
