@@ -206,6 +206,7 @@ def lib():
     _sig(L, "fx_rms_norm", i32, [vp, i32, i64, i64, i64, vp, i32, i64, vp, i64, vp, i32, C.c_float, vp, i32, i64, vp,
                                  i32, vp])
     _sig(L, "fx_w4_linear", i32, [vp, i32, i64, i64, vp, i32, vp, vp, i32, vp, i64, i64, i64, vp, vp, i32, i64, vp])
+    _sig(L, "fx_w4_device_status", i32, [i32])
     _sig(L, "fx_w4_quantize", i32, [vp, i32, i64, i64, i64, i64, vp, vp, i32, vp, vp])
     _sig(L, "fx_w4_dequantize", i32, [vp, vp, i32, vp, i64, i64, i64, vp, i32, i64, vp])
     _lib = L
@@ -333,6 +334,11 @@ def w4_linear_dev(x_ptr: int, y_ptr: int, rows: int, n: int, k: int, group: int,
     check(lib().fx_w4_linear(x_ptr, DTYPES[x_type], rows, x_stride, x_scale_ptr, SCALE_MODES[x_scale_mode], codes_ptr,
                              scales_ptr, DTYPES[scale_type], zeros_ptr, n, k, group, bias_ptr, y_ptr, DTYPES[y_type],
                              y_stride, stream))
+
+
+def w4_device_status(device: int = 0) -> None:
+    """fx_w4_device_status: raise if a bounded wait inside a 4-bit linear kernel gave up."""
+    check(lib().fx_w4_device_status(device))
 
 
 def w4_quantize_dev(w_ptr: int, n: int, k: int, group: int, codes_ptr: int, scales_ptr: int,

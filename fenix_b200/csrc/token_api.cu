@@ -3,6 +3,7 @@
 // refusals answer the same on a machine without a GPU.
 #include "fenix_b200.h"
 #include "token.cuh"
+#include "w4.cuh"
 
 #include <cuda_runtime.h>
 
@@ -219,6 +220,28 @@ fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t
         a.x_scale_mode = x_scale_mode;
         a.y_type = y_type;
         return done(fn, fxk::launch_w4_linear(a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+fx_status fx_w4_device_status(int device) {
+    static const char* const fn = "fx_w4_device_status";
+    return guarded([&]() -> fx_status {
+        int count = 0, cur = 0;
+        if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
+            cudaGetLastError();
+            return bad(fn, "no such device");
+        }
+        cudaGetDevice(&cur);
+        if (cudaError_t e = cudaSetDevice(device); e != cudaSuccess) return done(fn, e);
+        uint32_t few = 0, many = 0;
+        cudaError_t e = cudaDeviceSynchronize();
+        if (e == cudaSuccess) e = fxk::w4_few_status(&few);
+        if (e == cudaSuccess) e = fxk::w4_many_status(&many);
+        cudaSetDevice(cur);
+        if (e != cudaSuccess) return done(fn, e);
+        if (few || many)
+            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(few ? few : many));
+        return FX_OK;
     });
 }
 

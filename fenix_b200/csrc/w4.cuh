@@ -1,0 +1,77 @@
+// w4.cuh — what the kernels of the 4-bit linear layer share.
+#pragma once
+
+#include "ptx.cuh"
+#include "token.cuh"
+
+namespace fxk {
+
+cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s);
+// The status word of each file's kernels, cleared.
+cudaError_t w4_few_status(uint32_t* code);
+cudaError_t w4_many_status(uint32_t* code);
+
+#ifdef __CUDACC__
+// Set by a kernel of this file's includer whose bounded wait gave up; read and cleared by take_status.
+static __device__ uint32_t g_w4_status;
+__device__ __forceinline__ void set_w4_status(uint32_t code) { set_status(&g_w4_status, code); }
+
+// Bounded wait for a phase. Gives up after two seconds, or when another role of the block has. The clock is read only
+// after many tries (each may sleep for a while in hardware): an ordinary wait costs no more than itself.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile int* abort) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (it % 64 == 63) {
+            if (abort && *abort) return false;
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > 2000000000ull) return false;
+        }
+    }
+}
+
+// (w & mask) | bits
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+    return r;
+}
+
+// Eight e4m3 or 16-bit values at p as they lie in memory, e4m3 widened to f16; vec: p is aligned to eight of them.
+__device__ __forceinline__ uint4 in_order(const uint8_t* p, int x_type, bool vec) {
+    if (x_type == kTokE4M3) {
+        uint32_t v[2];
+        if (vec) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
+            v[0] = u.x, v[1] = u.y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                v[e] = __ldg(p + 4 * e) | __ldg(p + 4 * e + 1) << 8 | __ldg(p + 4 * e + 2) << 16 | __ldg(p + 4 * e + 3) << 24;
+        }
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v[i / 2] >> (16 * (i % 2))), __NV_E4M3);
+            r[i] = reinterpret_cast<const uint32_t&>(h);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+    if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+    const uint16_t* const q = reinterpret_cast<const uint16_t*>(p);
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __ldg(q + 2 * e) | static_cast<uint32_t>(__ldg(q + 2 * e + 1)) << 16;
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+static inline cudaError_t take_status(uint32_t* code) {
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_w4_status, sizeof *code);
+    const uint32_t zero = 0;
+    if (e == cudaSuccess && *code) e = cudaMemcpyToSymbol(g_w4_status, &zero, sizeof zero);
+    return e;
+}
+#endif
+
+}  // namespace fxk

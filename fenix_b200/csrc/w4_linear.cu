@@ -3,6 +3,7 @@
 #include "ptx.cuh"
 #include "tmap.hpp"
 #include "token.cuh"
+#include "w4.cuh"
 
 #include <atomic>
 
@@ -25,19 +26,6 @@ namespace {
 constexpr int kBlockK = 128;  // inputs of a consumer warp in a stage
 constexpr int kMaxConsumers = 16;
 
-// Bounded wait for a phase: gives up after some seconds' worth of tries (each may sleep for a while in hardware), or
-// when another role of the block has. No clock is read, so that a wait which has to sleep costs no more than that.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile int* abort) {
-    for (int it = 0; it < 1 << 24; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (it % 256 == 255 && abort && *abort) return false;
-    }
-    return false;
-}
-
-// Set by a kernel whose bounded wait gave up; read and cleared by w4_device_status.
-__device__ uint32_t g_w4_status;
-
 template <bool BF>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -56,12 +44,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 // Nibbles (i, i + 4) of a word of eight codes as two 16-bit floats, by or'ing them into the mantissa of a
 // power of two. bf16: 128 + code (three shifts for a word's four pairs). f16: 1024 + code or 1024 + 16 code
 // (one shift), from which one fused multiply-add makes code - zero; z = {1024 + zero, -(64 + zero)}.
-// (w & mask) | bits
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
-    return r;
-}
 template <bool BF>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, const uint32_t (&z)[2]) {
     if (BF) return and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
@@ -74,37 +56,10 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, const uint32_t 
     return r;
 }
 
-// Eight inputs of one row, given as they lie in memory, as 16-bit pairs (i, i + 4), i = 0..3: code_pair's order.
-__device__ __forceinline__ uint4 paired(const uint8_t* p, int x_type, bool vec) {
-    uint32_t v[4];
-    if (x_type == kTokE4M3) {
-        if (vec) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-            v[0] = u.x, v[1] = u.y;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                v[e] = __ldg(p + 4 * e) | __ldg(p + 4 * e + 1) << 8 | __ldg(p + 4 * e + 2) << 16 | __ldg(p + 4 * e + 3) << 24;
-        }
-        uint32_t r[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-                static_cast<__nv_fp8x2_storage_t>((v[0] >> (8 * i) & 0xff) | (v[1] >> (8 * i) & 0xff) << 8), __NV_E4M3);
-            r[i] = reinterpret_cast<const uint32_t&>(h);
-        }
-        return make_uint4(r[0], r[1], r[2], r[3]);
-    }
-    if (vec) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-    } else {
-        const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __ldg(q + 2 * e) | static_cast<uint32_t>(__ldg(q + 2 * e + 1)) << 16;
-    }
-    return make_uint4(__byte_perm(v[0], v[2], 0x5410), __byte_perm(v[0], v[2], 0x7632), __byte_perm(v[1], v[3], 0x5410),
-                      __byte_perm(v[1], v[3], 0x7632));
+// Eight 16-bit values as the pairs (i, i + 4), i = 0..3: code_pair's order.
+__device__ __forceinline__ uint4 paired(const uint4& v) {
+    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                      __byte_perm(v.y, v.w, 0x7632));
 }
 
 // How the few-rows kernel walks and where its parts lie in shared memory; made by the host.
@@ -217,7 +172,7 @@ __device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_
 // outputs each, and one that brings a tile's scales (and zero points: Z) to shared memory a tile ahead.
 template <bool BF, int CPF, bool Z>
 __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
-    w4_few_kernel(const __grid_constant__ W4LinearArgs a, const int row0, const __grid_constant__ FewPlan plan,
+    w4_few_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ FewPlan plan,
                   const __grid_constant__ CUtensorMap map_wide, const __grid_constant__ CUtensorMap map_narrow) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 4];  // ring full, ring empty, scales full, scales empty
@@ -226,14 +181,14 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
     const int warps = plan.consumers, warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int n = a.w.n, k = a.w.k, group = a.w.group;
     const int blocks = (k + kBlockK - 1) / kBlockK;
-    const int rows = min(a.rows - row0, 8);
+    const int rows = a.rows;  // at most 8
     const int stage_bytes = warps / 2 * kM * 128, s_bytes = kM * (plan.s_pitch + (Z ? plan.z_pitch : 0));
     const uint32_t ring = smem_u32(smem + plan.ring), full = smem_u32(bars), empty = full + 8 * kMaxStages;
     const uint32_t s_full = full + 16 * kMaxStages, s_empty = s_full + 16;
     auto tile_row = [&](int tile) { return tile < plan.wide ? tile * kM : plan.wide * kM + (tile - plan.wide) * 16; };
     auto gave_up = [&](uint32_t code) {
         abort_flag = 1;
-        set_status(&g_w4_status, code);
+        set_w4_status(code);
     };
 
     if (threadIdx.x == 0) {
@@ -310,9 +265,9 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
         {  // the rows' inputs of this segment
             const int kxb = a.x_type == kTokE4M3 ? 1 : 2, eights = min((seg_end - seg) * kBlockK, k - seg * kBlockK) / 8;
             for (int r = 0; r < rows; ++r) {
-                const uint8_t* const p = static_cast<const uint8_t*>(a.x) + (static_cast<int64_t>(row0 + r) * a.x_stride + seg * kBlockK) * kxb;
+                const uint8_t* const p = static_cast<const uint8_t*>(a.x) + (r * a.x_stride + seg * kBlockK) * kxb;
                 for (int i = threadIdx.x; i < eights; i += warps * 32)
-                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = paired(p + i * 8 * kxb, a.x_type, plan.x_vec);
+                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = paired(in_order(p + i * 8 * kxb, a.x_type, plan.x_vec));
             }
         }
         consumers_sync(warps);
@@ -372,9 +327,9 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                 if (seg_end < blocks) {
                     *kept = v;
                 } else {
-                    if (a.x_scale) v *= a.x_scale[a.x_scale_mode == kScaleRow ? row0 + r : 0];
+                    if (a.x_scale) v *= a.x_scale[a.x_scale_mode == kScaleRow ? r : 0];
                     if (a.bias) v += a.bias[o];
-                    tok_store(a.y, static_cast<int64_t>(row0 + r) * a.y_stride + o, a.y_type, v);
+                    tok_store(a.y, r * a.y_stride + o, a.y_type, v);
                 }
             }
             if (plan.red_bufs == 1) consumers_sync(warps);
@@ -440,10 +395,10 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
 }
 
 template <bool BF, int CPF, bool Z>
-cudaError_t launch_few(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t s) {
+cudaError_t launch_few(const W4LinearArgs& a, bool x_vec, cudaStream_t s) {
     auto* kern = w4_few_kernel<BF, CPF, Z>;
     int grid;
-    FewPlan p = few_plan(a, a.rows - row0 < 8 ? a.rows - row0 : 8, sm_count(), &grid);
+    FewPlan p = few_plan(a, a.rows, sm_count(), &grid);
     p.x_vec = x_vec;
     CUtensorMap wide, narrow;
     cudaError_t e = tmap_rows(&wide, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kM);
@@ -452,30 +407,41 @@ cudaError_t launch_few(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewSmem);
     if (e != cudaSuccess) return e;
     count_launch();
-    kern<<<grid, (p.consumers + 2) * 32, p.bytes, s>>>(a, row0, p, wide, narrow);
+    kern<<<grid, (p.consumers + 2) * 32, p.bytes, s>>>(a, p, wide, narrow);
     return cudaGetLastError();
 }
 template <bool BF, bool Z>
-cudaError_t launch_few_cpf(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t s) {
-    if (a.w.group % 128 == 0) return launch_few<BF, 4, Z>(a, row0, x_vec, s);
-    if (a.w.group % 64 == 0) return launch_few<BF, 2, Z>(a, row0, x_vec, s);
-    return launch_few<BF, 1, Z>(a, row0, x_vec, s);
+cudaError_t launch_few_cpf(const W4LinearArgs& a, bool x_vec, cudaStream_t s) {
+    if (a.w.group % 128 == 0) return launch_few<BF, 4, Z>(a, x_vec, s);
+    if (a.w.group % 64 == 0) return launch_few<BF, 2, Z>(a, x_vec, s);
+    return launch_few<BF, 1, Z>(a, x_vec, s);
 }
-cudaError_t launch_few_typed(const W4LinearArgs& a, int row0, bool x_vec, cudaStream_t s) {
-    if (a.x_type == kTokBF16) return a.w.zeros ? launch_few_cpf<true, true>(a, row0, x_vec, s) : launch_few_cpf<true, false>(a, row0, x_vec, s);
-    return a.w.zeros ? launch_few_cpf<false, true>(a, row0, x_vec, s) : launch_few_cpf<false, false>(a, row0, x_vec, s);
+cudaError_t launch_few_typed(const W4LinearArgs& a, bool x_vec, cudaStream_t s) {
+    if (a.x_type == kTokBF16) return a.w.zeros ? launch_few_cpf<true, true>(a, x_vec, s) : launch_few_cpf<true, false>(a, x_vec, s);
+    return a.w.zeros ? launch_few_cpf<false, true>(a, x_vec, s) : launch_few_cpf<false, false>(a, x_vec, s);
 }
 
 }  // namespace
 
 cudaError_t launch_w4_linear(const W4LinearArgs& a, cudaStream_t s) {
+    if (a.rows > 8) {
+        constexpr int kMost = 65535 * 16;  // rows of a launch: 65535 of the smallest tiles
+        for (int64_t row0 = 0; row0 < a.rows; row0 += kMost) {
+            W4LinearArgs b = a;
+            b.x = static_cast<const uint8_t*>(a.x) + row0 * a.x_stride * (a.x_type == kTokE4M3 ? 1 : 2);
+            b.y = static_cast<uint8_t*>(a.y) + row0 * a.y_stride * 2;
+            if (a.x_scale_mode == kScaleRow) b.x_scale = a.x_scale + row0;
+            b.rows = static_cast<int>(a.rows - row0 < kMost ? a.rows - row0 : kMost);
+            const cudaError_t e = launch_w4_many(b, sm_count(), s);
+            if (e != cudaSuccess) return e;
+        }
+        return cudaSuccess;
+    }
     const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
     const bool x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
-    for (int row0 = 0; row0 < a.rows; row0 += 8) {
-        const cudaError_t e = launch_few_typed(a, row0, x_vec, s);
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+    return launch_few_typed(a, x_vec, s);
 }
+
+cudaError_t w4_few_status(uint32_t* code) { return take_status(code); }
 
 }  // namespace fxk

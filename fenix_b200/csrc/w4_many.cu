@@ -1,0 +1,496 @@
+// w4_many.cu — linear layer with 4-bit weights and group scales, many rows: tcgen05.
+//
+// A tile is 128 or 256 outputs (the MMA's M) by up to 256 rows (its N). Codes come by TMA; eight warps turn
+// them into 16-bit weights in the MMA's swizzled layout, the rows come by TMA as they are (or, for e4m3 and
+// unaligned rows, through four loader warps); one thread issues the MMAs, which accumulate in TMEM in f32.
+// A weight scale * (code - zero) is rounded once to the rows' 16-bit type (f16 for e4m3 rows): code - zero is
+// exact, and the scale enters as the sum of two 16-bit values, one product and one fused multiply-add. In f16
+// each output's weights are divided by the power of two below its largest scale, so that no scale's size
+// overflows the type or sinks below it; the epilogue multiplies by it again.
+#include "counters.hpp"
+#include "ptx.cuh"
+#include "tmap.hpp"
+#include "token.cuh"
+#include "w4.cuh"
+
+#include <algorithm>
+
+namespace fxk {
+namespace {
+
+constexpr int kStageK = 256;  // inputs of a stage of codes: 128 bytes an output
+constexpr int kStepK = 64;    // inputs of a stage of operands: 128 bytes of 16-bit values a row
+constexpr int kMaxRing = 8;
+constexpr int kSmemMax = 226 * 1024;
+
+struct ManyPlan {
+    int tile_n;           // rows of a tile: a multiple of 16, at most 256
+    int rings[3];         // stages of codes, weights, rows
+    int codes, weights, rows, row_factor;  // offsets in shared memory
+    int bytes;
+    int split;            // blocks of a cluster that share a tile, each with a range of k
+    int stages_each;      // stages of codes of a block
+    int tmem_cols;
+    bool x_tma, x_vec;
+};
+
+// K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
+           static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}" : "=f"(v) : "r"(addr), "r"(rank));
+    return v;
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pair16(float a, float b) {
+    if (BF) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return reinterpret_cast<uint32_t&>(h);
+    }
+    __half2 h = __floats2half2_rn(a, b);
+    return reinterpret_cast<uint32_t&>(h);
+}
+template <bool BF>
+__device__ __forceinline__ float round16f(float v) {
+    return BF ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if (BF)
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    if (BF)
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    else
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+
+// Codes (2 i, 2 i + 1) of a word of eight as 16-bit floats code - zero, in their order; z from zero_terms.
+template <bool BF>
+__device__ __forceinline__ uint32_t code_pair_in_order(uint32_t w, uint32_t w4, int i, uint32_t z) {
+    uint32_t r;
+    if (BF) {  // 128 + code: the second code from the word shifted by four
+        const uint32_t v = and_or(__byte_perm(w, w4, 0x0000 + i + ((4 + i) << 8)), 0x000f000fu, 0x43004300u);
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(z));
+        return r;
+    }
+    // 1024 + code and 1024 + 16 code, times 1 and 1/16, less 1024 + zero and 64 + zero
+    const uint32_t v = and_or(__byte_perm(w, 0, 0x4040 + i + (i << 8)), 0x00f0000fu, 0x64006400u);
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0x2c003c00u), "r"(z));
+    return r;
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t zero_terms(uint32_t zero) {
+    if (BF) return 0x43004300u + 0x00010001u * zero;
+    return 0xd400e400u + 0x00100001u * zero;  // -(64 + zero), -(1024 + zero)
+}
+
+// 32 codes (16 bytes) under one scale as four 16-byte cells of weights.
+template <bool BF>
+__device__ __forceinline__ void weights32(const uint4& codes, uint32_t hi, uint32_t lo, uint32_t z, uint4 (&out)[4]) {
+    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t w4 = BF ? w[c] >> 4 : 0;
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = code_pair_in_order<BF>(w[c], w4, i, z);
+            r[i] = fma2<BF>(v, hi, mul2<BF>(v, lo));
+        }
+        out[c] = make_uint4(r[0], r[1], r[2], r[3]);
+    }
+}
+
+// TWO: 256 outputs a tile in two accumulators, else 128. Warps: 0 TMA, 1 MMA and TMEM, 2 and 3 idle, 4..11 weights
+// and epilogue, 12..15 (only without x_tma) rows.
+template <bool BF, bool TWO>
+__global__ void __launch_bounds__(512, 1)
+    w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
+                   const __grid_constant__ CUtensorMap rows_map) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[6 * kMaxRing + 1];
+    __shared__ uint32_t tmem_at;
+    __shared__ volatile int abort_flag;
+    constexpr int kTileM = TWO ? 256 : 128;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int n = a.w.n, k = a.w.k, group = a.w.group, groups = k / group;
+    const int tile_n = plan.tile_n, rank = plan.split > 1 ? static_cast<int>(blockIdx.x) % plan.split : 0;
+    const int o0 = static_cast<int>(blockIdx.x) / plan.split * kTileM;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * tile_n;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows) - r0, static_cast<int64_t>(tile_n)));
+    const int k_begin = rank * plan.stages_each * kStageK, k_end = min(k, k_begin + plan.stages_each * kStageK);
+    const int stages = k_begin < k_end ? (k_end - k_begin + kStageK - 1) / kStageK : 0;
+    const int steps = k_begin < k_end ? (k_end - k_begin + kStepK - 1) / kStepK : 0;
+    const uint32_t bar = smem_u32(bars);
+    const uint32_t c_full = bar, c_empty = bar + 8 * kMaxRing, w_full = bar + 16 * kMaxRing, w_empty = bar + 24 * kMaxRing,
+                   x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, done = bar + 48 * kMaxRing;
+    const uint32_t codes = smem_u32(smem + plan.codes), weights = smem_u32(smem + plan.weights), xrows = smem_u32(smem + plan.rows);
+    auto gave_up = [&](uint32_t code) {
+        abort_flag = 1;
+        set_w4_status(code);
+    };
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kMaxRing; ++i) {
+            mbar_init(c_full + 8 * i, 1);
+            mbar_init(c_empty + 8 * i, 8);
+            mbar_init(w_full + 8 * i, 8);
+            mbar_init(w_empty + 8 * i, 1);
+            mbar_init(x_full + 8 * i, plan.x_tma ? 1 : 4);
+            mbar_init(x_empty + 8 * i, 1);
+        }
+        mbar_init(done, 1);
+        abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_at), plan.tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int cs = 0, xs = 0, step = 0;
+            uint32_t cp = 0, xp = 0;
+            for (int st = 0; st < stages; ++st) {
+                if (!wait_phase(c_empty + 8 * cs, cp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                if (abort_flag) break;
+                mbar_arrive_expect_tx(c_full + 8 * cs, kTileM * 128);
+                tma_load_2d(codes + cs * kTileM * 128, &codes_map, (k_begin + st * kStageK) / 16, o0, c_full + 8 * cs);
+                if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
+                if (plan.x_tma)
+                    for (int i = 0; i < kStageK / kStepK && step < steps; ++i, ++step) {
+                        if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                        if (abort_flag) break;
+                        mbar_arrive_expect_tx(x_full + 8 * xs, tile_n * 128);
+                        tma_load_2d(xrows + xs * tile_n * 128, &rows_map, k_begin + step * kStepK, static_cast<int>(r0), x_full + 8 * xs);
+                        if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+                    }
+            }
+            if (abort_flag) {  // copies still on their way; the waits end by themselves
+                for (int i = 0; i < plan.rings[0]; ++i) wait_phase(c_full + 8 * i, (i < cs ? cp : cp ^ 1), nullptr);
+                if (plan.x_tma)
+                    for (int i = 0; i < plan.rings[2]; ++i) wait_phase(x_full + 8 * i, (i < xs ? xp : xp ^ 1), nullptr);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        const uint32_t idesc = instr_desc(128, 0, BF ? kOpBF16 : kOpF16) | static_cast<uint32_t>(tile_n >> 3) << 17;
+        int ws = 0, xs = 0;
+        uint32_t wp = 0, xp = 0;
+        for (int step = 0; step < steps; ++step) {
+            if (!wait_phase(w_full + 8 * ws, wp, &abort_flag)) gave_up(kStatusTimeoutFull);
+            if (!wait_phase(x_full + 8 * xs, xp, &abort_flag)) gave_up(kStatusTimeoutFull);
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t bd = desc_sw128(xrows + xs * tile_n * 128);
+#pragma unroll
+                for (int m = 0; m < (TWO ? 2 : 1); ++m) {
+                    const uint64_t ad = desc_sw128(weights + ws * kTileM * 128 + m * 128 * 128);
+#pragma unroll
+                    for (int i = 0; i < kStepK / 16; ++i)
+                        mma_f16(tmem + m * tile_n, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
+                }
+                mma_commit(w_empty + 8 * ws);
+                mma_commit(x_empty + 8 * xs);
+                if (step == steps - 1) mma_commit(done);
+            }
+            __syncwarp();
+            if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
+            if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+        }
+    } else if (warp >= 12) {  // rows that TMA does not bring: 16-byte cells of eight values, as the swizzle places them
+        const int tid = threadIdx.x - 384, cells = rows * 8, kxb = a.x_type == kTokE4M3 ? 1 : 2;
+        int xs = 0;
+        uint32_t xp = 0;
+        // a step's cells, eight at a time in flight
+        for (int step = 0; step < steps; ++step) {
+            const int k0 = k_begin + step * kStepK;
+            const uint8_t* const src = static_cast<const uint8_t*>(a.x) + (r0 * a.x_stride + k0) * kxb;
+            bool waited = false;
+            for (int c0 = 0; c0 < tile_n * 8; c0 += 8 * 128) {
+                uint4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int cell = c0 + i * 128 + tid, r = cell / 8, c = cell % 8;
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (cell < cells && k0 + c * 8 < k_end) v[i] = in_order(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
+                }
+                if (!waited && !wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                waited = true;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int cell = c0 + i * 128 + tid, r = cell / 8, c = cell % 8;
+                    if (cell < tile_n * 8) *reinterpret_cast<uint4*>(smem + plan.rows + xs * tile_n * 128 + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_full + 8 * xs);
+            if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+        }
+    } else if (warp >= 4) {
+        // thread: one output of two tiles, or half of each step's inputs of an output of one
+        const int tid = threadIdx.x - 128, row = TWO ? tid : tid % 128, half = TWO ? 0 : tid / 128;
+        const int o = min(o0 + row, n - 1);
+        const int64_t at = static_cast<int64_t>(o) * groups;
+        const bool wide = a.w.scale_type == kTokF32;
+        auto scale_at = [&](int g) { return tok_load(a.w.scales, at + g, a.w.scale_type); };
+        float back = 1.f, factor = 1.f;  // the output's power of two, and its reciprocal
+        if (!BF) {
+            float top = 0.f;
+            const int sb = wide ? 4 : 2;
+            const uint8_t* const p = static_cast<const uint8_t*>(a.w.scales) + at * sb;
+            int g = 0;
+            if (!wide && groups % 8 == 0 && reinterpret_cast<uintptr_t>(a.w.scales) % 16 == 0) {
+#pragma unroll 4
+                for (; g < groups; g += 8) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + g * 2));
+                    const uint32_t r[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t h = (i % 2 ? r[i / 2] >> 16 : r[i / 2]) & 0x7fffu;
+                        top = fmaxf(top, a.w.scale_type == kTokF16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16));
+                    }
+                }
+            }
+#pragma unroll 8
+            for (; g < groups; ++g) top = fmaxf(top, fabsf(scale_at(g)));
+            // 2^e <= top < 2^(e + 1), e kept where 2^e and 2^-e are normal; an infinity or zero keeps 1
+            if (top > 0.f && top < INFINITY) {
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
+                back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+                factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+            }
+        }
+        // scales and zero points of a stage's chunks of 32 inputs, a stage ahead
+        constexpr int kChunks = TWO ? 8 : 4;
+        float sc[kChunks];
+        uint32_t zo[kChunks];
+        const float inv_group = 1.f / static_cast<float>(group);
+        auto load_scales = [&](int k0) {
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int kc = k0 + (TWO ? c * 32 : c * 64 + half * 32);
+                sc[c] = 0.f;
+                zo[c] = 8;
+                if (kc < k_end) {
+                    // (kc + 1/2) / group truncated: exact while k < 2^21
+                    const int g = k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group;
+                    sc[c] = scale_at(g);
+                    if (a.w.zeros) zo[c] = __ldg(a.w.zeros + at + g);
+                }
+            }
+        };
+        load_scales(k_begin);
+        int cs = 0, ws = 0, step = 0;
+        uint32_t cp = 0, wp = 0;
+        for (int st = 0; st < stages; ++st) {
+            uint32_t hi[kChunks], lo[kChunks], z[kChunks];
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const float s = sc[c] * factor, h = round16f<BF>(s), l = s - h;
+                hi[c] = pair16<BF>(h, h);
+                lo[c] = l == l ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
+                z[c] = zero_terms<BF>(zo[c]);
+            }
+            if (st + 1 < stages) load_scales(k_begin + (st + 1) * kStageK);
+            if (!wait_phase(c_full + 8 * cs, cp, &abort_flag)) gave_up(kStatusTimeoutFull);
+            const uint32_t from = codes + cs * kTileM * 128 + row * 128;
+#pragma unroll
+            for (int b = 0; b < kStageK / kStepK; ++b) {
+                if (step >= steps) break;
+                ++step;
+                if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
+                const uint32_t to = weights + ws * kTileM * 128 + row * 128;
+#pragma unroll
+                for (int h = 0; h < (TWO ? 2 : 1); ++h) {
+                    const int part = TWO ? h : half, chunk = TWO ? 2 * b + h : b;
+                    uint4 v, out[4];
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(from + (((2 * b + part) ^ (row & 7)) << 4)));
+                    weights32<BF>(v, hi[chunk], lo[chunk], z[chunk], out);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((4 * part + c) ^ (row & 7)) << 4)), "r"(out[c].x),
+                                     "r"(out[c].y), "r"(out[c].z), "r"(out[c].w)
+                                     : "memory");
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(w_full + 8 * ws);
+                if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c_empty + 8 * cs);
+            if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
+        }
+        // epilogue: warp w reads TMEM lanes 32 (w % 4)..; two tiles: one tile each, one tile: half the columns each
+        if (steps && !wait_phase(done, 0, &abort_flag)) gave_up(kStatusTimeoutAcc);
+        tc_fence_after();
+        const int quad = warp % 4, part = (warp - 4) / 4;
+        const int out = o0 + (TWO ? part * 128 : 0) + quad * 32 + lane;
+        const int out_row = (TWO ? part * 128 : 0) + quad * 32 + lane;
+        // the power of two belongs to the output this thread made weights of, not the one it stores
+        float* const factors = reinterpret_cast<float*>(smem + plan.row_factor);
+        if (!BF) {
+            if (TWO || half == 0) factors[row] = back;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            back = factors[out_row];
+        }
+        const float bias = a.bias && out < n ? a.bias[out] : 0.f;
+        const int col0 = TWO ? 0 : part * (tile_n / 2), cols = TWO ? tile_n : tile_n / 2;
+        const uint32_t acc = tmem + (TWO ? part * tile_n : 0) + (static_cast<uint32_t>(quad * 32) << 16);
+        float* const partial = reinterpret_cast<float*>(smem);  // [row][output], over the rings
+        for (int c = 0; c < cols; c += 8) {
+            uint32_t v[8];
+            asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                         : "r"(acc + col0 + c));
+            tmem_wait();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i])::"memory");
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = col0 + c + i;
+                float f = steps ? __uint_as_float(v[i]) * back : 0.f;
+                if (plan.split > 1) {
+                    partial[r * kTileM + out_row] = f;
+                } else if (r < rows && out < n) {
+                    if (a.x_scale) f *= a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
+                    tok_store(a.y, (r0 + r) * a.y_stride + out, a.y_type, f + bias);
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    if (plan.split > 1) {  // each block adds up a share of the rows over the cluster
+        __syncwarp();
+        cluster_sync();
+        const uint32_t base = smem_u32(smem);
+        for (int i = threadIdx.x; i < rows * kTileM; i += blockDim.x) {
+            const int r = i / kTileM, o = i % kTileM;
+            if (r % plan.split != rank || o0 + o >= n) continue;
+            float f = 0.f;
+            for (int p = 0; p < plan.split; ++p) f += ld_cluster(base + i * 4, p);
+            if (a.x_scale) f *= a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
+            if (a.bias) f += a.bias[o0 + o];
+            tok_store(a.y, (r0 + r) * a.y_stride + o0 + o, a.y_type, f);
+        }
+        cluster_sync();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, plan.tmem_cols);
+    }
+}
+
+template <bool BF, bool TWO>
+cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
+    constexpr int kTileM = TWO ? 256 : 128;
+    auto* kern = w4_many_kernel<BF, TWO>;
+    CUtensorMap codes, rows;
+    cudaError_t e = tmap_rows(&codes, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kTileM);
+    if (e == cudaSuccess) {
+        if (p.x_tma)
+            e = tmap_rows(&rows, a.x, 2, a.w.k, a.rows, a.x_stride * 2, p.tile_n);
+        else
+            rows = codes;
+    }
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((a.w.n + kTileM - 1) / kTileM * p.split, (a.rows + p.tile_n - 1) / p.tile_n);
+    cfg.blockDim = dim3(p.x_tma ? 384 : 512);
+    cfg.dynamicSmemBytes = p.bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = p.split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = p.split > 1 ? 1 : 0;
+    count_launch();
+    e = cudaLaunchKernelEx(&cfg, kern, a, p, codes, rows);
+    return e == cudaSuccess ? cudaGetLastError() : e;
+}
+
+}  // namespace
+
+cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
+    ManyPlan p{};
+    const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
+    p.x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
+    p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
+    p.tile_n = a.rows >= 256 ? 256 : (a.rows + 15) / 16 * 16;
+    const int64_t tiles_n = (a.rows + p.tile_n - 1) / p.tile_n;
+    const bool two = (a.w.n + 255) / 256 * tiles_n >= sms;
+    const int tile_m = two ? 256 : 128;
+    const int64_t tiles = (a.w.n + tile_m - 1) / tile_m * tiles_n;
+    const int all_stages = (a.w.k + kStageK - 1) / kStageK;
+    // few tiles: a cluster shares one, each block a range of k, while a block keeps two stages of codes
+    p.split = 1;
+    while (!two && p.split < 8 && tiles * p.split * 2 <= sms && all_stages >= p.split * 4) p.split *= 2;
+    p.stages_each = (all_stages + p.split - 1) / p.split;
+    p.tmem_cols = 32;
+    while (p.tmem_cols < p.tile_n * (two ? 2 : 1)) p.tmem_cols *= 2;
+    const int factor_bytes = 1024;
+    // rings: half of the room left by two stages of weights for codes and weights in turn, at least two of each
+    int room = kSmemMax - factor_bytes;
+    const int w = tile_m * 128, x = p.tile_n * 128;
+    p.rings[0] = p.rings[1] = p.rings[2] = 2;
+    room -= 4 * w + 2 * x;
+    for (bool more = true; more;) {
+        more = false;
+        for (int i : {2, 0, 1}) {
+            const int cost = i == 2 ? x : w;
+            if (p.rings[i] < (i == 1 ? 4 : 6) && room >= cost) {
+                ++p.rings[i];
+                room -= cost;
+                more = true;
+            }
+        }
+    }
+    p.codes = 0;
+    p.weights = p.rings[0] * w;
+    p.rows = p.weights + p.rings[1] * w;
+    p.row_factor = p.rows + p.rings[2] * x;
+    p.bytes = p.row_factor + factor_bytes;
+    if (p.split > 1) {  // the partial sums lie over the rings
+        const int partial = p.tile_n * tile_m * 4;
+        if (partial > p.row_factor) {
+            p.row_factor = partial;
+            p.bytes = partial + factor_bytes;
+        }
+    }
+    if (a.x_type == kTokBF16) return two ? launch<true, true>(a, p, s) : launch<true, false>(a, p, s);
+    return two ? launch<false, true>(a, p, s) : launch<false, false>(a, p, s);
+}
+
+cudaError_t w4_many_status(uint32_t* code) { return take_status(code); }
+
+}  // namespace fxk

@@ -438,6 +438,10 @@ fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t
                        const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, const float* dev_bias,
                        void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream);
 
+/* FX_OK, or FX_INTERNAL when a wait inside an fx_w4_linear kernel on `device` gave up since the last call (every
+ * wait is bounded; such a kernel ends by itself and its outputs are undefined). Synchronises the device. */
+fx_status fx_w4_device_status(int device);
+
 /* The 4-bit form of weights [n][k] (f32, f16, bf16) in fx_w4_linear's layout, one scale (and zero point) per
  * `group` inputs, each quotient rounded to nearest, ties to even:
  *   dev_zeros NULL  scale = max |w| / 7 rounded to scale_type, code = clamp(round(w / scale) + 8, 0, 15)

@@ -576,6 +576,14 @@ def test_repeatable(cuda_torch):
             assert all(torch.equal(p, q) for p, q in zip(first, (b.sum, b.q.view(torch.uint8), b.qs, b.y)))
 
 
+def test_no_wait_gave_up(cuda_torch):
+    run_linear(cuda_torch, 3, 64, 256, 64)
+    run_linear(cuda_torch, 30, 64, 256, 64)
+    fx.w4_device_status(0)
+    with pytest.raises(fx.FxError):
+        fx.w4_device_status(-1)
+
+
 def test_host_pointers_are_refused(cuda_torch):
     torch = cuda_torch
     d = torch.zeros(64, 64, device="cuda", dtype=torch.bfloat16)
