@@ -1,82 +1,237 @@
 // rms_norm.cu — root-mean-square norm of token rows with the residual's addition and 8-bit output.
+//
+// Bound by memory: x, residual, sum and y pass once (7 bytes a value for bf16 to e4m3). A row's h = x + residual
+// stays in the registers of its team of threads, eight consecutive values a thread and turn, between the three
+// looks at it: the sum of squares, the largest magnitude, the output. A team is a warp or a block: a warp while
+// a row fits it, since its reductions need no barrier, else the smallest block that keeps 16 values a thread, so that an SM holds
+// many rows at different stages and its loads never pause.
 #include "counters.hpp"
 #include "token.cuh"
 
 namespace fxk {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kVec = 8;  // consecutive values of a thread: 16 bytes of a 16-bit type
 
-// Sum and maximum of a value over the block; every thread gets them.
-__device__ float block_sum(float v, float* red) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = 0.f;
-    for (int i = 0; i < kThreads / 32; ++i) v += red[i];
-    return v;
-}
-__device__ uint32_t block_max(uint32_t v, uint32_t* red) {
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = 0;
-    for (int i = 0; i < kThreads / 32; ++i) v = max(v, red[i]);
-    return v;
-}
-
-// One block per row, the row's h in shared memory.
-__global__ void __launch_bounds__(kThreads) rms_norm_kernel(const RmsNormArgs a) {
-    extern __shared__ float h[];
-    __shared__ float red[kThreads / 32];
-    const int64_t row = blockIdx.x;
-    float ss = 0.f;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-        float v = tok_load(a.x, row * a.x_stride + c, a.x_type);
-        if (a.residual) v += tok_load(a.residual, row * a.residual_stride + c, a.residual_type);
-        h[c] = v;
-        ss += v * v;
+// Eight 16-bit values, widened. The type's branch lies around the eight, not inside.
+__device__ __forceinline__ void unpack8(const uint4& v, int type, float (&f)[kVec]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if (type == kTokF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = __half22float2(reinterpret_cast<const __half2&>(w[j]));
+            f[2 * j] = t.x;
+            f[2 * j + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f[2 * j] = __uint_as_float(w[j] << 16);
+            f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
     }
-    ss = block_sum(ss, red);
+}
+
+// A thread's eight values of turn u in a row at p, widened. VEC: consecutive from column (u TEAM + me) 8 on, 16-byte
+// aligned; else one of every TEAM columns, so that neighbours read neighbours. Columns past the row are 0.
+template <int TEAM, bool VEC>
+__device__ __forceinline__ int column(int u, int j, int me) {
+    return VEC ? (u * TEAM + me) * kVec + j : (u * kVec + j) * TEAM + me;
+}
+template <int TEAM, bool VEC, bool CONST>
+__device__ __forceinline__ void load8(const void* p, int64_t row, int type, int u, int me, int cols, float (&f)[kVec]) {
+    if (VEC) {
+        const int c = column<TEAM, VEC>(u, 0, me);
+        if (c >= cols) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) f[j] = 0.f;
+        } else if (type == kTokF32) {
+            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + row + c);
+            const float4 a = CONST ? __ldg(q) : q[0], b = CONST ? __ldg(q + 1) : q[1];
+            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+        } else {
+            const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + row + c);
+            unpack8(CONST ? __ldg(q) : q[0], type, f);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            const int c = column<TEAM, VEC>(u, j, me);
+            f[j] = c < cols ? tok_load(p, row + c, type) : 0.f;
+        }
+    }
+}
+template <int TEAM, bool VEC>
+__device__ __forceinline__ void store8(void* p, int64_t row, int type, int u, int me, int cols, const float (&f)[kVec]) {
+    if (VEC) {
+        const int c = column<TEAM, VEC>(u, 0, me);
+        if (c >= cols) return;
+        if (type == kTokF32) {
+            float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + row + c);
+            q[0] = make_float4(f[0], f[1], f[2], f[3]);
+            q[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else if (type == kTokE4M3) {
+            uint32_t w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * j], f[4 * j + 1]), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * j + 2], f[4 * j + 3]), __NV_SATFINITE, __NV_E4M3);
+                w[j] = lo | hi << 16;
+            }
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p) + row + c) = make_uint2(w[0], w[1]);
+        } else {
+            uint32_t w[4];
+            if (type == kTokF16) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+                    w[j] = reinterpret_cast<const uint32_t&>(h);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                    w[j] = reinterpret_cast<const uint32_t&>(h);
+                }
+            }
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            const int c = column<TEAM, VEC>(u, j, me);
+            if (c < cols) tok_store(p, row + c, type, f[j]);
+        }
+    }
+}
+
+// Sum and maximum over the team; every thread gets them. red: a block's shared memory.
+template <int TEAM>
+__device__ __forceinline__ float team_sum(float v, float* red) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (TEAM == 32) return v;
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = threadIdx.x % 32 < TEAM / 32 ? red[threadIdx.x % 32] : 0.f;
+#pragma unroll
+    for (int o = TEAM / 64; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+template <int TEAM>
+__device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (TEAM == 32) return v;
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+    __syncthreads();
+    return __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32 < TEAM / 32 ? threadIdx.x % 32 : 0]);
+}
+
+// TEAM threads a row, TURNS times eight values each.
+template <int TEAM, int TURNS, bool VEC>
+__global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_kernel(const __grid_constant__ RmsNormArgs a) {
+    __shared__ float red[3][32];
+    const int me = threadIdx.x % TEAM;
+    const int64_t row = TEAM == 32 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+    if (row >= a.rows) return;
+    float h[TURNS][kVec];
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.x, row * a.x_stride, a.x_type, u, me, a.cols, h[u]);
+    if (a.residual) {
+        float r[TURNS][kVec];
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.residual, row * a.residual_stride, a.residual_type, u, me, a.cols, r[u]);
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) h[u][j] += r[u][j];
+    }
+    if (a.sum) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) store8<TEAM, VEC>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) ss = fmaf(h[u][j], h[u][j], ss);
+    ss = team_sum<TEAM>(ss, red[0]);
     float pre = 1.f;
     if (!(ss < 3.0e38f)) {  // squares past f32's range (or a NaN or infinity, which stays one): sum smaller ones
         pre = 8.2718061e-25f;  // 2^-80
         ss = 0.f;
-        for (int c = threadIdx.x; c < a.cols; c += kThreads) ss += (h[c] * pre) * (h[c] * pre);
-        ss = block_sum(ss, red);
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                h[u][j] *= pre;
+                ss = fmaf(h[u][j], h[u][j], ss);
+            }
+        ss = team_sum<TEAM>(ss, red[1]);
     }
     const float r = rsqrtf(ss / static_cast<float>(a.cols) + a.eps * pre * pre);
-    float scale = a.scale_mode == kScaleTensor ? a.scale[0] : 1.f;
-    uint32_t amax = 0;  // |v| as bits: a NaN is above every number
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
-        if (a.sum) tok_store(a.sum, row * a.sum_stride + c, a.residual_type, h[c]);
-        h[c] = h[c] * pre * r * (a.weight ? tok_load(a.weight, c, a.weight_type) : 1.f);
-        amax = max(amax, __float_as_uint(h[c]) & 0x7fffffffu);
+    // v = h weight r: r joins the scale, so that a value takes two products
+    float top = 0.f;
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+        if (a.weight) {
+            float w[kVec];
+            load8<TEAM, VEC, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) h[u][j] *= w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(h[u][j])));  // columns past the row are 0
     }
+    float times = r;
     if (a.scale_mode == kScaleRow) {
-        amax = block_max(amax, reinterpret_cast<uint32_t*>(red));
-        amax = max(amax, __float_as_uint(1e-30f));
-        scale = __uint_as_float(amax) / 448.f;
-        if (threadIdx.x == 0) a.scale[row] = scale;
+        // as bits a NaN is above every number
+        const uint32_t most = team_max<TEAM>(__float_as_uint(top * r) & 0x7fffffffu, reinterpret_cast<uint32_t*>(red[2]));
+        const float scale = __uint_as_float(max(most, __float_as_uint(1e-30f))) * (1.f / 448.f);
+        if (me == 0) a.scale[row] = scale;
+        times = r * (1.f / scale);
+    } else if (a.scale_mode == kScaleTensor) {
+        times = r * (1.f / a.scale[0]);
     }
-    const float inv = 1.f / scale;
-    for (int c = threadIdx.x; c < a.cols; c += kThreads) tok_store(a.y, row * a.y_stride + c, a.y_type, h[c] * inv);
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) h[u][j] *= times;
+        store8<TEAM, VEC>(a.y, row * a.y_stride, a.y_type, u, me, a.cols, h[u]);
+    }
+}
+
+template <int TEAM, int TURNS>
+cudaError_t launch(const RmsNormArgs& a, bool vec, cudaStream_t s) {
+    const int threads = TEAM == 32 ? 128 : TEAM, per = threads / TEAM;
+    const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + per - 1) / per);
+    count_launch();
+    if (vec)
+        rms_norm_kernel<TEAM, TURNS, true><<<grid, threads, 0, s>>>(a);
+    else
+        rms_norm_kernel<TEAM, TURNS, false><<<grid, threads, 0, s>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
 cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
-    const size_t smem = static_cast<size_t>(a.cols) * sizeof(float);
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(rms_norm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kRmsMaxCols * static_cast<int>(sizeof(float)));
-        if (e != cudaSuccess) return e;
-    }
-    count_launch();
-    rms_norm_kernel<<<a.rows, kThreads, smem, s>>>(a);
-    return cudaGetLastError();
+    auto ok = [&](const void* p, int64_t stride, int type) {  // 16-byte aligned rows (8-byte of e4m3)
+        const int64_t size = type == kTokF32 ? 4 : type == kTokE4M3 ? 1 : 2, unit = type == kTokE4M3 ? 8 : 16;
+        return !p || (reinterpret_cast<uintptr_t>(p) % unit == 0 && stride * size % unit == 0);
+    };
+    const bool vec = a.cols % kVec == 0 && ok(a.x, a.x_stride, a.x_type) && ok(a.residual, a.residual_stride, a.residual_type) &&
+                     ok(a.sum, a.sum_stride, a.residual_type) && ok(a.weight, 0, a.weight_type) && ok(a.y, a.y_stride, a.y_type);
+    // few rows: as many threads as the row has eights, for the shortest way through; many: 16 values a thread
+    const bool few = a.rows <= 148 * 2;
+    if (a.cols <= 256) return launch<32, 1>(a, vec, s);
+    if (a.cols <= 512) return launch<32, 2>(a, vec, s);
+    if (a.cols <= 1024) return few ? launch<128, 1>(a, vec, s) : launch<32, 4>(a, vec, s);
+    if (a.cols <= 2048) return few ? launch<256, 1>(a, vec, s) : launch<128, 2>(a, vec, s);
+    if (a.cols <= 4096) return few ? launch<512, 1>(a, vec, s) : launch<256, 2>(a, vec, s);
+    if (a.cols <= 8192) return few ? launch<1024, 1>(a, vec, s) : launch<512, 2>(a, vec, s);
+    if (a.cols <= 16384) return launch<1024, 2>(a, vec, s);
+    return launch<1024, 4>(a, vec, s);
 }
 
 }  // namespace fxk

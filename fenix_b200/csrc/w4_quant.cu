@@ -1,11 +1,20 @@
 // w4_quant.cu — weights to 4-bit codes with group scales (and zero points), and back.
+//
+// Bound by memory: a weight passes once (4 or 2 bytes against half a byte and its share of a scale). A team of
+// threads holds a group in registers between its extremes and its codes, eight consecutive weights a thread: 16 or
+// 32 bytes in, a word of codes out, the extremes by shuffles inside the warp. Codes are those of f32's correctly
+// rounded quotients: a product with the scale's reciprocal stands for the quotient unless it lies so near a half
+// that the two might round differently (or is not a small number); then the quotient is taken.
 #include "counters.hpp"
 #include "token.cuh"
+
+#include <algorithm>
 
 namespace fxk {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kEight = 8;
 
 // v rounded to the scale's type and back; past the type's range, its largest finite value.
 __device__ __forceinline__ float round_scale(float v, int type) {
@@ -18,66 +27,203 @@ __device__ __forceinline__ float code_of(float w, float scale, float zero) {
     return fminf(fmaxf(q, 0.f), 15.f);
 }
 
-// One warp per group.
-__global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* w, int w_type, int64_t w_stride, const W4Args q) {
-    const int lane = threadIdx.x % 32;
-    const int per_row = q.k / q.group;
-    const int64_t g = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + threadIdx.x / 32;
-    if (g >= static_cast<int64_t>(q.n) * per_row) return;
-    const int64_t base = g / per_row * w_stride + g % per_row * q.group;
-    float lo = 0.f, hi = 0.f;
-    for (int i = lane; i < q.group; i += 32) {
-        const float v = tok_load(w, base + i, w_type);
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
+// Eight codes in a word. The product t = w / scale is off by less than 2^-18 while |t| < 32, so that rounding it gives
+// the quotient's code if it is further than 2^-16 from a half. The magic constant puts t + zero into the low mantissa.
+__device__ __forceinline__ uint32_t codes_of(const float (&w)[kEight], float scale, float inv, float zero) {
+    const float magic = 12582912.f + zero, low = -zero, high = 15.f - zero;
+    uint32_t r = 0;
+    bool near = false;
+#pragma unroll
+    for (int j = kEight - 1; j >= 0; --j) {
+        const float t = w[j] * inv, m = fminf(fmaxf(t, low), high) + magic;
+        near |= !(fabsf(t - (m - magic)) <= 0.5f - 1.52587890625e-5f);
+        r = r * 16 + __float_as_uint(m);
     }
-    for (int o = 16; o; o >>= 1) {
+    r -= 0x4b400000u * 0x11111111u;  // the constants of the eight
+    if (near) {
+        r = 0;
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) r |= static_cast<uint32_t>(code_of(w[j], scale, zero)) << (4 * j);
+    }
+    return r;
+}
+
+template <bool VEC>
+__device__ __forceinline__ void load8(const void* p, int64_t i, int type, float (&f)[kEight]) {
+    if (VEC && type == kTokF32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 a = __ldcs(q), b = __ldcs(q + 1);
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else if (VEC) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (type == kTokF16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 t = __half22float2(reinterpret_cast<const __half2&>(w[j]));
+                f[2 * j] = t.x;
+                f[2 * j + 1] = t.y;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[2 * j] = __uint_as_float(w[j] << 16);
+                f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) f[j] = tok_load(p, i + j, type);
+    }
+}
+
+// TEAM lanes of a warp per group (4: groups of 32, ..., 32: any), HOLD times eight weights a lane in registers; a
+// longer group is read a second time for its codes.
+template <int TEAM, int HOLD, bool VEC>
+__global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __restrict__ w, int w_type, int64_t w_stride, const W4Args q) {
+    const int me = threadIdx.x % TEAM;
+    const uint32_t per_row = q.k / q.group, g32 = blockIdx.x * (kThreads / TEAM) + threadIdx.x / TEAM;  // below 2^31: the launcher's rows
+    const int64_t g = g32;
+    const bool on = g32 < q.n * per_row;  // lanes of no group run along: the shuffles are the warp's
+    const int64_t base = on ? static_cast<int64_t>(g32 / per_row) * w_stride + g32 % per_row * static_cast<int64_t>(q.group) : 0;
+    const int eights = on ? q.group / kEight : 0;
+    float f[HOLD][kEight], lo = 0.f, hi = 0.f;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (h * TEAM + me < eights) load8<VEC>(w, base + (h * TEAM + me) * kEight, w_type, f[h]);
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (h * TEAM + me < eights) {
+#pragma unroll
+            for (int j = 0; j < kEight; ++j) {
+                lo = fminf(lo, f[h][j]);
+                hi = fmaxf(hi, f[h][j]);
+            }
+        }
+    for (int e = HOLD * TEAM + me; e < eights; e += TEAM) {
+        float t[kEight];
+        load8<VEC>(w, base + static_cast<int64_t>(e) * kEight, w_type, t);
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) {
+            lo = fminf(lo, t[j]);
+            hi = fmaxf(hi, t[j]);
+        }
+    }
+#pragma unroll
+    for (int o = TEAM / 2; o; o >>= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     const float scale = round_scale(q.zeros ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f), q.scale_type);
     float zero = 8.f;
     if (q.zeros) zero = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(-lo, scale)), 0.f), 15.f) : 0.f;
-    if (lane == 0) {
+    if (on && me == 0) {
         tok_store(const_cast<void*>(q.scales), g, q.scale_type, scale);
         if (q.zeros) const_cast<uint8_t*>(q.zeros)[g] = static_cast<uint8_t>(zero);
     }
-    for (int i = 2 * lane; i < q.group; i += 64) {
-        const float a = code_of(tok_load(w, base + i, w_type), scale, zero);
-        const float b = code_of(tok_load(w, base + i + 1, w_type), scale, zero);
-        const_cast<uint8_t*>(q.codes)[(g * q.group + i) / 2] =
-            static_cast<uint8_t>(static_cast<int>(a) | static_cast<int>(b) << 4);
+    uint32_t* const codes = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(q.codes)) + g * (q.group / kEight);
+    const float inv = __fdiv_rn(1.f, scale);
+    auto put = [&](int e, const float(&v)[kEight]) { codes[e] = codes_of(v, scale, inv, zero); };
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if (h * TEAM + me < eights) put(h * TEAM + me, f[h]);
+    for (int e = HOLD * TEAM + me; e < eights; e += TEAM) {
+        float t[kEight];
+        load8<VEC>(w, base + static_cast<int64_t>(e) * kEight, w_type, t);
+        put(e, t);
     }
 }
 
-__global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const W4Args q, void* w, int w_type, int64_t w_stride) {
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) * 2;
-    if (i >= static_cast<int64_t>(q.n) * q.k) return;
-    const int64_t g = i / q.group, o = i / q.k * w_stride + i % q.k;
-    const int c = q.codes[i / 2];
-    const int z = q.zeros ? q.zeros[g] : 8;
+// A thread: a word of eight codes, eight consecutive values. A code is or'ed into the mantissa of 2^23.
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const W4Args q, void* __restrict__ w, int w_type, int64_t w_stride, int row0) {
+    const int e = blockIdx.x * kThreads + threadIdx.x, row = row0 + blockIdx.y;  // e: word of the row
+    if (e >= q.k / kEight) return;
+    // (e + 1/2) / words truncated: exact while e < 2^21, as k < 2^24
+    const int words = q.group / kEight, of_row = static_cast<int>((static_cast<float>(e) + 0.5f) * __frcp_rn(static_cast<float>(words)));
+    const int64_t g = static_cast<int64_t>(row) * (q.k / q.group) + of_row;
+    const uint32_t c = __ldcs(reinterpret_cast<const uint32_t*>(q.codes) + static_cast<int64_t>(row) * (q.k / kEight) + e);
     const float s = tok_load(q.scales, g, q.scale_type);
-    tok_store(w, o, w_type, s * static_cast<float>((c & 15) - z));
-    tok_store(w, o + 1, w_type, s * static_cast<float>((c >> 4) - z));
+    const float off = 8388608.f + (q.zeros ? static_cast<float>(q.zeros[g]) : 8.f);
+    float f[kEight];
+#pragma unroll
+    for (int j = 0; j < kEight; ++j) f[j] = s * (__uint_as_float((c >> (4 * j) & 15u) | 0x4b000000u) - off);
+    const int64_t o = row * w_stride + e * kEight;
+    if (VEC && w_type == kTokF32) {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(w) + o);
+        __stcs(p, make_float4(f[0], f[1], f[2], f[3]));
+        __stcs(p + 1, make_float4(f[4], f[5], f[6], f[7]));
+    } else if (VEC) {
+        uint32_t r[4];
+        if (w_type == kTokF16) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+                r[j] = reinterpret_cast<const uint32_t&>(h);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                r[j] = reinterpret_cast<const uint32_t&>(h);
+            }
+        }
+        __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(w) + o), make_uint4(r[0], r[1], r[2], r[3]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) tok_store(w, o + j, w_type, f[j]);
+    }
+}
+
+bool aligned_rows(const void* p, int64_t stride, int type) {
+    const int64_t size = type == kTokF32 ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+}
+
+template <int TEAM, int HOLD>
+cudaError_t quantize(const void* w, int w_type, int64_t w_stride, const W4Args& q, cudaStream_t s) {
+    const int64_t per_row = q.k / q.group, w_size = w_type == kTokF32 ? 4 : 2, s_size = q.scale_type == kTokF32 ? 4 : 2;
+    const int64_t most = std::max<int64_t>((int64_t{1} << 30) / per_row, 1);  // rows of a launch
+    for (int64_t row = 0; row < q.n; row += most) {
+        W4Args part = q;
+        part.n = static_cast<int>(std::min<int64_t>(most, q.n - row));
+        part.codes = q.codes + row * (q.k / 2);
+        part.scales = static_cast<const uint8_t*>(q.scales) + row * per_row * s_size;
+        if (q.zeros) part.zeros = q.zeros + row * per_row;
+        const void* const from = static_cast<const uint8_t*>(w) + row * w_stride * w_size;
+        const unsigned blocks = static_cast<unsigned>((part.n * per_row * TEAM + kThreads - 1) / kThreads);
+        count_launch();
+        if (aligned_rows(w, w_stride, w_type))
+            w4_quantize_kernel<TEAM, HOLD, true><<<blocks, kThreads, 0, s>>>(from, w_type, w_stride, part);
+        else
+            w4_quantize_kernel<TEAM, HOLD, false><<<blocks, kThreads, 0, s>>>(from, w_type, w_stride, part);
+        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace
 
 cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, const W4Args& q, cudaStream_t s) {
-    const int64_t groups = static_cast<int64_t>(q.n) * (q.k / q.group);
-    const int64_t blocks = (groups + kThreads / 32 - 1) / (kThreads / 32);
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    count_launch();
-    w4_quantize_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(w, w_type, w_stride, q);
-    return cudaGetLastError();
+    if (q.group == 32) return quantize<4, 1>(w, w_type, w_stride, q, s);
+    if (q.group <= 64) return quantize<8, 1>(w, w_type, w_stride, q, s);
+    if (q.group <= 128) return quantize<16, 1>(w, w_type, w_stride, q, s);
+    return quantize<32, 4>(w, w_type, w_stride, q, s);
 }
 
 cudaError_t launch_w4_dequantize(const W4Args& q, void* w, int w_type, int64_t w_stride, cudaStream_t s) {
-    const int64_t blocks = (static_cast<int64_t>(q.n) * q.k / 2 + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    count_launch();
-    w4_dequantize_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(q, w, w_type, w_stride);
-    return cudaGetLastError();
+    constexpr int kRows = 65535;  // of a launch
+    const unsigned across = (q.k / kEight + kThreads - 1) / kThreads;
+    for (int row0 = 0; row0 < q.n; row0 += kRows) {
+        const dim3 grid(across, static_cast<unsigned>(q.n - row0 < kRows ? q.n - row0 : kRows));
+        count_launch();
+        if (aligned_rows(w, w_stride, w_type))
+            w4_dequantize_kernel<true><<<grid, kThreads, 0, s>>>(q, w, w_type, w_stride, row0);
+        else
+            w4_dequantize_kernel<false><<<grid, kThreads, 0, s>>>(q, w, w_type, w_stride, row0);
+        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 }  // namespace fxk
