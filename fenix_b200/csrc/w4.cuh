@@ -38,32 +38,36 @@ __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t b
     return r;
 }
 
-// Eight e4m3 or 16-bit values at p as they lie in memory, e4m3 widened to f16; vec: p is aligned to eight of them.
-__device__ __forceinline__ uint4 in_order(const uint8_t* p, int x_type, bool vec) {
+// Eight e4m3 (in x, y) or 16-bit values at p as they lie in memory; vec: p is aligned to eight of them.
+__device__ __forceinline__ uint4 raw_eight(const uint8_t* p, int x_type, bool vec) {
+    uint32_t v[4] = {};
     if (x_type == kTokE4M3) {
-        uint32_t v[2];
         if (vec) {
             const uint2 u = __ldg(reinterpret_cast<const uint2*>(p));
-            v[0] = u.x, v[1] = u.y;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                v[e] = __ldg(p + 4 * e) | __ldg(p + 4 * e + 1) << 8 | __ldg(p + 4 * e + 2) << 16 | __ldg(p + 4 * e + 3) << 24;
+            return make_uint4(u.x, u.y, 0, 0);
         }
-        uint32_t r[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(v[i / 2] >> (16 * (i % 2))), __NV_E4M3);
-            r[i] = reinterpret_cast<const uint32_t&>(h);
-        }
-        return make_uint4(r[0], r[1], r[2], r[3]);
+        for (int e = 0; e < 2; ++e)
+            v[e] = __ldg(p + 4 * e) | __ldg(p + 4 * e + 1) << 8 | __ldg(p + 4 * e + 2) << 16 | __ldg(p + 4 * e + 3) << 24;
+        return make_uint4(v[0], v[1], 0, 0);
     }
     if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
     const uint16_t* const q = reinterpret_cast<const uint16_t*>(p);
-    uint32_t v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = __ldg(q + 2 * e) | static_cast<uint32_t>(__ldg(q + 2 * e + 1)) << 16;
     return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// Them as 16-bit values: e4m3 widened to f16, others as they are.
+__device__ __forceinline__ uint4 widened(const uint4& v, int x_type) {
+    if (x_type != kTokE4M3) return v;
+    const uint32_t w[2] = {v.x, v.y};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i / 2] >> (16 * (i % 2))), __NV_E4M3);
+        r[i] = reinterpret_cast<const uint32_t&>(h);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 static inline cudaError_t take_status(uint32_t* code) {

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             for (int r = 0; r < rows; ++r) {
                 const uint8_t* const p = static_cast<const uint8_t*>(a.x) + (r * a.x_stride + seg * kBlockK) * kxb;
                 for (int i = threadIdx.x; i < eights; i += warps * 32)
-                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = paired(in_order(p + i * 8 * kxb, a.x_type, plan.x_vec));
+                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = paired(widened(raw_eight(p + i * 8 * kxb, a.x_type, plan.x_vec), a.x_type));
             }
         }
         consumers_sync(warps);

@@ -1,8 +1,11 @@
 // w4_many.cu — linear layer with 4-bit weights and group scales, many rows: tcgen05.
 //
-// A tile is 128 or 256 outputs (the MMA's M) by up to 256 rows (its N). Codes come by TMA; eight warps turn
-// them into 16-bit weights in the MMA's swizzled layout, the rows come by TMA as they are (or, for e4m3 and
-// unaligned rows, through four loader warps); one thread issues the MMAs, which accumulate in TMEM in f32.
+// A tile is 256 outputs by up to 192 rows, or 128 by up to 256; outputs are the MMA's M, rows its N. Codes come by
+// TMA; sixteen warps turn them into 16-bit weights and put them into TMEM, from where the MMAs take their A operand:
+// shared memory, which an MMA of M = 128 already reads for its B operand at half its bandwidth, is spared a write and
+// a read of every weight. Two tiles of 128 outputs share each B operand, for the same reason and for the L2's. The
+// rows come by TMA as they are (or, for e4m3 and unaligned rows, through four loader warps); one thread issues the
+// MMAs, which accumulate in TMEM in f32.
 // A weight scale * (code - zero) is rounded once to the rows' 16-bit type (f16 for e4m3 rows): code - zero is
 // exact, and the scale enters as the sum of two 16-bit values, one product and one fused multiply-add. In f16
 // each output's weights are divided by the power of two below its largest scale, so that no scale's size
@@ -25,12 +28,13 @@ constexpr int kSmemMax = 226 * 1024;
 
 struct ManyPlan {
     int tile_n;           // rows of a tile: a multiple of 16, at most 256
-    int rings[3];         // stages of codes, weights, rows
-    int codes, weights, rows, row_factor;  // offsets in shared memory
+    int rings[3];         // stages of codes, weights, rows; at most kMaxRing
+    int codes, rows, row_factor;  // offsets in shared memory
     int bytes;
     int split;            // blocks of a cluster that share a tile, each with a range of k
     int stages_each;      // stages of codes of a block
     int tmem_cols;
+    int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
     bool x_tma, x_vec;
 };
 
@@ -38,6 +42,21 @@ struct ManyPlan {
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
     return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
            static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, f32 accumulate.
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Eight 32-bit columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -102,27 +121,26 @@ __device__ __forceinline__ uint32_t zero_terms(uint32_t zero) {
     return 0xd400e400u + 0x00100001u * zero;  // -(64 + zero), -(1024 + zero)
 }
 
-// 32 codes (16 bytes) under one scale as four 16-byte cells of weights.
+// 16 codes (two words) under one scale as eight pairs of weights.
 template <bool BF>
-__device__ __forceinline__ void weights32(const uint4& codes, uint32_t hi, uint32_t lo, uint32_t z, uint4 (&out)[4]) {
-    const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+__device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi, uint32_t lo, uint32_t z, uint32_t (&out)[8]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const uint32_t w4 = BF ? w[c] >> 4 : 0;
-        uint32_t r[4];
+    for (int c = 0; c < 2; ++c) {
+        const uint32_t w = c ? w1 : w0, w4 = BF ? w >> 4 : 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t v = code_pair_in_order<BF>(w[c], w4, i, z);
-            r[i] = fma2<BF>(v, hi, mul2<BF>(v, lo));
+            const uint32_t v = code_pair_in_order<BF>(w, w4, i, z);
+            out[4 * c + i] = fma2<BF>(v, hi, mul2<BF>(v, lo));
         }
-        out[c] = make_uint4(r[0], r[1], r[2], r[3]);
     }
 }
 
-// TWO: 256 outputs a tile in two accumulators, else 128. Warps: 0 TMA, 1 MMA and TMEM, 2 and 3 idle, 4..11 weights
-// and epilogue, 12..15 (only without x_tma) rows.
+// Warps: 0..15 weights and epilogue, 16 TMA, 17 MMA and TMEM, 18..21 (only without x_tma) rows.
+// TWO: 256 outputs a tile in two accumulators, else 128.
+constexpr int kMakers = 16;
+
 template <bool BF, bool TWO>
-__global__ void __launch_bounds__(512, 1)
+__global__ void __launch_bounds__(704, 1)
     w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
                    const __grid_constant__ CUtensorMap rows_map) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -142,7 +160,7 @@ __global__ void __launch_bounds__(512, 1)
     const uint32_t bar = smem_u32(bars);
     const uint32_t c_full = bar, c_empty = bar + 8 * kMaxRing, w_full = bar + 16 * kMaxRing, w_empty = bar + 24 * kMaxRing,
                    x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, done = bar + 48 * kMaxRing;
-    const uint32_t codes = smem_u32(smem + plan.codes), weights = smem_u32(smem + plan.weights), xrows = smem_u32(smem + plan.rows);
+    const uint32_t codes = smem_u32(smem + plan.codes), xrows = smem_u32(smem + plan.rows);
     auto gave_up = [&](uint32_t code) {
         abort_flag = 1;
         set_w4_status(code);
@@ -151,8 +169,8 @@ __global__ void __launch_bounds__(512, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxRing; ++i) {
             mbar_init(c_full + 8 * i, 1);
-            mbar_init(c_empty + 8 * i, 8);
-            mbar_init(w_full + 8 * i, 8);
+            mbar_init(c_empty + 8 * i, kMakers);
+            mbar_init(w_full + 8 * i, kMakers);
             mbar_init(w_empty + 8 * i, 1);
             mbar_init(x_full + 8 * i, plan.x_tma ? 1 : 4);
             mbar_init(x_empty + 8 * i, 1);
@@ -161,16 +179,16 @@ __global__ void __launch_bounds__(512, 1)
         abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 1) {
+    if (warp == 17) {
         tmem_alloc(smem_u32(&tmem_at), plan.tmem_cols);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_at;
+    const uint32_t tmem = tmem_at, weights = tmem + plan.weight_col;
 
-    if (warp == 0) {
+    if (warp == 16) {
         if (lane == 0) {
             int cs = 0, xs = 0, step = 0;
             uint32_t cp = 0, xp = 0;
@@ -196,7 +214,7 @@ __global__ void __launch_bounds__(512, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 1) {
+    } else if (warp == 17) {
         const uint32_t idesc = instr_desc(128, 0, BF ? kOpBF16 : kOpF16) | static_cast<uint32_t>(tile_n >> 3) << 17;
         int ws = 0, xs = 0;
         uint32_t wp = 0, xp = 0;
@@ -208,10 +226,10 @@ __global__ void __launch_bounds__(512, 1)
                 const uint64_t bd = desc_sw128(xrows + xs * tile_n * 128);
 #pragma unroll
                 for (int m = 0; m < (TWO ? 2 : 1); ++m) {
-                    const uint64_t ad = desc_sw128(weights + ws * kTileM * 128 + m * 128 * 128);
+                    const uint32_t ad = weights + (ws * (TWO ? 2 : 1) + m) * 32;
 #pragma unroll
                     for (int i = 0; i < kStepK / 16; ++i)
-                        mma_f16(tmem + m * tile_n, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
+                        mma_f16_ta(tmem + m * tile_n, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0);
                 }
                 mma_commit(w_empty + 8 * ws);
                 mma_commit(x_empty + 8 * xs);
@@ -221,29 +239,40 @@ __global__ void __launch_bounds__(512, 1)
             if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
             if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
         }
-    } else if (warp >= 12) {  // rows that TMA does not bring: 16-byte cells of eight values, as the swizzle places them
-        const int tid = threadIdx.x - 384, cells = rows * 8, kxb = a.x_type == kTokE4M3 ? 1 : 2;
+    } else if (warp >= 18) {
+        // rows that TMA does not bring: 16-byte cells of eight values, as the swizzle places them; a step's cells are
+        // on their way while the step before them is stored
+        constexpr int kCells = 8;
+        const int tid = threadIdx.x - 18 * 32, kxb = a.x_type == kTokE4M3 ? 1 : 2, batches = (tile_n * 8 + 128 * kCells - 1) / (128 * kCells);
         int xs = 0;
         uint32_t xp = 0;
-        // a step's cells, eight at a time in flight
-        for (int step = 0; step < steps; ++step) {
+        uint4 v[kCells];
+        auto load = [&](int step, int batch) {
             const int k0 = k_begin + step * kStepK;
             const uint8_t* const src = static_cast<const uint8_t*>(a.x) + (r0 * a.x_stride + k0) * kxb;
-            bool waited = false;
-            for (int c0 = 0; c0 < tile_n * 8; c0 += 8 * 128) {
-                uint4 v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int cell = c0 + i * 128 + tid, r = cell / 8, c = cell % 8;
-                    v[i] = make_uint4(0, 0, 0, 0);
-                    if (cell < cells && k0 + c * 8 < k_end) v[i] = in_order(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
-                }
-                if (!waited && !wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
-                waited = true;
+            for (int i = 0; i < kCells; ++i) {
+                const int cell = (batch * kCells + i) * 128 + tid, r = cell / 8, c = cell % 8;
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (step < steps && r < rows && k0 + c * 8 < k_end) v[i] = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
+            }
+        };
+        load(0, 0);
+        for (int step = 0; step < steps; ++step) {
+            if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+            for (int batch = 0; batch < batches; ++batch) {
+                uint4 w[kCells];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int cell = c0 + i * 128 + tid, r = cell / 8, c = cell % 8;
-                    if (cell < tile_n * 8) *reinterpret_cast<uint4*>(smem + plan.rows + xs * tile_n * 128 + r * 128 + ((c ^ (r & 7)) << 4)) = v[i];
+                for (int i = 0; i < kCells; ++i) w[i] = v[i];
+                if (batch + 1 < batches)
+                    load(step, batch + 1);
+                else
+                    load(step + 1, 0);
+#pragma unroll
+                for (int i = 0; i < kCells; ++i) {
+                    const int cell = (batch * kCells + i) * 128 + tid, r = cell / 8, c = cell % 8;
+                    if (r < tile_n)
+                        *reinterpret_cast<uint4*>(smem + plan.rows + xs * tile_n * 128 + r * 128 + ((c ^ (r & 7)) << 4)) = widened(w[i], a.x_type);
                 }
             }
             fence_async_shared();
@@ -251,18 +280,19 @@ __global__ void __launch_bounds__(512, 1)
             if (lane == 0) mbar_arrive(x_full + 8 * xs);
             if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
         }
-    } else if (warp >= 4) {
-        // thread: one output of two tiles, or half of each step's inputs of an output of one
-        const int tid = threadIdx.x - 128, row = TWO ? tid : tid % 128, half = TWO ? 0 : tid / 128;
-        const int o = min(o0 + row, n - 1);
-        const int64_t at = static_cast<int64_t>(o) * groups;
+    } else {
+        // a thread makes weights of one output, whose TMEM lane is its own: half of each step's inputs of an output of two
+        // tiles, or a quarter of an output of one
+        const int quad = warp % 4, part = warp / 4, row = (TWO ? part / 2 * 128 : 0) + quad * 32 + lane;
+        const int first = TWO ? part % 2 * 32 : part * 16;  // of the step's inputs
+        const int64_t at = static_cast<int64_t>(min(o0 + row, n - 1)) * groups;
         const bool wide = a.w.scale_type == kTokF32;
         auto scale_at = [&](int g) { return tok_load(a.w.scales, at + g, a.w.scale_type); };
-        float back = 1.f, factor = 1.f;  // the output's power of two, and its reciprocal
+        float factor = 1.f;  // reciprocal of the output's power of two
+        float* const factors = reinterpret_cast<float*>(smem + plan.row_factor);
         if (!BF) {
             float top = 0.f;
-            const int sb = wide ? 4 : 2;
-            const uint8_t* const p = static_cast<const uint8_t*>(a.w.scales) + at * sb;
+            const uint8_t* const p = static_cast<const uint8_t*>(a.w.scales) + at * (wide ? 4 : 2);
             int g = 0;
             if (!wide && groups % 8 == 0 && reinterpret_cast<uintptr_t>(a.w.scales) % 16 == 0) {
 #pragma unroll 4
@@ -279,21 +309,24 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll 8
             for (; g < groups; ++g) top = fmaxf(top, fabsf(scale_at(g)));
             // 2^e <= top < 2^(e + 1), e kept where 2^e and 2^-e are normal; an infinity or zero keeps 1
+            float back = 1.f;
             if (top > 0.f && top < INFINITY) {
                 const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
                 back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                 factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
             }
+            if (TWO ? part % 2 == 0 : part == 0) factors[row] = back;
+            asm volatile("bar.sync 1, %0;" ::"n"(kMakers * 32) : "memory");
         }
-        // scales and zero points of a stage's chunks of 32 inputs, a stage ahead
-        constexpr int kChunks = TWO ? 8 : 4;
-        float sc[kChunks];
-        uint32_t zo[kChunks];
+        // scales and zero points of a stage's steps, a stage ahead (a thread's inputs of a step lie in one chunk of 32)
+        constexpr int kSteps = kStageK / kStepK;
+        float sc[kSteps];
+        uint32_t zo[kSteps];
         const float inv_group = 1.f / static_cast<float>(group);
         auto load_scales = [&](int k0) {
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const int kc = k0 + (TWO ? c * 32 : c * 64 + half * 32);
+            for (int c = 0; c < kSteps; ++c) {
+                const int kc = k0 + c * kStepK + first / 32 * 32;
                 sc[c] = 0.f;
                 zo[c] = 8;
                 if (kc < k_end) {
@@ -305,12 +338,13 @@ __global__ void __launch_bounds__(512, 1)
             }
         };
         load_scales(k_begin);
+        const uint32_t to = weights + (TWO ? part / 2 * 32 : 0) + first / 2 + (static_cast<uint32_t>(quad * 32) << 16);
         int cs = 0, ws = 0, step = 0;
         uint32_t cp = 0, wp = 0;
         for (int st = 0; st < stages; ++st) {
-            uint32_t hi[kChunks], lo[kChunks], z[kChunks];
+            uint32_t hi[kSteps], lo[kSteps], z[kSteps];
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
+            for (int c = 0; c < kSteps; ++c) {
                 const float s = sc[c] * factor, h = round16f<BF>(s), l = s - h;
                 hi[c] = pair16<BF>(h, h);
                 lo[c] = l == l ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
@@ -320,26 +354,23 @@ __global__ void __launch_bounds__(512, 1)
             if (!wait_phase(c_full + 8 * cs, cp, &abort_flag)) gave_up(kStatusTimeoutFull);
             const uint32_t from = codes + cs * kTileM * 128 + row * 128;
 #pragma unroll
-            for (int b = 0; b < kStageK / kStepK; ++b) {
+            for (int b = 0; b < kSteps; ++b) {
                 if (step >= steps) break;
                 ++step;
+                uint32_t w[TWO ? 4 : 2], out[TWO ? 2 : 1][8];
+                const uint32_t cell = from + (((2 * b + first / 32) ^ (row & 7)) << 4);
+                if constexpr (TWO)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(cell));
+                else
+                    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(cell + first % 32 / 2));
+#pragma unroll
+                for (int h = 0; h < (TWO ? 2 : 1); ++h) weights16<BF>(w[2 * h], w[2 * h + 1], hi[b], lo[b], z[b], out[h]);
                 if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
-                const uint32_t to = weights + ws * kTileM * 128 + row * 128;
+                tc_fence_after();
 #pragma unroll
-                for (int h = 0; h < (TWO ? 2 : 1); ++h) {
-                    const int part = TWO ? h : half, chunk = TWO ? 2 * b + h : b;
-                    uint4 v, out[4];
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                 : "r"(from + (((2 * b + part) ^ (row & 7)) << 4)));
-                    weights32<BF>(v, hi[chunk], lo[chunk], z[chunk], out);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((4 * part + c) ^ (row & 7)) << 4)), "r"(out[c].x),
-                                     "r"(out[c].y), "r"(out[c].z), "r"(out[c].w)
-                                     : "memory");
-                }
-                fence_async_shared();
+                for (int h = 0; h < (TWO ? 2 : 1); ++h) tmem_st8(to + ws * (TWO ? 64 : 32) + 8 * h, out[h]);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_full + 8 * ws);
                 if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
@@ -348,37 +379,27 @@ __global__ void __launch_bounds__(512, 1)
             if (lane == 0) mbar_arrive(c_empty + 8 * cs);
             if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
         }
-        // epilogue: warp w reads TMEM lanes 32 (w % 4)..; two tiles: one tile each, one tile: half the columns each
+        // epilogue: a warp reads its TMEM lanes; the warps of a tile's quarter share its columns, eight at a time
         if (steps && !wait_phase(done, 0, &abort_flag)) gave_up(kStatusTimeoutAcc);
         tc_fence_after();
-        const int quad = warp % 4, part = (warp - 4) / 4;
-        const int out = o0 + (TWO ? part * 128 : 0) + quad * 32 + lane;
-        const int out_row = (TWO ? part * 128 : 0) + quad * 32 + lane;
-        // the power of two belongs to the output this thread made weights of, not the one it stores
-        float* const factors = reinterpret_cast<float*>(smem + plan.row_factor);
-        if (!BF) {
-            if (TWO || half == 0) factors[row] = back;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            back = factors[out_row];
-        }
-        const float bias = a.bias && out < n ? a.bias[out] : 0.f;
-        const int col0 = TWO ? 0 : part * (tile_n / 2), cols = TWO ? tile_n : tile_n / 2;
-        const uint32_t acc = tmem + (TWO ? part * tile_n : 0) + (static_cast<uint32_t>(quad * 32) << 16);
+        const int out = o0 + row;
+        const float back = BF ? 1.f : factors[row], bias = a.bias && out < n ? a.bias[out] : 0.f;
+        const uint32_t acc = tmem + (TWO ? part / 2 * tile_n : 0) + (static_cast<uint32_t>(quad * 32) << 16);
         float* const partial = reinterpret_cast<float*>(smem);  // [row][output], over the rings
-        for (int c = 0; c < cols; c += 8) {
+        for (int c = (TWO ? part % 2 : part) * 8; c < tile_n; c += TWO ? 16 : 32) {
             uint32_t v[8];
             asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                          : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                         : "r"(acc + col0 + c));
+                         : "r"(acc + c));
             tmem_wait();
 #pragma unroll
             for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i])::"memory");
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int r = col0 + c + i;
+                const int r = c + i;
                 float f = steps ? __uint_as_float(v[i]) * back : 0.f;
                 if (plan.split > 1) {
-                    partial[r * kTileM + out_row] = f;
+                    partial[r * kTileM + row] = f;
                 } else if (r < rows && out < n) {
                     if (a.x_scale) f *= a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
                     tok_store(a.y, (r0 + r) * a.y_stride + out, a.y_type, f + bias);
@@ -403,7 +424,7 @@ __global__ void __launch_bounds__(512, 1)
         cluster_sync();
     }
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 17) {
         tc_fence_after();
         tmem_dealloc(tmem, plan.tmem_cols);
     }
@@ -425,7 +446,7 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((a.w.n + kTileM - 1) / kTileM * p.split, (a.rows + p.tile_n - 1) / p.tile_n);
-    cfg.blockDim = dim3(p.x_tma ? 384 : 512);
+    cfg.blockDim = dim3(p.x_tma ? 18 * 32 : 22 * 32);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -446,29 +467,29 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
     p.x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
     p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
-    p.tile_n = a.rows >= 256 ? 256 : (a.rows + 15) / 16 * 16;
+    const bool two = (a.w.n + 255) / 256 * ((a.rows + 191) / 192) >= sms;
+    const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
+    p.tile_n = a.rows >= most_n ? most_n : (a.rows + 15) / 16 * 16;
     const int64_t tiles_n = (a.rows + p.tile_n - 1) / p.tile_n;
-    const bool two = (a.w.n + 255) / 256 * tiles_n >= sms;
-    const int tile_m = two ? 256 : 128;
     const int64_t tiles = (a.w.n + tile_m - 1) / tile_m * tiles_n;
     const int all_stages = (a.w.k + kStageK - 1) / kStageK;
     // few tiles: a cluster shares one, each block a range of k, while a block keeps two stages of codes
     p.split = 1;
     while (!two && p.split < 8 && tiles * p.split * 2 <= sms && all_stages >= p.split * 4) p.split *= 2;
     p.stages_each = (all_stages + p.split - 1) / p.split;
-    p.tmem_cols = 32;
-    while (p.tmem_cols < p.tile_n * (two ? 2 : 1)) p.tmem_cols *= 2;
-    const int factor_bytes = 1024;
-    // rings: half of the room left by two stages of weights for codes and weights in turn, at least two of each
-    int room = kSmemMax - factor_bytes;
-    const int w = tile_m * 128, x = p.tile_n * 128;
-    p.rings[0] = p.rings[1] = p.rings[2] = 2;
-    room -= 4 * w + 2 * x;
+    // TMEM, all of it (a block's shared memory leaves room for no other block): accumulators, then stages of weights
+    p.weight_col = (two ? 2 : 1) * p.tile_n;
+    p.tmem_cols = 512;
+    p.rings[1] = std::min((p.tmem_cols - p.weight_col) / (two ? 64 : 32), kMaxRing);
+    // shared memory: codes and rows in turn
+    const int factor_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128;
+    int room = kSmemMax - factor_bytes - 2 * w - 2 * x;
+    p.rings[0] = p.rings[2] = 2;
     for (bool more = true; more;) {
         more = false;
-        for (int i : {2, 0, 1}) {
+        for (int i : {2, 0}) {
             const int cost = i == 2 ? x : w;
-            if (p.rings[i] < (i == 1 ? 4 : 6) && room >= cost) {
+            if (p.rings[i] < kMaxRing && room >= cost) {
                 ++p.rings[i];
                 room -= cost;
                 more = true;
@@ -476,8 +497,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
         }
     }
     p.codes = 0;
-    p.weights = p.rings[0] * w;
-    p.rows = p.weights + p.rings[1] * w;
+    p.rows = p.rings[0] * w;
     p.row_factor = p.rows + p.rings[2] * x;
     p.bytes = p.row_factor + factor_bytes;
     if (p.split > 1) {  // the partial sums lie over the rings
