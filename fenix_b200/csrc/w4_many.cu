@@ -35,7 +35,7 @@ struct ManyPlan {
     int stages_each;      // stages of codes of a block
     int tmem_cols;
     int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
-    bool x_tma, x_vec;
+    bool x_tma, x_vec, x_vec16;  // rows by TMA; else aligned to eight values, to 16 e4m3 values
 };
 
 // K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 bytes apart.
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(704, 1)
         for (int i = 0; i < kMaxRing; ++i) {
             mbar_init(c_full + 8 * i, 1);
             mbar_init(c_empty + 8 * i, kMakers);
-            mbar_init(w_full + 8 * i, kMakers);
+            mbar_init(w_full + 8 * i, TWO ? 8 : 4);
             mbar_init(w_empty + 8 * i, 1);
             mbar_init(x_full + 8 * i, plan.x_tma ? 1 : 4);
             mbar_init(x_empty + 8 * i, 1);
@@ -257,8 +257,43 @@ __global__ void __launch_bounds__(704, 1)
                 if (step < steps && r < rows && k0 + c * 8 < k_end) v[i] = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
             }
         };
-        load(0, 0);
-        for (int step = 0; step < steps; ++step) {
+        // e4m3 rows of 16-byte alignment, two cells at a time: all of a step at once
+        auto load16 = [&](int step) {
+            const int k0 = k_begin + step * kStepK;
+            const uint8_t* const src = static_cast<const uint8_t*>(a.x) + r0 * a.x_stride + k0;
+#pragma unroll
+            for (int i = 0; i < kCells; ++i) {
+                const int r = (i * 128 + tid) / 4, c = tid % 4;
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (step < steps && r < rows && k0 + c * 16 < k_end)
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r) * a.x_stride + c * 16));
+            }
+        };
+        if (plan.x_vec16) {
+            load16(0);
+            for (int step = 0; step < steps; ++step) {
+                uint4 w[kCells];
+#pragma unroll
+                for (int i = 0; i < kCells; ++i) w[i] = v[i];
+                load16(step + 1);
+                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+#pragma unroll
+                for (int i = 0; i < kCells; ++i) {
+                    const int r = (i * 128 + tid) / 4, c = tid % 4 * 2;
+                    if (r < tile_n) {
+                        uint8_t* const to = smem + plan.rows + xs * tile_n * 128 + r * 128;
+                        *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = widened(w[i], kTokE4M3);
+                        *reinterpret_cast<uint4*>(to + (((c + 1) ^ (r & 7)) << 4)) = widened(make_uint4(w[i].z, w[i].w, 0, 0), kTokE4M3);
+                    }
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(x_full + 8 * xs);
+                if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+            }
+        }
+        if (!plan.x_vec16) load(0, 0);
+        for (int step = 0; step < steps && !plan.x_vec16; ++step) {
             if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
             for (int batch = 0; batch < batches; ++batch) {
                 uint4 w[kCells];
@@ -281,10 +316,10 @@ __global__ void __launch_bounds__(704, 1)
             if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
         }
     } else {
-        // a thread makes weights of one output, whose TMEM lane is its own: half of each step's inputs of an output of two
-        // tiles, or a quarter of an output of one
-        const int quad = warp % 4, part = warp / 4, row = (TWO ? part / 2 * 128 : 0) + quad * 32 + lane;
-        const int first = TWO ? part % 2 * 32 : part * 16;  // of the step's inputs
+        // a thread makes weights of one output, whose TMEM lane is its own; the four warps of a lane quarter take the steps
+        // in turn (with two tiles, two warps a tile), so that a step's latency is hidden behind the others'
+        constexpr int kSets = TWO ? 2 : 4;
+        const int quad = warp % 4, part = warp / 4, set = part % kSets, row = (TWO ? part / 2 * 128 : 0) + quad * 32 + lane;
         const int64_t at = static_cast<int64_t>(min(o0 + row, n - 1)) * groups;
         const bool wide = a.w.scale_type == kTokF32;
         auto scale_at = [&](int g) { return tok_load(a.w.scales, at + g, a.w.scale_type); };
@@ -315,65 +350,72 @@ __global__ void __launch_bounds__(704, 1)
                 back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                 factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
             }
-            if (TWO ? part % 2 == 0 : part == 0) factors[row] = back;
+            if (set == 0) factors[row] = back;
             asm volatile("bar.sync 1, %0;" ::"n"(kMakers * 32) : "memory");
         }
-        // scales and zero points of a stage's steps, a stage ahead (a thread's inputs of a step lie in one chunk of 32)
-        constexpr int kSteps = kStageK / kStepK;
-        float sc[kSteps];
-        uint32_t zo[kSteps];
+        // scales and zero points of a stage's chunks of 32 inputs, two a step, a stage ahead
+        constexpr int kMine = kStageK / kStepK / kSets;
+        float sc[kMine][2];
+        uint32_t zo[kMine][2];
         const float inv_group = 1.f / static_cast<float>(group);
         auto load_scales = [&](int k0) {
 #pragma unroll
-            for (int c = 0; c < kSteps; ++c) {
-                const int kc = k0 + c * kStepK + first / 32 * 32;
-                sc[c] = 0.f;
-                zo[c] = 8;
-                if (kc < k_end) {
-                    // (kc + 1/2) / group truncated: exact while k < 2^21
-                    const int g = k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group;
-                    sc[c] = scale_at(g);
-                    if (a.w.zeros) zo[c] = __ldg(a.w.zeros + at + g);
+            for (int c = 0; c < kMine; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int kc = k0 + (c * kSets + set) * kStepK + h * 32;
+                    sc[c][h] = 0.f;
+                    zo[c][h] = 8;
+                    if (kc < k_end) {
+                        // (kc + 1/2) / group truncated: exact while k < 2^21
+                        const int g = k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group;
+                        sc[c][h] = scale_at(g);
+                        if (a.w.zeros) zo[c][h] = __ldg(a.w.zeros + at + g);
+                    }
                 }
-            }
         };
         load_scales(k_begin);
-        const uint32_t to = weights + (TWO ? part / 2 * 32 : 0) + first / 2 + (static_cast<uint32_t>(quad * 32) << 16);
-        int cs = 0, ws = 0, step = 0;
+        const uint32_t to = weights + (TWO ? part / 2 * 32 : 0) + (static_cast<uint32_t>(quad * 32) << 16);
+        int cs = 0, ws = set, step = set;
         uint32_t cp = 0, wp = 0;
         for (int st = 0; st < stages; ++st) {
-            uint32_t hi[kSteps], lo[kSteps], z[kSteps];
+            uint32_t hi[kMine][2], lo[kMine][2], z[kMine][2];
 #pragma unroll
-            for (int c = 0; c < kSteps; ++c) {
-                const float s = sc[c] * factor, h = round16f<BF>(s), l = s - h;
-                hi[c] = pair16<BF>(h, h);
-                lo[c] = l == l ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
-                z[c] = zero_terms<BF>(zo[c]);
-            }
+            for (int c = 0; c < kMine; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float s = sc[c][h] * factor, r = round16f<BF>(s), l = s - r;
+                    hi[c][h] = pair16<BF>(r, r);
+                    lo[c][h] = l == l ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
+                    z[c][h] = zero_terms<BF>(zo[c][h]);
+                }
             if (st + 1 < stages) load_scales(k_begin + (st + 1) * kStageK);
             if (!wait_phase(c_full + 8 * cs, cp, &abort_flag)) gave_up(kStatusTimeoutFull);
             const uint32_t from = codes + cs * kTileM * 128 + row * 128;
 #pragma unroll
-            for (int b = 0; b < kSteps; ++b) {
+            for (int c = 0; c < kMine; ++c) {
                 if (step >= steps) break;
-                ++step;
-                uint32_t w[TWO ? 4 : 2], out[TWO ? 2 : 1][8];
-                const uint32_t cell = from + (((2 * b + first / 32) ^ (row & 7)) << 4);
-                if constexpr (TWO)
-                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(cell));
-                else
-                    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(cell + first % 32 / 2));
+                step += kSets;
+                while (ws >= plan.rings[1]) ws -= plan.rings[1], wp ^= 1;
+                uint32_t w[2][4];
 #pragma unroll
-                for (int h = 0; h < (TWO ? 2 : 1); ++h) weights16<BF>(w[2 * h], w[2 * h + 1], hi[b], lo[b], z[b], out[h]);
+                for (int h = 0; h < 2; ++h)
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(w[h][0]), "=r"(w[h][1]), "=r"(w[h][2]), "=r"(w[h][3])
+                                 : "r"(from + (((2 * (c * kSets + set) + h) ^ (row & 7)) << 4)));
+                uint32_t out[4][8];
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    weights16<BF>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2], lo[c][h / 2], z[c][h / 2], out[h]);
                 if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
                 tc_fence_after();
 #pragma unroll
-                for (int h = 0; h < (TWO ? 2 : 1); ++h) tmem_st8(to + ws * (TWO ? 64 : 32) + 8 * h, out[h]);
+                for (int h = 0; h < 4; ++h) tmem_st8(to + ws * (TWO ? 64 : 32) + 8 * h, out[h]);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_full + 8 * ws);
-                if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
+                ws += kSets;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(c_empty + 8 * cs);
@@ -467,6 +509,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
     p.x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
     p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
+    p.x_vec16 = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0;
     const bool two = (a.w.n + 255) / 256 * ((a.rows + 191) / 192) >= sms;
     const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
     p.tile_n = a.rows >= most_n ? most_n : (a.rows + 15) / 16 * 16;
