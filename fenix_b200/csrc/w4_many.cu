@@ -35,6 +35,7 @@ struct ManyPlan {
     int stages_each;      // stages of codes of a block
     int tmem_cols;
     int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
+    bool y_vec;           // results aligned to eight outputs
     bool x_tma, x_vec, x_vec16;  // rows by TMA; else aligned to eight values, to 16 e4m3 values
 };
 
@@ -77,10 +78,6 @@ __device__ __forceinline__ uint32_t pair16(float a, float b) {
     }
     __half2 h = __floats2half2_rn(a, b);
     return reinterpret_cast<uint32_t&>(h);
-}
-template <bool BF>
-__device__ __forceinline__ float round16f(float v) {
-    return BF ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
@@ -139,7 +136,8 @@ __device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi,
 // TWO: 256 outputs a tile in two accumulators, else 128.
 constexpr int kMakers = 16;
 
-template <bool BF, bool TWO>
+// CH: scales of a step of 64 inputs (1: groups are multiples of 64). Z: with zero points.
+template <bool BF, bool TWO, int CH, bool Z>
 __global__ void __launch_bounds__(704, 1)
     w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
                    const __grid_constant__ CUtensorMap rows_map) {
@@ -321,7 +319,7 @@ __global__ void __launch_bounds__(704, 1)
         constexpr int kSets = TWO ? 2 : 4;
         const int quad = warp % 4, part = warp / 4, set = part % kSets, row = (TWO ? part / 2 * 128 : 0) + quad * 32 + lane;
         const int64_t at = static_cast<int64_t>(min(o0 + row, n - 1)) * groups;
-        const bool wide = a.w.scale_type == kTokF32;
+        const bool wide = a.w.scale_type == kTokF32, is_f16 = a.w.scale_type == kTokF16;
         auto scale_at = [&](int g) { return tok_load(a.w.scales, at + g, a.w.scale_type); };
         float factor = 1.f;  // reciprocal of the output's power of two
         float* const factors = reinterpret_cast<float*>(smem + plan.row_factor);
@@ -353,24 +351,28 @@ __global__ void __launch_bounds__(704, 1)
             if (set == 0) factors[row] = back;
             asm volatile("bar.sync 1, %0;" ::"n"(kMakers * 32) : "memory");
         }
-        // scales and zero points of a stage's chunks of 32 inputs, two a step, a stage ahead
+        // scales, as they are stored, and zero points of a stage's steps, a stage ahead
         constexpr int kMine = kStageK / kStepK / kSets;
-        float sc[kMine][2];
-        uint32_t zo[kMine][2];
+        uint32_t sc[kMine][CH], zo[kMine][CH];
         const float inv_group = 1.f / static_cast<float>(group);
+        const uint8_t* const s_at = static_cast<const uint8_t*>(a.w.scales) + at * (wide ? 4 : 2);
+        const uint8_t* const z_at = Z ? a.w.zeros + at : nullptr;
         auto load_scales = [&](int k0) {
 #pragma unroll
             for (int c = 0; c < kMine; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < CH; ++h) {
                     const int kc = k0 + (c * kSets + set) * kStepK + h * 32;
-                    sc[c][h] = 0.f;
+                    sc[c][h] = 0;  // past the end weights are zeros
                     zo[c][h] = 8;
                     if (kc < k_end) {
                         // (kc + 1/2) / group truncated: exact while k < 2^21
                         const int g = k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group;
-                        sc[c][h] = scale_at(g);
-                        if (a.w.zeros) zo[c][h] = __ldg(a.w.zeros + at + g);
+                        if (wide)
+                            sc[c][h] = __ldg(reinterpret_cast<const uint32_t*>(s_at) + g);
+                        else
+                            sc[c][h] = __ldg(reinterpret_cast<const uint16_t*>(s_at) + g);
+                        if (Z) zo[c][h] = __ldg(z_at + g);
                     }
                 }
         };
@@ -379,14 +381,17 @@ __global__ void __launch_bounds__(704, 1)
         int cs = 0, ws = set, step = set;
         uint32_t cp = 0, wp = 0;
         for (int st = 0; st < stages; ++st) {
-            uint32_t hi[kMine][2], lo[kMine][2], z[kMine][2];
+            uint32_t hi[kMine][CH], lo[kMine][CH], z[kMine][CH];
 #pragma unroll
             for (int c = 0; c < kMine; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float s = sc[c][h] * factor, r = round16f<BF>(s), l = s - r;
-                    hi[c][h] = pair16<BF>(r, r);
-                    lo[c][h] = l == l ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
+                for (int h = 0; h < CH; ++h) {
+                    const uint32_t raw = sc[c][h];
+                    float v = wide ? __uint_as_float(raw) : is_f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(raw))) : __uint_as_float(raw << 16);
+                    if (!BF) v *= factor;
+                    hi[c][h] = pair16<BF>(v, v);
+                    const float l = v - (BF ? __uint_as_float(hi[c][h] << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(hi[c][h]))));
+                    lo[c][h] = fabsf(l) < INFINITY ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
                     z[c][h] = zero_terms<BF>(zo[c][h]);
                 }
             if (st + 1 < stages) load_scales(k_begin + (st + 1) * kStageK);
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(704, 1)
                 uint32_t out[4][8];
 #pragma unroll
                 for (int h = 0; h < 4; ++h)
-                    weights16<BF>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2], lo[c][h / 2], z[c][h / 2], out[h]);
+                    weights16<BF>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH], z[c][h / 2 % CH], out[h]);
                 if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
                 tc_fence_after();
 #pragma unroll
@@ -428,24 +433,51 @@ __global__ void __launch_bounds__(704, 1)
         const float back = BF ? 1.f : factors[row], bias = a.bias && out < n ? a.bias[out] : 0.f;
         const uint32_t acc = tmem + (TWO ? part / 2 * tile_n : 0) + (static_cast<uint32_t>(quad * 32) << 16);
         float* const partial = reinterpret_cast<float*>(smem);  // [row][output], over the rings
-        for (int c = (TWO ? part % 2 : part) * 8; c < tile_n; c += TWO ? 16 : 32) {
-            uint32_t v[8];
-            asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                         : "r"(acc + c));
+        // sixteen rows at a time; 16-bit results change places in shared memory (over the rings), so that a store is eight
+        // outputs of a row
+        uint8_t* const turned = smem + warp * (16 * 80);
+        const int o_warp = o0 + row - lane;
+        const bool vec = plan.y_vec && o_warp + 32 <= n;
+        for (int c = (TWO ? part % 2 : part) * 16; c < tile_n; c += TWO ? 32 : 64) {
+            uint32_t v[16];
+            tmem_ld16_nowait(acc + c, v);
             tmem_wait();
+            tmem_regs_ready(v);
+            float f[16];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) asm volatile("" : "+r"(v[i])::"memory");
+            for (int i = 0; i < 16; ++i) f[i] = steps ? __uint_as_float(v[i]) * back : 0.f;
+            if (plan.split > 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = c + i;
-                float f = steps ? __uint_as_float(v[i]) * back : 0.f;
-                if (plan.split > 1) {
-                    partial[r * kTileM + row] = f;
-                } else if (r < rows && out < n) {
-                    if (a.x_scale) f *= a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
-                    tok_store(a.y, (r0 + r) * a.y_stride + out, a.y_type, f + bias);
+                for (int i = 0; i < 16; ++i) partial[(c + i) * kTileM + row] = f[i];
+                continue;
+            }
+            if (a.x_scale) {
+                const int r = c + lane % 16;
+                const float xs = r < rows ? a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) f[i] *= __shfl_sync(0xffffffffu, xs, i);
+            }
+            uint16_t* const y = static_cast<uint16_t*>(a.y) + (r0 + c) * a.y_stride;
+            if (vec) {
+                if (a.y_type == kTokF16) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) *reinterpret_cast<__half*>(turned + i * 80 + lane * 2) = __float2half_rn(f[i] + bias);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) *reinterpret_cast<__nv_bfloat16*>(turned + i * 80 + lane * 2) = __float2bfloat16_rn(f[i] + bias);
                 }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = i * 8 + lane / 4;
+                    const uint4 w = *reinterpret_cast<const uint4*>(turned + r * 80 + lane % 4 * 16);
+                    if (c + r < rows) *reinterpret_cast<uint4*>(y + r * a.y_stride + o_warp + lane % 4 * 8) = w;
+                }
+                __syncwarp();
+            } else if (out < n) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (c + i < rows) tok_store(y, i * a.y_stride + out, a.y_type, f[i] + bias);
             }
         }
         tc_fence_before();
@@ -472,10 +504,10 @@ __global__ void __launch_bounds__(704, 1)
     }
 }
 
-template <bool BF, bool TWO>
+template <bool BF, bool TWO, int CH, bool Z>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     constexpr int kTileM = TWO ? 256 : 128;
-    auto* kern = w4_many_kernel<BF, TWO>;
+    auto* kern = w4_many_kernel<BF, TWO, CH, Z>;
     CUtensorMap codes, rows;
     cudaError_t e = tmap_rows(&codes, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kTileM);
     if (e == cudaSuccess) {
@@ -502,6 +534,12 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
+template <bool BF, bool TWO>
+cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
+    if (a.w.group % kStepK == 0) return a.w.zeros ? launch<BF, TWO, 1, true>(a, p, s) : launch<BF, TWO, 1, false>(a, p, s);
+    return a.w.zeros ? launch<BF, TWO, 2, true>(a, p, s) : launch<BF, TWO, 2, false>(a, p, s);
+}
+
 }  // namespace
 
 cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
@@ -509,6 +547,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
     p.x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
     p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
+    p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride % 8 == 0;
     p.x_vec16 = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0;
     const bool two = (a.w.n + 255) / 256 * ((a.rows + 191) / 192) >= sms;
     const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
