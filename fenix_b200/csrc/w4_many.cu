@@ -29,14 +29,15 @@ constexpr int kSmemMax = 226 * 1024;
 struct ManyPlan {
     int tile_n;           // rows of a tile: a multiple of 16, at most 256
     int rings[3];         // stages of codes, weights, rows; at most kMaxRing
-    int codes, rows, row_factor;  // offsets in shared memory
+    int codes, rows, raw, row_factor;  // offsets in shared memory
     int bytes;
     int split;            // blocks of a cluster that share a tile, each with a range of k
     int stages_each;      // stages of codes of a block
     int tmem_cols;
     int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
+    int raw_slots;        // of e4m3 rows by TMA, 128 inputs each
     bool y_vec;           // results aligned to eight outputs
-    bool x_tma, x_vec, x_vec16;  // rows by TMA; else aligned to eight values, to 16 e4m3 values
+    bool x_tma, x_vec;    // rows by TMA as they are; rows aligned to eight values
 };
 
 // K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 bytes apart.
@@ -64,9 +65,12 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}" : "=f"(v) : "r"(addr), "r"(rank));
+// Four f32 of a block of the cluster, at a shared-memory address of this one.
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {
+    float4 v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\tld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [r];\n\t}"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr), "r"(rank));
     return v;
 }
 
@@ -119,7 +123,7 @@ __device__ __forceinline__ uint32_t zero_terms(uint32_t zero) {
 }
 
 // 16 codes (two words) under one scale as eight pairs of weights.
-template <bool BF>
+template <bool BF, bool EX>
 __device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi, uint32_t lo, uint32_t z, uint32_t (&out)[8]) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -127,22 +131,26 @@ __device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi,
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t v = code_pair_in_order<BF>(w, w4, i, z);
-            out[4 * c + i] = fma2<BF>(v, hi, mul2<BF>(v, lo));
+            out[4 * c + i] = EX ? mul2<BF>(v, hi) : fma2<BF>(v, hi, mul2<BF>(v, lo));
         }
     }
 }
 
-// Warps: 0..15 weights and epilogue, 16 TMA, 17 MMA and TMEM, 18..21 (only without x_tma) rows.
+// Warps: 0..15 weights and epilogue, 16 codes by TMA, 17 MMA and TMEM, 18 rows by TMA, or 18 and 19 rows
+// that have to be widened or loaded.
 // TWO: 256 outputs a tile in two accumulators, else 128.
 constexpr int kMakers = 16;
 
-// CH: scales of a step of 64 inputs (1: groups are multiples of 64). Z: with zero points.
-template <bool BF, bool TWO, int CH, bool Z>
-__global__ void __launch_bounds__(704, 1)
+// XS: steps of 64 inputs that share a slot of the rows' ring (a constant: the issuing thread has no time to spare).
+// CH: scales of a step of 64 inputs (1: groups are multiples of 64). EX: the scales' type is the
+// operands', so that they have no second term (in f16 but for those 2^14 below their output's largest, whose last bits
+// are 2^-25 of it).
+template <bool BF, bool TWO, int XS, int CH, bool EX>
+__global__ void __launch_bounds__(640, 1)
     w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
                    const __grid_constant__ CUtensorMap rows_map) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[6 * kMaxRing + 1];
+    __shared__ __align__(8) uint64_t bars[7 * kMaxRing + 1];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int abort_flag;
     constexpr int kTileM = TWO ? 256 : 128;
@@ -157,7 +165,7 @@ __global__ void __launch_bounds__(704, 1)
     const int steps = k_begin < k_end ? (k_end - k_begin + kStepK - 1) / kStepK : 0;
     const uint32_t bar = smem_u32(bars);
     const uint32_t c_full = bar, c_empty = bar + 8 * kMaxRing, w_full = bar + 16 * kMaxRing, w_empty = bar + 24 * kMaxRing,
-                   x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, done = bar + 48 * kMaxRing;
+                   x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, raw_full = bar + 48 * kMaxRing, done = bar + 56 * kMaxRing;
     const uint32_t codes = smem_u32(smem + plan.codes), xrows = smem_u32(smem + plan.rows);
     auto gave_up = [&](uint32_t code) {
         abort_flag = 1;
@@ -170,7 +178,8 @@ __global__ void __launch_bounds__(704, 1)
             mbar_init(c_empty + 8 * i, kMakers);
             mbar_init(w_full + 8 * i, TWO ? 8 : 4);
             mbar_init(w_empty + 8 * i, 1);
-            mbar_init(x_full + 8 * i, plan.x_tma ? 1 : 4);
+            mbar_init(x_full + 8 * i, plan.x_tma ? 1 : 2);
+            mbar_init(raw_full + 8 * i, 1);
             mbar_init(x_empty + 8 * i, 1);
         }
         mbar_init(done, 1);
@@ -188,40 +197,48 @@ __global__ void __launch_bounds__(704, 1)
 
     if (warp == 16) {
         if (lane == 0) {
-            int cs = 0, xs = 0, step = 0;
-            uint32_t cp = 0, xp = 0;
+            int cs = 0;
+            uint32_t cp = 0;
             for (int st = 0; st < stages; ++st) {
                 if (!wait_phase(c_empty + 8 * cs, cp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
                 if (abort_flag) break;
                 mbar_arrive_expect_tx(c_full + 8 * cs, kTileM * 128);
                 tma_load_2d(codes + cs * kTileM * 128, &codes_map, (k_begin + st * kStageK) / 16, o0, c_full + 8 * cs);
                 if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
-                if (plan.x_tma)
-                    for (int i = 0; i < kStageK / kStepK && step < steps; ++i, ++step) {
-                        if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
-                        if (abort_flag) break;
-                        mbar_arrive_expect_tx(x_full + 8 * xs, tile_n * 128);
-                        tma_load_2d(xrows + xs * tile_n * 128, &rows_map, k_begin + step * kStepK, static_cast<int>(r0), x_full + 8 * xs);
-                        if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
-                    }
             }
-            if (abort_flag) {  // copies still on their way; the waits end by themselves
+            if (abort_flag)  // copies still on their way; the waits end by themselves
                 for (int i = 0; i < plan.rings[0]; ++i) wait_phase(c_full + 8 * i, (i < cs ? cp : cp ^ 1), nullptr);
-                if (plan.x_tma)
-                    for (int i = 0; i < plan.rings[2]; ++i) wait_phase(x_full + 8 * i, (i < xs ? xp : xp ^ 1), nullptr);
+        }
+        __syncwarp();
+    } else if (warp == 18 && plan.x_tma) {  // not the codes' thread: neither ring's waits hold up the other
+        if (lane == 0) {
+            int xs = 0;
+            uint32_t xp = 0;
+            for (int step = 0; step < steps; step += XS) {
+                const int boxes = min(XS, steps - step);
+                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                if (abort_flag) break;
+                mbar_arrive_expect_tx(x_full + 8 * xs, boxes * tile_n * 128);
+                for (int i = 0; i < boxes; ++i)
+                    tma_load_2d(xrows + (xs * XS + i) * tile_n * 128, &rows_map, k_begin + (step + i) * kStepK, static_cast<int>(r0),
+                                x_full + 8 * xs);
+                if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
+            if (abort_flag)
+                for (int i = 0; i < plan.rings[2]; ++i) wait_phase(x_full + 8 * i, (i < xs ? xp : xp ^ 1), nullptr);
         }
         __syncwarp();
     } else if (warp == 17) {
         const uint32_t idesc = instr_desc(128, 0, BF ? kOpBF16 : kOpF16) | static_cast<uint32_t>(tile_n >> 3) << 17;
-        int ws = 0, xs = 0;
+        int ws = 0, xs = 0, x_step = 0;
         uint32_t wp = 0, xp = 0;
         for (int step = 0; step < steps; ++step) {
+            if (x_step == 0 && !wait_phase(x_full + 8 * xs, xp, &abort_flag)) gave_up(kStatusTimeoutFull);
             if (!wait_phase(w_full + 8 * ws, wp, &abort_flag)) gave_up(kStatusTimeoutFull);
-            if (!wait_phase(x_full + 8 * xs, xp, &abort_flag)) gave_up(kStatusTimeoutFull);
             tc_fence_after();
+            const bool x_last = x_step == XS - 1 || step == steps - 1;
             if (elect_one()) {
-                const uint64_t bd = desc_sw128(xrows + xs * tile_n * 128);
+                const uint64_t bd = desc_sw128(xrows + (xs * XS + x_step) * tile_n * 128);
 #pragma unroll
                 for (int m = 0; m < (TWO ? 2 : 1); ++m) {
                     const uint32_t ad = weights + (ws * (TWO ? 2 : 1) + m) * 32;
@@ -230,88 +247,73 @@ __global__ void __launch_bounds__(704, 1)
                         mma_f16_ta(tmem + m * tile_n, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0);
                 }
                 mma_commit(w_empty + 8 * ws);
-                mma_commit(x_empty + 8 * xs);
+                if (x_last) mma_commit(x_empty + 8 * xs);
                 if (step == steps - 1) mma_commit(done);
             }
             __syncwarp();
             if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
-            if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+            if (++x_step == XS) {
+                x_step = 0;
+                if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+            }
         }
     } else if (warp >= 18) {
-        // rows that TMA does not bring: 16-byte cells of eight values, as the swizzle places them; a step's cells are
-        // on their way while the step before them is stored
-        constexpr int kCells = 8;
-        const int tid = threadIdx.x - 18 * 32, kxb = a.x_type == kTokE4M3 ? 1 : 2, batches = (tile_n * 8 + 128 * kCells - 1) / (128 * kCells);
-        int xs = 0;
-        uint32_t xp = 0;
-        uint4 v[kCells];
-        auto load = [&](int step, int batch) {
-            const int k0 = k_begin + step * kStepK;
-            const uint8_t* const src = static_cast<const uint8_t*>(a.x) + (r0 * a.x_stride + k0) * kxb;
-#pragma unroll
-            for (int i = 0; i < kCells; ++i) {
-                const int cell = (batch * kCells + i) * 128 + tid, r = cell / 8, c = cell % 8;
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (step < steps && r < rows && k0 + c * 8 < k_end) v[i] = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
-            }
-        };
-        // e4m3 rows of 16-byte alignment, two cells at a time: all of a step at once
-        auto load16 = [&](int step) {
-            const int k0 = k_begin + step * kStepK;
-            const uint8_t* const src = static_cast<const uint8_t*>(a.x) + r0 * a.x_stride + k0;
-#pragma unroll
-            for (int i = 0; i < kCells; ++i) {
-                const int r = (i * 128 + tid) / 4, c = tid % 4;
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (step < steps && r < rows && k0 + c * 16 < k_end)
-                    v[i] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r) * a.x_stride + c * 16));
-            }
-        };
-        if (plan.x_vec16) {
-            load16(0);
+        // rows that TMA does not bring as they are used: two warps write them in 16-byte cells of eight values, as the
+        // swizzle places them
+        const int tid = threadIdx.x - 18 * 32;
+        int xs = 0, rs = 0;
+        uint32_t xp = 0, rp = 0;
+        if (plan.raw_slots) {  // e4m3: TMA brings 128 inputs at a time, these warps widen them
+            auto fetch = [&](int step, int slot) {
+                if (tid == 0 && step < steps) {
+                    mbar_arrive_expect_tx(raw_full + 8 * slot, tile_n * 128);
+                    tma_load_2d(smem_u32(smem + plan.raw) + slot * tile_n * 128, &rows_map, (k_begin + step * kStepK) / 8, static_cast<int>(r0),
+                                raw_full + 8 * slot);
+                }
+            };
+            for (int i = 0; i < plan.raw_slots; ++i) fetch(2 * i, i);
             for (int step = 0; step < steps; ++step) {
-                uint4 w[kCells];
-#pragma unroll
-                for (int i = 0; i < kCells; ++i) w[i] = v[i];
-                load16(step + 1);
+                if (step % 2 == 0 && !wait_phase(raw_full + 8 * rs, rp, &abort_flag)) gave_up(kStatusTimeoutFull);
                 if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
-#pragma unroll
-                for (int i = 0; i < kCells; ++i) {
-                    const int r = (i * 128 + tid) / 4, c = tid % 4 * 2;
-                    if (r < tile_n) {
-                        uint8_t* const to = smem + plan.rows + xs * tile_n * 128 + r * 128;
-                        *reinterpret_cast<uint4*>(to + ((c ^ (r & 7)) << 4)) = widened(w[i], kTokE4M3);
-                        *reinterpret_cast<uint4*>(to + (((c + 1) ^ (r & 7)) << 4)) = widened(make_uint4(w[i].z, w[i].w, 0, 0), kTokE4M3);
-                    }
+                const uint8_t* const raw = smem + plan.raw + rs * tile_n * 128;
+                uint8_t* const to = smem + plan.rows + xs * tile_n * 128;
+#pragma unroll 4
+                for (int i = tid; i < tile_n * 4; i += 64) {
+                    const int r = i / 4, c = i % 4;
+                    const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 128 + (((4 * (step % 2) + c) ^ (r & 7)) << 4));
+                    *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = widened(v, kTokE4M3);
+                    *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = widened(make_uint4(v.z, v.w, 0, 0), kTokE4M3);
+                }
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(x_full + 8 * xs);
+                if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+                if (step % 2) {
+                    asm volatile("bar.sync 2, 64;" ::: "memory");  // both warps have read the slot
+                    fetch(step - 1 + 2 * plan.raw_slots, rs);
+                    if (++rs == plan.raw_slots) rs = 0, rp ^= 1;
+                }
+            }
+            if (abort_flag)  // copies still on their way
+                for (int i = 0; i < plan.raw_slots; ++i) wait_phase(raw_full + 8 * i, i < rs ? rp ^ 1 : rp, nullptr);
+        } else {  // value by value
+            const int kxb = a.x_type == kTokE4M3 ? 1 : 2;
+            for (int step = 0; step < steps; ++step) {
+                const int k0 = k_begin + step * kStepK;
+                const uint8_t* const src = static_cast<const uint8_t*>(a.x) + (r0 * a.x_stride + k0) * kxb;
+                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+#pragma unroll 2
+                for (int i = tid; i < tile_n * 8; i += 64) {
+                    const int r = i / 8, c = i % 8;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (r < rows && k0 + c * 8 < k_end) v = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
+                    *reinterpret_cast<uint4*>(smem + plan.rows + xs * tile_n * 128 + r * 128 + ((c ^ (r & 7)) << 4)) = widened(v, a.x_type);
                 }
                 fence_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(x_full + 8 * xs);
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
-        }
-        if (!plan.x_vec16) load(0, 0);
-        for (int step = 0; step < steps && !plan.x_vec16; ++step) {
-            if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
-            for (int batch = 0; batch < batches; ++batch) {
-                uint4 w[kCells];
-#pragma unroll
-                for (int i = 0; i < kCells; ++i) w[i] = v[i];
-                if (batch + 1 < batches)
-                    load(step, batch + 1);
-                else
-                    load(step + 1, 0);
-#pragma unroll
-                for (int i = 0; i < kCells; ++i) {
-                    const int cell = (batch * kCells + i) * 128 + tid, r = cell / 8, c = cell % 8;
-                    if (r < tile_n)
-                        *reinterpret_cast<uint4*>(smem + plan.rows + xs * tile_n * 128 + r * 128 + ((c ^ (r & 7)) << 4)) = widened(w[i], a.x_type);
-                }
-            }
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(x_full + 8 * xs);
-            if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
         }
     } else {
         // a thread makes weights of one output, whose TMEM lane is its own; the four warps of a lane quarter take the steps
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(704, 1)
         uint32_t sc[kMine][CH], zo[kMine][CH];
         const float inv_group = 1.f / static_cast<float>(group);
         const uint8_t* const s_at = static_cast<const uint8_t*>(a.w.scales) + at * (wide ? 4 : 2);
-        const uint8_t* const z_at = Z ? a.w.zeros + at : nullptr;
+        const uint8_t* const z_at = a.w.zeros ? a.w.zeros + at : nullptr;
         auto load_scales = [&](int k0) {
 #pragma unroll
             for (int c = 0; c < kMine; ++c)
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(704, 1)
                             sc[c][h] = __ldg(reinterpret_cast<const uint32_t*>(s_at) + g);
                         else
                             sc[c][h] = __ldg(reinterpret_cast<const uint16_t*>(s_at) + g);
-                        if (Z) zo[c][h] = __ldg(z_at + g);
+                        if (z_at) zo[c][h] = __ldg(z_at + g);
                     }
                 }
         };
@@ -390,11 +392,13 @@ __global__ void __launch_bounds__(704, 1)
                     float v = wide ? __uint_as_float(raw) : is_f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(raw))) : __uint_as_float(raw << 16);
                     if (!BF) v *= factor;
                     hi[c][h] = pair16<BF>(v, v);
+                    if (!EX) {
                     const float l = v - (BF ? __uint_as_float(hi[c][h] << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(hi[c][h]))));
                     lo[c][h] = fabsf(l) < INFINITY ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
+                    }
                     z[c][h] = zero_terms<BF>(zo[c][h]);
                 }
-            if (st + 1 < stages) load_scales(k_begin + (st + 1) * kStageK);
+            load_scales(k_begin + (st + 1) * kStageK);
             if (!wait_phase(c_full + 8 * cs, cp, &abort_flag)) gave_up(kStatusTimeoutFull);
             const uint32_t from = codes + cs * kTileM * 128 + row * 128;
 #pragma unroll
@@ -411,7 +415,7 @@ __global__ void __launch_bounds__(704, 1)
                 uint32_t out[4][8];
 #pragma unroll
                 for (int h = 0; h < 4; ++h)
-                    weights16<BF>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH], z[c][h / 2 % CH], out[h]);
+                    weights16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH], z[c][h / 2 % CH], out[h]);
                 if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
                 tc_fence_after();
 #pragma unroll
@@ -486,14 +490,23 @@ __global__ void __launch_bounds__(704, 1)
         __syncwarp();
         cluster_sync();
         const uint32_t base = smem_u32(smem);
-        for (int i = threadIdx.x; i < rows * kTileM; i += blockDim.x) {
-            const int r = i / kTileM, o = i % kTileM;
-            if (r % plan.split != rank || o0 + o >= n) continue;
-            float f = 0.f;
-            for (int p = 0; p < plan.split; ++p) f += ld_cluster(base + i * 4, p);
-            if (a.x_scale) f *= a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
-            if (a.bias) f += a.bias[o0 + o];
-            tok_store(a.y, (r0 + r) * a.y_stride + o0 + o, a.y_type, f);
+        const int mine = (rows - rank + plan.split - 1) / plan.split;  // rows rank, rank + split, ...
+        for (int i = threadIdx.x; i < mine * (kTileM / 4); i += blockDim.x) {
+            const int r = rank + i / (kTileM / 4) * plan.split, o = o0 + i % (kTileM / 4) * 4;
+            if (o >= n) continue;
+            const uint32_t at = base + (r * kTileM + i % (kTileM / 4) * 4) * 4;
+            float4 v[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < plan.split) v[p] = ld_cluster4(at, p);
+            float f[4] = {};
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+                if (p < plan.split) f[0] += v[p].x, f[1] += v[p].y, f[2] += v[p].z, f[3] += v[p].w;
+            const float xs = a.x_scale ? a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0] : 1.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (o + e < n) tok_store(a.y, (r0 + r) * a.y_stride + o + e, a.y_type, f[e] * xs + (a.bias ? a.bias[o + e] : 0.f));
         }
         cluster_sync();
     }
@@ -504,15 +517,17 @@ __global__ void __launch_bounds__(704, 1)
     }
 }
 
-template <bool BF, bool TWO, int CH, bool Z>
+template <bool BF, bool TWO, int XS, int CH, bool EX>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     constexpr int kTileM = TWO ? 256 : 128;
-    auto* kern = w4_many_kernel<BF, TWO, CH, Z>;
+    auto* kern = w4_many_kernel<BF, TWO, XS, CH, EX>;
     CUtensorMap codes, rows;
     cudaError_t e = tmap_rows(&codes, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kTileM);
     if (e == cudaSuccess) {
         if (p.x_tma)
             e = tmap_rows(&rows, a.x, 2, a.w.k, a.rows, a.x_stride * 2, p.tile_n);
+        else if (p.raw_slots)
+            e = tmap_rows(&rows, a.x, 8, a.w.k / 8, a.rows, a.x_stride, p.tile_n);
         else
             rows = codes;
     }
@@ -520,7 +535,7 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((a.w.n + kTileM - 1) / kTileM * p.split, (a.rows + p.tile_n - 1) / p.tile_n);
-    cfg.blockDim = dim3(p.x_tma ? 18 * 32 : 22 * 32);
+    cfg.blockDim = dim3(p.x_tma ? 19 * 32 : 20 * 32);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -534,10 +549,16 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-template <bool BF, bool TWO>
+template <bool BF, bool TWO, int XS>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
-    if (a.w.group % kStepK == 0) return a.w.zeros ? launch<BF, TWO, 1, true>(a, p, s) : launch<BF, TWO, 1, false>(a, p, s);
-    return a.w.zeros ? launch<BF, TWO, 2, true>(a, p, s) : launch<BF, TWO, 2, false>(a, p, s);
+    const bool exact = a.w.scale_type == (BF ? kTokBF16 : kTokF16);
+    if (a.w.group % kStepK == 0) return exact ? launch<BF, TWO, XS, 1, true>(a, p, s) : launch<BF, TWO, XS, 1, false>(a, p, s);
+    return exact ? launch<BF, TWO, XS, 2, true>(a, p, s) : launch<BF, TWO, XS, 2, false>(a, p, s);
+}
+template <bool BF>
+cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, bool two, int x_steps, cudaStream_t s) {
+    if (two) return launch<BF, true, 1>(a, p, s);
+    return x_steps == 1 ? launch<BF, false, 1>(a, p, s) : launch<BF, false, 4>(a, p, s);
 }
 
 }  // namespace
@@ -548,7 +569,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
     p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
     p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride % 8 == 0;
-    p.x_vec16 = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0;
+    p.raw_slots = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0 ? 2 : 0;
     const bool two = (a.w.n + 255) / 256 * ((a.rows + 191) / 192) >= sms;
     const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
     p.tile_n = a.rows >= most_n ? most_n : (a.rows + 15) / 16 * 16;
@@ -564,8 +585,9 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.tmem_cols = 512;
     p.rings[1] = std::min((p.tmem_cols - p.weight_col) / (two ? 64 : 32), kMaxRing);
     // shared memory: codes and rows in turn
-    const int factor_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128;
-    int room = kSmemMax - factor_bytes - 2 * w - 2 * x;
+    const int x_steps = p.x_tma && p.tile_n <= 64 ? 4 : 1;
+    const int factor_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128 * x_steps;
+    int room = kSmemMax - factor_bytes - 2 * w - 2 * x - p.raw_slots * p.tile_n * 128;
     p.rings[0] = p.rings[2] = 2;
     for (bool more = true; more;) {
         more = false;
@@ -580,7 +602,8 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     }
     p.codes = 0;
     p.rows = p.rings[0] * w;
-    p.row_factor = p.rows + p.rings[2] * x;
+    p.raw = p.rows + p.rings[2] * x;
+    p.row_factor = p.raw + p.raw_slots * p.tile_n * 128;
     p.bytes = p.row_factor + factor_bytes;
     if (p.split > 1) {  // the partial sums lie over the rings
         const int partial = p.tile_n * tile_m * 4;
@@ -589,8 +612,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
             p.bytes = partial + factor_bytes;
         }
     }
-    if (a.x_type == kTokBF16) return two ? launch<true, true>(a, p, s) : launch<true, false>(a, p, s);
-    return two ? launch<false, true>(a, p, s) : launch<false, false>(a, p, s);
+    return a.x_type == kTokBF16 ? launch<true>(a, p, two, x_steps, s) : launch<false>(a, p, two, x_steps, s);
 }
 
 cudaError_t w4_many_status(uint32_t* code) { return take_status(code); }
