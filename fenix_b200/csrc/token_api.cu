@@ -233,14 +233,15 @@ fx_status fx_w4_device_status(int device) {
         }
         cudaGetDevice(&cur);
         if (cudaError_t e = cudaSetDevice(device); e != cudaSuccess) return done(fn, e);
-        uint32_t few = 0, many = 0;
+        uint32_t few = 0, bf16 = 0, f16 = 0;
         cudaError_t e = cudaDeviceSynchronize();
         if (e == cudaSuccess) e = fxk::w4_few_status(&few);
-        if (e == cudaSuccess) e = fxk::w4_many_status(&many);
+        if (e == cudaSuccess) e = fxk::w4_many_bf16_status(&bf16);
+        if (e == cudaSuccess) e = fxk::w4_many_f16_status(&f16);
         cudaSetDevice(cur);
         if (e != cudaSuccess) return done(fn, e);
-        if (few || many)
-            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(few ? few : many));
+        if (few || bf16 || f16)
+            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(few ? few : bf16 ? bf16 : f16));
         return FX_OK;
     });
 }

@@ -6,10 +6,34 @@
 
 namespace fxk {
 
+constexpr int kStageK = 256;  // inputs of a stage of codes: 128 bytes an output
+constexpr int kStepK = 64;    // inputs of a stage of operands: 128 bytes of 16-bit values a row
+constexpr int kMaxRing = 8;
+constexpr int kSmemMax = 226 * 1024;
+
+struct ManyPlan {
+    int tile_n;           // rows of a tile: a multiple of 16, at most 256
+    int rings[3];         // stages of codes, weights, rows; at most kMaxRing
+    int codes, rows, raw, row_factor;  // offsets in shared memory
+    int bytes;
+    int split;            // blocks of a cluster that share a tile, each with a range of k
+    int stages_each;      // stages of codes of a block
+    int tmem_cols;
+    int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
+    int raw_slots;        // of e4m3 rows by TMA, 128 inputs each
+    bool y_vec;           // results aligned to eight outputs
+    int x_steps;          // steps of 64 inputs of a slot that TMA fills with rows as they are; 0: warps write the rows
+    bool x_vec;           // rows aligned to eight values
+    bool two;             // tiles of 256 outputs
+};
+
+cudaError_t w4_many_bf16(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s);
+cudaError_t w4_many_f16(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s);
 cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s);
 // The status word of each file's kernels, cleared.
 cudaError_t w4_few_status(uint32_t* code);
-cudaError_t w4_many_status(uint32_t* code);
+cudaError_t w4_many_bf16_status(uint32_t* code);
+cudaError_t w4_many_f16_status(uint32_t* code);
 
 #ifdef __CUDACC__
 // Set by a kernel of this file's includer whose bounded wait gave up; read and cleared by take_status.
