@@ -17,11 +17,11 @@ namespace {
 // warps, across tiles, so that memory never waits for a tile's end; each consumer takes 128 inputs of a
 // stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs, B: inputs x 8 rows); the rows lie in
 // shared memory for the whole walk, converted once and in the MMA's order.
-// Codes become exact 16-bit integers: in f16 code - zero, in bf16 128 + code, whose offset leaves in f32
-// with one more MMA of ones, shared by the m-tiles, that sums the inputs of a group:
-//   sum (code - zero) x = sum (128 + code) x - (128 + zero) sum x
-// (the difference loses 5 of f32's 24 bits). Scales are applied in f32 to a group's sum: no weight is
-// rounded. The consumers' partial sums meet in shared memory.
+// A code enters the MMA as offset + code, which costs one logical operation for two; what leaves again in f32, a group
+// at a time, are sums over the rows' inputs alone, made when those are brought in:
+//   sum (code - zero) x = sum (offset + code) x - sum offset x - zero sum x
+// (the difference loses 5 of f32's 24 bits in bf16, 8 in f16: 16 are left for results of 8 and 11). Scales are applied
+// in f32 to a group's sum: no weight is rounded. The consumers' partial sums meet in shared memory.
 
 constexpr int kBlockK = 128;  // inputs of a consumer warp in a stage
 constexpr int kMaxConsumers = 16;
@@ -41,25 +41,32 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Nibbles (i, i + 4) of a word of eight codes as two 16-bit floats, by or'ing them into the mantissa of a
-// power of two. bf16: 128 + code (three shifts for a word's four pairs). f16: 1024 + code or 1024 + 16 code
-// (one shift), from which one fused multiply-add makes code - zero; z = {1024 + zero, -(64 + zero)}.
+// Nibbles (i, i + 4) of a word of eight codes as two 16-bit floats offset + code, by or'ing them into the mantissa of
+// a power of two. bf16: 128 + code (three shifts for a word's four pairs). f16: 1024 + code, whose last place is one,
+// or 64 + code, whose last place is a sixteenth, wherever the nibble lies (one shift).
 template <bool BF>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, const uint32_t (&z)[2]) {
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
     if (BF) return and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
-    const uint32_t h = and_or(i >= 2 ? w >> 8 : w, i & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
-    uint32_t r;
-    if (i & 1)
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(h), "r"(0x2c002c00u), "r"(z[1]));
-    else
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(z[0]));
-    return r;
+    return and_or(i >= 2 ? w >> 8 : w, i & 1 ? 0x00f000f0u : 0x000f000fu, i & 1 ? 0x54005400u : 0x64006400u);
 }
-
 // Eight 16-bit values as the pairs (i, i + 4), i = 0..3: code_pair's order.
 __device__ __forceinline__ uint4 paired(const uint4& v) {
     return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                       __byte_perm(v.y, v.w, 0x7632));
+}
+
+// Sums over paired eight values: offset x, in code_pair's offsets, and x.
+template <bool BF>
+__device__ __forceinline__ float2 offset_sums(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float even = 0.f, odd = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = BF ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
+                            : __half22float2(reinterpret_cast<const __half2&>(w[i]));
+        (i & 1 ? odd : even) += f.x + f.y;
+    }
+    return make_float2(BF ? 128.f * (even + odd) : 1024.f * even + 64.f * odd, even + odd);
 }
 
 // How the few-rows kernel walks and where its parts lie in shared memory; made by the host.
@@ -72,7 +79,8 @@ struct FewPlan {
     int x_pitch;     // of a row's inputs: 64 modulo 128, so that 2 rows x 4 lanes of 16 bytes hit all banks once
     int s_pitch, z_pitch;  // of an output's scales and zero points: 16 modulo 128, so that 8 outputs hit different banks
     int red_bufs;
-    int x, scale, accum, red, ring, bytes;  // offsets; accum: the sums of earlier segments, by tile of this block
+    int sum_pitch;   // of a row's sums over units, in pairs
+    int x, sums, scale, accum, red, ring, bytes;  // offsets; accum: the sums of earlier segments, by tile of this block
     bool x_vec;
 };
 
@@ -111,12 +119,14 @@ __device__ __forceinline__ void rows_to_shared(uint8_t* to, int dst_pitch, const
 
 // CPF chunks of 32 inputs times MT m-tiles of 16 outputs into acc, under one scale per output. The codes of output
 // m 16 + h 8 (+ this lane's g, in `codes`) lie 128 bytes apart, 16-byte cell c of them at cell c ^ g (cell: of the first
-// chunk); `x`: this lane's rows; scales and zero points as they are stored.
+// chunk); x_at: this lane's row, sum0 and sum1: the sums of its results' rows; scales and zero points as they are stored.
 template <bool BF, int CPF, bool Z, int MT>
-__device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_t x_at, int cell, uint32_t s_at, int s_pitch,
+__device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_t x_at, const float2* sum0,
+                                     const float2* sum1, int cell, uint32_t s_at, int s_pitch,
                                      int scale_type, uint32_t z_at, int z_pitch) {
-    uint32_t x[CPF][4], w[MT][2][CPF], z[MT][2][2], zero[MT][2];
-    float scale[MT][2], part[MT][4] = {}, xs[4] = {};
+    uint32_t x[CPF][4], w[MT][2][CPF];
+    float scale[MT][2], zero[MT][2], part[MT][4] = {};
+    const float2 xs[2] = {*sum0, *sum1};
 #pragma unroll
     for (int c = 0; c < CPF; ++c) {
         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
@@ -140,28 +150,26 @@ __device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_
                 asm volatile("ld.shared.b16 %0, [%1];" : "=h"(raw) : "r"(at));
                 scale[m][h] = scale_type == kTokF16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float(static_cast<uint32_t>(raw) << 16);
             }
-            zero[m][h] = 8;
-            if (Z) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(zero[m][h]) : "r"(z_at + (m * 16 + h * 8) * z_pitch));
-            z[m][h][0] = 0x64006400u + 0x00010001u * zero[m][h];  // f16 pairs of 1024 + zero
-            z[m][h][1] = 0xd400d400u + 0x00100010u * zero[m][h];  // and -(64 + zero)
+            if (Z) {
+                uint32_t z;
+                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(z_at + (m * 16 + h * 8) * z_pitch));
+                zero[m][h] = static_cast<float>(z);
+            }
         }
 #pragma unroll
     for (int c = 0; c < CPF; ++c)
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-            if (BF) mma16816<BF>(xs, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u, x[c][i], x[c][i + 1]);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const uint32_t f0 = code_pair<BF>(w[m][0][c], i, z[m][0]), f1 = code_pair<BF>(w[m][1][c], i, z[m][1]);
-                const uint32_t f2 = code_pair<BF>(w[m][0][c], i + 1, z[m][0]), f3 = code_pair<BF>(w[m][1][c], i + 1, z[m][1]);
-                mma16816<BF>(part[m], f0, f1, f2, f3, x[c][i], x[c][i + 1]);
-            }
+            for (int m = 0; m < MT; ++m)
+                mma16816<BF>(part[m], code_pair<BF>(w[m][0][c], i), code_pair<BF>(w[m][1][c], i), code_pair<BF>(w[m][0][c], i + 1),
+                             code_pair<BF>(w[m][1][c], i + 1), x[c][i], x[c][i + 1]);
         }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float p = BF ? fmaf(-128.f - static_cast<float>(zero[m][e / 2]), xs[e % 2], part[m][e]) : part[m][e];
+            const float p = fmaf(Z ? -zero[m][e / 2] : -8.f, xs[e % 2].y, part[m][e] - xs[e % 2].x);
             acc[m][e] = fmaf(scale[m][e / 2], p, acc[m][e]);
         }
 }
@@ -257,6 +265,8 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
     }
 
     const uint32_t x_lane = smem_u32(smem + plan.x) + min(g, rows - 1) * plan.x_pitch + t * 16;  // rows past the last: nothing reads their sums
+    const float2* const sum0 = reinterpret_cast<const float2*>(smem + plan.sums) + min(2 * t, rows - 1) * plan.sum_pitch;
+    const float2* const sum1 = reinterpret_cast<const float2*>(smem + plan.sums) + min(2 * t + 1, rows - 1) * plan.sum_pitch;
     const float inv_group = 1.f / static_cast<float>(group);
     int red_buf = 0;
     for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
@@ -266,8 +276,22 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             const int kxb = a.x_type == kTokE4M3 ? 1 : 2, eights = min((seg_end - seg) * kBlockK, k - seg * kBlockK) / 8;
             for (int r = 0; r < rows; ++r) {
                 const uint8_t* const p = static_cast<const uint8_t*>(a.x) + (r * a.x_stride + seg * kBlockK) * kxb;
-                for (int i = threadIdx.x; i < eights; i += warps * 32)
-                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = paired(widened(raw_eight(p + i * 8 * kxb, a.x_type, plan.x_vec), a.x_type));
+                float2* const sums = reinterpret_cast<float2*>(smem + plan.sums) + r * plan.sum_pitch;
+                for (int i0 = warp * 32; i0 < eights; i0 += warps * 32) {
+                    const int i = i0 + lane;
+                    float2 f = {};
+                    if (i < eights) {
+                        const uint4 v = paired(widened(raw_eight(p + i * 8 * kxb, a.x_type, plan.x_vec), a.x_type));
+                        *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = v;
+                        f = offset_sums<BF>(v);
+                    }
+#pragma unroll
+                    for (int o = 2 * CPF; o; o >>= 1) {
+                        f.x += __shfl_xor_sync(0xffffffffu, f.x, o);
+                        f.y += __shfl_xor_sync(0xffffffffu, f.y, o);
+                    }
+                    if (lane % (4 * CPF) == 0 && i < eights) sums[i / (4 * CPF)] = f;
+                }
             }
         }
         consumers_sync(warps);
@@ -294,10 +318,10 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                         // (kc + 1/2) / group truncated: exact while k < 2^21
                         const int gi = (k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group) - g0;
                         if (wide)
-                            unit<BF, CPF, Z, 2>(acc, cw, xw + u * CPF * 64, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
+                            unit<BF, CPF, Z, 2>(acc, cw, xw + u * CPF * 64, sum0 + (blk - seg) * kUnits + u, sum1 + (blk - seg) * kUnits + u, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
                                                 a.w.scale_type, z_at + gi, plan.z_pitch);
                         else
-                            unit<BF, CPF, Z, 1>(acc, cw, xw + u * CPF * 64, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
+                            unit<BF, CPF, Z, 1>(acc, cw, xw + u * CPF * 64, sum0 + (blk - seg) * kUnits + u, sum1 + (blk - seg) * kUnits + u, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
                                                 a.w.scale_type, z_at + gi, plan.z_pitch);
                     }
                 }
@@ -378,7 +402,9 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
     if (p.tiles < sms) *grid = p.tiles;
     p.red_bufs = rows <= 4 ? 2 : 1;
     p.x = 0;
-    p.scale = round_up(rows * p.x_pitch, 128);
+    p.sums = round_up(rows * p.x_pitch, 128);
+    p.sum_pitch = p.seg_blocks * (a.w.group % 128 == 0 ? 1 : a.w.group % 64 == 0 ? 2 : 4) + 1;
+    p.scale = p.sums + round_up(rows * p.sum_pitch * 8, 128);
     p.accum = p.scale + round_up(2 * kM * (p.s_pitch + (a.w.zeros ? p.z_pitch : 0)), 128);
     p.red = p.accum;
     if (p.seg_blocks < blocks) {  // room for the sums of a block's tiles between segments
