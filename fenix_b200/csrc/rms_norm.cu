@@ -8,6 +8,8 @@
 #include "counters.hpp"
 #include "token.cuh"
 
+#include <atomic>
+
 namespace fxk {
 namespace {
 
@@ -127,29 +129,9 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
     return __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32 < TEAM / 32 ? threadIdx.x % 32 : 0]);
 }
 
-// TEAM threads a row, TURNS times eight values each.
+// From a row's h on: the norm, the scale, the output. red: three rows of 32 floats that no thread of the team still reads.
 template <int TEAM, int TURNS, bool VEC>
-__global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_kernel(const __grid_constant__ RmsNormArgs a) {
-    __shared__ float red[3][32];
-    const int me = threadIdx.x % TEAM;
-    const int64_t row = TEAM == 32 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-    if (row >= a.rows) return;
-    float h[TURNS][kVec];
-#pragma unroll
-    for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.x, row * a.x_stride, a.x_type, u, me, a.cols, h[u]);
-    if (a.residual) {
-        float r[TURNS][kVec];
-#pragma unroll
-        for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.residual, row * a.residual_stride, a.residual_type, u, me, a.cols, r[u]);
-#pragma unroll
-        for (int u = 0; u < TURNS; ++u)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) h[u][j] += r[u][j];
-    }
-    if (a.sum) {
-#pragma unroll
-        for (int u = 0; u < TURNS; ++u) store8<TEAM, VEC>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
-    }
+__device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, int me, float (&h)[TURNS][kVec], float (*red)[32]) {
     float ss = 0.f;
 #pragma unroll
     for (int u = 0; u < TURNS; ++u)
@@ -201,6 +183,76 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_kernel(const
     }
 }
 
+// TEAM threads a row, TURNS times eight values each.
+template <int TEAM, int TURNS, bool VEC>
+__global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_kernel(const __grid_constant__ RmsNormArgs a) {
+    __shared__ float red[3][32];
+    const int me = threadIdx.x % TEAM;
+    const int64_t row = TEAM == 32 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+    if (row >= a.rows) return;
+    float h[TURNS][kVec];
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.x, row * a.x_stride, a.x_type, u, me, a.cols, h[u]);
+    if (a.residual) {
+        float r[TURNS][kVec];
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.residual, row * a.residual_stride, a.residual_type, u, me, a.cols, r[u]);
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) h[u][j] += r[u][j];
+    }
+    if (a.sum) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) store8<TEAM, VEC>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
+    }
+    finish_row<TEAM, TURNS, VEC>(a, row, me, h, red);
+}
+
+// Many rows of 16-bit x (and residual): the blocks stay and walk over the rows, a row's values on their way while the row
+// before it is worked on, so that memory does not wait for the reductions.
+template <int TEAM, int TURNS, bool RES>
+__global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_stream_kernel(const __grid_constant__ RmsNormArgs a) {
+    __shared__ float red[2][3][32];
+    const int me = threadIdx.x % TEAM, per = TEAM == 32 ? blockDim.x / 32 : 1;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * per;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / TEAM;
+    uint4 x[TURNS], r[RES ? TURNS : 1];
+    auto fetch = [&](int64_t at) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            const int c = column<TEAM, true>(u, 0, me);
+            if (at >= a.rows || c >= a.cols) continue;
+            x[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + at * a.x_stride + c);
+            if (RES) r[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.residual) + at * a.residual_stride + c);
+        }
+    };
+    fetch(row);
+    for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
+        float h[TURNS][kVec];
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            unpack8(x[u], a.x_type, h[u]);
+            if (RES) {
+                float f[kVec];
+                unpack8(r[u], a.residual_type, f);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) h[u][j] += f[j];
+            }
+            if (column<TEAM, true>(u, 0, me) >= a.cols) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) h[u][j] = 0.f;
+            }
+        }
+        fetch(row + step);
+        if (a.sum) {
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u) store8<TEAM, true>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
+        }
+        finish_row<TEAM, TURNS, true>(a, row, me, h, red[turn]);  // a row's barrier lies between two uses of a half of red
+    }
+}
+
 template <int TEAM, int TURNS>
 cudaError_t launch(const RmsNormArgs& a, bool vec, cudaStream_t s) {
     const int threads = TEAM == 32 ? 128 : TEAM, per = threads / TEAM;
@@ -213,6 +265,27 @@ cudaError_t launch(const RmsNormArgs& a, bool vec, cudaStream_t s) {
     return cudaGetLastError();
 }
 
+template <int TEAM, int TURNS, bool RES>
+cudaError_t launch_stream(const RmsNormArgs& a, cudaStream_t s) {
+    auto* kern = rms_norm_stream_kernel<TEAM, TURNS, RES>;
+    constexpr int threads = TEAM == 32 ? 128 : TEAM, per = threads / TEAM;
+    static std::atomic<int> known;  // blocks that are resident at once on an SM; the same on every sm_100
+    int resident = known.load(std::memory_order_relaxed);
+    if (!resident) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, 0);
+        if (e != cudaSuccess) return e;
+        known.store(resident, std::memory_order_relaxed);
+    }
+    const int64_t need = (static_cast<int64_t>(a.rows) + per - 1) / per, fit = static_cast<int64_t>(sm_count()) * resident;
+    count_launch();
+    kern<<<static_cast<unsigned>(need < fit ? need : fit), threads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+template <int TEAM, int TURNS>
+cudaError_t launch_stream(const RmsNormArgs& a, cudaStream_t s) {
+    return a.residual ? launch_stream<TEAM, TURNS, true>(a, s) : launch_stream<TEAM, TURNS, false>(a, s);
+}
+
 }  // namespace
 
 cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
@@ -222,14 +295,23 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
     };
     const bool vec = a.cols % kVec == 0 && ok(a.x, a.x_stride, a.x_type) && ok(a.residual, a.residual_stride, a.residual_type) &&
                      ok(a.sum, a.sum_stride, a.residual_type) && ok(a.weight, 0, a.weight_type) && ok(a.y, a.y_stride, a.y_type);
-    // few rows: as many threads as the row has eights, for the shortest way through; many: 16 values a thread
     const bool few = a.rows <= 148 * 2;
+    if (vec && !few && a.x_type != kTokF32 && (!a.residual || a.residual_type != kTokF32)) {
+        if (a.cols <= 256) return launch_stream<32, 1>(a, s);
+        if (a.cols <= 512) return launch_stream<32, 2>(a, s);
+        if (a.cols <= 1024) return launch_stream<32, 4>(a, s);
+        if (a.cols <= 2048) return launch_stream<128, 2>(a, s);
+        if (a.cols <= 4096) return launch_stream<256, 2>(a, s);
+        if (a.cols <= 8192) return launch_stream<512, 2>(a, s);
+        if (a.cols <= 16384) return launch_stream<1024, 2>(a, s);
+    }
+    // few rows: as many threads as the row has eights, for the shortest way through
     if (a.cols <= 256) return launch<32, 1>(a, vec, s);
     if (a.cols <= 512) return launch<32, 2>(a, vec, s);
     if (a.cols <= 1024) return few ? launch<128, 1>(a, vec, s) : launch<32, 4>(a, vec, s);
-    if (a.cols <= 2048) return few ? launch<256, 1>(a, vec, s) : launch<128, 2>(a, vec, s);
-    if (a.cols <= 4096) return few ? launch<512, 1>(a, vec, s) : launch<256, 2>(a, vec, s);
-    if (a.cols <= 8192) return few ? launch<1024, 1>(a, vec, s) : launch<512, 2>(a, vec, s);
+    if (a.cols <= 2048) return launch<256, 1>(a, vec, s);
+    if (a.cols <= 4096) return launch<512, 1>(a, vec, s);
+    if (a.cols <= 8192) return launch<1024, 1>(a, vec, s);
     if (a.cols <= 16384) return launch<1024, 2>(a, vec, s);
     return launch<1024, 4>(a, vec, s);
 }

@@ -27,6 +27,9 @@ struct RmsNormArgs {
     int x_type, residual_type, weight_type, y_type, scale_mode;
     float eps;
 };
+// SMs of the current device.
+int sm_count();
+
 cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s);
 
 struct W4Args {

@@ -16,6 +16,22 @@ fx_status abi_error(int code, const std::string& msg);
 fx_status abi_exception();
 }  // namespace fxh
 
+namespace fxk {
+
+int sm_count() {
+    static std::atomic<int> count[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int c = dev < 64 ? count[dev].load(std::memory_order_relaxed) : 0;
+    if (!c) {
+        cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
+        if (dev < 64) count[dev].store(c, std::memory_order_relaxed);
+    }
+    return c;
+}
+
+}  // namespace fxk
+
 namespace {
 
 constexpr int64_t kMaxExtent = int64_t{1} << 30;  // rows, columns and strides: byte offsets stay below 2^62

@@ -5,8 +5,6 @@
 #include "token.cuh"
 #include "w4.cuh"
 
-#include <atomic>
-
 namespace fxk {
 namespace {
 
@@ -359,18 +357,6 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             if (plan.red_bufs == 1) consumers_sync(warps);
         }
     }
-}
-
-int sm_count() {
-    static std::atomic<int> count[64];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int c = dev < 64 ? count[dev].load(std::memory_order_relaxed) : 0;
-    if (!c) {
-        cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
-        if (dev < 64) count[dev].store(c, std::memory_order_relaxed);
-    }
-    return c;
 }
 
 constexpr int kFewSmem = 226 * 1024;  // a block's shared memory, less the barriers

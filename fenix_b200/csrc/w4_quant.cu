@@ -134,44 +134,58 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __res
     }
 }
 
-// A thread: a word of eight codes, eight consecutive values. A code is or'ed into the mantissa of 2^23.
+constexpr int kWords = 4;  // of a thread, kThreads apart
+
+// A word of eight codes makes eight consecutive values. A code is or'ed into the mantissa of 2^23.
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const W4Args q, void* __restrict__ w, int w_type, int64_t w_stride, int row0) {
-    const int e = blockIdx.x * kThreads + threadIdx.x, row = row0 + blockIdx.y;  // e: word of the row
-    if (e >= q.k / kEight) return;
-    // (e + 1/2) / words truncated: exact while e < 2^21, as k < 2^24
-    const int words = q.group / kEight, of_row = static_cast<int>((static_cast<float>(e) + 0.5f) * __frcp_rn(static_cast<float>(words)));
-    const int64_t g = static_cast<int64_t>(row) * (q.k / q.group) + of_row;
-    const uint32_t c = __ldcs(reinterpret_cast<const uint32_t*>(q.codes) + static_cast<int64_t>(row) * (q.k / kEight) + e);
-    const float s = tok_load(q.scales, g, q.scale_type);
-    const float off = 8388608.f + (q.zeros ? static_cast<float>(q.zeros[g]) : 8.f);
-    float f[kEight];
+    const int row = row0 + blockIdx.y, words = q.k / kEight;  // of the row
+    const float inv = __frcp_rn(static_cast<float>(q.group / kEight));
+    const uint32_t* const codes = reinterpret_cast<const uint32_t*>(q.codes) + static_cast<int64_t>(row) * words;
+    const int64_t g0 = static_cast<int64_t>(row) * (q.k / q.group);
+    uint32_t c[kWords];
+    float s[kWords], off[kWords];
 #pragma unroll
-    for (int j = 0; j < kEight; ++j) f[j] = s * (__uint_as_float((c >> (4 * j) & 15u) | 0x4b000000u) - off);
-    const int64_t o = row * w_stride + e * kEight;
-    if (VEC && w_type == kTokF32) {
-        float4* p = reinterpret_cast<float4*>(static_cast<float*>(w) + o);
-        __stcs(p, make_float4(f[0], f[1], f[2], f[3]));
-        __stcs(p + 1, make_float4(f[4], f[5], f[6], f[7]));
-    } else if (VEC) {
-        uint32_t r[4];
-        if (w_type == kTokF16) {
+    for (int i = 0; i < kWords; ++i) {
+        const int e = (blockIdx.x * kWords + i) * kThreads + threadIdx.x;
+        if (e >= words) continue;
+        c[i] = __ldcs(codes + e);
+        const int64_t g = g0 + static_cast<int>((static_cast<float>(e) + 0.5f) * inv);  // exact while e < 2^21, as k < 2^24
+        s[i] = tok_load(q.scales, g, q.scale_type);
+        off[i] = 8388608.f + (q.zeros ? static_cast<float>(__ldg(q.zeros + g)) : 8.f);
+    }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-                r[j] = reinterpret_cast<const uint32_t&>(h);
+    for (int i = 0; i < kWords; ++i) {
+        const int e = (blockIdx.x * kWords + i) * kThreads + threadIdx.x;
+        if (e >= words) continue;
+        float f[kEight];
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) f[j] = s[i] * (__uint_as_float((c[i] >> (4 * j) & 15u) | 0x4b000000u) - off[i]);
+        const int64_t o = row * w_stride + e * kEight;
+        if (VEC && w_type == kTokF32) {
+            float4* p = reinterpret_cast<float4*>(static_cast<float*>(w) + o);
+            __stcs(p, make_float4(f[0], f[1], f[2], f[3]));
+            __stcs(p + 1, make_float4(f[4], f[5], f[6], f[7]));
+        } else if (VEC) {
+            uint32_t r[4];
+            if (w_type == kTokF16) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+                    r[j] = reinterpret_cast<const uint32_t&>(h);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                    r[j] = reinterpret_cast<const uint32_t&>(h);
+                }
             }
+            __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(w) + o), make_uint4(r[0], r[1], r[2], r[3]));
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-                r[j] = reinterpret_cast<const uint32_t&>(h);
-            }
+            for (int j = 0; j < kEight; ++j) tok_store(w, o + j, w_type, f[j]);
         }
-        __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(w) + o), make_uint4(r[0], r[1], r[2], r[3]));
-    } else {
-#pragma unroll
-        for (int j = 0; j < kEight; ++j) tok_store(w, o + j, w_type, f[j]);
     }
 }
 
@@ -205,15 +219,19 @@ cudaError_t quantize(const void* w, int w_type, int64_t w_stride, const W4Args& 
 }  // namespace
 
 cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, const W4Args& q, cudaStream_t s) {
-    if (q.group == 32) return quantize<4, 1>(w, w_type, w_stride, q, s);
-    if (q.group <= 64) return quantize<8, 1>(w, w_type, w_stride, q, s);
-    if (q.group <= 128) return quantize<16, 1>(w, w_type, w_stride, q, s);
+    // 32 weights a thread share what is done once a group (8192 x 8192 f32 in groups of 128: 50 us, 83 with 8 a thread);
+    // a matrix that leaves SMs idle that way takes 8 a thread (1003 x 1088 bf16 in groups of 32: 3.7 us, 5.2 with 32)
+    const bool small = static_cast<int64_t>(q.n) * q.k < int64_t{148} * 1024 * 32;
+    if (q.group == 32) return small ? quantize<4, 1>(w, w_type, w_stride, q, s) : quantize<1, 4>(w, w_type, w_stride, q, s);
+    if (q.group == 64) return small ? quantize<8, 1>(w, w_type, w_stride, q, s) : quantize<2, 4>(w, w_type, w_stride, q, s);
+    if (q.group == 128) return small ? quantize<16, 1>(w, w_type, w_stride, q, s) : quantize<4, 4>(w, w_type, w_stride, q, s);
+    if (q.group == 256 && !small) return quantize<8, 4>(w, w_type, w_stride, q, s);
     return quantize<32, 4>(w, w_type, w_stride, q, s);
 }
 
 cudaError_t launch_w4_dequantize(const W4Args& q, void* w, int w_type, int64_t w_stride, cudaStream_t s) {
     constexpr int kRows = 65535;  // of a launch
-    const unsigned across = (q.k / kEight + kThreads - 1) / kThreads;
+    const unsigned across = (q.k / kEight + kThreads * kWords - 1) / (kThreads * kWords);
     for (int row0 = 0; row0 < q.n; row0 += kRows) {
         const dim3 grid(across, static_cast<unsigned>(q.n - row0 < kRows ? q.n - row0 : kRows));
         count_launch();
