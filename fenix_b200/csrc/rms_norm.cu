@@ -55,12 +55,22 @@ __device__ __forceinline__ void load8(const void* p, int64_t row, int type, int 
             const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + row + c);
             unpack8(CONST ? __ldg(q) : q[0], type, f);
         }
-    } else {
+    } else if (type == kTokF32) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
             const int c = column<TEAM, VEC>(u, j, me);
-            f[j] = c < cols ? tok_load(p, row + c, type) : 0.f;
+            f[j] = c < cols ? static_cast<const float*>(p)[row + c] : 0.f;
         }
+    } else {
+        uint16_t v[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            const int c = column<TEAM, VEC>(u, j, me);
+            v[j] = c < cols ? static_cast<const uint16_t*>(p)[row + c] : uint16_t{0};
+        }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+            f[j] = type == kTokF16 ? __half2float(__ushort_as_half(v[j])) : __uint_as_float(static_cast<uint32_t>(v[j]) << 16);
     }
 }
 template <int TEAM, bool VEC>
@@ -107,12 +117,13 @@ __device__ __forceinline__ void store8(void* p, int64_t row, int type, int u, in
     }
 }
 
-// Sum and maximum over the team; every thread gets them. red: a block's shared memory.
+// Sum and maximum over the team; every thread gets them. red: a block's shared memory. Teams inside a warp take part
+// together, as all lanes of a warp run through the same rows.
 template <int TEAM>
 __device__ __forceinline__ float team_sum(float v, float* red) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (TEAM == 32) return v;
+    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (TEAM <= 32) return v;
     if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
     __syncthreads();
     v = threadIdx.x % 32 < TEAM / 32 ? red[threadIdx.x % 32] : 0.f;
@@ -122,6 +133,11 @@ __device__ __forceinline__ float team_sum(float v, float* red) {
 }
 template <int TEAM>
 __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
+    if (TEAM < 32) {
+#pragma unroll
+        for (int o = TEAM / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
     v = __reduce_max_sync(0xffffffffu, v);
     if (TEAM == 32) return v;
     if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
@@ -129,9 +145,9 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
     return __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32 < TEAM / 32 ? threadIdx.x % 32 : 0]);
 }
 
-// From a row's h on: the norm, the scale, the output. red: three rows of 32 floats that no thread of the team still reads.
+// From a row's h on: the norm, the scale, the output; cols 0: no row, nothing is stored. red: three rows of 32 floats that no thread of the team still reads.
 template <int TEAM, int TURNS, bool VEC>
-__device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, int me, float (&h)[TURNS][kVec], float (*red)[32]) {
+__device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, int me, int cols, float (&h)[TURNS][kVec], float (*red)[32]) {
     float ss = 0.f;
 #pragma unroll
     for (int u = 0; u < TURNS; ++u)
@@ -139,8 +155,10 @@ __device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, in
         for (int j = 0; j < kVec; ++j) ss = fmaf(h[u][j], h[u][j], ss);
     ss = team_sum<TEAM>(ss, red[0]);
     float pre = 1.f;
-    if (!(ss < 3.0e38f)) {  // squares past f32's range (or a NaN or infinity, which stays one): sum smaller ones
-        pre = 8.2718061e-25f;  // 2^-80
+    // squares past f32's range (or a NaN or infinity, which stays one): sum smaller ones
+    const bool past = !(ss < 3.0e38f);
+    if (TEAM < 32 ? __any_sync(0xffffffffu, past) : past) {
+        if (past) pre = 8.2718061e-25f;  // 2^-80
         ss = 0.f;
 #pragma unroll
         for (int u = 0; u < TURNS; ++u)
@@ -170,7 +188,7 @@ __device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, in
         // as bits a NaN is above every number
         const uint32_t most = team_max<TEAM>(__float_as_uint(top * r) & 0x7fffffffu, reinterpret_cast<uint32_t*>(red[2]));
         const float scale = __uint_as_float(max(most, __float_as_uint(1e-30f))) * (1.f / 448.f);
-        if (me == 0) a.scale[row] = scale;
+        if (me == 0 && cols) a.scale[row] = scale;
         times = r * (1.f / scale);
     } else if (a.scale_mode == kScaleTensor) {
         times = r * (1.f / a.scale[0]);
@@ -179,7 +197,7 @@ __device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, in
     for (int u = 0; u < TURNS; ++u) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j) h[u][j] *= times;
-        store8<TEAM, VEC>(a.y, row * a.y_stride, a.y_type, u, me, a.cols, h[u]);
+        store8<TEAM, VEC>(a.y, row * a.y_stride, a.y_type, u, me, cols, h[u]);
     }
 }
 
@@ -206,15 +224,15 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_kernel(const
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) store8<TEAM, VEC>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
     }
-    finish_row<TEAM, TURNS, VEC>(a, row, me, h, red);
+    finish_row<TEAM, TURNS, VEC>(a, row, me, a.cols, h, red);
 }
 
 // Many rows of 16-bit x (and residual): the blocks stay and walk over the rows, a row's values on their way while the row
 // before it is worked on, so that memory does not wait for the reductions.
 template <int TEAM, int TURNS, bool RES>
-__global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_stream_kernel(const __grid_constant__ RmsNormArgs a) {
+__global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) rms_norm_stream_kernel(const __grid_constant__ RmsNormArgs a) {
     __shared__ float red[2][3][32];
-    const int me = threadIdx.x % TEAM, per = TEAM == 32 ? blockDim.x / 32 : 1;
+    const int me = threadIdx.x % TEAM, per = TEAM <= 32 ? 128 / TEAM : 1;
     const int64_t step = static_cast<int64_t>(gridDim.x) * per;
     int64_t row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / TEAM;
     uint4 x[TURNS], r[RES ? TURNS : 1];
@@ -228,7 +246,9 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_stream_kerne
         }
     };
     fetch(row);
-    for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
+    int turn = 0;
+    const int64_t first = TEAM < 32 ? row - threadIdx.x % 32 / TEAM : row;  // of the warp's teams: they end together
+    for (int64_t lead = first; lead < a.rows; lead += step, row += step, turn ^= 1) {
         float h[TURNS][kVec];
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
@@ -245,11 +265,12 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) rms_norm_stream_kerne
             }
         }
         fetch(row + step);
+        const int cols = TEAM < 32 && row >= a.rows ? 0 : a.cols;  // a team past the last row stores nothing
         if (a.sum) {
 #pragma unroll
-            for (int u = 0; u < TURNS; ++u) store8<TEAM, true>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
+            for (int u = 0; u < TURNS; ++u) store8<TEAM, true>(a.sum, row * a.sum_stride, a.residual_type, u, me, cols, h[u]);
         }
-        finish_row<TEAM, TURNS, true>(a, row, me, h, red[turn]);  // a row's barrier lies between two uses of a half of red
+        finish_row<TEAM, TURNS, true>(a, row, me, cols, h, red[turn]);  // a row's barrier lies between two uses of a half of red
     }
 }
 
@@ -268,7 +289,7 @@ cudaError_t launch(const RmsNormArgs& a, bool vec, cudaStream_t s) {
 template <int TEAM, int TURNS, bool RES>
 cudaError_t launch_stream(const RmsNormArgs& a, cudaStream_t s) {
     auto* kern = rms_norm_stream_kernel<TEAM, TURNS, RES>;
-    constexpr int threads = TEAM == 32 ? 128 : TEAM, per = threads / TEAM;
+    constexpr int threads = TEAM <= 32 ? 128 : TEAM, per = threads / TEAM;
     static std::atomic<int> known;  // blocks that are resident at once on an SM; the same on every sm_100
     int resident = known.load(std::memory_order_relaxed);
     if (!resident) {
@@ -297,8 +318,13 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
                      ok(a.sum, a.sum_stride, a.residual_type) && ok(a.weight, 0, a.weight_type) && ok(a.y, a.y_stride, a.y_type);
     const bool few = a.rows <= 148 * 2;
     if (vec && !few && a.x_type != kTokF32 && (!a.residual || a.residual_type != kTokF32)) {
-        if (a.cols <= 256) return launch_stream<32, 1>(a, s);
-        if (a.cols <= 512) return launch_stream<32, 2>(a, s);
+        // narrow rows: several to a warp, so that its lanes are busy and have loads enough on their way (200003 x 320 bf16
+        // to bf16: 50 us, 69 with a warp a row)
+        if (a.cols <= 64) return launch_stream<8, 1>(a, s);
+        if (a.cols <= 128) return launch_stream<8, 2>(a, s);
+        if (a.cols <= 256) return launch_stream<8, 4>(a, s);
+        if (a.cols <= 320) return launch_stream<8, 5>(a, s);
+        if (a.cols <= 512) return launch_stream<16, 4>(a, s);
         if (a.cols <= 1024) return launch_stream<32, 4>(a, s);
         if (a.cols <= 2048) return launch_stream<128, 2>(a, s);
         if (a.cols <= 4096) return launch_stream<256, 2>(a, s);

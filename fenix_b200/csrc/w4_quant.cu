@@ -134,10 +134,9 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __res
     }
 }
 
-constexpr int kWords = 4;  // of a thread, kThreads apart
-
-// A word of eight codes makes eight consecutive values. A code is or'ed into the mantissa of 2^23.
-template <bool VEC>
+// A word of eight codes makes eight consecutive values; a thread takes kWords of them, kThreads apart. A code is or'ed
+// into the mantissa of 2^23.
+template <bool VEC, int kWords>
 __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const W4Args q, void* __restrict__ w, int w_type, int64_t w_stride, int row0) {
     const int row = row0 + blockIdx.y, words = q.k / kEight;  // of the row
     const float inv = __frcp_rn(static_cast<float>(q.group / kEight));
@@ -231,14 +230,17 @@ cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, cons
 
 cudaError_t launch_w4_dequantize(const W4Args& q, void* w, int w_type, int64_t w_stride, cudaStream_t s) {
     constexpr int kRows = 65535;  // of a launch
-    const unsigned across = (q.k / kEight + kThreads * kWords - 1) / (kThreads * kWords);
+    // 16-bit values: four words a thread (4096 x 14336: 35 us, 39 with one); f32 ones fill a thread's stores alone
+    // (8192 x 8192: 60 us, 69 with four)
+    const int words = w_type == kTokF32 ? 1 : 4;
+    const bool vec = aligned_rows(w, w_stride, w_type);
+    const unsigned across = (q.k / kEight + kThreads * words - 1) / (kThreads * words);
     for (int row0 = 0; row0 < q.n; row0 += kRows) {
         const dim3 grid(across, static_cast<unsigned>(q.n - row0 < kRows ? q.n - row0 : kRows));
+        auto* kern = words == 1 ? (vec ? w4_dequantize_kernel<true, 1> : w4_dequantize_kernel<false, 1>)
+                                : (vec ? w4_dequantize_kernel<true, 4> : w4_dequantize_kernel<false, 4>);
         count_launch();
-        if (aligned_rows(w, w_stride, w_type))
-            w4_dequantize_kernel<true><<<grid, kThreads, 0, s>>>(q, w, w_type, w_stride, row0);
-        else
-            w4_dequantize_kernel<false><<<grid, kThreads, 0, s>>>(q, w, w_type, w_stride, row0);
+        kern<<<grid, kThreads, 0, s>>>(q, w, w_type, w_stride, row0);
         if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     }
     return cudaSuccess;
