@@ -123,26 +123,30 @@ template <int TEAM>
 __device__ __forceinline__ float team_sum(float v, float* red) {
 #pragma unroll
     for (int o = (TEAM < 32 ? TEAM : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (TEAM <= 32) return v;
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = threadIdx.x % 32 < TEAM / 32 ? red[threadIdx.x % 32] : 0.f;
+    if constexpr (TEAM > 32) {
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = threadIdx.x % 32 < TEAM / 32 ? red[threadIdx.x % 32] : 0.f;
 #pragma unroll
-    for (int o = TEAM / 64; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return __shfl_sync(0xffffffffu, v, 0);
+        for (int o = TEAM / 64; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        v = __shfl_sync(0xffffffffu, v, 0);
+    }
+    return v;
 }
 template <int TEAM>
 __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
-    if (TEAM < 32) {
+    if constexpr (TEAM < 32) {
 #pragma unroll
         for (int o = TEAM / 2; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-        return v;
+    } else {
+        v = __reduce_max_sync(0xffffffffu, v);
     }
-    v = __reduce_max_sync(0xffffffffu, v);
-    if (TEAM == 32) return v;
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
-    __syncthreads();
-    return __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32 < TEAM / 32 ? threadIdx.x % 32 : 0]);
+    if constexpr (TEAM > 32) {
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = __reduce_max_sync(0xffffffffu, red[threadIdx.x % 32 < TEAM / 32 ? threadIdx.x % 32 : 0]);
+    }
+    return v;
 }
 
 // From a row's h on: the norm, the scale, the output; cols 0: no row, nothing is stored. red: three rows of 32 floats that no thread of the team still reads.

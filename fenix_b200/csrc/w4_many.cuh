@@ -27,12 +27,13 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
            static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
 
-// D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, f32 accumulate.
-__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, f32 accumulate: every lane runs the code, on warp-uniform
+// operands, and the lane with issue != 0 executes it.
+__device__ __forceinline__ void mma_f16_ta_if(uint32_t issue, uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
         : "memory");
 }
 // Eight 32-bit columns of this thread's TMEM lane.
@@ -212,33 +213,32 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
         __syncwarp();
     } else if (warp == 17) {
         const uint32_t idesc = instr_desc(128, 0, BF ? kOpBF16 : kOpF16) | static_cast<uint32_t>(tile_n >> 3) << 17;
+        // All of TMEM is this block's, so its first column is 0, a constant that the issuing loop has at no cost; it keeps
+        // to warp-uniform values throughout, as its own time bounds short steps.
+        if (tmem != 0) gave_up(kStatusBadTmem);
+        const uint32_t issue = elect_one();
         int ws = 0, xs = 0, x_step = 0;
         uint32_t wp = 0, xp = 0;
         for (int step = 0; step < steps; ++step) {
             if (x_step == 0 && !wait_phase(x_full + 8 * xs, xp, &abort_flag)) gave_up(kStatusTimeoutFull);
             if (!wait_phase(w_full + 8 * ws, wp, &abort_flag)) gave_up(kStatusTimeoutFull);
             tc_fence_after();
-            const bool x_last = x_step == kSlotSteps - 1 || step == steps - 1;
-            if (elect_one()) {
-                const uint64_t bd = desc_sw128(xrows + (xs * kSlotSteps + x_step) * tile_n * 128);
+            const uint64_t bd = desc_sw128(xrows + (xs * kSlotSteps + x_step) * tile_n * 128);
 #pragma unroll
-                for (int m = 0; m < (TWO ? 2 : 1); ++m) {
-                    const uint32_t ad = weights + (ws * (TWO ? 2 : 1) + m) * 32;
+            for (int m = 0; m < (TWO ? 2 : 1); ++m) {
+                const uint32_t ad = plan.weight_col + (ws * (TWO ? 2 : 1) + m) * 32;
 #pragma unroll
-                    for (int i = 0; i < kStepK / 16; ++i)
-                        mma_f16_ta(tmem + m * tile_n, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0);
-                }
-                mma_commit(w_empty + 8 * ws);
-                if (x_last) mma_commit(x_empty + 8 * xs);
-                if (step == steps - 1) mma_commit(done);
+                for (int i = 0; i < kStepK / 16; ++i) mma_f16_ta_if(issue, m * tile_n, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0);
             }
-            __syncwarp();
+            mma_commit_if(issue, w_empty + 8 * ws);
             if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
-            if (++x_step == kSlotSteps) {
+            if (++x_step == kSlotSteps || step == steps - 1) {
+                mma_commit_if(issue, x_empty + 8 * xs);
                 x_step = 0;
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
         }
+        if (steps) mma_commit_if(issue, done);
     } else if (!XS && warp >= 18) {
         // rows that TMA does not bring as they are used: four warps write them in 16-byte cells of eight values, as the
         // swizzle places them
