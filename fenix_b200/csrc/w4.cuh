@@ -14,7 +14,7 @@ constexpr int kSmemMax = 226 * 1024;
 struct ManyPlan {
     int tile_n;           // rows of a tile: a multiple of 16, at most 256
     int rings[3];         // stages of codes, weights, rows; at most kMaxRing
-    int codes, rows, raw, row_factor;  // offsets in shared memory
+    int codes, rows, raw, tops;  // offsets in shared memory
     int bytes;
     int split;            // blocks of a cluster that share a tile, each with a range of k
     int stages_each;      // stages of codes of a block
@@ -22,8 +22,8 @@ struct ManyPlan {
     int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
     int raw_slots;        // of e4m3 rows by TMA, 128 inputs each
     bool y_vec;           // results aligned to eight outputs
-    int x_steps;          // steps of 64 inputs of a slot that TMA fills with rows as they are; 0: warps write the rows
-    bool x_vec;           // rows aligned to eight values
+    int slot_steps;       // steps of 64 inputs that share a slot of the rows' ring
+    bool x_tma, x_vec;    // rows come by TMA as they are; rows aligned to eight values
     bool two;             // tiles of 256 outputs
 };
 

@@ -9,7 +9,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     ManyPlan p{};
     const int64_t xb = a.x_type == kTokE4M3 ? 1 : 2;
     p.x_vec = reinterpret_cast<uintptr_t>(a.x) % (8 * xb) == 0 && a.x_stride % 8 == 0;
-    const bool x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
+    p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
     p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride % 8 == 0;
     p.raw_slots = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0 ? 2 : 0;
     const bool two = p.two = (a.w.n + 255) / 256 * ((a.rows + 191) / 192) >= sms;
@@ -27,9 +27,11 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.tmem_cols = 512;
     p.rings[1] = std::min((p.tmem_cols - p.weight_col) / (two ? 64 : 32), kMaxRing);
     // shared memory: codes and rows in turn
-    p.x_steps = !x_tma ? 0 : !two && p.tile_n <= 64 ? 4 : 1;
-    const int factor_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128 * std::max(p.x_steps, 1);
-    int room = kSmemMax - factor_bytes - 2 * w - 2 * x - p.raw_slots * p.tile_n * 128;
+    // short steps: four to a slot, for fewer waits
+    p.slot_steps = !two && p.tile_n <= 64 ? 4 : 1;
+    if (p.raw_slots && p.slot_steps == 4) p.raw_slots = 4;
+    const int tops_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128 * p.slot_steps;
+    int room = kSmemMax - tops_bytes - 2 * w - 2 * x - p.raw_slots * p.tile_n * 128;
     p.rings[0] = p.rings[2] = 2;
     for (bool more = true; more;) {
         more = false;
@@ -45,13 +47,13 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.codes = 0;
     p.rows = p.rings[0] * w;
     p.raw = p.rows + p.rings[2] * x;
-    p.row_factor = p.raw + p.raw_slots * p.tile_n * 128;
-    p.bytes = p.row_factor + factor_bytes;
+    p.tops = p.raw + p.raw_slots * p.tile_n * 128;
+    p.bytes = p.tops + tops_bytes;
     if (p.split > 1) {  // the partial sums lie over the rings
         const int partial = p.tile_n * tile_m * 4;
-        if (partial > p.row_factor) {
-            p.row_factor = partial;
-            p.bytes = partial + factor_bytes;
+        if (partial > p.tops) {
+            p.tops = partial;
+            p.bytes = partial + tops_bytes;
         }
     }
     return a.x_type == kTokBF16 ? w4_many_bf16(a, p, s) : w4_many_f16(a, p, s);

@@ -123,20 +123,20 @@ __device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi,
 // TWO: 256 outputs a tile in two accumulators, else 128.
 constexpr int kMakers = 16;
 
-// XS: steps of 64 inputs that share a slot of the rows' ring (a constant: the issuing thread has no time to spare), 0: one,
-// written by four warps.
+// TMA: the rows come as they are, else four warps write them. SS: steps of 64 inputs that share a slot of the rows' ring (a
+// constant: the issuing thread has no time to spare).
 // CH: scales of a step of 64 inputs (1: groups are multiples of 64). EX: the scales' type is the
 // operands', so that they have no second term (in f16 but for those 2^14 below their output's largest, whose last bits
 // are 2^-25 of it).
-template <bool BF, bool TWO, int XS, int CH, bool EX>
-__global__ void __launch_bounds__(XS ? 608 : 704, 1)
+template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX>
+__global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
                    const __grid_constant__ CUtensorMap rows_map) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[7 * kMaxRing + 1];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int abort_flag;
-    constexpr int kTileM = TWO ? 256 : 128, kSlotSteps = XS ? XS : 1, kRowWarps = 4;
+    constexpr int kTileM = TWO ? 256 : 128, kRowWarps = 4;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int n = a.w.n, k = a.w.k, group = a.w.group, groups = k / group;
     const int tile_n = plan.tile_n, rank = plan.split > 1 ? static_cast<int>(blockIdx.x) % plan.split : 0;
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
             mbar_init(c_empty + 8 * i, kMakers);
             mbar_init(w_full + 8 * i, TWO ? 8 : 4);
             mbar_init(w_empty + 8 * i, 1);
-            mbar_init(x_full + 8 * i, XS ? 1 : kRowWarps);
+            mbar_init(x_full + 8 * i, TMA ? 1 : kRowWarps);
             mbar_init(raw_full + 8 * i, 1);
             mbar_init(x_empty + 8 * i, 1);
         }
@@ -193,17 +193,17 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
                 for (int i = 0; i < plan.rings[0]; ++i) wait_phase(c_full + 8 * i, (i < cs ? cp : cp ^ 1), nullptr);
         }
         __syncwarp();
-    } else if (XS && warp == 18) {  // not the codes' thread: neither ring's waits hold up the other
+    } else if (TMA && warp == 18) {  // not the codes' thread: neither ring's waits hold up the other
         if (lane == 0) {
             int xs = 0;
             uint32_t xp = 0;
-            for (int step = 0; step < steps; step += kSlotSteps) {
-                const int boxes = min(kSlotSteps, steps - step);
+            for (int step = 0; step < steps; step += SS) {
+                const int boxes = min(SS, steps - step);
                 if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
                 if (abort_flag) break;
                 mbar_arrive_expect_tx(x_full + 8 * xs, boxes * tile_n * 128);
                 for (int i = 0; i < boxes; ++i)
-                    tma_load_2d(xrows + (xs * kSlotSteps + i) * tile_n * 128, &rows_map, k_begin + (step + i) * kStepK, static_cast<int>(r0),
+                    tma_load_2d(xrows + (xs * SS + i) * tile_n * 128, &rows_map, k_begin + (step + i) * kStepK, static_cast<int>(r0),
                                 x_full + 8 * xs);
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
             if (x_step == 0 && !wait_phase(x_full + 8 * xs, xp, &abort_flag)) gave_up(kStatusTimeoutFull);
             if (!wait_phase(w_full + 8 * ws, wp, &abort_flag)) gave_up(kStatusTimeoutFull);
             tc_fence_after();
-            const uint64_t bd = desc_sw128(xrows + (xs * kSlotSteps + x_step) * tile_n * 128);
+            const uint64_t bd = desc_sw128(xrows + (xs * SS + x_step) * tile_n * 128);
 #pragma unroll
             for (int m = 0; m < (TWO ? 2 : 1); ++m) {
                 const uint32_t ad = plan.weight_col + (ws * (TWO ? 2 : 1) + m) * 32;
@@ -232,71 +232,75 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
             }
             mma_commit_if(issue, w_empty + 8 * ws);
             if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
-            if (++x_step == kSlotSteps || step == steps - 1) {
+            if (++x_step == SS || step == steps - 1) {
                 mma_commit_if(issue, x_empty + 8 * xs);
                 x_step = 0;
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
         }
         if (steps) mma_commit_if(issue, done);
-    } else if (!XS && warp >= 18) {
+    } else if (!TMA && warp >= 18) {
         // rows that TMA does not bring as they are used: four warps write them in 16-byte cells of eight values, as the
         // swizzle places them
-        const int tid = threadIdx.x - 18 * 32;
+        // (a step each where four share a slot, so that a step's latency is hidden behind the others', else together)
+        constexpr bool kApart = SS == kRowWarps;
+        const int tid = threadIdx.x - 18 * 32, kxb = a.x_type == kTokE4M3 ? 1 : 2;
+        const int from = kApart ? lane : tid, by = kApart ? 32 : kRowWarps * 32;
         int xs = 0, rs = 0;
         uint32_t xp = 0, rp = 0;
-        if (plan.raw_slots) {  // e4m3: TMA brings 128 inputs at a time, these warps widen them
-            auto fetch = [&](int step, int slot) {
-                if (tid == 0 && step < steps) {
-                    mbar_arrive_expect_tx(raw_full + 8 * slot, tile_n * 128);
-                    tma_load_2d(smem_u32(smem + plan.raw) + slot * tile_n * 128, &rows_map, (k_begin + step * kStepK) / 8, static_cast<int>(r0),
-                                raw_full + 8 * slot);
-                }
-            };
+        auto fetch = [&](int step, int slot) {  // e4m3: TMA brings 128 inputs at a time, these warps widen them
+            if (step < steps) {
+                mbar_arrive_expect_tx(raw_full + 8 * slot, tile_n * 128);
+                tma_load_2d(smem_u32(smem + plan.raw) + slot * tile_n * 128, &rows_map, (k_begin + step * kStepK) / 8, static_cast<int>(r0),
+                            raw_full + 8 * slot);
+            }
+        };
+        if (tid == 0)
             for (int i = 0; i < plan.raw_slots; ++i) fetch(2 * i, i);
-            for (int step = 0; step < steps; ++step) {
-                if (step % 2 == 0 && !wait_phase(raw_full + 8 * rs, rp, &abort_flag)) gave_up(kStatusTimeoutFull);
-                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+        for (int step0 = 0; step0 < steps; step0 += SS) {
+            const int step = step0 + (kApart ? tid / 32 : 0), pair = step / 2;
+            if (plan.raw_slots) rs = pair % plan.raw_slots, rp = pair / plan.raw_slots & 1;
+            if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+            uint8_t* const to = smem + plan.rows + (xs * SS + step - step0) * tile_n * 128;
+            if (step < steps && plan.raw_slots) {
+                if (!wait_phase(raw_full + 8 * rs, rp, &abort_flag)) gave_up(kStatusTimeoutFull);
                 const uint8_t* const raw = smem + plan.raw + rs * tile_n * 128;
-                uint8_t* const to = smem + plan.rows + xs * tile_n * 128;
 #pragma unroll 4
-                for (int i = tid; i < tile_n * 4; i += kRowWarps * 32) {
+                for (int i = from; i < tile_n * 4; i += by) {
                     const int r = i / 4, c = i % 4;
                     const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 128 + (((4 * (step % 2) + c) ^ (r & 7)) << 4));
                     *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = widened(v, kTokE4M3);
                     *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = widened(make_uint4(v.z, v.w, 0, 0), kTokE4M3);
                 }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(x_full + 8 * xs);
-                if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
-                if (step % 2) {
-                    asm volatile("bar.sync 2, %0;" ::"n"(kRowWarps * 32) : "memory");  // all of them have read the slot
-                    fetch(step - 1 + 2 * plan.raw_slots, rs);
-                    if (++rs == plan.raw_slots) rs = 0, rp ^= 1;
-                }
-            }
-            if (abort_flag)  // copies still on their way
-                for (int i = 0; i < plan.raw_slots; ++i) wait_phase(raw_full + 8 * i, i < rs ? rp ^ 1 : rp, nullptr);
-        } else {  // value by value
-            const int kxb = a.x_type == kTokE4M3 ? 1 : 2;
-            for (int step = 0; step < steps; ++step) {
+            } else if (step < steps) {
                 const int k0 = k_begin + step * kStepK;
                 const uint8_t* const src = static_cast<const uint8_t*>(a.x) + (r0 * a.x_stride + k0) * kxb;
-                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
 #pragma unroll 2
-                for (int i = tid; i < tile_n * 8; i += kRowWarps * 32) {
+                for (int i = from; i < tile_n * 8; i += by) {
                     const int r = i / 8, c = i % 8;
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (r < rows && k0 + c * 8 < k_end) v = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
-                    *reinterpret_cast<uint4*>(smem + plan.rows + xs * tile_n * 128 + r * 128 + ((c ^ (r & 7)) << 4)) = widened(v, a.x_type);
+                    *reinterpret_cast<uint4*>(to + r * 128 + ((c ^ (r & 7)) << 4)) = widened(v, a.x_type);
                 }
-                fence_async_shared();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(x_full + 8 * xs);
-                if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(x_full + 8 * xs);
+            if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
+            if (plan.raw_slots && (kApart || step % 2)) {  // the slot's readers (two warps, or all) are done with it
+                if (kApart)
+                    asm volatile("bar.sync %0, 64;" ::"r"(2 + tid / 64) : "memory");
+                else
+                    asm volatile("bar.sync 2, %0;" ::"n"(kRowWarps * 32) : "memory");
+                if (kApart ? tid % 64 == 0 : tid == 0) fetch(step / 2 * 2 + 2 * plan.raw_slots, rs);
             }
         }
+        __syncwarp();
+        if (abort_flag)  // copies still on their way: either phase may be the last that was asked for
+            for (int i = 0; i < plan.raw_slots; ++i) {
+                wait_phase(raw_full + 8 * i, 0, nullptr);
+                wait_phase(raw_full + 8 * i, 1, nullptr);
+            }
     } else {
         // a thread makes weights of one output, whose TMEM lane is its own; the four warps of a lane quarter take the steps
         // in turn (with two tiles, two warps a tile), so that a step's latency is hidden behind the others'
@@ -305,35 +309,38 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
         const int64_t at = static_cast<int64_t>(min(o0 + row, n - 1)) * groups;
         const bool wide = a.w.scale_type == kTokF32, is_f16 = a.w.scale_type == kTokF16;
         auto scale_at = [&](int g) { return tok_load(a.w.scales, at + g, a.w.scale_type); };
-        float factor = 1.f;  // reciprocal of the output's power of two
-        float* const factors = reinterpret_cast<float*>(smem + plan.row_factor);
+        float back = 1.f, factor = 1.f;  // the output's power of two, and its reciprocal
         if (!BF) {
+            // the warps of a lane quarter look through a share of the scales each
+            uint32_t* const tops = reinterpret_cast<uint32_t*>(smem + plan.tops);
+            if (set == 0) tops[row] = 0;
+            asm volatile("bar.sync 1, %0;" ::"n"(kMakers * 32) : "memory");
             float top = 0.f;
             const uint8_t* const p = static_cast<const uint8_t*>(a.w.scales) + at * (wide ? 4 : 2);
-            int g = 0;
             if (!wide && groups % 8 == 0 && reinterpret_cast<uintptr_t>(a.w.scales) % 16 == 0) {
 #pragma unroll 4
-                for (; g < groups; g += 8) {
+                for (int g = set * 8; g < groups; g += kSets * 8) {
                     const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + g * 2));
                     const uint32_t r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const uint32_t h = (i % 2 ? r[i / 2] >> 16 : r[i / 2]) & 0x7fffu;
-                        top = fmaxf(top, a.w.scale_type == kTokF16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16));
+                        top = fmaxf(top, is_f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16));
                     }
                 }
-            }
+            } else {
 #pragma unroll 8
-            for (; g < groups; ++g) top = fmaxf(top, fabsf(scale_at(g)));
+                for (int g = set; g < groups; g += kSets) top = fmaxf(top, fabsf(scale_at(g)));
+            }
+            atomicMax(tops + row, __float_as_uint(top));  // of numbers that are not negative the bits are in order
+            asm volatile("bar.sync 1, %0;" ::"n"(kMakers * 32) : "memory");
+            top = __uint_as_float(tops[row]);
             // 2^e <= top < 2^(e + 1), e kept where 2^e and 2^-e are normal; an infinity or zero keeps 1
-            float back = 1.f;
             if (top > 0.f && top < INFINITY) {
                 const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -126), 126);
                 back = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
                 factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
             }
-            if (set == 0) factors[row] = back;
-            asm volatile("bar.sync 1, %0;" ::"n"(kMakers * 32) : "memory");
         }
         // scales, as they are stored, and zero points of a stage's steps, a stage ahead
         constexpr int kMine = kStageK / kStepK / kSets;
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
         if (steps && !wait_phase(done, 0, &abort_flag)) gave_up(kStatusTimeoutAcc);
         tc_fence_after();
         const int out = o0 + row;
-        const float back = BF ? 1.f : factors[row], bias = a.bias && out < n ? a.bias[out] : 0.f;
+        const float bias = a.bias && out < n ? a.bias[out] : 0.f;
         const uint32_t acc = tmem + (TWO ? part / 2 * tile_n : 0) + (static_cast<uint32_t>(quad * 32) << 16);
         float* const partial = reinterpret_cast<float*>(smem);  // [row][output], over the rings
         // sixteen rows at a time; 16-bit results change places in shared memory (over the rings), so that a store is eight
@@ -499,14 +506,14 @@ __global__ void __launch_bounds__(XS ? 608 : 704, 1)
     }
 }
 
-template <bool BF, bool TWO, int XS, int CH, bool EX>
+template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     constexpr int kTileM = TWO ? 256 : 128;
-    auto* kern = w4_many_kernel<BF, TWO, XS, CH, EX>;
+    auto* kern = w4_many_kernel<BF, TWO, TMA, SS, CH, EX>;
     CUtensorMap codes, rows;
     cudaError_t e = tmap_rows(&codes, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kTileM);
     if (e == cudaSuccess) {
-        if (XS)
+        if (TMA)
             e = tmap_rows(&rows, a.x, 2, a.w.k, a.rows, a.x_stride * 2, p.tile_n);
         else if (p.raw_slots)
             e = tmap_rows(&rows, a.x, 8, a.w.k / 8, a.rows, a.x_stride, p.tile_n);
@@ -517,7 +524,7 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((a.w.n + kTileM - 1) / kTileM * p.split, (a.rows + p.tile_n - 1) / p.tile_n);
-    cfg.blockDim = dim3(XS ? 19 * 32 : 22 * 32);
+    cfg.blockDim = dim3(TMA ? 19 * 32 : 22 * 32);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
@@ -531,16 +538,17 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-template <bool BF, bool TWO, int XS>
+template <bool BF, bool TWO, bool TMA, int SS>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     const bool exact = a.w.scale_type == (BF ? kTokBF16 : kTokF16);
-    if (a.w.group % kStepK == 0) return exact ? launch<BF, TWO, XS, 1, true>(a, p, s) : launch<BF, TWO, XS, 1, false>(a, p, s);
-    return exact ? launch<BF, TWO, XS, 2, true>(a, p, s) : launch<BF, TWO, XS, 2, false>(a, p, s);
+    if (a.w.group % kStepK == 0) return exact ? launch<BF, TWO, TMA, SS, 1, true>(a, p, s) : launch<BF, TWO, TMA, SS, 1, false>(a, p, s);
+    return exact ? launch<BF, TWO, TMA, SS, 2, true>(a, p, s) : launch<BF, TWO, TMA, SS, 2, false>(a, p, s);
 }
 template <bool BF>
 cudaError_t launch_typed(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
-    if (p.two) return p.x_steps ? launch<BF, true, 1>(a, p, s) : launch<BF, true, 0>(a, p, s);
-    return p.x_steps == 4 ? launch<BF, false, 4>(a, p, s) : p.x_steps ? launch<BF, false, 1>(a, p, s) : launch<BF, false, 0>(a, p, s);
+    if (p.two) return p.x_tma ? launch<BF, true, true, 1>(a, p, s) : launch<BF, true, false, 1>(a, p, s);
+    if (p.slot_steps == 1) return p.x_tma ? launch<BF, false, true, 1>(a, p, s) : launch<BF, false, false, 1>(a, p, s);
+    return p.x_tma ? launch<BF, false, true, 4>(a, p, s) : launch<BF, false, false, 4>(a, p, s);
 }
 
 }  // namespace
