@@ -9,6 +9,7 @@ namespace fxk {
 constexpr int kStageK = 256;  // inputs of a stage of codes: 128 bytes an output
 constexpr int kStepK = 64;    // inputs of a stage of operands: 128 bytes of 16-bit values a row
 constexpr int kMaxRing = 8;
+constexpr int kRowWarps = 4;  // that write rows which TMA does not bring
 constexpr int kSmemMax = 226 * 1024;
 
 struct ManyPlan {

@@ -31,8 +31,12 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.slot_steps = !two && p.tile_n <= 64 ? 4 : 1;
     if (p.raw_slots && p.slot_steps == 4) p.raw_slots = 4;
     const int tops_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128 * p.slot_steps;
-    int room = kSmemMax - tops_bytes - 2 * w - 2 * x - p.raw_slots * p.tile_n * 128;
-    p.rings[0] = p.rings[2] = 2;
+    // Warps that write a slot each, taking steps in turn, tell a slot's uses apart by parity: a ring as long as they are
+    // many keeps one that runs ahead from meeting a slot two uses behind.
+    p.rings[0] = 2;
+    p.rings[2] = !p.x_tma && p.slot_steps == 1 ? kRowWarps : 2;
+    int room = kSmemMax - tops_bytes - p.rings[0] * w - p.rings[2] * x - p.raw_slots * p.tile_n * 128;
+    if (room < 0) return cudaErrorInvalidConfiguration;
     for (bool more = true; more;) {
         more = false;
         for (int i : {2, 0}) {

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     __shared__ __align__(8) uint64_t bars[7 * kMaxRing + 1];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int abort_flag;
-    constexpr int kTileM = TWO ? 256 : 128, kRowWarps = 4;
+    constexpr int kTileM = TWO ? 256 : 128;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int n = a.w.n, k = a.w.k, group = a.w.group, groups = k / group;
     const int tile_n = plan.tile_n, rank = plan.split > 1 ? static_cast<int>(blockIdx.x) % plan.split : 0;
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             mbar_init(c_empty + 8 * i, kMakers);
             mbar_init(w_full + 8 * i, TWO ? 8 : 4);
             mbar_init(w_empty + 8 * i, 1);
-            mbar_init(x_full + 8 * i, TMA ? 1 : kRowWarps);
+            mbar_init(x_full + 8 * i, TMA ? 1 : SS);  // SS warps write a slot
             mbar_init(raw_full + 8 * i, 1);
             mbar_init(x_empty + 8 * i, 1);
         }
@@ -242,12 +242,9 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     } else if (!TMA && warp >= 18) {
         // rows that TMA does not bring as they are used: four warps write them in 16-byte cells of eight values, as the
         // swizzle places them
-        // (a step each where four share a slot, so that a step's latency is hidden behind the others', else together)
-        constexpr bool kApart = SS == kRowWarps;
+        // (a step each, so that a step's latency is hidden behind the others')
+        static_assert(SS == 1 || SS == kRowWarps, "a slot is one warp's or all warps'");
         const int tid = threadIdx.x - 18 * 32, kxb = a.x_type == kTokE4M3 ? 1 : 2;
-        const int from = kApart ? lane : tid, by = kApart ? 32 : kRowWarps * 32;
-        int xs = 0, rs = 0;
-        uint32_t xp = 0, rp = 0;
         auto fetch = [&](int step, int slot) {  // e4m3: TMA brings 128 inputs at a time, these warps widen them
             if (step < steps) {
                 mbar_arrive_expect_tx(raw_full + 8 * slot, tile_n * 128);
@@ -257,16 +254,18 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
         };
         if (tid == 0)
             for (int i = 0; i < plan.raw_slots; ++i) fetch(2 * i, i);
-        for (int step0 = 0; step0 < steps; step0 += SS) {
-            const int step = step0 + (kApart ? tid / 32 : 0), pair = step / 2;
-            if (plan.raw_slots) rs = pair % plan.raw_slots, rp = pair / plan.raw_slots & 1;
+        for (int step0 = 0; step0 < steps; step0 += kRowWarps) {
+            const int step = step0 + tid / 32, pair = step / 2, slots = plan.raw_slots ? plan.raw_slots : 1, rs = pair % slots;
+            if (SS == 1 && step >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
+            const int xs = step / SS % plan.rings[2];
+            const uint32_t xp = step / SS / plan.rings[2] & 1, rp = pair / slots & 1;
             if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
-            uint8_t* const to = smem + plan.rows + (xs * SS + step - step0) * tile_n * 128;
+            uint8_t* const to = smem + plan.rows + (xs * SS + step % SS) * tile_n * 128;
             if (step < steps && plan.raw_slots) {
                 if (!wait_phase(raw_full + 8 * rs, rp, &abort_flag)) gave_up(kStatusTimeoutFull);
                 const uint8_t* const raw = smem + plan.raw + rs * tile_n * 128;
 #pragma unroll 4
-                for (int i = from; i < tile_n * 4; i += by) {
+                for (int i = lane; i < tile_n * 4; i += 32) {
                     const int r = i / 4, c = i % 4;
                     const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 128 + (((4 * (step % 2) + c) ^ (r & 7)) << 4));
                     *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = widened(v, kTokE4M3);
@@ -276,7 +275,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                 const int k0 = k_begin + step * kStepK;
                 const uint8_t* const src = static_cast<const uint8_t*>(a.x) + (r0 * a.x_stride + k0) * kxb;
 #pragma unroll 2
-                for (int i = from; i < tile_n * 8; i += by) {
+                for (int i = lane; i < tile_n * 8; i += 32) {
                     const int r = i / 8, c = i % 8;
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (r < rows && k0 + c * 8 < k_end) v = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
@@ -286,13 +285,9 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(x_full + 8 * xs);
-            if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
-            if (plan.raw_slots && (kApart || step % 2)) {  // the slot's readers (two warps, or all) are done with it
-                if (kApart)
-                    asm volatile("bar.sync %0, 64;" ::"r"(2 + tid / 64) : "memory");
-                else
-                    asm volatile("bar.sync 2, %0;" ::"n"(kRowWarps * 32) : "memory");
-                if (kApart ? tid % 64 == 0 : tid == 0) fetch(step / 2 * 2 + 2 * plan.raw_slots, rs);
+            if (plan.raw_slots && pair * 2 + 2 * plan.raw_slots < steps) {  // another use: both warps are done with the raw slot
+                asm volatile("bar.sync %0, 64;" ::"r"(2 + tid / 64) : "memory");
+                if (tid % 64 == 0) fetch(pair * 2 + 2 * plan.raw_slots, rs);
             }
         }
         __syncwarp();

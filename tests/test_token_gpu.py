@@ -419,6 +419,21 @@ def test_linear_large(cuda_torch):
     run_linear(cuda_torch, 1500, 3000, 2048, 64, "e4m3", "f16", zeros=True, bias=True)
 
 
+@pytest.mark.parametrize("xt,zeros,group,offset", [("bf16", False, 128, 0), ("f16", True, 64, 0), ("e4m3", False, 128, 0),
+                                                   ("e4m3", True, 32, 0), ("e4m3", False, 64, 1), ("bf16", True, 32, 1)])
+def test_linear_tiles_that_fill_the_gpu(cuda_torch, xt, zeros, group, offset):
+    """Tiles of 256 outputs: more of them than SMs, ragged at both edges, rows by TMA, widened, and value by value."""
+    run_linear(cuda_torch, 2005, 5003, 1120 if group == 32 else 1152, group, xt, "f16" if xt == "f16" else "bf16", zeros=zeros,
+               bias=True, offset=offset)
+
+
+@pytest.mark.parametrize("xt,offset", [("bf16", 0), ("f16", 1), ("e4m3", 0), ("e4m3", 1)])
+def test_linear_inputs_over_a_cluster(cuda_torch, xt, offset):
+    """One tile of outputs and many inputs: a cluster shares it, some of its blocks without inputs of their own."""
+    for rows, k in ((9, 28672), (70, 8192 + 256), (250, 9 * 1024), (16, 4 * 1024 + 32 * 8)):
+        run_linear(cuda_torch, rows, 100, k, 32, xt, "bf16", zeros=True, bias=True, offset=offset)
+
+
 def test_linear_rows_past_32_bits(cuda_torch):
     torch = cuda_torch
     if torch.cuda.mem_get_info()[0] < 40 << 30:
