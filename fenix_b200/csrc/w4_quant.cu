@@ -134,38 +134,39 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __res
     }
 }
 
-// A word of eight codes makes eight consecutive values; a thread takes kWords of them, kThreads apart. A code is or'ed
+// A thread makes PIECES times N consecutive values (16 bytes of them where VEC), pieces kThreads apart. A code is or'ed
 // into the mantissa of 2^23.
-template <bool VEC, int kWords>
+template <bool VEC, int N, int PIECES>
 __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const W4Args q, void* __restrict__ w, int w_type, int64_t w_stride, int row0) {
-    const int row = row0 + blockIdx.y, words = q.k / kEight;  // of the row
-    const float inv = __frcp_rn(static_cast<float>(q.group / kEight));
-    const uint32_t* const codes = reinterpret_cast<const uint32_t*>(q.codes) + static_cast<int64_t>(row) * words;
+    const int row = row0 + blockIdx.y, pieces = q.k / N;  // of the row
+    const float inv = __frcp_rn(static_cast<float>(q.group / N));
+    const uint8_t* const codes = q.codes + static_cast<int64_t>(row) * (q.k / 2);
     const int64_t g0 = static_cast<int64_t>(row) * (q.k / q.group);
-    uint32_t c[kWords];
-    float s[kWords], off[kWords];
+    uint32_t c[PIECES];
+    float s[PIECES], off[PIECES];
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-        const int e = (blockIdx.x * kWords + i) * kThreads + threadIdx.x;
-        if (e >= words) continue;
-        c[i] = __ldcs(codes + e);
-        const int64_t g = g0 + static_cast<int>((static_cast<float>(e) + 0.5f) * inv);  // exact while e < 2^21, as k < 2^24
+    for (int i = 0; i < PIECES; ++i) {
+        const int e = (blockIdx.x * PIECES + i) * kThreads + threadIdx.x;
+        if (e >= pieces) continue;
+        if constexpr (N == 8)
+            c[i] = __ldcs(reinterpret_cast<const uint32_t*>(codes) + e);
+        else
+            c[i] = __ldcs(reinterpret_cast<const uint16_t*>(codes) + e);
+        const int64_t g = g0 + static_cast<int>((static_cast<float>(e) + 0.5f) * inv);  // exact while e < 2^22, as k < 2^24
         s[i] = tok_load(q.scales, g, q.scale_type);
         off[i] = 8388608.f + (q.zeros ? static_cast<float>(__ldg(q.zeros + g)) : 8.f);
     }
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-        const int e = (blockIdx.x * kWords + i) * kThreads + threadIdx.x;
-        if (e >= words) continue;
-        float f[kEight];
+    for (int i = 0; i < PIECES; ++i) {
+        const int e = (blockIdx.x * PIECES + i) * kThreads + threadIdx.x;
+        if (e >= pieces) continue;
+        float f[N];
 #pragma unroll
-        for (int j = 0; j < kEight; ++j) f[j] = s[i] * (__uint_as_float((c[i] >> (4 * j) & 15u) | 0x4b000000u) - off[i]);
-        const int64_t o = row * w_stride + e * kEight;
-        if (VEC && w_type == kTokF32) {
-            float4* p = reinterpret_cast<float4*>(static_cast<float*>(w) + o);
-            __stcs(p, make_float4(f[0], f[1], f[2], f[3]));
-            __stcs(p + 1, make_float4(f[4], f[5], f[6], f[7]));
-        } else if (VEC) {
+        for (int j = 0; j < N; ++j) f[j] = s[i] * (__uint_as_float((c[i] >> (4 * j) & 15u) | 0x4b000000u) - off[i]);
+        const int64_t o = row * w_stride + e * N;
+        if constexpr (VEC && N == 4) {
+            __stcs(reinterpret_cast<float4*>(static_cast<float*>(w) + o), make_float4(f[0], f[1], f[2], f[3]));
+        } else if constexpr (VEC) {
             uint32_t r[4];
             if (w_type == kTokF16) {
 #pragma unroll
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const W4Args q,
             __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(w) + o), make_uint4(r[0], r[1], r[2], r[3]));
         } else {
 #pragma unroll
-            for (int j = 0; j < kEight; ++j) tok_store(w, o + j, w_type, f[j]);
+            for (int j = 0; j < N; ++j) tok_store(w, o + j, w_type, f[j]);
         }
     }
 }
@@ -230,15 +231,15 @@ cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, cons
 
 cudaError_t launch_w4_dequantize(const W4Args& q, void* w, int w_type, int64_t w_stride, cudaStream_t s) {
     constexpr int kRows = 65535;  // of a launch
-    // 16-bit values: four words a thread (4096 x 14336: 35 us, 39 with one); f32 ones fill a thread's stores alone
-    // (8192 x 8192: 60 us, 69 with four)
-    const int words = w_type == kTokF32 ? 1 : 4;
+    // A store is 16 bytes a thread and whole lines a warp: four codes of f32 values (8192 x 8192: 54 us; 60 with eight
+    // codes, whose two stores write half of every sector each), eight of 16-bit ones; four pieces a thread
+    const int n = w_type == kTokF32 ? 4 : 8;
     const bool vec = aligned_rows(w, w_stride, w_type);
-    const unsigned across = (q.k / kEight + kThreads * words - 1) / (kThreads * words);
+    const unsigned across = (q.k / n + kThreads * 4 - 1) / (kThreads * 4);
     for (int row0 = 0; row0 < q.n; row0 += kRows) {
         const dim3 grid(across, static_cast<unsigned>(q.n - row0 < kRows ? q.n - row0 : kRows));
-        auto* kern = words == 1 ? (vec ? w4_dequantize_kernel<true, 1> : w4_dequantize_kernel<false, 1>)
-                                : (vec ? w4_dequantize_kernel<true, 4> : w4_dequantize_kernel<false, 4>);
+        auto* kern = n == 4 ? (vec ? w4_dequantize_kernel<true, 4, 4> : w4_dequantize_kernel<false, 4, 4>)
+                            : (vec ? w4_dequantize_kernel<true, 8, 4> : w4_dequantize_kernel<false, 8, 4>);
         count_launch();
         kern<<<grid, kThreads, 0, s>>>(q, w, w_type, w_stride, row0);
         if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
