@@ -207,6 +207,23 @@ def test_norm_extreme_rows(cuda_torch, cols):
                 check_close(torch, got[fine], (v[fine] / 0.02).clamp(-448, 448), HALF["e4m3"] + NORM_TOL + U, TINY["e4m3"])
 
 
+@pytest.mark.parametrize("xt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(4, 100), (4, 4096), (300, 64), (300, 1024), (300, 8192)])
+def test_norm_rows_near_zero(cuda_torch, rows, cols, xt):
+    """1 / sqrt(eps) times the least row scale's reciprocal is past f32's range."""
+    torch, eps = cuda_torch, 1e-12
+    x = torch.zeros(rows, cols, dtype=tt(torch, xt), device="cuda")
+    x[1::3] = (torch.arange(cols, device="cuda") % 15 - 7) * 2.0 ** -125  # v of some 1e-31, below the least maximum
+    x[2::3] = torch.randn(cols, device="cuda").to(x.dtype)
+    y = torch.empty(rows, cols, dtype=tt(torch, "e4m3"), device="cuda")
+    scale = torch.zeros(rows, device="cuda")
+    fx.rms_norm_dev(ptr(x), ptr(y), rows, cols, xt, "e4m3", scale_ptr=ptr(scale), scale_mode="row", eps=eps, stream=stream(torch))
+    _, v = norm_want(torch, x, None, None, eps)
+    check_close(torch, scale, v.abs().amax(1).clamp(min=1e-30) / 448, NORM_TOL, 0)
+    assert bool((y[0::3].float() == 0).all())
+    check_close(torch, y.float(), v / scale.double()[:, None], HALF["e4m3"] + NORM_TOL, TINY["e4m3"])
+
+
 # ---- 4-bit weights ----------------------------------------------------------------------------------------------
 
 
