@@ -328,7 +328,10 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
     };
     const bool vec = a.cols % kVec == 0 && ok(a.x, a.x_stride, a.x_type) && ok(a.residual, a.residual_stride, a.residual_type) &&
                      ok(a.sum, a.sum_stride, a.residual_type) && ok(a.weight, 0, a.weight_type) && ok(a.y, a.y_stride, a.y_type);
-    const bool few = a.rows <= 148 * 2;
+    // little work: a block a row with as many threads as it has eights, for the shortest way through; more: blocks that stay
+    // (us, the one and the other: 444 x 320 3.2 and 4.0, 4736 x 320 6.1 and 6.2, 9472 x 320 10.3 and 7.1, 222 x 4096 4.3
+    // and 4.4, 370 x 8192 8.8 and 7.5; rows of eights to a warp's quarter: 444 x 64 2.3 and 1.8)
+    const bool few = a.cols <= 256 ? a.rows <= 148 * 2 : static_cast<int64_t>(a.rows) * a.cols <= 148 * 8192;
     if (vec && !few && a.x_type != kTokF32 && (!a.residual || a.residual_type != kTokF32)) {
         // narrow rows: several to a warp, so that its lanes are busy and have loads enough on their way (200003 x 320 bf16
         // to bf16: 50 us, 69 with a warp a row)
@@ -343,7 +346,6 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
         if (a.cols <= 8192) return launch_stream<512, 2>(a, s);
         if (a.cols <= 16384) return launch_stream<1024, 2>(a, s);
     }
-    // few rows: as many threads as the row has eights, for the shortest way through
     if (a.cols <= 256) return launch<32, 1>(a, vec, s);
     if (a.cols <= 512) return launch<32, 2>(a, vec, s);
     if (a.cols <= 1024) return few ? launch<128, 1>(a, vec, s) : launch<32, 4>(a, vec, s);

@@ -12,13 +12,20 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.x_tma = xb == 2 && p.x_vec && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
     p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride % 8 == 0;
     p.raw_slots = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0 ? 2 : 0;
-    const bool two = p.two = (a.w.n + 255) / 256 * ((a.rows + 191) / 192) >= sms;
+    // Tiles of 128 outputs by up to 256 rows, or of 256 by 192, of the size that spreads the rows evenly. A turn of 148 of
+    // the larger ones takes 1.5 times as long, or 1.1 times where warps bring the rows, which then bound it (us, smaller
+    // against larger; bf16: 1536 x 4096 -> 4096 50 and 40, 1024 x 4096 -> 14336 102 and 119, 4096 rows 370 and 370; e4m3:
+    // 1024 x 4096 -> 4096 54 and 58, 576 x 4096 -> 14336 158 and 115)
+    auto across = [&](int m) { return (a.w.n + m - 1) / m; };
+    auto turns = [&](int m, int most) { return (across(m) * ((static_cast<int64_t>(a.rows) + most - 1) / most) + sms - 1) / sms; };
+    const bool two = p.two = p.x_tma ? turns(256, 192) * 3 < turns(128, 256) * 2 : turns(256, 192) * 11 < turns(128, 256) * 10;
     const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
-    p.tile_n = a.rows >= most_n ? most_n : (a.rows + 15) / 16 * 16;
-    const int64_t tiles_n = (a.rows + p.tile_n - 1) / p.tile_n;
-    const int64_t tiles = (a.w.n + tile_m - 1) / tile_m * tiles_n;
+    const int64_t tiles_n = (static_cast<int64_t>(a.rows) + most_n - 1) / most_n;
+    p.tile_n = static_cast<int>((a.rows + tiles_n * 16 - 1) / (tiles_n * 16)) * 16;
+    const int64_t tiles = across(tile_m) * tiles_n;
     const int all_stages = (a.w.k + kStageK - 1) / kStageK;
-    // few tiles: a cluster shares one, each block a range of k, while a block keeps two stages of codes
+    // few tiles: a cluster shares one, each block a range of k, while a block keeps two stages of codes (us without and
+    // with: 16 x 4096 -> 4096 18.5 and 10.0, 256 x 4096 -> 4096 26.5 and 16.5, 192 x 8192 -> 8192 46 and 29)
     p.split = 1;
     while (!two && p.split < 8 && tiles * p.split * 2 <= sms && all_stages >= p.split * 4) p.split *= 2;
     p.stages_each = (all_stages + p.split - 1) / p.split;
@@ -26,15 +33,17 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.weight_col = (two ? 2 : 1) * p.tile_n;
     p.tmem_cols = 512;
     p.rings[1] = std::min((p.tmem_cols - p.weight_col) / (two ? 64 : 32), kMaxRing);
-    // shared memory: codes and rows in turn
-    // short steps: four to a slot, for fewer waits
-    p.slot_steps = !two && p.tile_n <= 64 ? 4 : 1;
+    // the issuing thread's waits bound short steps: four or two of them share a slot of the rows, as room allows (4096 ->
+    // 14336 bf16, us, one step a slot against more: 16 rows 23.6 and 19.5, 128 rows 25.6 and 22.3; 1024 x 4096 -> 4096
+    // 28.2 and 26.9)
+    p.slot_steps = two ? 1 : p.tile_n <= 128 ? 4 : 2;
     if (p.raw_slots && p.slot_steps == 4) p.raw_slots = 4;
     const int tops_bytes = 1024, w = tile_m * 128, x = p.tile_n * 128 * p.slot_steps;
     // Warps that write a slot each, taking steps in turn, tell a slot's uses apart by parity: a ring as long as they are
     // many keeps one that runs ahead from meeting a slot two uses behind.
     p.rings[0] = 2;
     p.rings[2] = !p.x_tma && p.slot_steps == 1 ? kRowWarps : 2;
+    // the rest: codes and rows in turn
     int room = kSmemMax - tops_bytes - p.rings[0] * w - p.rings[2] * x - p.raw_slots * p.tile_n * 128;
     if (room < 0) return cudaErrorInvalidConfiguration;
     for (bool more = true; more;) {

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
         // rows that TMA does not bring as they are used: four warps write them in 16-byte cells of eight values, as the
         // swizzle places them
         // (a step each, so that a step's latency is hidden behind the others')
-        static_assert(SS == 1 || SS == kRowWarps, "a slot is one warp's or all warps'");
+        static_assert(kRowWarps % SS == 0, "a slot is written in one turn of the warps");
         const int tid = threadIdx.x - 18 * 32, kxb = a.x_type == kTokE4M3 ? 1 : 2;
         auto fetch = [&](int step, int slot) {  // e4m3: TMA brings 128 inputs at a time, these warps widen them
             if (step < steps) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             for (int i = 0; i < plan.raw_slots; ++i) fetch(2 * i, i);
         for (int step0 = 0; step0 < steps; step0 += kRowWarps) {
             const int step = step0 + tid / 32, pair = step / 2, slots = plan.raw_slots ? plan.raw_slots : 1, rs = pair % slots;
-            if (SS == 1 && step >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
+            if (step / SS * SS >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
             const int xs = step / SS % plan.rings[2];
             const uint32_t xp = step / SS / plan.rings[2] & 1, rp = pair / slots & 1;
             if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
@@ -543,6 +543,7 @@ template <bool BF>
 cudaError_t launch_typed(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     if (p.two) return p.x_tma ? launch<BF, true, true, 1>(a, p, s) : launch<BF, true, false, 1>(a, p, s);
     if (p.slot_steps == 1) return p.x_tma ? launch<BF, false, true, 1>(a, p, s) : launch<BF, false, false, 1>(a, p, s);
+    if (p.slot_steps == 2) return p.x_tma ? launch<BF, false, true, 2>(a, p, s) : launch<BF, false, false, 2>(a, p, s);
     return p.x_tma ? launch<BF, false, true, 4>(a, p, s) : launch<BF, false, false, 4>(a, p, s);
 }
 
