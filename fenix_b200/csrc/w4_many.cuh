@@ -256,20 +256,23 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             for (int i = 0; i < plan.raw_slots; ++i) fetch(2 * i, i);
         for (int step0 = 0; step0 < steps; step0 += kRowWarps) {
             const int step = step0 + tid / 32, pair = step / 2, slots = plan.raw_slots ? plan.raw_slots : 1, rs = pair % slots;
-            if (step / SS * SS >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
+            if (SS < kRowWarps && step / SS * SS >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
             const int xs = step / SS % plan.rings[2];
             const uint32_t xp = step / SS / plan.rings[2] & 1, rp = pair / slots & 1;
             if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
             uint8_t* const to = smem + plan.rows + (xs * SS + step % SS) * tile_n * 128;
             if (step < steps && plan.raw_slots) {
                 if (!wait_phase(raw_full + 8 * rs, rp, &abort_flag)) gave_up(kStatusTimeoutFull);
-                const uint8_t* const raw = smem + plan.raw + rs * tile_n * 128;
+                // eight lanes take a cell of eight rows each: every bank once, read and written
+                const int at = lane % 8, c = lane / 8;
+                const uint8_t* const raw = smem + plan.raw + rs * tile_n * 128 + at * 128 + (((4 * (step % 2) + c) ^ at) << 4);
+                uint8_t* const lo = to + at * 128 + (((2 * c) ^ at) << 4);
+                uint8_t* const hi = to + at * 128 + (((2 * c + 1) ^ at) << 4);
 #pragma unroll 4
-                for (int i = lane; i < tile_n * 4; i += 32) {
-                    const int r = i / 4, c = i % 4;
-                    const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 128 + (((4 * (step % 2) + c) ^ (r & 7)) << 4));
-                    *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c) ^ (r & 7)) << 4)) = widened(v, kTokE4M3);
-                    *reinterpret_cast<uint4*>(to + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4)) = widened(make_uint4(v.z, v.w, 0, 0), kTokE4M3);
+                for (int r = 0; r < tile_n * 128; r += 1024) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(raw + r);
+                    *reinterpret_cast<uint4*>(lo + r) = widened(v, kTokE4M3);
+                    *reinterpret_cast<uint4*>(hi + r) = widened(make_uint4(v.z, v.w, 0, 0), kTokE4M3);
                 }
             } else if (step < steps) {
                 const int k0 = k_begin + step * kStepK;
