@@ -2,9 +2,12 @@
 //
 // Bound by memory: x, residual, sum and y pass once (7 bytes a value for bf16 to e4m3). A row's h = x + residual
 // stays in the registers of its team of threads, eight consecutive values a thread and turn, between the three
-// looks at it: the sum of squares, the largest magnitude, the output. A team is a warp or a block: a warp while
-// a row fits it, since its reductions need no barrier, else the smallest block that keeps 16 values a thread, so that an SM holds
-// many rows at different stages and its loads never pause.
+// looks at it: the sum of squares, the largest magnitude, the output. A team is a part of a warp, a warp or a block.
+// Where rows are many, blocks stay and walk over them with the next row's loads on their way during a row's
+// reductions (16384 x 4096 bf16 with residual to e4m3: 75 us, 6.2 TB/s; 99 us with a block a row); where they are few,
+// a block a row has as many threads as the row has eights (1 x 4096: 2.5 us, launch and two reductions). Rows that are
+// no multiple of eight values, or not aligned, are read one value at a time, neighbours by neighbours (1031 x 5119 f16
+// with residual: 23 us, 1.6 TB/s: four times the loads of a vector, each waited for).
 #include "counters.hpp"
 #include "token.cuh"
 

@@ -9,12 +9,16 @@ namespace fxk {
 namespace {
 
 // ---- few rows ----------------------------------------------------------------------------------
-// With few token rows the time is the weights' way from memory: 4.5 bits a weight, each used once per
-// row, and the bound close behind is the instructions that make operands of the codes. One block per SM
-// walks over tiles of 16 MT outputs: a producer warp keeps a ring of bulk copies ahead of the consumer
-// warps, across tiles, so that memory never waits for a tile's end; each consumer takes 128 inputs of a
-// stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs, B: inputs x 8 rows); the rows lie in
-// shared memory for the whole walk, converted once and in the MMA's order.
+// With up to 8 token rows the floor is the weights' way from memory: 4.1 bits a weight, each used once per row. What
+// bounds the kernel before that is the instructions that make operands of the codes and the time a warp's chain of
+// them takes (1 x 8192 -> 28672 f16: 34 us, 3.5 TB/s, 54% of the copy's rate; 1 x 4096 -> 4096: 6.7 us, of which half
+// is launch, first loads and the reduction; 8 x 4096 -> 14336 e4m3 with zero points: 19.7 us). One block per SM walks
+// over tiles of 32 outputs (the last of them over tiles of 16, so that all blocks have as much to do): a producer warp
+// keeps a ring of TMA boxes, 32 outputs x 256 inputs, ahead of the consumer warps, across tiles, so that memory never
+// waits for a tile's end (a bulk copy for each row of a tile costs its thread some 60 ns); each consumer takes 128 inputs of a stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs,
+// B: inputs x 8 rows), whose 8 columns are what few rows can fill: a tcgen05 operand would have to be written before
+// it is read (all of it: 1 x 4096 -> 4096 9.7 us, 1 x 8192 -> 28672 67). The rows lie in shared memory for the whole
+// walk, converted once and in the MMA's order.
 // A code enters the MMA as offset + code, which costs one logical operation for two; what leaves again in f32, a group
 // at a time, are sums over the rows' inputs alone, made when those are brought in:
 //   sum (code - zero) x = sum (offset + code) x - sum offset x - zero sum x
@@ -436,6 +440,8 @@ cudaError_t launch_few_typed(const W4LinearArgs& a, bool x_vec, cudaStream_t s) 
 }  // namespace
 
 cudaError_t launch_w4_linear(const W4LinearArgs& a, cudaStream_t s) {
+    // 8 rows are an MMA's columns; the kernels meet there (us, few rows' and many rows': 4 x 4096 -> 14336 15.9 and 20.0,
+    // 8 x 4096 -> 4096 10.7 and 10.1, 8 x 4096 -> 14336 18.9 and 19.9, 8 x 8192 -> 28672 55 and 67)
     if (a.rows > 8) {
         constexpr int kMost = 65535 * 16;  // rows of a launch: 65535 of the smallest tiles
         for (int64_t row0 = 0; row0 < a.rows; row0 += kMost) {

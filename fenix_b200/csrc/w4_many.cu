@@ -14,8 +14,8 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.raw_slots = xb == 1 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 16 == 0 ? 2 : 0;
     // Tiles of 128 outputs by up to 256 rows, or of 256 by 192, of the size that spreads the rows evenly. A turn of 148 of
     // the larger ones takes 1.5 times as long, or 1.1 times where warps bring the rows, which then bound it (us, smaller
-    // against larger; bf16: 1536 x 4096 -> 4096 50 and 40, 1024 x 4096 -> 14336 102 and 119, 4096 rows 370 and 370; e4m3:
-    // 1024 x 4096 -> 4096 54 and 58, 576 x 4096 -> 14336 158 and 115)
+    // against larger; bf16: 1536 x 4096 -> 4096 50 and 40, 1024 x 4096 -> 14336 102 and 119, 4096 rows 352 and 364; e4m3:
+    // 1024 x 4096 -> 4096 49 and 49, 576 x 4096 -> 14336 109 and 107, 4096 rows 609 and 483)
     auto across = [&](int m) { return (a.w.n + m - 1) / m; };
     auto turns = [&](int m, int most) { return (across(m) * ((static_cast<int64_t>(a.rows) + most - 1) / most) + sms - 1) / sms; };
     const bool two = p.two = p.x_tma ? turns(256, 192) * 3 < turns(128, 256) * 2 : turns(256, 192) * 11 < turns(128, 256) * 10;

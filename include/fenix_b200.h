@@ -401,9 +401,9 @@ fx_status fx_accum_finalize(const float* dev_acc, int64_t dz, int64_t dy, int64_
  * Common to these calls: matrices are row-major with their rows `*_stride` elements apart (at least the
  * row's length; 0: packed) and their elements at least element-aligned. Every pointer of a call is device
  * memory of one device, which need not be the current one; `stream` (NULL: that device's default stream)
- * belongs to that device. The calls enqueue one kernel, allocate nothing, keep nothing between calls and
- * do not synchronise, so any number may run at once and be captured into graphs. Extents and strides are
- * below 2^30. No row (rows or n = 0) is not an error: nothing is done. */
+ * belongs to that device. The calls enqueue one kernel (a few in a row for extents past 65535), allocate
+ * nothing, keep nothing between calls and do not synchronise, so any number may run at once and be captured
+ * into graphs. Extents and strides are below 2^30. No row (rows or n = 0) is not an error: nothing is done. */
 typedef enum fx_dtype { FX_F32 = 0, FX_F16 = 1, FX_BF16 = 2, FX_E4M3 = 3 } fx_dtype;
 /* Scale of 8-bit rows (value = e4m3 * scale): none, one for the tensor, or one per row. */
 typedef enum fx_scale { FX_SCALE_NONE = 0, FX_SCALE_TENSOR = 1, FX_SCALE_ROW = 2 } fx_scale;
@@ -417,7 +417,8 @@ typedef enum fx_scale { FX_SCALE_NONE = 0, FX_SCALE_TENSOR = 1, FX_SCALE_ROW = 2
  *   FX_SCALE_ROW     scale[row] = max(max |v|, 1e-30) / 448, written to dev_scale [rows]
  *   FX_SCALE_TENSOR  scale = dev_scale[0], read (a calibrated activation scale)
  * A row that holds a NaN or infinity follows the formula: its values (and a row scale) come out NaN, save
- * the finite values of a row of infinities under a tensor scale and in 16 / 32 bits, which become zero.
+ * the finite values of a row of infinities under a tensor scale and in 16 / 32 bits, which become zero. The mean is
+ * held in f32: of squares below 2^-126 only eps is left.
  * In place: dev_sum may be dev_residual or dev_x, and dev_y may be dev_x, at equal types and strides; no
  * other overlap. 1 <= cols <= 32768, eps > 0. Extents that are multiples of 8 with 16-byte aligned rows
  * take 16-byte accesses. */
@@ -432,7 +433,11 @@ fx_status fx_rms_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t 
  * aligned), scales [n][k / group] of scale_type (f32, f16, bf16) and zero points [n][k / group] of 0..15
  * (NULL: 8 everywhere). group is a multiple of 32 that divides k < 2^24; rows and n are any numbers. x is f16,
  * bf16, or e4m3 with x_scale (f32: FX_SCALE_TENSOR one value, FX_SCALE_ROW [rows]); y is f16 or bf16,
- * rounded once; bias is f32 [n] or NULL. Sums are held in f32. y overlaps no input. */
+ * rounded once; bias is f32 [n] or NULL. Sums are held in f32. y overlaps no input.
+ * Up to 8 rows no weight is rounded, but the outputs need 1039 |x| summed over a group to stay in f32's range (f16 and
+ * e4m3 always do); from 9 rows on a weight is rounded once to x's 16-bit type (f16 for e4m3, relative to its output's
+ * largest scale). A row that holds a NaN or infinity, and an output with such a scale, come out not finite (NaN or
+ * infinite, which is not specified); other rows and outputs are untouched by them. Results repeat exactly. */
 fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t x_stride, const float* dev_x_scale,
                        fx_scale x_scale_mode, const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
                        const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, const float* dev_bias,
