@@ -30,6 +30,8 @@ struct ManyPlan {
 
 cudaError_t w4_many_bf16(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s);
 cudaError_t w4_many_f16(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s);
+// Clusters of `size` blocks that the current device runs at once.
+cudaError_t w4_many_clusters(int size, int* count);
 cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s);
 // The status word of each file's kernels, cleared.
 cudaError_t w4_few_status(uint32_t* code);

@@ -24,11 +24,19 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     p.tile_n = static_cast<int>((a.rows + tiles_n * 16 - 1) / (tiles_n * 16)) * 16;
     const int64_t tiles = across(tile_m) * tiles_n;
     const int all_stages = (a.w.k + kStageK - 1) / kStageK;
-    // few tiles: a cluster shares one, each block a range of k, while a block keeps two stages of codes (us without and
-    // with: 16 x 4096 -> 4096 18.5 and 10.0, 256 x 4096 -> 4096 26.5 and 16.5, 192 x 8192 -> 8192 46 and 29)
-    p.split = 1;
-    while (!two && p.split < 8 && tiles * p.split * 2 <= sms && all_stages >= p.split * 4) p.split *= 2;
-    p.stages_each = (all_stages + p.split - 1) / p.split;
+    // few tiles: a cluster shares one, each block a range of k, in the largest clusters that all run at once (on a GPU of
+    // 148 SMs 74 of 2, 45 of 3, 33 of 4, 26 of 5, 22 of 6, 15 of 8) and leave a block two stages of codes (us without and
+    // with: 16 x 4096 -> 4096 18.5 and 10.0, 256 x 4096 -> 4096 26.5 and 16.5, 192 x 8192 -> 8192 46 and 29; clusters of
+    // 4, three of 36 left over for a second turn, against 3: 24 x 4096 -> 4608 18.7 and 11.9)
+    int split = 1;
+    for (int c = 8; !two && c > 1 && split == 1; --c) {
+        if (tiles * c > sms || all_stages < 2 * c) continue;
+        int most = 0;
+        if (const cudaError_t e = w4_many_clusters(c, &most); e != cudaSuccess) return e;
+        if (tiles <= most) split = c;
+    }
+    p.stages_each = (all_stages + split - 1) / split;
+    p.split = (all_stages + p.stages_each - 1) / p.stages_each;  // no block without a stage
     // TMEM, all of it (a block's shared memory leaves room for no other block): accumulators, then stages of weights
     p.weight_col = (two ? 2 : 1) * p.tile_n;
     p.tmem_cols = 512;

@@ -451,6 +451,13 @@ def test_linear_inputs_over_a_cluster(cuda_torch, xt, offset):
         run_linear(cuda_torch, rows, 100, k, 32, xt, "bf16", zeros=True, bias=True, offset=offset)
 
 
+@pytest.mark.parametrize("tiles", [9, 15, 16, 22, 23, 26, 27, 33, 34, 45, 46, 74, 75])
+def test_linear_clusters_of_every_size(cuda_torch, tiles):
+    """Tiles of 128 outputs, shared by clusters of as many blocks as the GPU runs at once; the last tile is a part."""
+    run_linear(cuda_torch, 20, tiles * 128 - 5, 3584, 128, "bf16", "bf16", zeros=True, bias=True)
+    run_linear(cuda_torch, 130, tiles * 128 - 64, 2176, 64, "e4m3", "f16", mode="row")
+
+
 def test_linear_rows_past_32_bits(cuda_torch):
     torch = cuda_torch
     if torch.cuda.mem_get_info()[0] < 40 << 30:
