@@ -11,6 +11,7 @@
 #include "token.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fxk {
 namespace {
@@ -50,38 +51,68 @@ __device__ __forceinline__ uint32_t codes_of(const float (&w)[kEight], float sca
     return r;
 }
 
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* p, int64_t i, int type, float (&f)[kEight]) {
-    if (VEC && type == kTokF32) {
-        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 a = __ldcs(q), b = __ldcs(q + 1);
-        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else if (VEC) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        if (type == kTokF16) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 t = __half22float2(reinterpret_cast<const __half2&>(w[j]));
-                f[2 * j] = t.x;
-                f[2 * j + 1] = t.y;
-            }
+// How eight weights are read and held: one at a time (any type), or 16 bytes at a time of one type.
+enum Kind { kAny, kVecF32, kVecF16, kVecBF16 };
+template <Kind KIND>
+struct Eight {  // f32, or 16-bit values as they lie in memory
+    float f[kEight];
+    __device__ __forceinline__ void load(const void* p, int64_t i, int type) {
+        if (KIND == kVecF32) {
+            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+            const float4 a = __ldcs(q), b = __ldcs(q + 1);
+            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[2 * j] = __uint_as_float(w[j] << 16);
-                f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
+            for (int j = 0; j < kEight; ++j) f[j] = tok_load(p, i + j, type);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kEight; ++j) f[j] = tok_load(p, i + j, type);
     }
-}
+    __device__ __forceinline__ void extremes(float& lo, float& hi) const {
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) {
+            lo = fminf(lo, f[j]);
+            hi = fmaxf(hi, f[j]);
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[kEight]) const {
+#pragma unroll
+        for (int j = 0; j < kEight; ++j) v[j] = f[j];
+    }
+};
+template <class T2>
+struct Eight16 {
+    uint4 raw;
+    __device__ __forceinline__ static float2 pair(uint32_t w) {
+        if constexpr (std::is_same_v<T2, __half2>)
+            return __half22float2(reinterpret_cast<const __half2&>(w));
+        else
+            return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    __device__ __forceinline__ void load(const void* p, int64_t i, int) { raw = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i)); }
+    __device__ __forceinline__ void extremes(float& lo, float& hi) const {  // two at a time; a NaN loses against a number
+        const T2* const v = reinterpret_cast<const T2*>(&raw);
+        const T2 l = __hmin2(__hmin2(v[0], v[1]), __hmin2(v[2], v[3])), h = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
+        const float2 a = pair(reinterpret_cast<const uint32_t&>(l)), b = pair(reinterpret_cast<const uint32_t&>(h));
+        lo = fminf(lo, fminf(a.x, a.y));
+        hi = fmaxf(hi, fmaxf(b.x, b.y));
+    }
+    __device__ __forceinline__ void values(float (&v)[kEight]) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 t = pair(w[j]);
+            v[2 * j] = t.x;
+            v[2 * j + 1] = t.y;
+        }
+    }
+};
+template <>
+struct Eight<kVecF16> : Eight16<__half2> {};
+template <>
+struct Eight<kVecBF16> : Eight16<__nv_bfloat162> {};
 
-// TEAM lanes of a warp per group (4: groups of 32, ..., 32: any), HOLD times eight weights a lane in registers; a
+// TEAM lanes of a warp per group (1: groups of 32, ..., 32: any), HOLD times eight weights a lane in registers; a
 // longer group is read a second time for its codes.
-template <int TEAM, int HOLD, bool VEC>
+template <int TEAM, int HOLD, Kind KIND>
 __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __restrict__ w, int w_type, int64_t w_stride, const W4Args q) {
     const int me = threadIdx.x % TEAM;
     const uint32_t per_row = q.k / q.group, g32 = blockIdx.x * (kThreads / TEAM) + threadIdx.x / TEAM;  // below 2^31: the launcher's rows
@@ -89,27 +120,18 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __res
     const bool on = g32 < q.n * per_row;  // lanes of no group run along: the shuffles are the warp's
     const int64_t base = on ? static_cast<int64_t>(g32 / per_row) * w_stride + g32 % per_row * static_cast<int64_t>(q.group) : 0;
     const int eights = on ? q.group / kEight : 0;
-    float f[HOLD][kEight], lo = 0.f, hi = 0.f;
+    Eight<KIND> f[HOLD];
+    float lo = 0.f, hi = 0.f;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
-        if (h * TEAM + me < eights) load8<VEC>(w, base + (h * TEAM + me) * kEight, w_type, f[h]);
+        if (h * TEAM + me < eights) f[h].load(w, base + (h * TEAM + me) * kEight, w_type);
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
-        if (h * TEAM + me < eights) {
-#pragma unroll
-            for (int j = 0; j < kEight; ++j) {
-                lo = fminf(lo, f[h][j]);
-                hi = fmaxf(hi, f[h][j]);
-            }
-        }
+        if (h * TEAM + me < eights) f[h].extremes(lo, hi);
     for (int e = HOLD * TEAM + me; e < eights; e += TEAM) {
-        float t[kEight];
-        load8<VEC>(w, base + static_cast<int64_t>(e) * kEight, w_type, t);
-#pragma unroll
-        for (int j = 0; j < kEight; ++j) {
-            lo = fminf(lo, t[j]);
-            hi = fmaxf(hi, t[j]);
-        }
+        Eight<KIND> t;
+        t.load(w, base + static_cast<int64_t>(e) * kEight, w_type);
+        t.extremes(lo, hi);
     }
 #pragma unroll
     for (int o = TEAM / 2; o; o >>= 1) {
@@ -124,14 +146,18 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __res
         if (q.zeros) const_cast<uint8_t*>(q.zeros)[g] = static_cast<uint8_t>(zero);
     }
     uint32_t* const codes = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(q.codes)) + g * (q.group / kEight);
-    const float inv = __fdiv_rn(1.f, scale);
-    auto put = [&](int e, const float(&v)[kEight]) { codes[e] = codes_of(v, scale, inv, zero); };
+    const float inv = 1.f / scale;
+    auto put = [&](int e, const Eight<KIND>& t) {
+        float v[kEight];
+        t.values(v);
+        codes[e] = codes_of(v, scale, inv, zero);
+    };
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
         if (h * TEAM + me < eights) put(h * TEAM + me, f[h]);
     for (int e = HOLD * TEAM + me; e < eights; e += TEAM) {
-        float t[kEight];
-        load8<VEC>(w, base + static_cast<int64_t>(e) * kEight, w_type, t);
+        Eight<KIND> t;
+        t.load(w, base + static_cast<int64_t>(e) * kEight, w_type);
         put(e, t);
     }
 }
@@ -209,10 +235,11 @@ cudaError_t quantize(const void* w, int w_type, int64_t w_stride, const W4Args& 
         const void* const from = static_cast<const uint8_t*>(w) + row * w_stride * w_size;
         const unsigned blocks = static_cast<unsigned>((part.n * per_row * TEAM + kThreads - 1) / kThreads);
         count_launch();
-        if (aligned_rows(w, w_stride, w_type))
-            w4_quantize_kernel<TEAM, HOLD, true><<<blocks, kThreads, 0, s>>>(from, w_type, w_stride, part);
-        else
-            w4_quantize_kernel<TEAM, HOLD, false><<<blocks, kThreads, 0, s>>>(from, w_type, w_stride, part);
+        auto* kern = !aligned_rows(w, w_stride, w_type) ? w4_quantize_kernel<TEAM, HOLD, kAny>
+                     : w_type == kTokF32                ? w4_quantize_kernel<TEAM, HOLD, kVecF32>
+                     : w_type == kTokF16                ? w4_quantize_kernel<TEAM, HOLD, kVecF16>
+                                                        : w4_quantize_kernel<TEAM, HOLD, kVecBF16>;
+        kern<<<blocks, kThreads, 0, s>>>(from, w_type, w_stride, part);
         if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     }
     return cudaSuccess;
