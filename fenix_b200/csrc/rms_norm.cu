@@ -7,7 +7,8 @@
 // reductions (16384 x 4096 bf16 with residual to e4m3: 75 us, 6.2 TB/s; 99 us with a block a row); where they are few,
 // a block a row has as many threads as the row has eights (1 x 4096: 2.5 us, launch and two reductions). Rows that are
 // no multiple of eight values, or not aligned, are read one value at a time, neighbours by neighbours (1031 x 5119 f16
-// with residual: 23 us, 1.6 TB/s: four times the loads of a vector, each waited for).
+// with residual: 15 us, 2.5 TB/s, bound by the instructions of a value; with the next row brought to shared memory in
+// 16-byte pieces 19).
 #include "counters.hpp"
 #include "token.cuh"
 
@@ -71,9 +72,13 @@ __device__ __forceinline__ void load8(const void* p, int64_t row, int type, int 
             const int c = column<TEAM, VEC>(u, j, me);
             v[j] = c < cols ? static_cast<const uint16_t*>(p)[row + c] : uint16_t{0};
         }
+        if (type == kTokF16) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j)
-            f[j] = type == kTokF16 ? __half2float(__ushort_as_half(v[j])) : __uint_as_float(static_cast<uint32_t>(v[j]) << 16);
+            for (int j = 0; j < kVec; ++j) f[j] = __half2float(__ushort_as_half(v[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) f[j] = __uint_as_float(static_cast<uint32_t>(v[j]) << 16);
+        }
     }
 }
 template <int TEAM, bool VEC>
@@ -112,11 +117,22 @@ __device__ __forceinline__ void store8(void* p, int64_t row, int type, int u, in
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + row + c) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     } else {
+        auto each = [&](auto* q, auto&& make) {
+            q += row;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-            const int c = column<TEAM, VEC>(u, j, me);
-            if (c < cols) tok_store(p, row + c, type, f[j]);
-        }
+            for (int j = 0; j < kVec; ++j) {
+                const int c = column<TEAM, VEC>(u, j, me);
+                if (c < cols) q[c] = make(f[j]);
+            }
+        };
+        if (type == kTokF32)
+            each(static_cast<float*>(p), [](float v) { return v; });
+        else if (type == kTokF16)
+            each(static_cast<__half*>(p), [](float v) { return __float2half_rn(v); });
+        else if (type == kTokBF16)
+            each(static_cast<__nv_bfloat16*>(p), [](float v) { return __float2bfloat16_rn(v); });
+        else
+            each(static_cast<__nv_fp8_storage_t*>(p), [](float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); });
     }
 }
 
@@ -131,7 +147,7 @@ __device__ __forceinline__ float team_sum(float v, float* red) {
         __syncthreads();
         v = threadIdx.x % 32 < TEAM / 32 ? red[threadIdx.x % 32] : 0.f;
 #pragma unroll
-        for (int o = TEAM / 64; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int o = TEAM > 512 ? 16 : TEAM > 256 ? 8 : TEAM / 64; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         v = __shfl_sync(0xffffffffu, v, 0);
     }
     return v;
@@ -346,6 +362,9 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
         if (a.cols <= 1024) return launch_stream<32, 4>(a, s);
         if (a.cols <= 2048) return launch_stream<128, 2>(a, s);
         if (a.cols <= 4096) return launch_stream<256, 2>(a, s);
+        // (8192 x 5120 51 us, 64 with 512 threads; a team of 448 for 7168 columns is no faster)
+        if (a.cols <= 5120) return launch_stream<320, 2>(a, s);
+        if (a.cols <= 6144) return launch_stream<384, 2>(a, s);
         if (a.cols <= 8192) return launch_stream<512, 2>(a, s);
         if (a.cols <= 16384) return launch_stream<1024, 2>(a, s);
     }
@@ -354,6 +373,10 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
     if (a.cols <= 1024) return few ? launch<128, 1>(a, vec, s) : launch<32, 4>(a, vec, s);
     if (a.cols <= 2048) return launch<256, 1>(a, vec, s);
     if (a.cols <= 4096) return launch<512, 1>(a, vec, s);
+    // (teams between the powers of two: 1031 x 5119 15 us, 20 with 1024 threads)
+    if (a.cols <= 5120) return launch<640, 1>(a, vec, s);
+    if (a.cols <= 6144) return launch<768, 1>(a, vec, s);
+    if (a.cols <= 7168) return launch<896, 1>(a, vec, s);
     if (a.cols <= 8192) return launch<1024, 1>(a, vec, s);
     if (a.cols <= 16384) return launch<1024, 2>(a, vec, s);
     return launch<1024, 4>(a, vec, s);

@@ -1,8 +1,8 @@
 // w4_quant.cu — weights to 4-bit codes with group scales (and zero points), and back.
 //
 // Bound by memory with f32 weights: a weight passes once (4 bytes against half a byte and its share of a scale; 8192 x
-// 8192 in groups of 128: 51 us, 6.0 TB/s, and 54 back), with 16-bit ones by the instructions of a weight (4096 x 14336
-// bf16 with zero points: 63 us, 2.4 TB/s, and 34 back, 4.3 TB/s). A team of
+// 8192 in groups of 128: 47 us, 6.4 TB/s, and 54 back), with 16-bit ones by the instructions of a weight (4096 x 14336
+// bf16 with zero points: 46 us, 3.2 TB/s, and 34 back, 4.3 TB/s). A team of
 // threads holds a group in registers between its extremes and its codes, eight consecutive weights a thread: 16 or
 // 32 bytes in, a word of codes out, the extremes by shuffles inside the warp. Codes are those of f32's correctly
 // rounded quotients: a product with the scale's reciprocal stands for the quotient unless it lies so near a half
@@ -256,8 +256,8 @@ cudaError_t quantize(const void* w, int w_type, int64_t w_stride, const W4Args& 
 }  // namespace
 
 cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, const W4Args& q, cudaStream_t s) {
-    // 32 weights a thread share what is done once a group (8192 x 8192 f32 in groups of 128: 50 us, 83 with 8 a thread);
-    // a matrix that leaves SMs idle that way takes 8 a thread (1003 x 1088 bf16 in groups of 32: 3.7 us, 5.2 with 32)
+    // 32 weights a thread share what is done once a group (8192 x 8192 f32 in groups of 128: 47 us, 83 with 8 a thread);
+    // a matrix that leaves SMs idle that way takes 8 a thread (1003 x 1088 bf16 in groups of 32: 3.1 us, 5.2 with 32)
     const bool small = static_cast<int64_t>(q.n) * q.k < int64_t{148} * 1024 * 32;
     if (q.group == 32) return small ? quantize<4, 1>(w, w_type, w_stride, q, s) : quantize<1, 4>(w, w_type, w_stride, q, s);
     if (q.group == 64) return small ? quantize<8, 1>(w, w_type, w_stride, q, s) : quantize<2, 4>(w, w_type, w_stride, q, s);

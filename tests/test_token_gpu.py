@@ -114,6 +114,12 @@ def test_norm_extents(cuda_torch, rows, cols):
     run_norm(cuda_torch, rows, cols, yt="bf16", residual=False, keep_sum=False, seed=cols + 1)
 
 
+@pytest.mark.parametrize("cols", [4097, 4104, 5120, 5121, 5128, 6143, 6144, 6145, 7000, 7168, 7169, 7176])
+@pytest.mark.parametrize("rows", [2, 400])
+def test_norm_teams_between_powers_of_two(cuda_torch, rows, cols):
+    run_norm(cuda_torch, rows, cols, yt="e4m3", mode="row", seed=cols)
+
+
 @pytest.mark.parametrize("xt,yt,rt", list(itertools.product(["f32", "f16", "bf16"], ["f32", "f16", "bf16", "e4m3"],
                                                         ["f32", "f16", "bf16"])))
 def test_norm_types(cuda_torch, xt, yt, rt):
