@@ -5,14 +5,16 @@
 #include "token.cuh"
 #include "w4.cuh"
 
+#include <algorithm>
+
 namespace fxk {
 namespace {
 
 // ---- few rows ----------------------------------------------------------------------------------
 // With up to 8 token rows the floor is the weights' way from memory: 4.1 bits a weight, each used once per row. What
 // bounds the kernel before that is the instructions that make operands of the codes and the time a warp's chain of
-// them takes (1 x 8192 -> 28672 f16: 34 us, 3.5 TB/s, 54% of the copy's rate; 1 x 4096 -> 4096: 6.7 us, of which half
-// is launch, first loads and the reduction; 8 x 4096 -> 14336 e4m3 with zero points: 19.7 us). One block per SM walks
+// them takes (1 x 8192 -> 28672 f16: 31 us, 3.9 TB/s, 59% of the copy's rate; 1 x 4096 -> 4096: 6.6 us, of which half
+// is launch, first loads and the reduction; 8 x 4096 -> 14336 e4m3 with zero points: 18.9 us). One block per SM walks
 // over tiles of 32 outputs (the last of them over tiles of 16, so that all blocks have as much to do): a producer warp
 // keeps a ring of TMA boxes, 32 outputs x 256 inputs, ahead of the consumer warps, across tiles, so that memory never
 // waits for a tile's end (a bulk copy for each row of a tile costs its thread some 60 ns); each consumer takes 128 inputs of a stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs,
@@ -80,7 +82,7 @@ struct FewPlan {
     int tiles;
     int x_pitch;     // of a row's inputs: 64 modulo 128, so that 2 rows x 4 lanes of 16 bytes hit all banks once
     int s_pitch, z_pitch;  // of an output's scales and zero points: 16 modulo 128, so that 8 outputs hit different banks
-    int red_bufs;
+    int red_bufs;  // tiles whose partial sums have room
     int sum_pitch;   // of a row's sums over units, in pairs
     int x, sums, scale, accum, red, ring, bytes;  // offsets; accum: the sums of earlier segments, by tile of this block
     bool x_vec;
@@ -270,7 +272,6 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
     const float2* const sum0 = reinterpret_cast<const float2*>(smem + plan.sums) + min(2 * t, rows - 1) * plan.sum_pitch;
     const float2* const sum1 = reinterpret_cast<const float2*>(smem + plan.sums) + min(2 * t + 1, rows - 1) * plan.sum_pitch;
     const float inv_group = 1.f / static_cast<float>(group);
-    int red_buf = 0;
     for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
         const int seg_end = min(seg + plan.seg_blocks, blocks), g0 = seg * kBlockK / group;
         if (seg) consumers_sync(warps);  // the last segment's rows are read
@@ -297,10 +298,9 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             }
         }
         consumers_sync(warps);
-        int turn = 0;
+        int turn = 0, added = 0;  // tiles of this block, and those added up
         for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x, ++turn) {
             const bool wide = tile < plan.wide;
-            const int per = wide ? kM : 16;
             float acc[2][4] = {};
             if (!wait_phase(s_full + 8 * s_slot, s_phase, &abort_flag))
                 gave_up(kStatusTimeoutFull);
@@ -333,22 +333,30 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             }
             if (lane == 0) mbar_arrive(s_empty + 8 * s_slot);
             if (++s_slot == 2) s_slot = 0, s_phase ^= 1;
-            // partial sums [warp][row][output]; with two buffers the next tile's go to the other one, and its barrier
-            // comes after every thread's reads of this one
-            float* const red = reinterpret_cast<float*>(smem + plan.red) + red_buf * warps * rows * kM;
-            if (plan.red_bufs == 2) red_buf ^= 1;
+            // partial sums [tile][warp][row][output]: warps go on to the next tile, and add up when the buffers are full
+            const int per_tile = rows * kM;
+            float* const red = reinterpret_cast<float*>(smem + plan.red) + (turn - added) * warps * per_tile;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (2 * t + (e & 1) < rows) red[(warp * rows + 2 * t + (e & 1)) * kM + m * 16 + (e / 2) * 8 + g] = acc[m][e];
+                    if (2 * t + (e & 1) < rows) red[warp * per_tile + (2 * t + (e & 1)) * kM + m * 16 + (e / 2) * 8 + g] = acc[m][e];
+            const bool last = tile + static_cast<int>(gridDim.x) >= plan.tiles;
+            if (turn + 1 - added < plan.red_bufs && !last) continue;
             consumers_sync(warps);
-            for (int i = threadIdx.x; i < rows * kM; i += warps * 32) {
-                const int r = i / kM, o = tile_row(tile) + i % kM;
-                if (i % kM >= per || o >= n) continue;
-                float v = 0.f;
-                for (int w = 0; w < warps; ++w) v += red[w * rows * kM + i];
-                float* const kept = reinterpret_cast<float*>(smem + plan.accum) + turn * rows * kM + i;
+            for (int i = threadIdx.x; i < (turn + 1 - added) * per_tile; i += warps * 32) {
+                const int nth = i / per_tile, r = i % per_tile / kM, from = tile - (turn - added - nth) * static_cast<int>(gridDim.x);
+                const int o = tile_row(from) + i % kM;
+                if (i % kM >= (from < plan.wide ? kM : 16) || o >= n) continue;
+                const float* const part = reinterpret_cast<float*>(smem + plan.red) + nth * warps * per_tile + i % per_tile;
+                float v = 0.f, v1 = 0.f;
+#pragma unroll 4
+                for (int w = 0; w < warps; w += 2) {
+                    v += part[w * per_tile];
+                    v1 += part[(w + 1) * per_tile];
+                }
+                v += v1;
+                float* const kept = reinterpret_cast<float*>(smem + plan.accum) + added * per_tile + i;
                 if (seg) v += *kept;
                 if (seg_end < blocks) {
                     *kept = v;
@@ -358,7 +366,8 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                     tok_store(a.y, r * a.y_stride + o, a.y_type, v);
                 }
             }
-            if (plan.red_bufs == 1) consumers_sync(warps);
+            added = turn + 1;
+            if (!last) consumers_sync(warps);
         }
     }
 }
@@ -390,7 +399,6 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
     p.wide = a.w.n / kM / sms * sms;
     p.tiles = p.wide + (a.w.n - p.wide * kM + 15) / 16;
     if (p.tiles < sms) *grid = p.tiles;
-    p.red_bufs = rows <= 4 ? 2 : 1;
     p.x = 0;
     p.sums = round_up(rows * p.x_pitch, 128);
     p.sum_pitch = p.seg_blocks * (a.w.group % 128 == 0 ? 1 : a.w.group % 64 == 0 ? 2 : 4) + 1;
@@ -402,10 +410,16 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
         if ((p.tiles + *grid - 1) / *grid > per) *grid = (p.tiles + per - 1) / per;
         p.red += round_up((p.tiles + *grid - 1) / *grid * rows * kM * 4, 128);
     }
-    p.ring = round_up(p.red + p.red_bufs * p.consumers * rows * kM * 4, 1024);
-    const int stage = p.consumers / 2 * kM * 128;
-    p.stages = (kFewSmem - p.ring) / stage;
-    if (p.stages > kMaxStages) p.stages = kMaxStages;
+    // partial sums of as many tiles as have room beside three stages: a warp need not wait for the others at a tile's end
+    // (1 x 8192 -> 28672 f16 31.4 us, 33.5 with two buffers; 8 x 8192 -> 8192 24.5 us with three, 26.5 with one)
+    const int stage = p.consumers / 2 * kM * 128, per_tile = p.consumers * rows * kM * 4;
+    p.red_bufs = std::clamp(48 * 1024 / per_tile, 1, (p.tiles + *grid - 1) / *grid);
+    auto place = [&] {
+        p.ring = round_up(p.red + p.red_bufs * per_tile, 1024);
+        p.stages = std::min((kFewSmem - p.ring) / stage, kMaxStages);
+        return p.stages >= 3 || p.red_bufs == 1;
+    };
+    while (!place()) --p.red_bufs;
     p.bytes = p.ring + p.stages * stage;
     return p;
 }
@@ -440,8 +454,8 @@ cudaError_t launch_few_typed(const W4LinearArgs& a, bool x_vec, cudaStream_t s) 
 }  // namespace
 
 cudaError_t launch_w4_linear(const W4LinearArgs& a, cudaStream_t s) {
-    // 8 rows are an MMA's columns; the kernels meet there (us, few rows' and many rows': 4 x 4096 -> 14336 15.9 and 20.0,
-    // 8 x 4096 -> 4096 10.7 and 10.1, 8 x 4096 -> 14336 18.9 and 19.9, 8 x 8192 -> 28672 55 and 67)
+    // 8 rows are an MMA's columns; the kernels meet there (us, few rows' and many rows': 4 x 4096 -> 14336 15.0 and 20.0,
+    // 8 x 4096 -> 4096 10.1 and 10.1, 8 x 4096 -> 14336 18.0 and 19.9, 8 x 8192 -> 28672 52 and 67)
     if (a.rows > 8) {
         constexpr int kMost = 65535 * 16;  // rows of a launch: 65535 of the smallest tiles
         for (int64_t row0 = 0; row0 < a.rows; row0 += kMost) {
