@@ -13,19 +13,18 @@ namespace {
 // ---- few rows ----------------------------------------------------------------------------------
 // With up to 8 token rows the floor is the weights' way from memory: 4.1 bits a weight, each used once per row. What
 // bounds the kernel before that is the instructions that make operands of the codes and the time a warp's chain of
-// them takes (1 x 8192 -> 28672 f16: 31 us, 3.9 TB/s, 59% of the copy's rate; 1 x 4096 -> 4096: 6.6 us, of which half
-// is launch, first loads and the reduction; 8 x 4096 -> 14336 e4m3 with zero points: 18.9 us). One block per SM walks
+// them takes (1 x 8192 -> 28672 f16: 32 us, 3.7 TB/s, 57% of the copy's rate; 1 x 4096 -> 4096: 6.5 us, of which half
+// is launch, first loads and the reduction; 8 x 4096 -> 14336 e4m3 with zero points: 18.5 us). One block per SM walks
 // over tiles of 32 outputs (the last of them over tiles of 16, so that all blocks have as much to do): a producer warp
 // keeps a ring of TMA boxes, 32 outputs x 256 inputs, ahead of the consumer warps, across tiles, so that memory never
-// waits for a tile's end (a bulk copy for each row of a tile costs its thread some 60 ns); each consumer takes 128 inputs of a stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs,
-// B: inputs x 8 rows), whose 8 columns are what few rows can fill: a tcgen05 operand would have to be written before
-// it is read (all of it: 1 x 4096 -> 4096 9.7 us, 1 x 8192 -> 28672 67). The rows lie in shared memory for the whole
-// walk, converted once and in the MMA's order.
-// A code enters the MMA as offset + code, which costs one logical operation for two; what leaves again in f32, a group
-// at a time, are sums over the rows' inputs alone, made when those are brought in:
-//   sum (code - zero) x = sum (offset + code) x - sum offset x - zero sum x
-// (the difference loses 5 of f32's 24 bits in bf16, 8 in f16: 16 are left for results of 8 and 11). Scales are applied
-// in f32 to a group's sum: no weight is rounded. The consumers' partial sums meet in shared memory.
+// waits for a tile's end (a bulk copy for each row of a tile costs its thread some 60 ns); each consumer takes 128
+// inputs of a stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs, B: inputs x 8 rows), whose 8 columns are
+// what few rows can fill: a tcgen05 operand would have to be written before it is read (all of it: 1 x 4096 -> 4096
+// 9.7 us, 1 x 8192 -> 28672 67). The rows lie in shared memory for the whole walk, converted once and in the MMA's order.
+// A weight enters the MMA as code - zero, a whole number (in bf16 times 2^-11), made of two codes at a time by one
+// logical operation and one packed subtraction, both exact. So every product is exact, the sums hold nothing but the
+// result's own terms, and scales are applied in f32 to the sum of a group's inputs: no weight is rounded. The consumers'
+// partial sums meet in shared memory.
 
 constexpr int kBlockK = 128;  // inputs of a consumer warp in a stage
 constexpr int kMaxConsumers = 16;
@@ -45,32 +44,33 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Nibbles (i, i + 4) of a word of eight codes as two 16-bit floats offset + code, by or'ing them into the mantissa of
-// a power of two. bf16: 128 + code (three shifts for a word's four pairs). f16: 1024 + code, whose last place is one,
-// or 64 + code, whose last place is a sixteenth, wherever the nibble lies (one shift).
+// Nibbles (i, i + 4) of a word of eight codes as two 16-bit floats code - zero, by or'ing them into the mantissa of a
+// power of two and taking off that and the zero point. f16: 1024 + code, whose last place is one, or 64 + code, whose
+// last place is a sixteenth, wherever the nibble lies (one shift for a word's four pairs). bf16: (128 + code) 2^-11
+// (three shifts); the factor keeps the sum of 128 inputs of any size, times up to 15 each, inside f32's range.
 template <bool BF>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
-    if (BF) return and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
-    return and_or(i >= 2 ? w >> 8 : w, i & 1 ? 0x00f000f0u : 0x000f000fu, i & 1 ? 0x54005400u : 0x64006400u);
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, const uint32_t (&offset)[2]) {
+    const uint32_t v = BF ? and_or(w >> (4 * i), 0x000f000fu, 0x3d803d80u)
+                          : and_or(i >= 2 ? w >> 8 : w, i & 1 ? 0x00f000f0u : 0x000f000fu, i & 1 ? 0x54005400u : 0x64006400u);
+    uint32_t r;
+    if (BF)
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(offset[0]));
+    else
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(offset[i & 1]));
+    return r;
 }
+// What code_pair takes off for a zero point, for even and odd i.
+template <bool BF>
+__device__ __forceinline__ void code_offsets(uint32_t zero, uint32_t (&offset)[2]) {
+    offset[0] = (BF ? 0x3d803d80u : 0x64006400u) + 0x00010001u * zero;
+    offset[1] = 0x54005400u + 0x00100010u * zero;
+}
+constexpr float kBackBF16 = 2048.f;  // bf16's factor leaves with the scales' sum
+
 // Eight 16-bit values as the pairs (i, i + 4), i = 0..3: code_pair's order.
 __device__ __forceinline__ uint4 paired(const uint4& v) {
     return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
                       __byte_perm(v.y, v.w, 0x7632));
-}
-
-// Sums over paired eight values: offset x, in code_pair's offsets, and x.
-template <bool BF>
-__device__ __forceinline__ float2 offset_sums(const uint4& v) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float even = 0.f, odd = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = BF ? make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u))
-                            : __half22float2(reinterpret_cast<const __half2&>(w[i]));
-        (i & 1 ? odd : even) += f.x + f.y;
-    }
-    return make_float2(BF ? 128.f * (even + odd) : 1024.f * even + 64.f * odd, even + odd);
 }
 
 // How the few-rows kernel walks and where its parts lie in shared memory; made by the host.
@@ -83,8 +83,7 @@ struct FewPlan {
     int x_pitch;     // of a row's inputs: 64 modulo 128, so that 2 rows x 4 lanes of 16 bytes hit all banks once
     int s_pitch, z_pitch;  // of an output's scales and zero points: 16 modulo 128, so that 8 outputs hit different banks
     int red_bufs;  // tiles whose partial sums have room
-    int sum_pitch;   // of a row's sums over units, in pairs
-    int x, sums, scale, accum, red, ring, bytes;  // offsets; accum: the sums of earlier segments, by tile of this block
+    int x, scale, accum, red, ring, bytes;  // offsets; accum: the sums of earlier segments, by tile of this block
     bool x_vec;
 };
 
@@ -123,14 +122,12 @@ __device__ __forceinline__ void rows_to_shared(uint8_t* to, int dst_pitch, const
 
 // CPF chunks of 32 inputs times MT m-tiles of 16 outputs into acc, under one scale per output. The codes of output
 // m 16 + h 8 (+ this lane's g, in `codes`) lie 128 bytes apart, 16-byte cell c of them at cell c ^ g (cell: of the first
-// chunk); x_at: this lane's row, sum0 and sum1: the sums of its results' rows; scales and zero points as they are stored.
+// chunk); x_at: this lane's row; scales and zero points as they are stored.
 template <bool BF, int CPF, bool Z, int MT>
-__device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_t x_at, const float2* sum0,
-                                     const float2* sum1, int cell, uint32_t s_at, int s_pitch,
+__device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_t x_at, int cell, uint32_t s_at, int s_pitch,
                                      int scale_type, uint32_t z_at, int z_pitch) {
-    uint32_t x[CPF][4], w[MT][2][CPF];
-    float scale[MT][2], zero[MT][2], part[MT][4] = {};
-    const float2 xs[2] = {*sum0, *sum1};
+    uint32_t x[CPF][4], w[MT][2][CPF], offset[MT][2][2];
+    float scale[MT][2], part[MT][4] = {};
 #pragma unroll
     for (int c = 0; c < CPF; ++c) {
         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
@@ -154,11 +151,9 @@ __device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_
                 asm volatile("ld.shared.b16 %0, [%1];" : "=h"(raw) : "r"(at));
                 scale[m][h] = scale_type == kTokF16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float(static_cast<uint32_t>(raw) << 16);
             }
-            if (Z) {
-                uint32_t z;
-                asm volatile("ld.shared.u8 %0, [%1];" : "=r"(z) : "r"(z_at + (m * 16 + h * 8) * z_pitch));
-                zero[m][h] = static_cast<float>(z);
-            }
+            uint32_t zero = 8;
+            if (Z) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(zero) : "r"(z_at + (m * 16 + h * 8) * z_pitch));
+            code_offsets<BF>(zero, offset[m][h]);
         }
 #pragma unroll
     for (int c = 0; c < CPF; ++c)
@@ -166,16 +161,14 @@ __device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_
         for (int i = 0; i < 4; i += 2) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                mma16816<BF>(part[m], code_pair<BF>(w[m][0][c], i), code_pair<BF>(w[m][1][c], i), code_pair<BF>(w[m][0][c], i + 1),
-                             code_pair<BF>(w[m][1][c], i + 1), x[c][i], x[c][i + 1]);
+                mma16816<BF>(part[m], code_pair<BF>(w[m][0][c], i, offset[m][0]), code_pair<BF>(w[m][1][c], i, offset[m][1]),
+                             code_pair<BF>(w[m][0][c], i + 1, offset[m][0]), code_pair<BF>(w[m][1][c], i + 1, offset[m][1]),
+                             x[c][i], x[c][i + 1]);
         }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p = fmaf(Z ? -zero[m][e / 2] : -8.f, xs[e % 2].y, part[m][e] - xs[e % 2].x);
-            acc[m][e] = fmaf(scale[m][e / 2], p, acc[m][e]);
-        }
+        for (int e = 0; e < 4; ++e) acc[m][e] = fmaf(scale[m][e / 2], part[m][e], acc[m][e]);
 }
 
 // CPF: the scale changes every CPF chunks of 32 inputs at most (4: groups are multiples of 128, 2: of 64, 1: of 32);
@@ -269,8 +262,6 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
     }
 
     const uint32_t x_lane = smem_u32(smem + plan.x) + min(g, rows - 1) * plan.x_pitch + t * 16;  // rows past the last: nothing reads their sums
-    const float2* const sum0 = reinterpret_cast<const float2*>(smem + plan.sums) + min(2 * t, rows - 1) * plan.sum_pitch;
-    const float2* const sum1 = reinterpret_cast<const float2*>(smem + plan.sums) + min(2 * t + 1, rows - 1) * plan.sum_pitch;
     const float inv_group = 1.f / static_cast<float>(group);
     for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
         const int seg_end = min(seg + plan.seg_blocks, blocks), g0 = seg * kBlockK / group;
@@ -279,22 +270,9 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             const int kxb = a.x_type == kTokE4M3 ? 1 : 2, eights = min((seg_end - seg) * kBlockK, k - seg * kBlockK) / 8;
             for (int r = 0; r < rows; ++r) {
                 const uint8_t* const p = static_cast<const uint8_t*>(a.x) + (r * a.x_stride + seg * kBlockK) * kxb;
-                float2* const sums = reinterpret_cast<float2*>(smem + plan.sums) + r * plan.sum_pitch;
-                for (int i0 = warp * 32; i0 < eights; i0 += warps * 32) {
-                    const int i = i0 + lane;
-                    float2 f = {};
-                    if (i < eights) {
-                        const uint4 v = paired(widened(raw_eight(p + i * 8 * kxb, a.x_type, plan.x_vec), a.x_type));
-                        *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) = v;
-                        f = offset_sums<BF>(v);
-                    }
-#pragma unroll
-                    for (int o = 2 * CPF; o; o >>= 1) {
-                        f.x += __shfl_xor_sync(0xffffffffu, f.x, o);
-                        f.y += __shfl_xor_sync(0xffffffffu, f.y, o);
-                    }
-                    if (lane % (4 * CPF) == 0 && i < eights) sums[i / (4 * CPF)] = f;
-                }
+                for (int i = warp * 32 + lane; i < eights; i += warps * 32)
+                    *reinterpret_cast<uint4*>(smem + plan.x + r * plan.x_pitch + i * 16) =
+                        paired(widened(raw_eight(p + i * 8 * kxb, a.x_type, plan.x_vec), a.x_type));
             }
         }
         consumers_sync(warps);
@@ -319,12 +297,13 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                         if (CPF < 4 && kc >= k) break;
                         // (kc + 1/2) / group truncated: exact while k < 2^21
                         const int gi = (k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group) - g0;
+                        const int cell = (4 * (warp & 1) + u * CPF) ^ g;
                         if (wide)
-                            unit<BF, CPF, Z, 2>(acc, cw, xw + u * CPF * 64, sum0 + (blk - seg) * kUnits + u, sum1 + (blk - seg) * kUnits + u, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
-                                                a.w.scale_type, z_at + gi, plan.z_pitch);
+                            unit<BF, CPF, Z, 2>(acc, cw, xw + u * CPF * 64, cell, s_at + gi * sb, plan.s_pitch, a.w.scale_type,
+                                                z_at + gi, plan.z_pitch);
                         else
-                            unit<BF, CPF, Z, 1>(acc, cw, xw + u * CPF * 64, sum0 + (blk - seg) * kUnits + u, sum1 + (blk - seg) * kUnits + u, (4 * (warp & 1) + u * CPF) ^ g, s_at + gi * sb, plan.s_pitch,
-                                                a.w.scale_type, z_at + gi, plan.z_pitch);
+                            unit<BF, CPF, Z, 1>(acc, cw, xw + u * CPF * 64, cell, s_at + gi * sb, plan.s_pitch, a.w.scale_type,
+                                                z_at + gi, plan.z_pitch);
                     }
                 }
                 __syncwarp();
@@ -361,6 +340,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                 if (seg_end < blocks) {
                     *kept = v;
                 } else {
+                    if (BF) v *= kBackBF16;
                     if (a.x_scale) v *= a.x_scale[a.x_scale_mode == kScaleRow ? r : 0];
                     if (a.bias) v += a.bias[o];
                     tok_store(a.y, r * a.y_stride + o, a.y_type, v);
@@ -400,9 +380,7 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
     p.tiles = p.wide + (a.w.n - p.wide * kM + 15) / 16;
     if (p.tiles < sms) *grid = p.tiles;
     p.x = 0;
-    p.sums = round_up(rows * p.x_pitch, 128);
-    p.sum_pitch = p.seg_blocks * (a.w.group % 128 == 0 ? 1 : a.w.group % 64 == 0 ? 2 : 4) + 1;
-    p.scale = p.sums + round_up(rows * p.sum_pitch * 8, 128);
+    p.scale = round_up(rows * p.x_pitch, 128);
     p.accum = p.scale + round_up(2 * kM * (p.s_pitch + (a.w.zeros ? p.z_pitch : 0)), 128);
     p.red = p.accum;
     if (p.seg_blocks < blocks) {  // room for the sums of a block's tiles between segments

@@ -434,10 +434,10 @@ fx_status fx_rms_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t 
  * (NULL: 8 everywhere). group is a multiple of 32 that divides k < 2^24; rows and n are any numbers. x is f16,
  * bf16, or e4m3 with x_scale (f32: FX_SCALE_TENSOR one value, FX_SCALE_ROW [rows]); y is f16 or bf16,
  * rounded once; bias is f32 [n] or NULL. Sums are held in f32. y overlaps no input.
- * Up to 8 rows no weight is rounded, but the outputs need 1039 |x| summed over a group to stay in f32's range (f16 and
- * e4m3 always do); from 9 rows on a weight is rounded once to x's 16-bit type (f16 for e4m3, relative to its output's
- * largest scale). A row that holds a NaN or infinity, and an output with such a scale, come out not finite (NaN or
- * infinite, which is not specified); other rows and outputs are untouched by them. Results repeat exactly. */
+ * Up to 8 rows no weight is rounded; from 9 rows on a weight is rounded once to x's 16-bit type (f16 for e4m3, relative
+ * to its output's largest scale). A row that holds a NaN or infinity, and an output with such a scale, come out not
+ * finite (NaN or infinite, which is not specified); other rows and outputs are untouched by them. Results repeat
+ * exactly. */
 fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t x_stride, const float* dev_x_scale,
                        fx_scale x_scale_mode, const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
                        const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, const float* dev_bias,
