@@ -20,12 +20,13 @@ struct ManyPlan {
     int split;            // blocks of a cluster that share a tile, each with a range of k
     int stages_each;      // stages of codes of a block
     int tmem_cols;
-    int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs and stage
+    int weight_col;       // of the weights in TMEM, behind the accumulators: 32 columns per 128 outputs, stage and term
     int raw_slots;        // of e4m3 rows by TMA, 128 inputs each
     bool y_vec;           // results aligned to eight outputs
     int slot_steps;       // steps of 64 inputs that share a slot of the rows' ring
     bool x_tma, x_vec;    // rows come by TMA as they are; rows aligned to eight values
     bool two;             // tiles of 256 outputs
+    bool terms;           // a weight is the sum of two 16-bit values
 };
 
 cudaError_t w4_many_bf16(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s);

@@ -18,7 +18,9 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     // 1024 x 4096 -> 4096 49 and 49, 576 x 4096 -> 14336 109 and 107, 4096 rows 609 and 483)
     auto across = [&](int m) { return (a.w.n + m - 1) / m; };
     auto turns = [&](int m, int most) { return (across(m) * ((static_cast<int64_t>(a.rows) + most - 1) / most) + sms - 1) / sms; };
-    const bool two = p.two = p.x_tma ? turns(256, 192) * 3 < turns(128, 256) * 2 : turns(256, 192) * 11 < turns(128, 256) * 10;
+    // f16 results of bf16 rows hold more bits than a bf16 weight: a weight is two terms there, an MMA each
+    p.terms = a.x_type == kTokBF16 && a.y_type == kTokF16;
+    const bool two = p.two = p.terms ? false : p.x_tma ? turns(256, 192) * 3 < turns(128, 256) * 2 : turns(256, 192) * 11 < turns(128, 256) * 10;
     const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
     const int64_t tiles_n = (static_cast<int64_t>(a.rows) + most_n - 1) / most_n;
     p.tile_n = static_cast<int>((a.rows + tiles_n * 16 - 1) / (tiles_n * 16)) * 16;
@@ -40,7 +42,7 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     // TMEM, all of it (a block's shared memory leaves room for no other block): accumulators, then stages of weights
     p.weight_col = (two ? 2 : 1) * p.tile_n;
     p.tmem_cols = 512;
-    p.rings[1] = std::min((p.tmem_cols - p.weight_col) / (two ? 64 : 32), kMaxRing);
+    p.rings[1] = std::min((p.tmem_cols - p.weight_col) / (two || p.terms ? 64 : 32), kMaxRing);
     // the issuing thread's waits bound short steps: four or two of them share a slot of the rows, as room allows (4096 ->
     // 14336 bf16, us, one step a slot against more: 16 rows 23.6 and 19.5, 128 rows 25.6 and 22.3; 1024 x 4096 -> 4096
     // 28.2 and 26.9)

@@ -15,6 +15,9 @@
 // exact, and the scale enters as the sum of two 16-bit values, one product and one fused multiply-add. In f16
 // each output's weights are divided by the power of two below its largest scale, so that no scale's size
 // overflows the type or sinks below it; the epilogue multiplies by it again.
+// f16 results of bf16 rows hold eight times finer steps than bf16 weights: there a weight is the sum of two bf16 values,
+// right to 2^-15 of it, each multiplied by the rows in an MMA of its own (root mean square error 2.1e-4 of the result's
+// size, f16's own rounding, 1.7e-3 with one term; 64 x 4096 -> 14336 27 us, 20 with one; 4096 rows 605 and 354).
 #pragma once
 
 #include "counters.hpp"
@@ -123,6 +126,22 @@ __device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi,
     }
 }
 
+// The same as the sum of two 16-bit values: the weight rounded, and what that left (exact where EX).
+template <bool BF, bool EX>
+__device__ __forceinline__ void weight_terms16(uint32_t w0, uint32_t w1, uint32_t hi, uint32_t lo, uint32_t z, uint32_t (&out)[8],
+                                               uint32_t (&rest)[8]) {
+    weights16<BF, EX>(w0, w1, hi, lo, z, out);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const uint32_t w = c ? w1 : w0, w4 = BF ? w >> 4 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = code_pair_in_order<BF>(w, w4, i, z), left = fma2<BF>(v, hi, out[4 * c + i] ^ 0x80008000u);
+            rest[4 * c + i] = EX ? left : fma2<BF>(v, lo, left);
+        }
+    }
+}
+
 // Warps: 0..15 weights and epilogue, 16 codes by TMA, 17 MMA and TMEM, 18 rows by TMA, or 18..21 rows
 // that have to be widened or loaded.
 // TWO: 256 outputs a tile in two accumulators, else 128.
@@ -132,8 +151,8 @@ constexpr int kMakers = 16;
 // constant: the issuing thread has no time to spare).
 // CH: scales of a step of 64 inputs (1: groups are multiples of 64). EX: the scales' type is the
 // operands', so that they have no second term (in f16 but for those 2^14 below their output's largest, whose last bits
-// are 2^-25 of it).
-template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX>
+// are 2^-25 of it). TERMS: a weight is two terms.
+template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX, bool TERMS>
 __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
                    const __grid_constant__ CUtensorMap rows_map) {
@@ -141,7 +160,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     __shared__ __align__(8) uint64_t bars[7 * kMaxRing + 1];
     __shared__ uint32_t tmem_at;
     __shared__ volatile int abort_flag;
-    constexpr int kTileM = TWO ? 256 : 128;
+    static_assert(!(TWO && TERMS), "two blocks of weights a step at most");
+    constexpr int kTileM = TWO ? 256 : 128, kWeightCols = TWO || TERMS ? 64 : 32;  // of a step
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int n = a.w.n, k = a.w.k, group = a.w.group, groups = k / group;
     const int tile_n = plan.tile_n, rank = plan.split > 1 ? static_cast<int>(blockIdx.x) % plan.split : 0;
@@ -230,10 +250,11 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             tc_fence_after();
             const uint64_t bd = desc_sw128(xrows + (xs * SS + x_step) * tile_n * 128);
 #pragma unroll
-            for (int m = 0; m < (TWO ? 2 : 1); ++m) {
-                const uint32_t ad = plan.weight_col + (ws * (TWO ? 2 : 1) + m) * 32;
+            for (int m = 0; m < kWeightCols / 32; ++m) {
+                const uint32_t ad = plan.weight_col + ws * kWeightCols + m * 32;
 #pragma unroll
-                for (int i = 0; i < kStepK / 16; ++i) mma_f16_ta_if(issue, m * tile_n, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0);
+                for (int i = 0; i < kStepK / 16; ++i)
+                    mma_f16_ta_if(issue, TWO ? m * tile_n : 0, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0 || (TERMS && m > 0));
             }
             mma_commit_if(issue, w_empty + 8 * ws);
             if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
@@ -404,14 +425,29 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                                  : "=r"(w[h][0]), "=r"(w[h][1]), "=r"(w[h][2]), "=r"(w[h][3])
                                  : "r"(from + (((2 * (c * kSets + set) + h) ^ (row & 7)) << 4)));
-                uint32_t out[4][8];
+                const uint32_t slot = to + ws * kWeightCols;
+                if constexpr (TERMS) {  // sixteen weights at a time: both terms of all would not fit the registers
+                    if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
+                    tc_fence_after();
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                    weights16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH], z[c][h / 2 % CH], out[h]);
-                if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
-                tc_fence_after();
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t out[8], rest[8];
+                        weight_terms16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH],
+                                               z[c][h / 2 % CH], out, rest);
+                        tmem_st8(slot + 8 * h, out);
+                        tmem_st8(slot + 32 + 8 * h, rest);
+                    }
+                } else {
+                    uint32_t out[4][8];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) tmem_st8(to + ws * (TWO ? 64 : 32) + 8 * h, out[h]);
+                    for (int h = 0; h < 4; ++h)
+                        weights16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH],
+                                          z[c][h / 2 % CH], out[h]);
+                    if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
+                    tc_fence_after();
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) tmem_st8(slot + 8 * h, out[h]);
+                }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -509,10 +545,10 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     }
 }
 
-template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX>
+template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX, bool TERMS>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     constexpr int kTileM = TWO ? 256 : 128;
-    auto* kern = w4_many_kernel<BF, TWO, TMA, SS, CH, EX>;
+    auto* kern = w4_many_kernel<BF, TWO, TMA, SS, CH, EX, TERMS>;
     CUtensorMap codes, rows;
     cudaError_t e = tmap_rows(&codes, a.w.codes, 8, a.w.k / 16, a.w.n, a.w.k / 2, kTileM);
     if (e == cudaSuccess) {
@@ -541,14 +577,18 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-template <bool BF, bool TWO, bool TMA, int SS>
+template <bool BF, bool TWO, bool TMA, int SS, bool TERMS = false>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     const bool exact = a.w.scale_type == (BF ? kTokBF16 : kTokF16);
-    if (a.w.group % kStepK == 0) return exact ? launch<BF, TWO, TMA, SS, 1, true>(a, p, s) : launch<BF, TWO, TMA, SS, 1, false>(a, p, s);
-    return exact ? launch<BF, TWO, TMA, SS, 2, true>(a, p, s) : launch<BF, TWO, TMA, SS, 2, false>(a, p, s);
+    if (a.w.group % kStepK == 0) return exact ? launch<BF, TWO, TMA, SS, 1, true, TERMS>(a, p, s) : launch<BF, TWO, TMA, SS, 1, false, TERMS>(a, p, s);
+    return exact ? launch<BF, TWO, TMA, SS, 2, true, TERMS>(a, p, s) : launch<BF, TWO, TMA, SS, 2, false, TERMS>(a, p, s);
 }
 template <bool BF>
 cudaError_t launch_typed(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
+    if constexpr (BF) {
+        if (p.terms && p.slot_steps == 2) return p.x_tma ? launch<BF, false, true, 2, true>(a, p, s) : launch<BF, false, false, 2, true>(a, p, s);
+        if (p.terms) return p.x_tma ? launch<BF, false, true, 4, true>(a, p, s) : launch<BF, false, false, 4, true>(a, p, s);
+    }
     if (p.two) return p.x_tma ? launch<BF, true, true, 1>(a, p, s) : launch<BF, true, false, 1>(a, p, s);
     if (p.slot_steps == 1) return p.x_tma ? launch<BF, false, true, 1>(a, p, s) : launch<BF, false, false, 1>(a, p, s);
     if (p.slot_steps == 2) return p.x_tma ? launch<BF, false, true, 2>(a, p, s) : launch<BF, false, false, 2>(a, p, s);

@@ -14,7 +14,7 @@ cudaError_t w4_many_clusters(int size, int* count) {
     cudaGetDevice(&dev);
     *count = dev < 64 ? known[dev][size].load(std::memory_order_relaxed) : 0;
     if (*count) return cudaSuccess;
-    auto* kern = w4_many_kernel<true, false, true, 4, 1, true>;  // as any other: a block has its SM to itself
+    auto* kern = w4_many_kernel<true, false, true, 4, 1, true, false>;  // as any other: a block has its SM to itself
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};

@@ -435,9 +435,9 @@ fx_status fx_rms_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t 
  * bf16, or e4m3 with x_scale (f32: FX_SCALE_TENSOR one value, FX_SCALE_ROW [rows]); y is f16 or bf16,
  * rounded once; bias is f32 [n] or NULL. Sums are held in f32. y overlaps no input.
  * Up to 8 rows no weight is rounded; from 9 rows on a weight is rounded once to x's 16-bit type (f16 for e4m3, relative
- * to its output's largest scale). A row that holds a NaN or infinity, and an output with such a scale, come out not
- * finite (NaN or infinite, which is not specified); other rows and outputs are untouched by them. Results repeat
- * exactly. */
+ * to its output's largest scale), or to the sum of two bf16 values where x is bf16 and y f16. A row that holds a NaN
+ * or infinity, and an output with such a scale, come out not finite (NaN or infinite, which is not specified); other
+ * rows and outputs are untouched by them. Results repeat exactly. */
 fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t x_stride, const float* dev_x_scale,
                        fx_scale x_scale_mode, const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
                        const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, const float* dev_bias,

@@ -98,3 +98,33 @@ def test_bf16_rows_at_the_ends_of_the_range(cuda_torch, rows, power):
         y = linear(torch, x, "bf16", "bf16", codes, scales, "f32", zp, group)
         want = x.double() @ unpack(torch, codes, scales, zp, group).t()
         assert torch.equal(y, want.float().bfloat16())
+
+
+@pytest.mark.parametrize("rows", [9, 20, 128, 130, 257, 513])
+@pytest.mark.parametrize("st,zeros,group", [("f16", False, 128), ("f32", True, 64), ("bf16", True, 32)])
+def test_f16_results_of_many_bf16_rows(cuda_torch, rows, st, zeros, group):
+    """A result held in 11 bits is not made of weights held in 8. A weight is two bf16 terms (and so is a scale of
+    more bits): off by at most HALF^2 each, 2^-15 |w| together, with an input's sign, so that 4 2^-15 sqrt(sum (w x)^2)
+    bounds their sum as in test_token_gpu, and one rounding to f16 remains."""
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    worst = 0.0
+    for n, k, stride, kind in ((200, 512, 0, "random"), (700, 2048, 0, "random"), (65, 1152, 1160, "one sign"),
+                               (130, 512, 515, "random")):
+        codes, scales, zp = base.make_layer(torch, n, k, group, st, zeros, g, False)
+        _, x = base.rows_of(torch, rows, k, torch.bfloat16, stride)
+        x.copy_(torch.randn(rows, k, generator=g, device="cuda"))
+        if kind == "one sign":
+            x.abs_()
+        y = torch.empty(rows, n, dtype=torch.float16, device="cuda")
+        fx.w4_linear_dev(ptr(x), ptr(y), rows, n, k, group, ptr(codes), ptr(scales), ptr(zp), "bf16", "f16", st, stride,
+                         stream=stream(torch))
+        torch.cuda.synchronize()
+        xv, w = x.double(), unpack(torch, codes, scales, zp, group)
+        want = xv @ w.t()
+        lim = (4 * 2.0 ** -15 * (xv.square() @ w.square().t()).sqrt() + k / 16 * 2.0 ** -22 * (xv.abs() @ w.abs().t())
+               + (HALF["f16"] + 4 * U) * want.abs() + TINY["f16"])
+        err = (y.double() - want).abs()
+        worst = max(worst, (err / lim).max().item())
+        print(rows, st, n, k, "rms error / rms result %.2e" % (err.square().mean().sqrt() / want.square().mean().sqrt()).item())
+    assert worst <= 1, worst
