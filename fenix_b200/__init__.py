@@ -207,6 +207,7 @@ def lib():
                                  i32, vp])
     _sig(L, "fx_w4_linear", i32, [vp, i32, i64, i64, vp, i32, vp, vp, i32, vp, i64, i64, i64, vp, vp, i32, i64, vp])
     _sig(L, "fx_w4_device_status", i32, [i32])
+    _sig(L, "fx_selftest_w4_wait_timeout", i32, [i32, i32, i32, C.c_uint64])
     _sig(L, "fx_w4_quantize", i32, [vp, i32, i64, i64, i64, i64, vp, vp, i32, vp, vp])
     _sig(L, "fx_w4_dequantize", i32, [vp, vp, i32, vp, i64, i64, i64, vp, i32, i64, vp])
     _lib = L

@@ -48,6 +48,8 @@ struct W4LinearArgs {
     int64_t x_stride, y_stride;
     int rows;
     int x_type, x_scale_mode, y_type;
+    bool hold_codes;   // failure self-test only: no codes are brought, so that the waits for them run out
+    uint64_t wait_ns;  // limit of each wait inside the kernel
 };
 cudaError_t launch_w4_linear(const W4LinearArgs& a, cudaStream_t s);
 // codes, scales and zeros of w are written

@@ -35,6 +35,7 @@ int sm_count() {
 namespace {
 
 constexpr int64_t kMaxExtent = int64_t{1} << 30;  // rows, columns and strides: byte offsets stay below 2^62
+constexpr uint64_t kWaitNs = 2000000000;          // limit of a wait inside a 4-bit linear kernel
 constexpr int64_t kMaxInner = int64_t{1} << 24;   // k of a 4-bit layer: 32-bit offsets inside 128 of its rows
 
 fx_status bad(const char* fn, const char* what) {
@@ -235,6 +236,7 @@ fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t
         a.x_type = x_type;
         a.x_scale_mode = x_scale_mode;
         a.y_type = y_type;
+        a.wait_ns = kWaitNs;
         return done(fn, fxk::launch_w4_linear(a, static_cast<cudaStream_t>(stream)));
     });
 }
@@ -259,6 +261,52 @@ fx_status fx_w4_device_status(int device) {
         if (few || bf16 || f16)
             return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(few ? few : bf16 ? bf16 : f16));
         return FX_OK;
+    });
+}
+
+fx_status fx_selftest_w4_wait_timeout(int device, fx_dtype x_type, int rows, uint64_t wait_ns) {
+    static const char* const fn = "fx_selftest_w4_wait_timeout";
+    return guarded([&]() -> fx_status {
+        int count = 0;
+        if (x_type != FX_F16 && x_type != FX_BF16 && x_type != FX_E4M3) return bad(fn, "x is f16, bf16 or e4m3");
+        if (rows < 1 || rows > 4096 || wait_ns == 0) return bad(fn, "rows must be 1..4096 and the limit positive");
+        if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
+            cudaGetLastError();
+            return bad(fn, "no such device");
+        }
+        constexpr int kOut = 1024, kIn = 4096, kGroup = 128;
+        struct Scratch {  // zeros: the layer's operands and results
+            int back = -1;
+            void* p = nullptr;
+            ~Scratch() {
+                cudaFree(p);
+                if (back >= 0) cudaSetDevice(back);
+            }
+        } sc;
+        cudaGetDevice(&sc.back);
+        const size_t codes = size_t{kOut} * kIn / 2, scales = size_t{kOut} * kIn / kGroup * 2, x = size_t(rows) * kIn * 2,
+                     y = size_t(rows) * kOut * 2, all = codes + scales + x + y + 256;
+        cudaError_t e = cudaSetDevice(device);
+        if (e == cudaSuccess) e = cudaMalloc(&sc.p, all);
+        if (e == cudaSuccess) e = cudaMemset(sc.p, 0, all);
+        if (e != cudaSuccess) return done(fn, e);
+        uint8_t* const at = static_cast<uint8_t*>(sc.p);
+        fxk::W4LinearArgs a{};
+        a.w = w4_args(at, at + codes, FX_F16, nullptr, kOut, kIn, kGroup);
+        a.x = at + codes + scales;
+        a.y = at + codes + scales + x;
+        a.x_scale = x_type == FX_E4M3 ? reinterpret_cast<const float*>(at + codes + scales + x + y) : nullptr;
+        a.x_scale_mode = x_type == FX_E4M3 ? FX_SCALE_TENSOR : FX_SCALE_NONE;
+        a.x_stride = kIn;
+        a.y_stride = kOut;
+        a.rows = rows;
+        a.x_type = x_type;
+        a.y_type = x_type == FX_BF16 ? FX_BF16 : FX_F16;
+        a.hold_codes = true;
+        a.wait_ns = wait_ns;
+        e = fxk::launch_w4_linear(a, nullptr);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        return done(fn, e);
     });
 }
 

@@ -215,7 +215,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
     if (warp == warps) {  // codes
         if (lane) return;
         int issued = 0;
-        for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
+        for (int seg = 0; seg < blocks && !a.hold_codes; seg += plan.seg_blocks) {
             const int seg_end = min(seg + plan.seg_blocks, blocks);
             for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x) {
                 const bool wide = tile < plan.wide;
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                 const int o0 = tile_row(tile), box_bytes = (wide ? kM : 16) * 128;
                 for (int blk = seg; blk < seg_end; blk += warps) {
                     const int boxes = (min(warps, seg_end - blk) + 1) / 2;  // of 256 inputs; past the end they read as zeros
-                    if (!wait_phase(empty + 8 * slot, phase ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                    if (!wait_phase(empty + 8 * slot, phase ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
                     if (abort_flag) break;
                     mbar_arrive_expect_tx(full + 8 * slot, boxes * box_bytes);
                     for (int i = 0; i < boxes; ++i)
@@ -233,11 +233,11 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                 }
             }
         }
-        if (abort_flag)  // the consumers no longer wait for the copies still on their way
-            for (int i = min(issued, plan.stages); i > 0; --i) {
-                if (slot-- == 0) slot = plan.stages - 1, phase ^= 1;
-                wait_phase(full + 8 * slot, phase, nullptr);
-            }
+        // consumers that give up, now or later, no longer wait for the copies still on their way
+        for (int i = min(issued, plan.stages); i > 0; --i) {
+            if (slot-- == 0) slot = plan.stages - 1, phase ^= 1;
+            wait_phase(full + 8 * slot, phase, nullptr, a.wait_ns);
+        }
         return;
     }
     const int sb = a.w.scale_type == kTokF32 ? 4 : 2;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
             const int seg_end = min(seg + plan.seg_blocks, blocks);
             const int g0 = seg * kBlockK / group, gn = (min(seg_end * kBlockK, k) - 1) / group + 1 - g0;
             for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x) {
-                if (!wait_phase(s_empty + 8 * s_slot, s_phase ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                if (!wait_phase(s_empty + 8 * s_slot, s_phase ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
                 uint8_t* const to = smem + plan.scale + s_slot * s_bytes;
                 const int o0 = tile_row(tile), per = min(tile < plan.wide ? kM : 16, n - o0);
                 const int64_t at = static_cast<int64_t>(o0) * groups + g0;
@@ -280,13 +280,13 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
         for (int tile = blockIdx.x; tile < plan.tiles; tile += gridDim.x, ++turn) {
             const bool wide = tile < plan.wide;
             float acc[2][4] = {};
-            if (!wait_phase(s_full + 8 * s_slot, s_phase, &abort_flag))
+            if (!wait_phase(s_full + 8 * s_slot, s_phase, &abort_flag, a.wait_ns))
                 gave_up(kStatusTimeoutFull);
             const uint32_t s_at = smem_u32(smem + plan.scale + s_slot * s_bytes) + g * plan.s_pitch;
             const uint32_t z_at = smem_u32(smem + plan.scale + s_slot * s_bytes) + kM * plan.s_pitch + g * plan.z_pitch;
             for (int blk0 = seg; blk0 < seg_end; blk0 += warps) {
                 const int blk = blk0 + warp, k0 = blk * kBlockK;
-                if (!wait_phase(full + 8 * slot, phase, &abort_flag))
+                if (!wait_phase(full + 8 * slot, phase, &abort_flag, a.wait_ns))
                     gave_up(kStatusTimeoutFull);
                 if (blk < seg_end) {
                     const uint32_t cw = ring + slot * stage_bytes + warp / 2 * kM * 128 + g * 128 + t * 4;

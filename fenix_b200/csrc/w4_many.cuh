@@ -207,15 +207,15 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
         if (lane == 0) {
             int cs = 0;
             uint32_t cp = 0;
-            for (int st = 0; st < stages; ++st) {
-                if (!wait_phase(c_empty + 8 * cs, cp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+            for (int st = 0; st < stages && !a.hold_codes; ++st) {
+                if (!wait_phase(c_empty + 8 * cs, cp ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
                 if (abort_flag) break;
                 mbar_arrive_expect_tx(c_full + 8 * cs, kTileM * 128);
                 tma_load_2d(codes + cs * kTileM * 128, &codes_map, (k_begin + st * kStageK) / 16, o0, c_full + 8 * cs);
                 if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
             }
-            if (abort_flag)  // copies still on their way; the waits end by themselves
-                for (int i = 0; i < plan.rings[0]; ++i) wait_phase(c_full + 8 * i, (i < cs ? cp : cp ^ 1), nullptr);
+            // copies still on their way, which roles that give up, now or later, no longer wait for
+            for (int i = 0; i < plan.rings[0]; ++i) wait_phase(c_full + 8 * i, (i < cs ? cp : cp ^ 1), nullptr, a.wait_ns);
         }
         __syncwarp();
     } else if (TMA && warp == 18) {  // not the codes' thread: neither ring's waits hold up the other
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             uint32_t xp = 0;
             for (int step = 0; step < steps; step += SS) {
                 const int boxes = min(SS, steps - step);
-                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+                if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
                 if (abort_flag) break;
                 mbar_arrive_expect_tx(x_full + 8 * xs, boxes * tile_n * 128);
                 for (int i = 0; i < boxes; ++i)
@@ -232,8 +232,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                                 x_full + 8 * xs);
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
-            if (abort_flag)
-                for (int i = 0; i < plan.rings[2]; ++i) wait_phase(x_full + 8 * i, (i < xs ? xp : xp ^ 1), nullptr);
+            for (int i = 0; i < plan.rings[2]; ++i) wait_phase(x_full + 8 * i, (i < xs ? xp : xp ^ 1), nullptr, a.wait_ns);
         }
         __syncwarp();
     } else if (warp == 17) {
@@ -245,8 +244,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
         int ws = 0, xs = 0, x_step = 0;
         uint32_t wp = 0, xp = 0;
         for (int step = 0; step < steps; ++step) {
-            if (x_step == 0 && !wait_phase(x_full + 8 * xs, xp, &abort_flag)) gave_up(kStatusTimeoutFull);
-            if (!wait_phase(w_full + 8 * ws, wp, &abort_flag)) gave_up(kStatusTimeoutFull);
+            if (x_step == 0 && !wait_phase(x_full + 8 * xs, xp, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
+            if (!wait_phase(w_full + 8 * ws, wp, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
             tc_fence_after();
             const uint64_t bd = desc_sw128(xrows + (xs * SS + x_step) * tile_n * 128);
 #pragma unroll
@@ -264,7 +263,10 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
         }
-        if (steps) mma_commit_if(issue, done);
+        if (steps) {
+            mma_commit_if(issue, done);
+            wait_phase(done, 0, nullptr, a.wait_ns);  // the epilogue may have given up: no MMA outlives its TMEM
+        }
     } else if (!TMA && warp >= 18) {
         // rows that TMA does not bring as they are used: four warps write them in 16-byte cells of eight values, as the
         // swizzle places them
@@ -285,10 +287,10 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             if (SS < kRowWarps && step / SS * SS >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
             const int xs = step / SS % plan.rings[2];
             const uint32_t xp = step / SS / plan.rings[2] & 1, rp = pair / slots & 1;
-            if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag)) gave_up(kStatusTimeoutEmpty);
+            if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
             uint8_t* const to = smem + plan.rows + (xs * SS + step % SS) * tile_n * 128;
             if (step < steps && plan.raw_slots) {
-                if (!wait_phase(raw_full + 8 * rs, rp, &abort_flag)) gave_up(kStatusTimeoutFull);
+                if (!wait_phase(raw_full + 8 * rs, rp, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
                 // eight lanes take a cell of eight rows each: every bank once, read and written
                 const int at = lane % 8, c = lane / 8;
                 const uint8_t* const raw = smem + plan.raw + rs * tile_n * 128 + at * 128 + (((4 * (step % 2) + c) ^ at) << 4);
@@ -322,8 +324,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
         __syncwarp();
         if (abort_flag)  // copies still on their way: either phase may be the last that was asked for
             for (int i = 0; i < plan.raw_slots; ++i) {
-                wait_phase(raw_full + 8 * i, 0, nullptr);
-                wait_phase(raw_full + 8 * i, 1, nullptr);
+                wait_phase(raw_full + 8 * i, 0, nullptr, a.wait_ns);
+                wait_phase(raw_full + 8 * i, 1, nullptr, a.wait_ns);
             }
     } else {
         // a thread makes weights of one output, whose TMEM lane is its own; the four warps of a lane quarter take the steps
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                     z[c][h] = zero_terms<BF>(zo[c][h]);
                 }
             load_scales(k_begin + (st + 1) * kStageK);
-            if (!wait_phase(c_full + 8 * cs, cp, &abort_flag)) gave_up(kStatusTimeoutFull);
+            if (!wait_phase(c_full + 8 * cs, cp, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
             const uint32_t from = codes + cs * kTileM * 128 + row * 128;
 #pragma unroll
             for (int c = 0; c < kMine; ++c) {
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                                  : "r"(from + (((2 * (c * kSets + set) + h) ^ (row & 7)) << 4)));
                 const uint32_t slot = to + ws * kWeightCols;
                 if constexpr (TERMS) {  // sixteen weights at a time: both terms of all would not fit the registers
-                    if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
+                    if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAccFree);
                     tc_fence_after();
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                     for (int h = 0; h < 4; ++h)
                         weights16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH],
                                           z[c][h / 2 % CH], out[h]);
-                    if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag)) gave_up(kStatusTimeoutAccFree);
+                    if (!wait_phase(w_empty + 8 * ws, wp ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAccFree);
                     tc_fence_after();
 #pragma unroll
                     for (int h = 0; h < 4; ++h) tmem_st8(slot + 8 * h, out[h]);
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
         }
         // epilogue: a warp reads its TMEM lanes; the warps of a tile's quarter share its columns, eight at a time
-        if (steps && !wait_phase(done, 0, &abort_flag)) gave_up(kStatusTimeoutAcc);
+        if (steps && !wait_phase(done, 0, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAcc);
         tc_fence_after();
         const int out = o0 + row;
         const float bias = a.bias && out < n ? a.bias[out] : 0.f;

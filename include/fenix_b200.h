@@ -447,6 +447,11 @@ fx_status fx_w4_linear(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t
  * wait is bounded; such a kernel ends by itself and its outputs are undefined). Synchronises the device. */
 fx_status fx_w4_device_status(int device);
 
+/* Failure self-test of those waits: one layer of 1024 outputs and 4096 inputs over `rows` rows of x_type (f16, bf16,
+ * e4m3) on `device` whose codes are never brought, with a limit of wait_ns a wait. FX_OK once the launch has ended by
+ * itself; fx_w4_device_status then reports the wait that gave up, and the context stays usable. Synchronises. */
+fx_status fx_selftest_w4_wait_timeout(int device, fx_dtype x_type, int rows, uint64_t wait_ns);
+
 /* The 4-bit form of weights [n][k] (f32, f16, bf16) in fx_w4_linear's layout, one scale (and zero point) per
  * `group` inputs, each quotient rounded to nearest, ties to even:
  *   dev_zeros NULL  scale = max |w| / 7 rounded to scale_type, code = clamp(round(w / scale) + 8, 0, 15)
