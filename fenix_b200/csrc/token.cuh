@@ -57,23 +57,20 @@ cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, cons
 cudaError_t launch_w4_dequantize(const W4Args& q, void* w, int w_type, int64_t w_stride, cudaStream_t s);
 
 #ifdef __CUDACC__
+// f32, f16 or bf16
 __device__ __forceinline__ float tok_load(const void* p, int64_t i, int type) {
     if (type == kTokF32) return static_cast<const float*>(p)[i];
     if (type == kTokF16) return __half2float(static_cast<const __half*>(p)[i]);
-    if (type == kTokBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    __half_raw h = __nv_cvt_fp8_to_halfraw(static_cast<const __nv_fp8_storage_t*>(p)[i], __NV_E4M3);
-    return __half2float(__half(h));
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
-// v rounded to nearest; f16 past its range becomes infinite, e4m3 saturates
+// v rounded to nearest; f16 past its range becomes infinite
 __device__ __forceinline__ void tok_store(void* p, int64_t i, int type, float v) {
     if (type == kTokF32)
         static_cast<float*>(p)[i] = v;
     else if (type == kTokF16)
         static_cast<__half*>(p)[i] = __float2half_rn(v);
-    else if (type == kTokBF16)
-        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
     else
-        static_cast<__nv_fp8_storage_t*>(p)[i] = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+        static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 #endif
 

@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * tile_n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows) - r0, static_cast<int64_t>(tile_n)));
     const int k_begin = rank * plan.stages_each * kStageK, k_end = min(k, k_begin + plan.stages_each * kStageK);
-    const int stages = k_begin < k_end ? (k_end - k_begin + kStageK - 1) / kStageK : 0;
-    const int steps = k_begin < k_end ? (k_end - k_begin + kStepK - 1) / kStepK : 0;
+    const int stages = (k_end - k_begin + kStageK - 1) / kStageK;  // at least one: the planner's split
+    const int steps = (k_end - k_begin + kStepK - 1) / kStepK;
     const uint32_t bar = smem_u32(bars);
     const uint32_t c_full = bar, c_empty = bar + 8 * kMaxRing, w_full = bar + 16 * kMaxRing, w_empty = bar + 24 * kMaxRing,
                    x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, raw_full = bar + 48 * kMaxRing, done = bar + 56 * kMaxRing;
@@ -263,10 +263,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
         }
-        if (steps) {
-            mma_commit_if(issue, done);
-            wait_phase(done, 0, nullptr, a.wait_ns);  // the epilogue may have given up: no MMA outlives its TMEM
-        }
+        mma_commit_if(issue, done);
+        wait_phase(done, 0, nullptr, a.wait_ns);  // the epilogue may have given up: no MMA outlives its TMEM
     } else if (!TMA && warp >= 18) {
         // rows that TMA does not bring as they are used: four warps write them in 16-byte cells of eight values, as the
         // swizzle places them
@@ -461,7 +459,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             if (++cs == plan.rings[0]) cs = 0, cp ^= 1;
         }
         // epilogue: a warp reads its TMEM lanes; the warps of a tile's quarter share its columns, eight at a time
-        if (steps && !wait_phase(done, 0, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAcc);
+        if (!wait_phase(done, 0, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAcc);
         tc_fence_after();
         const int out = o0 + row;
         const float bias = a.bias && out < n ? a.bias[out] : 0.f;
@@ -479,7 +477,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             tmem_regs_ready(v);
             float f[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) f[i] = steps ? __uint_as_float(v[i]) * back : 0.f;
+            for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]) * back;
             if (plan.split > 1) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) partial[(c + i) * kTileM + row] = f[i];
@@ -592,7 +590,6 @@ cudaError_t launch_typed(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t 
         if (p.terms) return p.x_tma ? launch<BF, false, true, 4, true>(a, p, s) : launch<BF, false, false, 4, true>(a, p, s);
     }
     if (p.two) return p.x_tma ? launch<BF, true, true, 1>(a, p, s) : launch<BF, true, false, 1>(a, p, s);
-    if (p.slot_steps == 1) return p.x_tma ? launch<BF, false, true, 1>(a, p, s) : launch<BF, false, false, 1>(a, p, s);
     if (p.slot_steps == 2) return p.x_tma ? launch<BF, false, true, 2>(a, p, s) : launch<BF, false, false, 2>(a, p, s);
     return p.x_tma ? launch<BF, false, true, 4>(a, p, s) : launch<BF, false, false, 4>(a, p, s);
 }
