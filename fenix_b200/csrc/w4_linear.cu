@@ -92,8 +92,9 @@ constexpr int kMaxStages = 6;
 
 __device__ __forceinline__ void consumers_sync(int warps) { asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory"); }
 
-// Bytes [0, bytes) of each of `rows` rows, `src_pitch` apart, to shared memory rows `dst_pitch` apart by one warp,
-// asynchronously in pieces of UNIT bytes where the addresses allow it (the caller's mbarrier arrival follows them).
+// Bytes [0, bytes) of each of `rows` rows, `src_pitch` apart, to shared memory rows `dst_pitch` apart by one warp:
+// asynchronously in pieces of UNIT bytes where the addresses allow it, else by plain stores, byte by byte (the result:
+// whether asynchronously).
 template <int UNIT>
 __device__ __forceinline__ void rows_async(uint32_t dst, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
     const int lane = threadIdx.x % 32;
@@ -105,19 +106,20 @@ __device__ __forceinline__ void rows_async(uint32_t dst, int dst_pitch, const ui
                 asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + r * dst_pitch + at), "l"(src + r * src_pitch + at) : "memory");
         }
 }
-__device__ __forceinline__ void rows_to_shared(uint8_t* to, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
+__device__ __forceinline__ bool rows_to_shared(uint8_t* to, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
     const int64_t all = static_cast<int64_t>(reinterpret_cast<uintptr_t>(src)) | src_pitch;
     if (all % 16 == 0 && bytes % 16 == 0) {
         rows_async<16>(smem_u32(to), dst_pitch, src, src_pitch, rows, bytes);
+        return true;
     } else if (all % 4 == 0 && bytes % 4 == 0) {
         rows_async<4>(smem_u32(to), dst_pitch, src, src_pitch, rows, bytes);
-    } else {
-        const int lane = threadIdx.x % 32;
-        for (int r = lane / 4; r < rows; r += 8)
-#pragma unroll 8
-            for (int at = lane % 4; at < bytes; at += 4) to[r * dst_pitch + at] = __ldg(src + r * src_pitch + at);
-        __threadfence_block();
+        return true;
     }
+    const int lane = threadIdx.x % 32;
+    for (int r = lane / 4; r < rows; r += 8)
+#pragma unroll 8
+        for (int at = lane % 4; at < bytes; at += 4) to[r * dst_pitch + at] = __ldg(src + r * src_pitch + at);
+    return false;
 }
 
 // CPF chunks of 32 inputs times MT m-tiles of 16 outputs into acc, under one scale per output. The codes of output
@@ -251,9 +253,15 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                 uint8_t* const to = smem + plan.scale + s_slot * s_bytes;
                 const int o0 = tile_row(tile), per = min(tile < plan.wide ? kM : 16, n - o0);
                 const int64_t at = static_cast<int64_t>(o0) * groups + g0;
-                rows_to_shared(to, plan.s_pitch, static_cast<const uint8_t*>(a.w.scales) + at * sb, static_cast<int64_t>(groups) * sb, per, gn * sb);
-                if (Z) rows_to_shared(to + kM * plan.s_pitch, plan.z_pitch, a.w.zeros + at, groups, per, gn);
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(s_full + 8 * s_slot) : "memory");
+                bool async = rows_to_shared(to, plan.s_pitch, static_cast<const uint8_t*>(a.w.scales) + at * sb,
+                                            static_cast<int64_t>(groups) * sb, per, gn * sb);
+                if (Z) async &= rows_to_shared(to + kM * plan.s_pitch, plan.z_pitch, a.w.zeros + at, groups, per, gn);
+                if (async) {
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(s_full + 8 * s_slot) : "memory");
+                } else {  // an arrival of this thread's own, which releases its plain stores, too
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    mbar_arrive(s_full + 8 * s_slot);
+                }
                 if (++s_slot == 2) s_slot = 0, s_phase ^= 1;
             }
         }
