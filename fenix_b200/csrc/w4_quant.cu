@@ -146,7 +146,9 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const void* __res
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    const float scale = round_scale(q.zeros ? __fdiv_rn(hi - lo, 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f), q.scale_type);
+    float range = q.zeros ? hi - lo : fmaxf(hi, -lo), steps = q.zeros ? 15.f : 7.f;
+    if (range == INFINITY && q.zeros) range = 0.5f * hi - 0.5f * lo, steps = 7.5f;  // past f32's largest value: halves
+    const float scale = round_scale(__fdiv_rn(range, steps), q.scale_type);
     float zero = 8.f;
     if (q.zeros) zero = scale > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(-lo, scale)), 0.f), 15.f) : 0.f;
     if (on && me == 0) {

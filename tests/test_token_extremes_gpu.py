@@ -1,0 +1,35 @@
+"""The token-row calls at the ends of f32's range, where a sum, a difference or a reciprocal of the formulas' leaves it
+although the result does not."""
+import pytest
+import test_token_gpu as base
+from test_token_gpu import tt
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("wt", ["f32", "bf16"])
+@pytest.mark.parametrize("st", ["f32", "bf16"])
+@pytest.mark.parametrize("group", [32, 64, 128, 512])
+def test_quantize_ranges_past_f32(cuda_torch, wt, st, group):
+    """hi - lo is past f32's largest value, (hi - lo) / 15 is not."""
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(group)
+    n, k = 7, 512
+    w = ((2 * torch.rand(n, k, generator=g, device="cuda") - 0.94) * 3.1e38).to(tt(torch, wt))
+    assert bool(w.isfinite().all())
+    w.view(n, k // group, group)[:, :, 3] = -2.9e38
+    w.view(n, k // group, group)[:, :, 7] = 3.2e38
+    w[1] *= 0.01  # and an ordinary row between
+    codes, scales, zp = base.quantize(torch, w, wt, group, st, True)
+    v = w.double().view(n, k // group, group)
+    lo, hi = v.amin(2).clamp(max=0), v.amax(2).clamp(min=0)
+    want = ((hi / 2).float() - (lo / 2).float()) / torch.full_like(scales, 7.5, dtype=torch.float32)  # f32's quotient
+    want = want.to(tt(torch, st))
+    assert torch.equal(scales, want)
+    s = scales.double()
+    z = torch.round(-lo / s).clamp(0, 15)
+    assert torch.equal(zp.double(), z)
+    q = torch.round(v / s[..., None])
+    near = ((v / s[..., None]).frac().abs() - 0.5).abs() < 2.0 ** -20  # quotients that f32 may round either way
+    got = torch.stack((codes & 15, codes >> 4), 2).view(n, k // group, group).double()
+    assert bool(((got - (q + z[..., None]).clamp(0, 15)).abs() <= near).all())  # by one there, by none elsewhere
