@@ -178,8 +178,8 @@ __device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, in
         for (int j = 0; j < kVec; ++j) ss = fmaf(h[u][j], h[u][j], ss);
     ss = team_sum<TEAM>(ss, red[0]);
     float pre = 1.f;
-    // squares past f32's range (or a NaN or infinity, which stays one): sum smaller ones
-    const bool past = !(ss < 3.0e38f);
+    // squares (and eps) past f32's range, or a NaN or infinity, which stays one: sum smaller ones
+    const bool past = !(ss + a.eps < 3.0e38f);
     if (TEAM < 32 ? __any_sync(0xffffffffu, past) : past) {
         if (past) pre = 8.2718061e-25f;  // 2^-80
         ss = 0.f;

@@ -2,7 +2,9 @@
 although the result does not."""
 import pytest
 import test_token_gpu as base
-from test_token_gpu import tt
+from test_token_gpu import HALF, NORM_TOL, TINY, ptr, stream, tt
+
+import fenix_b200 as fx
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +35,19 @@ def test_quantize_ranges_past_f32(cuda_torch, wt, st, group):
     near = ((v / s[..., None]).frac().abs() - 0.5).abs() < 2.0 ** -20  # quotients that f32 may round either way
     got = torch.stack((codes & 15, codes >> 4), 2).view(n, k // group, group).double()
     assert bool(((got - (q + z[..., None]).clamp(0, 15)).abs() <= near).all())  # by one there, by none elsewhere
+
+
+@pytest.mark.parametrize("rows", [1, 5, 1000])
+@pytest.mark.parametrize("yt", ["f32", "bf16"])
+def test_norm_eps_and_squares_past_f32_together(cuda_torch, rows, yt):
+    torch = cuda_torch
+    eps = 2.9e38
+    for cols in (1, 2, 64):
+        x = torch.full((rows, cols), 1.6e19 / cols ** 0.5, device="cuda")
+        x[::2] *= -0.9
+        y = torch.empty(rows, cols, dtype=tt(torch, yt), device="cuda")
+        fx.rms_norm_dev(ptr(x), ptr(y), rows, cols, "f32", yt, eps=eps, stream=stream(torch))
+        torch.cuda.synchronize()
+        eps32 = float(torch.tensor(eps, dtype=torch.float32))
+        _, v = base.norm_want(torch, x, None, None, eps32)
+        base.check_close(torch, y, v, HALF[yt] + NORM_TOL, TINY[yt])
