@@ -206,23 +206,25 @@ __device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, in
 #pragma unroll
         for (int j = 0; j < kVec; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(h[u][j])));  // columns past the row are 0
     }
-    float times = r, inv = 1.f;
+    float times = r, scale = 1.f;
     if (a.scale_mode == kScaleRow) {
         // as bits a NaN is above every number
         const uint32_t most = team_max<TEAM>(__float_as_uint(top * r) & 0x7fffffffu, reinterpret_cast<uint32_t*>(red[2]));
-        const float scale = __uint_as_float(max(most, __float_as_uint(1e-30f))) * (1.f / 448.f);
+        scale = __uint_as_float(max(most, __float_as_uint(1e-30f))) * (1.f / 448.f);
         if (me == 0 && cols) a.scale[row] = scale;
-        inv = 1.f / scale;
+        times = r * (1.f / scale);
     } else if (a.scale_mode == kScaleTensor) {
-        inv = 1.f / a.scale[0];
+        scale = a.scale[0];
+        times = r * (1.f / scale);
     }
-    times *= inv;
-    if (times == INFINITY) {  // a row near zero under a small eps (its zeros stay zeros): one product after the other
+    // a row near zero under a small eps, or a scale near zero: one product after the other (zeros stay zeros)
+    if (fabsf(times) == INFINITY) {
+        const float inv = 1.f / (scale * 1.8446744e19f);  // 2^64
 #pragma unroll
         for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) h[u][j] *= r;
-        times = inv;
+            for (int j = 0; j < kVec; ++j) h[u][j] = h[u][j] * r * inv;
+        times = 1.8446744e19f;
     }
 #pragma unroll
     for (int u = 0; u < TURNS; ++u) {

@@ -51,3 +51,23 @@ def test_norm_eps_and_squares_past_f32_together(cuda_torch, rows, yt):
         eps32 = float(torch.tensor(eps, dtype=torch.float32))
         _, v = base.norm_want(torch, x, None, None, eps32)
         base.check_close(torch, y, v, HALF[yt] + NORM_TOL, TINY[yt])
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 100), (2, 4096), (600, 64), (900, 2048)])
+@pytest.mark.parametrize("scale", [2.0 ** -128, 2.0 ** -149, 2.0 ** -127 * 1.5])
+def test_norm_tensor_scales_whose_reciprocal_is_past_f32(cuda_torch, rows, cols, scale):
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(rows, cols, generator=g, device="cuda").bfloat16()
+    x[:, ::5] = 0.0
+    w = torch.full((cols,), 2.0 ** -125, device="cuda")
+    w[:cols // 2] = 2.0
+    sc = torch.tensor([scale], device="cuda", dtype=torch.float64).float()
+    y = torch.empty(rows, cols, dtype=torch.float8_e4m3fn, device="cuda")
+    fx.rms_norm_dev(ptr(x), ptr(y), rows, cols, "bf16", "e4m3", ptr(w), "f32", 1e-5, scale_ptr=ptr(sc), scale_mode="tensor",
+                    stream=stream(torch))
+    torch.cuda.synchronize()
+    _, v = base.norm_want(torch, x, None, w, float(torch.tensor(1e-5, dtype=torch.float32)))
+    # v itself comes close to f32's smallest normal value: half a subnormal step of it, over the scale, is added
+    want = (v / sc.double()).clamp(-448, 448)
+    base.check_close(torch, y.float(), want, HALF["e4m3"] + NORM_TOL, TINY["e4m3"] + 2.0 ** -150 / scale * (1 + HALF["e4m3"]))
