@@ -352,7 +352,8 @@ cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s) {
     // little work: a block a row with as many threads as it has eights, for the shortest way through; more: blocks that stay
     // (us, the one and the other: 444 x 320 3.2 and 4.0, 4736 x 320 6.1 and 6.2, 9472 x 320 10.3 and 7.1, 222 x 4096 4.3
     // and 4.4, 370 x 8192 8.8 and 7.5; rows of eights to a warp's quarter: 444 x 64 2.3 and 1.8)
-    const bool few = a.cols <= 256 ? a.rows <= 148 * 2 : static_cast<int64_t>(a.rows) * a.cols <= 148 * 8192;
+    const int64_t sms = sm_count();
+    const bool few = a.cols <= 256 ? a.rows <= sms * 2 : static_cast<int64_t>(a.rows) * a.cols <= sms * 8192;
     if (vec && !few && a.x_type != kTokF32 && (!a.residual || a.residual_type != kTokF32)) {
         // narrow rows: several to a warp, so that its lanes are busy and have loads enough on their way (200003 x 320 bf16
         // to bf16: 50 us, 69 with a warp a row)

@@ -260,7 +260,7 @@ cudaError_t quantize(const void* w, int w_type, int64_t w_stride, const W4Args& 
 cudaError_t launch_w4_quantize(const void* w, int w_type, int64_t w_stride, const W4Args& q, cudaStream_t s) {
     // 32 weights a thread share what is done once a group (8192 x 8192 f32 in groups of 128: 47 us, 83 with 8 a thread);
     // a matrix that leaves SMs idle that way takes 8 a thread (1003 x 1088 bf16 in groups of 32: 3.1 us, 5.2 with 32)
-    const bool small = static_cast<int64_t>(q.n) * q.k < int64_t{148} * 1024 * 32;
+    const bool small = static_cast<int64_t>(q.n) * q.k < int64_t{sm_count()} * 1024 * 32;
     if (q.group == 32) return small ? quantize<4, 1>(w, w_type, w_stride, q, s) : quantize<1, 4>(w, w_type, w_stride, q, s);
     if (q.group == 64) return small ? quantize<8, 1>(w, w_type, w_stride, q, s) : quantize<2, 4>(w, w_type, w_stride, q, s);
     if (q.group == 128) return small ? quantize<16, 1>(w, w_type, w_stride, q, s) : quantize<4, 4>(w, w_type, w_stride, q, s);
