@@ -72,6 +72,11 @@ __device__ __forceinline__ void tok_store(void* p, int64_t i, int type, float v)
     else
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
+// the same of a 16-bit type, one store whichever it is
+__device__ __forceinline__ void tok_store16(void* p, int64_t i, int type, float v) {
+    static_cast<uint16_t*>(p)[i] =
+        type == kTokF16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
 #endif
 
 }  // namespace fxk

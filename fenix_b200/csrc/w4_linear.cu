@@ -351,7 +351,7 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                     if (BF) v *= kBackBF16;
                     if (a.x_scale) v *= a.x_scale[a.x_scale_mode == kScaleRow ? r : 0];
                     if (a.bias) v += a.bias[o];
-                    tok_store(a.y, r * a.y_stride + o, a.y_type, v);
+                    tok_store16(a.y, r * a.y_stride + o, a.y_type, v);
                 }
             }
             added = turn + 1;

@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             } else if (out < n) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (c + i < rows) tok_store(y, i * a.y_stride + out, a.y_type, f[i] + bias);
+                    if (c + i < rows) tok_store16(y, i * a.y_stride + out, a.y_type, f[i] + bias);
             }
         }
         tc_fence_before();
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             const float xs = a.x_scale ? a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0] : 1.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (o + e < n) tok_store(a.y, (r0 + r) * a.y_stride + o + e, a.y_type, f[e] * xs + (a.bias ? a.bias[o + e] : 0.f));
+                if (o + e < n) tok_store16(a.y, (r0 + r) * a.y_stride + o + e, a.y_type, f[e] * xs + (a.bias ? a.bias[o + e] : 0.f));
         }
         cluster_sync();
     }
