@@ -127,3 +127,27 @@ def test_norm_many_rows_that_no_team_walks_over(cuda_torch, cols, xt):
 @pytest.mark.parametrize("xt", ["f32", "bf16"])
 def test_norm_longest_rows(cuda_torch, cols, xt):
     base.run_norm(cuda_torch, 500, cols, xt, "e4m3", xt, xt, "row", seed=cols)
+
+
+# ---- inputs past 2^21, where a group's number no longer comes from a product ---------------------------------------
+
+
+@pytest.mark.parametrize("rows", [1, 8, 12])
+@pytest.mark.parametrize("group", [96, 32])
+def test_inputs_past_two_million(cuda_torch, rows, group):
+    k = (1 << 21) // group * group + 5 * group
+    base.run_linear(cuda_torch, rows, 37, k, group, "bf16" if rows != 8 else "e4m3", "bf16", zeros=True, bias=True)
+    cuda_torch.cuda.empty_cache()
+
+
+def test_quantize_rows_past_two_million(cuda_torch):
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = 96 * 21900
+    w = torch.randn(3, k, generator=g, device="cuda").bfloat16()
+    codes, scales, zp = base.quantize(torch, w, "bf16", 96, "f16", True)
+    want = base.quantize_want(torch, w, 96, "f16", True)
+    assert torch.equal(codes, want[0]) and torch.equal(scales.float(), want[1]) and torch.equal(zp, want[2])
+    out = torch.empty(3, k, device="cuda")
+    fx.w4_dequantize_dev(ptr(codes), ptr(scales), 3, k, 96, ptr(out), ptr(zp), "f32", "f16", stream=stream(torch))
+    assert torch.equal(out.double(), unpack(torch, codes, scales, zp, 96))

@@ -128,3 +128,40 @@ def test_f16_results_of_many_bf16_rows(cuda_torch, rows, st, zeros, group):
         worst = max(worst, (err / lim).max().item())
         print(rows, st, n, k, "rms error / rms result %.2e" % (err.square().mean().sqrt() / want.square().mean().sqrt()).item())
     assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("rows", [9, 130, 300])
+def test_two_terms_keep_what_is_not_finite_apart(cuda_torch, rows):
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    n, k, group = 300, 512, 64
+    codes, scales, zp = base.make_layer(torch, n, k, group, "f32", True, g, True)
+    x = torch.randint(-4, 5, (rows, k), generator=g, device="cuda").bfloat16()
+    want = (x.double() @ unpack(torch, codes, scales, zp, group).t()).half()
+    x[2, 7], x[5, 100] = float("inf"), float("nan")
+    scales[3, 1], scales[4, 0] = float("inf"), float("nan")
+    y = linear(torch, x, "bf16", "f16", codes, scales, "f32", zp, group)
+    fine_rows = [r for r in range(rows) if r not in (2, 5)]
+    fine_outs = [o for o in range(n) if o not in (3, 4)]
+    assert torch.equal(y[fine_rows][:, fine_outs], want[fine_rows][:, fine_outs])
+    assert not bool(y[[2, 5]].isfinite().any()) and not bool(y[:, [3, 4]].isfinite().any())
+
+
+def test_two_terms_captured_and_repeated(cuda_torch):
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(8)
+    n, k, group = 640, 4096, 128
+    codes, scales, zp = base.make_layer(torch, n, k, group, "f16", False, g, False)
+    for rows in (20, 300):
+        x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+        first = linear(torch, x, "bf16", "f16", codes, scales, "f16", zp, group)
+        y = torch.zeros(rows, n, dtype=torch.float16, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            fx.w4_linear_dev(ptr(x), ptr(y), rows, n, k, group, ptr(codes), ptr(scales), x_type="bf16", y_type="f16",
+                             stream=stream(torch))
+        for _ in range(3):
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, first)
