@@ -168,9 +168,11 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
     return v;
 }
 
-// From a row's h on: the norm, the scale, the output; cols 0: no row, nothing is stored. red: three rows of 32 floats that no thread of the team still reads.
+// From a row's h on: the norm, the scale, the output; cols 0: no row, nothing is stored. red: three rows of 32 floats that
+// no thread of the team still reads.
 template <int TEAM, int TURNS, bool VEC>
-__device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, int me, int cols, float (&h)[TURNS][kVec], float (*red)[32]) {
+__device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, int me, int cols, float (&h)[TURNS][kVec],
+                                           float (*red)[32]) {
     float ss = 0.f;
 #pragma unroll
     for (int u = 0; u < TURNS; ++u)
@@ -204,7 +206,8 @@ __device__ __forceinline__ void finish_row(const RmsNormArgs& a, int64_t row, in
             for (int j = 0; j < kVec; ++j) h[u][j] *= w[j];
         }
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(h[u][j])));  // columns past the row are 0
+        for (int j = 0; j < kVec; ++j)  // columns past the row are 0
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(h[u][j])));
     }
     float times = r, scale = 1.f;
     if (a.scale_mode == kScaleRow) {

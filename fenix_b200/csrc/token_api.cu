@@ -259,7 +259,8 @@ fx_status fx_w4_device_status(int device) {
         cudaSetDevice(cur);
         if (e != cudaSuccess) return done(fn, e);
         if (few || bf16 || f16)
-            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(few ? few : bf16 ? bf16 : f16));
+            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " +
+                                                   std::to_string(few ? few : bf16 ? bf16 : f16));
         return FX_OK;
     });
 }

@@ -96,17 +96,21 @@ __device__ __forceinline__ void consumers_sync(int warps) { asm volatile("bar.sy
 // asynchronously in pieces of UNIT bytes where the addresses allow it, else by plain stores, byte by byte (the result:
 // whether asynchronously).
 template <int UNIT>
-__device__ __forceinline__ void rows_async(uint32_t dst, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
+__device__ __forceinline__ void rows_async(uint32_t dst, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows,
+                                           int bytes) {
     const int lane = threadIdx.x % 32;
     for (int r = lane / 4; r < rows; r += 8)
         for (int at = lane % 4 * UNIT; at < bytes; at += 4 * UNIT) {
+            const uint32_t to = dst + r * dst_pitch + at;
+            const uint8_t* const from = src + r * src_pitch + at;
             if constexpr (UNIT == 16)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + r * dst_pitch + at), "l"(src + r * src_pitch + at) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
             else
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + r * dst_pitch + at), "l"(src + r * src_pitch + at) : "memory");
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
         }
 }
-__device__ __forceinline__ bool rows_to_shared(uint8_t* to, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows, int bytes) {
+__device__ __forceinline__ bool rows_to_shared(uint8_t* to, int dst_pitch, const uint8_t* src, int64_t src_pitch, int rows,
+                                               int bytes) {
     const int64_t all = static_cast<int64_t>(reinterpret_cast<uintptr_t>(src)) | src_pitch;
     if (all % 16 == 0 && bytes % 16 == 0) {
         rows_async<16>(smem_u32(to), dst_pitch, src, src_pitch, rows, bytes);
@@ -139,7 +143,8 @@ __device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[m][h][c]) : "r"(at + (m * 16 + h * 8) * 128));
+            for (int h = 0; h < 2; ++h)
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[m][h][c]) : "r"(at + (m * 16 + h * 8) * 128));
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -151,7 +156,8 @@ __device__ __forceinline__ void unit(float (&acc)[2][4], uint32_t codes, uint32_
             } else {
                 unsigned short raw;
                 asm volatile("ld.shared.b16 %0, [%1];" : "=h"(raw) : "r"(at));
-                scale[m][h] = scale_type == kTokF16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float(static_cast<uint32_t>(raw) << 16);
+                scale[m][h] = scale_type == kTokF16 ? __half2float(__ushort_as_half(raw))
+                                                    : __uint_as_float(static_cast<uint32_t>(raw) << 16);
             }
             uint32_t zero = 8;
             if (Z) asm volatile("ld.shared.u8 %0, [%1];" : "=r"(zero) : "r"(z_at + (m * 16 + h * 8) * z_pitch));
@@ -269,7 +275,8 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
         return;
     }
 
-    const uint32_t x_lane = smem_u32(smem + plan.x) + min(g, rows - 1) * plan.x_pitch + t * 16;  // rows past the last: nothing reads their sums
+    // (rows past the last: nothing reads their sums)
+    const uint32_t x_lane = smem_u32(smem + plan.x) + min(g, rows - 1) * plan.x_pitch + t * 16;
     const float inv_group = 1.f / static_cast<float>(group);
     for (int seg = 0; seg < blocks; seg += plan.seg_blocks) {
         const int seg_end = min(seg + plan.seg_blocks, blocks), g0 = seg * kBlockK / group;
@@ -304,7 +311,8 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
                         const int kc = k0 + u * 32 * CPF;
                         if (CPF < 4 && kc >= k) break;
                         // (kc + 1/2) / group truncated: exact while k < 2^21
-                        const int gi = (k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group) - g0;
+                        const int gi =
+                            (k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group) - g0;
                         const int cell = (4 * (warp & 1) + u * CPF) ^ g;
                         if (wide)
                             unit<BF, CPF, Z, 2>(acc, cw, xw + u * CPF * 64, cell, s_at + gi * sb, plan.s_pitch, a.w.scale_type,
@@ -326,13 +334,16 @@ __global__ void __launch_bounds__((kMaxConsumers + 2) * 32, 1)
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (2 * t + (e & 1) < rows) red[warp * per_tile + (2 * t + (e & 1)) * kM + m * 16 + (e / 2) * 8 + g] = acc[m][e];
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 2 * t + (e & 1);
+                    if (r < rows) red[warp * per_tile + r * kM + m * 16 + (e / 2) * 8 + g] = acc[m][e];
+                }
             const bool last = tile + static_cast<int>(gridDim.x) >= plan.tiles;
             if (turn + 1 - added < plan.red_bufs && !last) continue;
             consumers_sync(warps);
             for (int i = threadIdx.x; i < (turn + 1 - added) * per_tile; i += warps * 32) {
-                const int nth = i / per_tile, r = i % per_tile / kM, from = tile - (turn - added - nth) * static_cast<int>(gridDim.x);
+                const int nth = i / per_tile, r = i % per_tile / kM;
+                const int from = tile - (turn - added - nth) * static_cast<int>(gridDim.x);
                 const int o = tile_row(from) + i % kM;
                 if (i % kM >= (from < plan.wide ? kM : 16) || o >= n) continue;
                 const float* const part = reinterpret_cast<float*>(smem + plan.red) + nth * warps * per_tile + i % per_tile;
@@ -373,7 +384,8 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
     p.consumers = round_up((blocks + turns - 1) / turns, 2);
     const int x_fit = kXRoom / rows / (p.consumers * kBlockK * 2 + 64);
     const int sb = a.w.scale_type == kTokF32 ? 4 : 2;
-    const int64_t s_fit = static_cast<int64_t>((kScaleRoom / kM - 2 * 128) / (a.w.zeros ? sb + 1 : sb) - 1) * a.w.group / (p.consumers * kBlockK);
+    const int64_t s_room = (kScaleRoom / kM - 2 * 128) / (a.w.zeros ? sb + 1 : sb) - 1;
+    const int64_t s_fit = s_room * a.w.group / (p.consumers * kBlockK);
     int fit = x_fit < s_fit ? x_fit : static_cast<int>(s_fit);
     if (fit < 1) fit = 1;
     const int segs = (turns + fit - 1) / fit;
@@ -433,7 +445,8 @@ cudaError_t launch_few_cpf(const W4LinearArgs& a, bool x_vec, cudaStream_t s) {
     return launch_few<BF, 1, Z>(a, x_vec, s);
 }
 cudaError_t launch_few_typed(const W4LinearArgs& a, bool x_vec, cudaStream_t s) {
-    if (a.x_type == kTokBF16) return a.w.zeros ? launch_few_cpf<true, true>(a, x_vec, s) : launch_few_cpf<true, false>(a, x_vec, s);
+    if (a.x_type == kTokBF16)
+        return a.w.zeros ? launch_few_cpf<true, true>(a, x_vec, s) : launch_few_cpf<true, false>(a, x_vec, s);
     return a.w.zeros ? launch_few_cpf<false, true>(a, x_vec, s) : launch_few_cpf<false, false>(a, x_vec, s);
 }
 

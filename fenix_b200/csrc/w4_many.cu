@@ -17,10 +17,14 @@ cudaError_t launch_w4_many(const W4LinearArgs& a, int sms, cudaStream_t s) {
     // against larger; bf16: 1536 x 4096 -> 4096 50 and 40, 1024 x 4096 -> 14336 102 and 119, 4096 rows 352 and 364; e4m3:
     // 1024 x 4096 -> 4096 49 and 49, 576 x 4096 -> 14336 109 and 107, 4096 rows 609 and 483)
     auto across = [&](int m) { return (a.w.n + m - 1) / m; };
-    auto turns = [&](int m, int most) { return (across(m) * ((static_cast<int64_t>(a.rows) + most - 1) / most) + sms - 1) / sms; };
+    auto turns = [&](int m, int most) {
+        return (across(m) * ((static_cast<int64_t>(a.rows) + most - 1) / most) + sms - 1) / sms;
+    };
     // f16 results of bf16 rows hold more bits than a bf16 weight: a weight is two terms there, an MMA each
     p.terms = a.x_type == kTokBF16 && a.y_type == kTokF16;
-    const bool two = p.two = p.terms ? false : p.x_tma ? turns(256, 192) * 3 < turns(128, 256) * 2 : turns(256, 192) * 11 < turns(128, 256) * 10;
+    const bool two = p.two = p.terms   ? false
+                             : p.x_tma ? turns(256, 192) * 3 < turns(128, 256) * 2
+                                       : turns(256, 192) * 11 < turns(128, 256) * 10;
     const int tile_m = two ? 256 : 128, most_n = two ? 192 : 256;
     const int64_t tiles_n = (static_cast<int64_t>(a.rows) + most_n - 1) / most_n;
     p.tile_n = static_cast<int>((a.rows + tiles_n * 16 - 1) / (tiles_n * 16)) * 16;

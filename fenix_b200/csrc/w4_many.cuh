@@ -31,13 +31,14 @@ namespace {
 
 // K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 | static_cast<uint64_t>(1024 >> 4) << 32 |
-           static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
 }
 
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, f32 accumulate: every lane runs the code, on warp-uniform
 // operands, and the lane with issue != 0 executes it.
-__device__ __forceinline__ void mma_f16_ta_if(uint32_t issue, uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_f16_ta_if(uint32_t issue, uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
@@ -72,6 +73,10 @@ __device__ __forceinline__ uint32_t pair16(float a, float b) {
     }
     __half2 h = __floats2half2_rn(a, b);
     return reinterpret_cast<uint32_t&>(h);
+}
+// A 16-bit value's bits (the low half) as f32.
+__device__ __forceinline__ float value16(uint32_t bits, bool is_f16) {
+    return is_f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(bits))) : __uint_as_float(bits << 16);
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
@@ -128,8 +133,8 @@ __device__ __forceinline__ void weights16(uint32_t w0, uint32_t w1, uint32_t hi,
 
 // The same as the sum of two 16-bit values: the weight rounded, and what that left (exact where EX).
 template <bool BF, bool EX>
-__device__ __forceinline__ void weight_terms16(uint32_t w0, uint32_t w1, uint32_t hi, uint32_t lo, uint32_t z, uint32_t (&out)[8],
-                                               uint32_t (&rest)[8]) {
+__device__ __forceinline__ void weight_terms16(uint32_t w0, uint32_t w1, uint32_t hi, uint32_t lo, uint32_t z,
+                                               uint32_t (&out)[8], uint32_t (&rest)[8]) {
     weights16<BF, EX>(w0, w1, hi, lo, z, out);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -154,8 +159,8 @@ constexpr int kMakers = 16;
 // are 2^-25 of it). TERMS: a weight is two terms.
 template <bool BF, bool TWO, bool TMA, int SS, int CH, bool EX, bool TERMS>
 __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
-    w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan, const __grid_constant__ CUtensorMap codes_map,
-                   const __grid_constant__ CUtensorMap rows_map) {
+    w4_many_kernel(const __grid_constant__ W4LinearArgs a, const __grid_constant__ ManyPlan plan,
+                   const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ CUtensorMap rows_map) {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[7 * kMaxRing + 1];
     __shared__ uint32_t tmem_at;
@@ -173,7 +178,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
     const int steps = (k_end - k_begin + kStepK - 1) / kStepK;
     const uint32_t bar = smem_u32(bars);
     const uint32_t c_full = bar, c_empty = bar + 8 * kMaxRing, w_full = bar + 16 * kMaxRing, w_empty = bar + 24 * kMaxRing,
-                   x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, raw_full = bar + 48 * kMaxRing, done = bar + 56 * kMaxRing;
+                   x_full = bar + 32 * kMaxRing, x_empty = bar + 40 * kMaxRing, raw_full = bar + 48 * kMaxRing,
+                   done = bar + 56 * kMaxRing;
     const uint32_t codes = smem_u32(smem + plan.codes), xrows = smem_u32(smem + plan.rows);
     auto gave_up = [&](uint32_t code) {
         abort_flag = 1;
@@ -228,8 +234,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                 if (abort_flag) break;
                 mbar_arrive_expect_tx(x_full + 8 * xs, boxes * tile_n * 128);
                 for (int i = 0; i < boxes; ++i)
-                    tma_load_2d(xrows + (xs * SS + i) * tile_n * 128, &rows_map, k_begin + (step + i) * kStepK, static_cast<int>(r0),
-                                x_full + 8 * xs);
+                    tma_load_2d(xrows + (xs * SS + i) * tile_n * 128, &rows_map, k_begin + (step + i) * kStepK,
+                                static_cast<int>(r0), x_full + 8 * xs);
                 if (++xs == plan.rings[2]) xs = 0, xp ^= 1;
             }
             for (int i = 0; i < plan.rings[2]; ++i) wait_phase(x_full + 8 * i, (i < xs ? xp : xp ^ 1), nullptr, a.wait_ns);
@@ -253,7 +259,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                 const uint32_t ad = plan.weight_col + ws * kWeightCols + m * 32;
 #pragma unroll
                 for (int i = 0; i < kStepK / 16; ++i)
-                    mma_f16_ta_if(issue, TWO ? m * tile_n : 0, ad + 8 * i, bd + 2 * i, idesc, step > 0 || i > 0 || (TERMS && m > 0));
+                    mma_f16_ta_if(issue, TWO ? m * tile_n : 0, ad + 8 * i, bd + 2 * i, idesc,
+                                  step > 0 || i > 0 || (TERMS && m > 0));
             }
             mma_commit_if(issue, w_empty + 8 * ws);
             if (++ws == plan.rings[1]) ws = 0, wp ^= 1;
@@ -274,15 +281,16 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
         auto fetch = [&](int step, int slot) {  // e4m3: TMA brings 128 inputs at a time, these warps widen them
             if (step < steps) {
                 mbar_arrive_expect_tx(raw_full + 8 * slot, tile_n * 128);
-                tma_load_2d(smem_u32(smem + plan.raw) + slot * tile_n * 128, &rows_map, (k_begin + step * kStepK) / 8, static_cast<int>(r0),
-                            raw_full + 8 * slot);
+                tma_load_2d(smem_u32(smem + plan.raw) + slot * tile_n * 128, &rows_map, (k_begin + step * kStepK) / 8,
+                            static_cast<int>(r0), raw_full + 8 * slot);
             }
         };
         if (tid == 0)
             for (int i = 0; i < plan.raw_slots; ++i) fetch(2 * i, i);
         for (int step0 = 0; step0 < steps; step0 += kRowWarps) {
             const int step = step0 + tid / 32, pair = step / 2, slots = plan.raw_slots ? plan.raw_slots : 1, rs = pair % slots;
-            if (SS < kRowWarps && step / SS * SS >= steps) break;  // (the warp that shares its raw slot has asked for the last one)
+            // (the warp that shares its raw slot has asked for the last one)
+            if (SS < kRowWarps && step / SS * SS >= steps) break;
             const int xs = step / SS % plan.rings[2];
             const uint32_t xp = step / SS / plan.rings[2] & 1, rp = pair / slots & 1;
             if (!wait_phase(x_empty + 8 * xs, xp ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
@@ -307,14 +315,16 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                 for (int i = lane; i < tile_n * 8; i += 32) {
                     const int r = i / 8, c = i % 8;
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < rows && k0 + c * 8 < k_end) v = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
+                    if (r < rows && k0 + c * 8 < k_end)
+                        v = raw_eight(src + (static_cast<int64_t>(r) * a.x_stride + c * 8) * kxb, a.x_type, plan.x_vec);
                     *reinterpret_cast<uint4*>(to + r * 128 + ((c ^ (r & 7)) << 4)) = widened(v, a.x_type);
                 }
             }
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(x_full + 8 * xs);
-            if (plan.raw_slots && pair * 2 + 2 * plan.raw_slots < steps) {  // another use: both warps are done with the raw slot
+            // another use: both warps are done with the raw slot
+            if (plan.raw_slots && pair * 2 + 2 * plan.raw_slots < steps) {
                 asm volatile("bar.sync %0, 64;" ::"r"(2 + tid / 64) : "memory");
                 if (tid % 64 == 0) fetch(pair * 2 + 2 * plan.raw_slots, rs);
             }
@@ -348,8 +358,7 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                     const uint32_t r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const uint32_t h = (i % 2 ? r[i / 2] >> 16 : r[i / 2]) & 0x7fffu;
-                        top = fmaxf(top, is_f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(h))) : __uint_as_float(h << 16));
+                        top = fmaxf(top, value16((i % 2 ? r[i / 2] >> 16 : r[i / 2]) & 0x7fffu, is_f16));
                     }
                 }
             } else {
@@ -382,7 +391,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
                     zo[c][h] = 8;
                     if (kc < k_end) {
                         // (kc + 1/2) / group truncated: exact while k < 2^21
-                        const int g = k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group;
+                        const int g =
+                            k < (1 << 21) ? static_cast<int>((static_cast<float>(kc) + 0.5f) * inv_group) : kc / group;
                         if (wide)
                             sc[c][h] = __ldg(reinterpret_cast<const uint32_t*>(s_at) + g);
                         else
@@ -402,11 +412,11 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
 #pragma unroll
                 for (int h = 0; h < CH; ++h) {
                     const uint32_t raw = sc[c][h];
-                    float v = wide ? __uint_as_float(raw) : is_f16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(raw))) : __uint_as_float(raw << 16);
+                    float v = wide ? __uint_as_float(raw) : value16(raw, is_f16);
                     if (!BF) v *= factor;
                     hi[c][h] = pair16<BF>(v, v);
                     if (!EX) {
-                        const float l = v - (BF ? __uint_as_float(hi[c][h] << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(hi[c][h]))));
+                        const float l = v - value16(hi[c][h], !BF);
                         lo[c][h] = fabsf(l) < INFINITY ? pair16<BF>(l, l) : 0;  // an infinite scale has no remainder
                     }
                     z[c][h] = zero_terms<BF>(zo[c][h]);
@@ -432,8 +442,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         uint32_t out[8], rest[8];
-                        weight_terms16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH], lo[c][h / 2 % CH],
-                                               z[c][h / 2 % CH], out, rest);
+                        weight_terms16<BF, EX>(w[h / 2][h % 2 * 2], w[h / 2][h % 2 * 2 + 1], hi[c][h / 2 % CH],
+                                               lo[c][h / 2 % CH], z[c][h / 2 % CH], out, rest);
                         tmem_st8(slot + 8 * h, out);
                         tmem_st8(slot + 32 + 8 * h, rest);
                     }
@@ -493,10 +503,12 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             if (vec) {
                 if (a.y_type == kTokF16) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) *reinterpret_cast<__half*>(turned + i * 80 + lane * 2) = __float2half_rn(f[i] + bias);
+                    for (int i = 0; i < 16; ++i)
+                        *reinterpret_cast<__half*>(turned + i * 80 + lane * 2) = __float2half_rn(f[i] + bias);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) *reinterpret_cast<__nv_bfloat16*>(turned + i * 80 + lane * 2) = __float2bfloat16_rn(f[i] + bias);
+                    for (int i = 0; i < 16; ++i)
+                        *reinterpret_cast<__nv_bfloat16*>(turned + i * 80 + lane * 2) = __float2bfloat16_rn(f[i] + bias);
                 }
                 __syncwarp();
 #pragma unroll
@@ -534,7 +546,8 @@ __global__ void __launch_bounds__(TMA ? 608 : 704, 1)
             const float xs = a.x_scale ? a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0] : 1.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (o + e < n) tok_store16(a.y, (r0 + r) * a.y_stride + o + e, a.y_type, f[e] * xs + (a.bias ? a.bias[o + e] : 0.f));
+                if (o + e < n)
+                    tok_store16(a.y, (r0 + r) * a.y_stride + o + e, a.y_type, f[e] * xs + (a.bias ? a.bias[o + e] : 0.f));
         }
         cluster_sync();
     }
@@ -580,13 +593,15 @@ cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
 template <bool BF, bool TWO, bool TMA, int SS, bool TERMS = false>
 cudaError_t launch(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     const bool exact = a.w.scale_type == (BF ? kTokBF16 : kTokF16);
-    if (a.w.group % kStepK == 0) return exact ? launch<BF, TWO, TMA, SS, 1, true, TERMS>(a, p, s) : launch<BF, TWO, TMA, SS, 1, false, TERMS>(a, p, s);
+    if (a.w.group % kStepK == 0)
+        return exact ? launch<BF, TWO, TMA, SS, 1, true, TERMS>(a, p, s) : launch<BF, TWO, TMA, SS, 1, false, TERMS>(a, p, s);
     return exact ? launch<BF, TWO, TMA, SS, 2, true, TERMS>(a, p, s) : launch<BF, TWO, TMA, SS, 2, false, TERMS>(a, p, s);
 }
 template <bool BF>
 cudaError_t launch_typed(const W4LinearArgs& a, const ManyPlan& p, cudaStream_t s) {
     if constexpr (BF) {
-        if (p.terms && p.slot_steps == 2) return p.x_tma ? launch<BF, false, true, 2, true>(a, p, s) : launch<BF, false, false, 2, true>(a, p, s);
+        if (p.terms && p.slot_steps == 2)
+            return p.x_tma ? launch<BF, false, true, 2, true>(a, p, s) : launch<BF, false, false, 2, true>(a, p, s);
         if (p.terms) return p.x_tma ? launch<BF, false, true, 4, true>(a, p, s) : launch<BF, false, false, 4, true>(a, p, s);
     }
     if (p.two) return p.x_tma ? launch<BF, true, true, 1>(a, p, s) : launch<BF, true, false, 1>(a, p, s);
