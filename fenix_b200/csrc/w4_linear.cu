@@ -20,13 +20,14 @@ namespace {
 // waits for a tile's end (a bulk copy for each row of a tile costs its thread some 60 ns); each consumer takes 128
 // inputs of a stage. Codes meet the rows in m16n8k16 MMAs (A: outputs x inputs, B: inputs x 8 rows), whose 8 columns are
 // what few rows can fill: a tcgen05 operand would have to be written before it is read (all of it: 1 x 4096 -> 4096
-// 9.7 us, 1 x 8192 -> 28672 67). The rows lie in shared memory for the whole walk, converted once and in the MMA's order.
+// 9.5 us, 1 x 8192 -> 28672 f16 57). The rows lie in shared memory for the whole walk, converted once and in the MMA's order.
 // A weight enters the MMA as code - zero, a whole number (in bf16 times 2^-11), made of two codes at a time by one
 // logical operation and one packed subtraction, both exact. So every product is exact, the sums hold nothing but the
 // result's own terms, and scales are applied in f32 to the sum of a group's inputs: no weight is rounded. The consumers'
 // partial sums meet in shared memory.
 
 constexpr int kBlockK = 128;  // inputs of a consumer warp in a stage
+// (us, with 16, 18 and 22: 1 x 8192 -> 28672 f16 32.3, 33.6 and 33.0, 8 x 8192 -> 8192 22.8, 23.4 and 32.7)
 constexpr int kMaxConsumers = 16;
 
 template <bool BF>
@@ -409,7 +410,7 @@ FewPlan few_plan(const W4LinearArgs& a, int rows, int sms, int* grid) {
         p.red += round_up((p.tiles + *grid - 1) / *grid * rows * kM * 4, 128);
     }
     // partial sums of as many tiles as have room beside three stages: a warp need not wait for the others at a tile's end
-    // (1 x 8192 -> 28672 f16 31.4 us, 33.5 with two buffers; 8 x 8192 -> 8192 24.5 us with three, 26.5 with one)
+    // (1 x 8192 -> 28672 f16 32.3 us, 35.4 with two buffers; 8 x 8192 -> 8192 22.8 us with three, 25.0 with one)
     const int stage = p.consumers / 2 * kM * 128, per_tile = p.consumers * rows * kM * 4;
     p.red_bufs = std::clamp(48 * 1024 / per_tile, 1, (p.tiles + *grid - 1) / *grid);
     auto place = [&] {
@@ -453,8 +454,9 @@ cudaError_t launch_few_typed(const W4LinearArgs& a, bool x_vec, cudaStream_t s) 
 }  // namespace
 
 cudaError_t launch_w4_linear(const W4LinearArgs& a, cudaStream_t s) {
-    // 8 rows are an MMA's columns; the kernels meet there (us, few rows' and many rows': 4 x 4096 -> 14336 15.0 and 20.0,
-    // 8 x 4096 -> 4096 10.1 and 10.1, 8 x 4096 -> 14336 18.0 and 19.9, 8 x 8192 -> 28672 52 and 67)
+    // 8 rows are an MMA's columns; the kernels meet there (us, few rows' and many rows': 4 x 4096 -> 14336 14.8 and 20.0,
+    // 8 x 4096 -> 4096 9.1 and 9.9, 8 x 4096 -> 14336 17.3 and 20.0, 8 x 8192 -> 8192 22.8 and 21.4, 8 x 8192 -> 28672 50
+    // and 60)
     if (a.rows > 8) {
         constexpr int kMost = 65535 * 16;  // rows of a launch: 65535 of the smallest tiles
         for (int64_t row0 = 0; row0 < a.rows; row0 += kMost) {

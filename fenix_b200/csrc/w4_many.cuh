@@ -7,10 +7,11 @@
 // rows come by TMA as they are (or, for e4m3 and unaligned rows, through four loader warps); one thread issues the
 // MMAs, which accumulate in TMEM in f32. Few tiles share a cluster each, by ranges of k, and add up over its shared
 // memory.
-// Bounds: with many rows the tensor cores under the power limit (4096 x 4096 -> 14336 bf16: 352 us, 1.37 PFLOP/s, 85% of
-// a burst's and 100% of a sustained library product's rate); up to 64 rows the making of weights, some two
+// Bounds: with many rows the tensor cores under the power limit, whose clock goes with the operands and the GPU's heat
+// (4096 x 4096 -> 14336 bf16: 353 us on uniform codes, 1.36 PFLOP/s, 99% of a sustained library product's rate; 359 on
+// normal weights, up to 411 with other rows each time and between other work, 1.17 PFLOP/s); up to 64 rows the making of weights, some two
 // instructions a weight on pipes of half rate (64 x 4096 -> 14336: 20 us, as long as 16 rows take); with e4m3 rows
-// their widening (4096 rows 487 us).
+// their widening (4096 rows 486 to 585 us).
 // A weight scale * (code - zero) is rounded once to the rows' 16-bit type (f16 for e4m3 rows): code - zero is
 // exact, and the scale enters as the sum of two 16-bit values, one product and one fused multiply-add. In f16
 // each output's weights are divided by the power of two below its largest scale, so that no scale's size

@@ -462,7 +462,8 @@ fx_status fx_selftest_w4_wait_timeout(int device, fx_dtype x_type, int rows, uin
  * code = zero (8; 0 with zero points); a NaN is left out of the extremes and gets code = zero. */
 fx_status fx_w4_quantize(const void* dev_w, fx_dtype w_type, int64_t n, int64_t k, int64_t w_stride, int64_t group,
                          uint8_t* dev_codes, void* dev_scales, fx_dtype scale_type, uint8_t* dev_zeros, void* stream);
-/* The values such weights stand for: w = scale * (code - zero), rounded once to w_type (f32, f16, bf16). */
+/* The values such weights stand for: w = scale * (code - zero) in f32 (exact with f16 and bf16 scales), rounded to w_type
+ * (f32, f16, bf16). */
 fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
                            const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, void* dev_w,
                            fx_dtype w_type, int64_t w_stride, void* stream);
