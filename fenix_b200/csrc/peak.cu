@@ -12,7 +12,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <chrono>
 #include <string>
+#include <thread>
 #include <vector>
 
 namespace fxh {
@@ -127,6 +129,9 @@ extern "C" fx_status fx_tc_rate(int device, int precision, int n_cols, double ms
     run(n0);
     const double ms0 = std::max(run(n0), 1e-3);
     const long long n = std::max<long long>(n0, static_cast<long long>(static_cast<double>(n0) * ms_per_run / ms0));
+    // from rest: right after other work the power limit holds the first runs' clock down (f16 1570 to 1960 TFLOP/s without
+    // the pause, 1950 to 1965 with it)
+    std::this_thread::sleep_for(std::chrono::milliseconds(100));
     double best = 0.0, sum = 0.0;
     for (int r = 0; r < runs; ++r) {
         const double ms = run(n);

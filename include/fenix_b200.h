@@ -288,7 +288,8 @@ fx_status fx_net_profile_read(fx_net* net, double* conv_ms, double* conv_flops, 
 int fx_net_profile_read_layers(fx_net* net, double* layer_ms, int cap);
 /* The dense tcgen05 tensor rate of `device`, measured with this library's own kernel: one CTA per SM
  * issuing M = 128, N = 256 MMAs back to back on shared-memory-resident operands (kind::f8f6f4 e4m3
- * for FX_PREC_FP8, kind::f16 for bf16 / f16) into TMEM. `runs` launches of about ms_per_run each:
+ * for FX_PREC_FP8, kind::f16 for bf16 / f16) into TMEM. `runs` launches of about ms_per_run each, from rest (the GPU
+ * idles for 0.1 s before them, so that the power limit's state is not the work's before):
  * *best_tflops = the fastest (the burst rate), *mean_tflops (may be NULL) = their mean; a single long
  * run gives the sustained, power-capped rate. No reference counterpart (the reference measures
  * none). */
