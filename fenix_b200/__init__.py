@@ -31,7 +31,7 @@ STATUS_NAMES = {
 }
 PREC_BF16, PREC_FP8, PREC_F16 = 0, 1, 2
 PRECISIONS = {"bf16": PREC_BF16, "fp8": PREC_FP8, "f16": PREC_F16}
-DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}  # fx_dtype
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3, "i8": 4}  # fx_dtype
 SCALE_MODES = {None: 0, "tensor": 1, "row": 2}  # fx_scale
 
 
@@ -206,6 +206,14 @@ def lib():
     _sig(L, "fx_rms_norm", i32, [vp, i32, i64, i64, i64, vp, i32, i64, vp, i64, vp, i32, C.c_float, vp, i32, i64, vp,
                                  i32, vp])
     _sig(L, "fx_w4_linear", i32, [vp, i32, i64, i64, vp, i32, vp, vp, i32, vp, i64, i64, i64, vp, vp, i32, i64, vp])
+    _sig(L, "fx_layer_norm", i32, [vp, i32, i64, i64, i64, vp, i32, i64, vp, i64, vp, vp, i32, C.c_float, vp, i32, i64, vp,
+                                   vp, vp, i32, vp])
+    _sig(L, "fx_layer_norm_backward_workspace", C.c_uint64, [i64, i64])
+    _sig(L, "fx_layer_norm_backward", i32, [vp, i32, i64, i64, i64, vp, i32, i64, vp, vp, vp, i32, vp, i64, vp, i32, i64, vp,
+                                            vp, i32, vp, C.c_uint64, vp])
+    _sig(L, "fx_i8_quantize", i32, [vp, i32, i64, i64, i64, vp, i64, vp, i32, vp])
+    _sig(L, "fx_i8_dequantize", i32, [vp, i64, vp, i32, i64, i64, vp, i32, i64, vp])
+    _sig(L, "fx_i8_linear", i32, [vp, i64, i64, vp, i32, vp, i64, vp, i64, i64, vp, vp, i32, i64, vp])
     _sig(L, "fx_w4_device_status", i32, [i32])
     _sig(L, "fx_selftest_w4_wait_timeout", i32, [i32, i32, i32, C.c_uint64])
     _sig(L, "fx_w4_quantize", i32, [vp, i32, i64, i64, i64, i64, vp, vp, i32, vp, vp])
@@ -356,6 +364,62 @@ def w4_dequantize_dev(codes_ptr: int, scales_ptr: int, n: int, k: int, group: in
     """fx_w4_dequantize: the values that 4-bit codes, scales and zero points stand for."""
     check(lib().fx_w4_dequantize(codes_ptr, scales_ptr, DTYPES[scale_type], zeros_ptr, n, k, group, w_ptr,
                                  DTYPES[w_type], w_stride, stream))
+
+
+def layer_norm_dev(x_ptr: int, y_ptr: int, rows: int, cols: int, x_type: str = "bf16", y_type: str = "bf16",
+                   weight_ptr: int | None = None, bias_ptr: int | None = None, weight_type: str = "bf16",
+                   eps: float = 1e-5, x_stride: int = 0, y_stride: int = 0, residual_ptr: int | None = None,
+                   residual_type: str = "bf16", residual_stride: int = 0, sum_ptr: int | None = None, sum_stride: int = 0,
+                   mean_ptr: int | None = None, rstd_ptr: int | None = None, scale_ptr: int | None = None,
+                   scale_mode: str | None = None, stream: int | None = None) -> None:
+    """fx_layer_norm: y = layer norm of x + residual, the sum stored at ``sum_ptr``, the rows' statistics (f32 [rows]) at
+    ``mean_ptr`` and ``rstd_ptr``. Types are "f32", "f16" or "bf16"; ``y_type`` "e4m3" or "i8" with ``scale_mode`` "row"
+    (scales written to ``scale_ptr`` [rows]) or "tensor" (one scale read there). Strides are in elements, 0 for packed rows."""
+    check(lib().fx_layer_norm(x_ptr, DTYPES[x_type], rows, cols, x_stride, residual_ptr, DTYPES[residual_type],
+                              residual_stride, sum_ptr, sum_stride, weight_ptr, bias_ptr, DTYPES[weight_type], eps, y_ptr,
+                              DTYPES[y_type], y_stride, mean_ptr, rstd_ptr, scale_ptr, SCALE_MODES[scale_mode], stream))
+
+
+def layer_norm_backward_workspace(rows: int, cols: int) -> int:
+    """fx_layer_norm_backward_workspace: bytes that layer_norm_backward_dev needs for the weight's and bias's gradients."""
+    return lib().fx_layer_norm_backward_workspace(rows, cols)
+
+
+def layer_norm_backward_dev(dy_ptr: int, h_ptr: int, mean_ptr: int, rstd_ptr: int, rows: int, cols: int,
+                            dy_type: str = "bf16", h_type: str = "bf16", weight_ptr: int | None = None,
+                            weight_type: str = "bf16", dsum_ptr: int | None = None, dx_ptr: int | None = None,
+                            dx_type: str = "bf16", dweight_ptr: int | None = None, dbias_ptr: int | None = None,
+                            accumulate: bool = False, work_ptr: int | None = None, work_bytes: int = 0, dy_stride: int = 0,
+                            h_stride: int = 0, dsum_stride: int = 0, dx_stride: int = 0, stream: int | None = None) -> None:
+    """fx_layer_norm_backward: dx (with ``dsum_ptr``, the gradient beside the norm, added), and f32 dweight and dbias, which
+    need a workspace of layer_norm_backward_workspace(rows, cols) bytes. ``h_ptr`` holds what layer_norm_dev normalised."""
+    check(lib().fx_layer_norm_backward(dy_ptr, DTYPES[dy_type], rows, cols, dy_stride, h_ptr, DTYPES[h_type], h_stride,
+                                       mean_ptr, rstd_ptr, weight_ptr, DTYPES[weight_type], dsum_ptr, dsum_stride, dx_ptr,
+                                       DTYPES[dx_type], dx_stride, dweight_ptr, dbias_ptr, int(accumulate), work_ptr,
+                                       work_bytes, stream))
+
+
+def i8_quantize_dev(x_ptr: int, rows: int, cols: int, codes_ptr: int, scales_ptr: int, x_type: str = "bf16",
+                    scale_mode: str = "row", x_stride: int = 0, codes_stride: int = 0, stream: int | None = None) -> None:
+    """fx_i8_quantize: rows to int8 codes, with a scale per row (written) or one for the tensor (read)."""
+    check(lib().fx_i8_quantize(x_ptr, DTYPES[x_type], rows, cols, x_stride, codes_ptr, codes_stride, scales_ptr,
+                               SCALE_MODES[scale_mode], stream))
+
+
+def i8_dequantize_dev(codes_ptr: int, scales_ptr: int, rows: int, cols: int, y_ptr: int, y_type: str = "bf16",
+                      scale_mode: str = "row", codes_stride: int = 0, y_stride: int = 0, stream: int | None = None) -> None:
+    """fx_i8_dequantize: the values that int8 codes and scales stand for."""
+    check(lib().fx_i8_dequantize(codes_ptr, codes_stride, scales_ptr, SCALE_MODES[scale_mode], rows, cols, y_ptr,
+                                 DTYPES[y_type], y_stride, stream))
+
+
+def i8_linear_dev(x_ptr: int, y_ptr: int, rows: int, n: int, k: int, codes_ptr: int, scales_ptr: int, x_scale_ptr: int,
+                  y_type: str = "bf16", x_scale_mode: str = "row", x_stride: int = 0, y_stride: int = 0,
+                  codes_stride: int = 0, bias_ptr: int | None = None, stream: int | None = None) -> None:
+    """fx_i8_linear: y [rows][n] = int8 x [rows][k] times int8 weights [n][k], scaled by token and by channel, plus bias
+    (f32). Codes and scales are i8_quantize_dev's or layer_norm_dev's."""
+    check(lib().fx_i8_linear(x_ptr, rows, x_stride, x_scale_ptr, SCALE_MODES[x_scale_mode], codes_ptr, codes_stride,
+                             scales_ptr, n, k, bias_ptr, y_ptr, DTYPES[y_type], y_stride, stream))
 
 
 # ---- nets ----------------------------------------------------------------------------------

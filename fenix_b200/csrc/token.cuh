@@ -1,5 +1,5 @@
-// token.cuh — operators over token rows: RMS norm with the residual's addition and 8-bit output, the
-// linear layer with 4-bit weights, the 4-bit quantiser. Types are fx_dtype's values.
+// token.cuh — operators over token rows: RMS norm and layer norm with the residual's addition and 8-bit output, the layer
+// norm's backward pass, the linear layers with 4-bit and 8-bit weights, their quantisers. Types are fx_dtype's values.
 #pragma once
 
 #include <cstdint>
@@ -10,10 +10,12 @@
 
 namespace fxk {
 
-enum TokType : int { kTokF32 = 0, kTokF16 = 1, kTokBF16 = 2, kTokE4M3 = 3 };
+enum TokType : int { kTokF32 = 0, kTokF16 = 1, kTokBF16 = 2, kTokE4M3 = 3, kTokI8 = 4 };
 enum TokScale : int { kScaleNone = 0, kScaleTensor = 1, kScaleRow = 2 };
 
 constexpr int kRmsMaxCols = 32768;
+constexpr int kLnMaxCols = 32768;
+constexpr int kI8MaxInner = 131071;  // inputs of an 8-bit layer: sums of products of two bytes stay below 2^31
 
 struct RmsNormArgs {
     const void* x;
@@ -31,6 +33,70 @@ struct RmsNormArgs {
 int sm_count();
 
 cudaError_t launch_rms_norm(const RmsNormArgs& a, cudaStream_t s);
+
+struct LayerNormArgs {
+    const void* x;
+    const void* residual;  // may be null
+    void* sum;             // may be null
+    const void* weight;    // may be null
+    const void* bias;      // may be null
+    void* y;
+    float* mean;   // may be null
+    float* rstd;   // may be null
+    float* scale;  // read (kScaleTensor) or written (kScaleRow); null with kScaleNone
+    int64_t x_stride, residual_stride, sum_stride, y_stride;
+    int rows, cols;
+    int x_type, residual_type, weight_type, y_type, scale_mode;
+    float eps;
+};
+cudaError_t launch_layer_norm(const LayerNormArgs& a, cudaStream_t s);
+
+struct LayerNormBackwardArgs {
+    const void* dy;
+    const void* h;
+    const float* mean;
+    const float* rstd;
+    const void* weight;  // may be null
+    const void* dsum;    // may be null; of dx_type
+    void* dx;            // may be null
+    float* dweight;      // may be null
+    float* dbias;        // may be null
+    float* work;         // [blocks][2][cols] sums of dweight and dbias
+    int64_t dy_stride, h_stride, dsum_stride, dx_stride;
+    int rows, cols;
+    int dy_type, h_type, weight_type, dx_type;
+    bool accumulate;
+};
+// Blocks whose sums of the weight's gradient wait in the workspace, at most: the same on every device.
+int64_t layer_norm_backward_blocks(int64_t rows, int64_t cols);
+cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStream_t s);
+
+struct I8RowsArgs {  // values [rows][cols] beside their 8-bit form
+    const void* x;   // read by the quantiser
+    void* y;         // written by the way back
+    int8_t* codes;
+    float* scale;  // one (kScaleTensor) or [rows]
+    int64_t stride, codes_stride;
+    int rows, cols;
+    int type, scale_mode;
+};
+cudaError_t launch_i8_quantize(const I8RowsArgs& a, cudaStream_t s);
+cudaError_t launch_i8_dequantize(const I8RowsArgs& a, cudaStream_t s);
+
+struct I8LinearArgs {
+    const int8_t* x;
+    const int8_t* codes;   // [n][k]
+    const float* x_scale;  // one (kScaleTensor) or [rows]
+    const float* scales;   // [n]
+    const float* bias;     // may be null
+    void* y;
+    int64_t x_stride, codes_stride, y_stride;
+    int rows, n, k;
+    int x_scale_mode, y_type;
+    bool hold_codes;   // failure self-test only: no codes are brought, so that the waits for them run out
+    uint64_t wait_ns;  // limit of each wait inside the kernel
+};
+cudaError_t launch_i8_linear(const I8LinearArgs& a, cudaStream_t s);
 
 struct W4Args {
     const uint8_t* codes;  // [n][k / 2]

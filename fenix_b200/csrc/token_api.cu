@@ -35,7 +35,7 @@ int sm_count() {
 namespace {
 
 constexpr int64_t kMaxExtent = int64_t{1} << 30;  // rows, columns and strides: byte offsets stay below 2^62
-constexpr uint64_t kWaitNs = 2000000000;          // limit of a wait inside a 4-bit linear kernel
+constexpr uint64_t kWaitNs = 2000000000;          // limit of a wait inside a linear kernel
 constexpr int64_t kMaxInner = int64_t{1} << 24;   // k of a 4-bit layer: 32-bit offsets inside 128 of its rows
 
 fx_status bad(const char* fn, const char* what) {
@@ -43,7 +43,7 @@ fx_status bad(const char* fn, const char* what) {
 }
 
 bool is_float(int t) { return t == FX_F32 || t == FX_F16 || t == FX_BF16; }
-int64_t type_size(int t) { return t == FX_F32 ? 4 : t == FX_E4M3 ? 1 : 2; }
+int64_t type_size(int t) { return t == FX_F32 ? 4 : t == FX_E4M3 || t == FX_I8 ? 1 : 2; }
 bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(to) == 0; }
 
 // Packed rows for a stride of 0; false when the stride is out of range.
@@ -120,6 +120,15 @@ fx_status check_w4(const char* fn, const uint8_t* codes, const void* scales, int
     if (!codes || !scales) return bad(fn, "null codes or scales");
     if (!aligned(codes, 16)) return bad(fn, "codes must be 16-byte aligned");
     if (!aligned(scales, type_size(scale_type))) return bad(fn, "scales are not aligned to their type");
+    return FX_OK;
+}
+
+// Rows of values and of codes: everything that needs no device.
+fx_status check_i8_rows(const char* fn, int64_t rows, int64_t cols, int64_t& stride, int64_t& codes_stride, int scale_mode) {
+    if (rows < 0 || rows >= kMaxExtent || cols < 1 || cols >= kMaxExtent) return bad(fn, "rows or cols out of range");
+    if (scale_mode != FX_SCALE_TENSOR && scale_mode != FX_SCALE_ROW) return bad(fn, "codes take a tensor or a row scale");
+    if (!fix_stride(stride, cols) || !fix_stride(codes_stride, cols))
+        return bad(fn, "a stride is shorter than a row or out of range");
     return FX_OK;
 }
 
@@ -344,6 +353,237 @@ fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_
         if (fx_status r = on.enter(fn, {dev_codes, dev_scales, dev_zeros, dev_w})) return r;
         return done(fn, fxk::launch_w4_dequantize(w4_args(dev_codes, dev_scales, scale_type, dev_zeros, n, k, group),
                                                   dev_w, w_type, w_stride, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+fx_status fx_layer_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                        const void* dev_residual, fx_dtype residual_type, int64_t residual_stride, void* dev_sum,
+                        int64_t sum_stride, const void* dev_weight, const void* dev_bias, fx_dtype weight_type, float eps,
+                        void* dev_y, fx_dtype y_type, int64_t y_stride, float* dev_mean, float* dev_rstd, float* dev_scale,
+                        fx_scale scale_mode, void* stream) {
+    static const char* const fn = "fx_layer_norm";
+    return guarded([&]() -> fx_status {
+        if (rows < 0 || rows >= kMaxExtent) return bad(fn, "rows out of range");
+        if (cols < 1 || cols > fxk::kLnMaxCols) return bad(fn, "cols must be 1..32768");
+        if (!(eps > 0.f) || eps > 3.0e38f) return bad(fn, "eps must be positive and finite");
+        if (!is_float(x_type) || !is_float(residual_type) || !is_float(weight_type))
+            return bad(fn, "x, residual and weight are f32, f16 or bf16");
+        const bool eight = y_type == FX_E4M3 || y_type == FX_I8;
+        if (!is_float(y_type) && !eight) return bad(fn, "y is f32, f16, bf16, e4m3 or i8");
+        if (eight ? (scale_mode != FX_SCALE_TENSOR && scale_mode != FX_SCALE_ROW) : scale_mode != FX_SCALE_NONE)
+            return bad(fn, "an 8-bit y takes a tensor or a row scale, another y none");
+        if (!fix_stride(x_stride, cols) || !fix_stride(residual_stride, cols) || !fix_stride(sum_stride, cols) ||
+            !fix_stride(y_stride, cols))
+            return bad(fn, "a stride is shorter than a row or out of range");
+        if (rows == 0) return FX_OK;
+        if (!dev_x || !dev_y) return bad(fn, "null x or y");
+        if (eight && !dev_scale) return bad(fn, "an 8-bit y needs dev_scale");
+        if (!aligned(dev_x, type_size(x_type)) || !aligned(dev_y, type_size(y_type)) ||
+            !aligned(dev_residual, type_size(residual_type)) || !aligned(dev_sum, type_size(residual_type)) ||
+            !aligned(dev_weight, type_size(weight_type)) || !aligned(dev_bias, type_size(weight_type)) ||
+            !aligned(dev_mean, 4) || !aligned(dev_rstd, 4) || !aligned(dev_scale, 4))
+            return bad(fn, "a pointer is not aligned to its type");
+        if (dev_y == dev_x && (y_type != x_type || (rows > 1 && y_stride != x_stride)))
+            return bad(fn, "y in place of x needs x's type and stride");
+        if (dev_sum && dev_sum == dev_x && (residual_type != x_type || (rows > 1 && sum_stride != x_stride)))
+            return bad(fn, "sum in place of x needs x's type and stride");
+        if (dev_sum && dev_sum == dev_residual && rows > 1 && sum_stride != residual_stride)
+            return bad(fn, "sum in place of residual needs its stride");
+        if (dev_y == dev_sum || dev_y == dev_residual) return bad(fn, "y may not be sum or residual");
+        if (scale_mode == FX_SCALE_NONE) dev_scale = nullptr;
+        if ((dev_mean && (dev_mean == dev_rstd || dev_mean == dev_scale)) || (dev_rstd && dev_rstd == dev_scale))
+            return bad(fn, "mean, rstd and scale may not be one another");
+        OnDevice on;
+        if (fx_status r = on.enter(fn, {dev_x, dev_y, dev_residual, dev_sum, dev_weight, dev_bias, dev_mean, dev_rstd, dev_scale}))
+            return r;
+        fxk::LayerNormArgs a{};
+        a.x = dev_x;
+        a.residual = dev_residual;
+        a.sum = dev_sum;
+        a.weight = dev_weight;
+        a.bias = dev_bias;
+        a.y = dev_y;
+        a.mean = dev_mean;
+        a.rstd = dev_rstd;
+        a.scale = dev_scale;
+        a.x_stride = x_stride;
+        a.residual_stride = residual_stride;
+        a.sum_stride = sum_stride;
+        a.y_stride = y_stride;
+        a.rows = static_cast<int>(rows);
+        a.cols = static_cast<int>(cols);
+        a.x_type = x_type;
+        a.residual_type = residual_type;
+        a.weight_type = weight_type;
+        a.y_type = y_type;
+        a.scale_mode = scale_mode;
+        a.eps = eps;
+        return done(fn, fxk::launch_layer_norm(a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+uint64_t fx_layer_norm_backward_workspace(int64_t rows, int64_t cols) {
+    if (rows < 0 || rows >= kMaxExtent || cols < 1 || cols > fxk::kLnMaxCols) return 0;
+    return static_cast<uint64_t>(fxk::layer_norm_backward_blocks(rows, cols)) * 8 * static_cast<uint64_t>(cols);
+}
+
+fx_status fx_layer_norm_backward(const void* dev_dy, fx_dtype dy_type, int64_t rows, int64_t cols, int64_t dy_stride,
+                                 const void* dev_h, fx_dtype h_type, int64_t h_stride, const float* dev_mean,
+                                 const float* dev_rstd, const void* dev_weight, fx_dtype weight_type, const void* dev_dsum,
+                                 int64_t dsum_stride, void* dev_dx, fx_dtype dx_type, int64_t dx_stride, float* dev_dweight,
+                                 float* dev_dbias, int accumulate, void* dev_work, uint64_t work_bytes, void* stream) {
+    static const char* const fn = "fx_layer_norm_backward";
+    return guarded([&]() -> fx_status {
+        if (rows < 0 || rows >= kMaxExtent) return bad(fn, "rows out of range");
+        if (cols < 1 || cols > fxk::kLnMaxCols) return bad(fn, "cols must be 1..32768");
+        if (!is_float(dy_type) || !is_float(h_type) || !is_float(weight_type) || !is_float(dx_type))
+            return bad(fn, "dy, h, weight and dx are f32, f16 or bf16");
+        if (!fix_stride(dy_stride, cols) || !fix_stride(h_stride, cols) || !fix_stride(dsum_stride, cols) ||
+            !fix_stride(dx_stride, cols))
+            return bad(fn, "a stride is shorter than a row or out of range");
+        const bool sums = dev_dweight || dev_dbias;
+        if (rows == 0 && !sums) return FX_OK;
+        if (!dev_dx && !sums) return bad(fn, "dx, dweight and dbias are all null");
+        if (rows && (!dev_dy || !dev_h || !dev_mean || !dev_rstd)) return bad(fn, "null dy, h, mean or rstd");
+        if (!aligned(dev_dy, type_size(dy_type)) || !aligned(dev_h, type_size(h_type)) || !aligned(dev_mean, 4) ||
+            !aligned(dev_rstd, 4) || !aligned(dev_weight, type_size(weight_type)) ||
+            !aligned(dev_dsum, type_size(dx_type)) || !aligned(dev_dx, type_size(dx_type)) || !aligned(dev_dweight, 4) ||
+            !aligned(dev_dbias, 4))
+            return bad(fn, "a pointer is not aligned to its type");
+        if (dev_dx && ((dev_dx == dev_dy && (dx_type != dy_type || (rows > 1 && dx_stride != dy_stride))) ||
+                       (dev_dx == dev_h && (dx_type != h_type || (rows > 1 && dx_stride != h_stride))) ||
+                       (dev_dx == dev_dsum && rows > 1 && dx_stride != dsum_stride)))
+            return bad(fn, "dx in place of an input needs its type and stride");
+        if (dev_dweight && dev_dweight == dev_dbias) return bad(fn, "dweight may not be dbias");
+        if (sums && rows) {
+            if (!dev_work || !aligned(dev_work, 16)) return bad(fn, "dweight and dbias need a 16-byte aligned workspace");
+            if (work_bytes < fx_layer_norm_backward_workspace(rows, cols)) return bad(fn, "the workspace is too small");
+        } else {
+            dev_work = nullptr;
+        }
+        if (!dev_dx) dev_dsum = nullptr;
+        OnDevice on;
+        if (fx_status r = on.enter(fn, {dev_dy, dev_h, dev_mean, dev_rstd, dev_weight, dev_dsum, dev_dx, dev_dweight, dev_dbias,
+                                        dev_work}))
+            return r;
+        fxk::LayerNormBackwardArgs a{};
+        a.dy = dev_dy;
+        a.h = dev_h;
+        a.mean = dev_mean;
+        a.rstd = dev_rstd;
+        a.weight = dev_weight;
+        a.dsum = dev_dsum;
+        a.dx = dev_dx;
+        a.dweight = dev_dweight;
+        a.dbias = dev_dbias;
+        a.work = static_cast<float*>(dev_work);
+        a.dy_stride = dy_stride;
+        a.h_stride = h_stride;
+        a.dsum_stride = dsum_stride;
+        a.dx_stride = dx_stride;
+        a.rows = static_cast<int>(rows);
+        a.cols = static_cast<int>(cols);
+        a.dy_type = dy_type;
+        a.h_type = h_type;
+        a.weight_type = weight_type;
+        a.dx_type = dx_type;
+        a.accumulate = accumulate != 0;
+        return done(fn, fxk::launch_layer_norm_backward(a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+fx_status fx_i8_quantize(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                         int8_t* dev_codes, int64_t codes_stride, float* dev_scales, fx_scale scale_mode, void* stream) {
+    static const char* const fn = "fx_i8_quantize";
+    return guarded([&]() -> fx_status {
+        if (!is_float(x_type)) return bad(fn, "x is f32, f16 or bf16");
+        if (fx_status r = check_i8_rows(fn, rows, cols, x_stride, codes_stride, scale_mode)) return r;
+        if (rows == 0) return FX_OK;
+        if (!dev_x || !dev_codes || !dev_scales) return bad(fn, "null x, codes or scales");
+        if (!aligned(dev_x, type_size(x_type)) || !aligned(dev_scales, 4))
+            return bad(fn, "a pointer is not aligned to its type");
+        if (dev_x == dev_codes) return bad(fn, "codes may not be x");
+        OnDevice on;
+        if (fx_status r = on.enter(fn, {dev_x, dev_codes, dev_scales})) return r;
+        fxk::I8RowsArgs a{};
+        a.x = dev_x;
+        a.codes = dev_codes;
+        a.scale = dev_scales;
+        a.stride = x_stride;
+        a.codes_stride = codes_stride;
+        a.rows = static_cast<int>(rows);
+        a.cols = static_cast<int>(cols);
+        a.type = x_type;
+        a.scale_mode = scale_mode;
+        return done(fn, fxk::launch_i8_quantize(a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+fx_status fx_i8_dequantize(const int8_t* dev_codes, int64_t codes_stride, const float* dev_scales, fx_scale scale_mode,
+                           int64_t rows, int64_t cols, void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream) {
+    static const char* const fn = "fx_i8_dequantize";
+    return guarded([&]() -> fx_status {
+        if (!is_float(y_type)) return bad(fn, "y is f32, f16 or bf16");
+        if (fx_status r = check_i8_rows(fn, rows, cols, y_stride, codes_stride, scale_mode)) return r;
+        if (rows == 0) return FX_OK;
+        if (!dev_y || !dev_codes || !dev_scales) return bad(fn, "null codes, scales or y");
+        if (!aligned(dev_y, type_size(y_type)) || !aligned(dev_scales, 4))
+            return bad(fn, "a pointer is not aligned to its type");
+        if (dev_y == dev_codes) return bad(fn, "y may not be codes");
+        OnDevice on;
+        if (fx_status r = on.enter(fn, {dev_codes, dev_scales, dev_y})) return r;
+        fxk::I8RowsArgs a{};
+        a.y = dev_y;
+        a.codes = const_cast<int8_t*>(dev_codes);
+        a.scale = const_cast<float*>(dev_scales);
+        a.stride = y_stride;
+        a.codes_stride = codes_stride;
+        a.rows = static_cast<int>(rows);
+        a.cols = static_cast<int>(cols);
+        a.type = y_type;
+        a.scale_mode = scale_mode;
+        return done(fn, fxk::launch_i8_dequantize(a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+fx_status fx_i8_linear(const int8_t* dev_x, int64_t rows, int64_t x_stride, const float* dev_x_scale, fx_scale x_scale_mode,
+                       const int8_t* dev_codes, int64_t codes_stride, const float* dev_scales, int64_t n, int64_t k,
+                       const float* dev_bias, void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream) {
+    static const char* const fn = "fx_i8_linear";
+    return guarded([&]() -> fx_status {
+        if (rows < 0 || rows >= kMaxExtent || n < 0 || n >= kMaxExtent) return bad(fn, "rows or n out of range");
+        if (k < 1 || k > fxk::kI8MaxInner) return bad(fn, "k must be 1..131071");
+        if (!is_float(y_type)) return bad(fn, "y is f32, f16 or bf16");
+        if (x_scale_mode != FX_SCALE_TENSOR && x_scale_mode != FX_SCALE_ROW)
+            return bad(fn, "x takes a tensor or a row scale");
+        if (!fix_stride(x_stride, k) || !fix_stride(codes_stride, k) || !fix_stride(y_stride, n))
+            return bad(fn, "a stride is shorter than a row or out of range");
+        if (rows == 0 || n == 0) return FX_OK;
+        if (!dev_x || !dev_x_scale || !dev_codes || !dev_scales || !dev_y)
+            return bad(fn, "null x, codes, scales or y");
+        if (!aligned(dev_x_scale, 4) || !aligned(dev_scales, 4) || !aligned(dev_bias, 4) ||
+            !aligned(dev_y, type_size(y_type)))
+            return bad(fn, "a pointer is not aligned to its type");
+        if (dev_y == dev_x || dev_y == dev_codes) return bad(fn, "y may not be x or codes");
+        OnDevice on;
+        if (fx_status r = on.enter(fn, {dev_x, dev_x_scale, dev_codes, dev_scales, dev_bias, dev_y})) return r;
+        fxk::I8LinearArgs a{};
+        a.x = dev_x;
+        a.codes = dev_codes;
+        a.x_scale = dev_x_scale;
+        a.scales = dev_scales;
+        a.bias = dev_bias;
+        a.y = dev_y;
+        a.x_stride = x_stride;
+        a.codes_stride = codes_stride;
+        a.y_stride = y_stride;
+        a.rows = static_cast<int>(rows);
+        a.n = static_cast<int>(n);
+        a.k = static_cast<int>(k);
+        a.x_scale_mode = x_scale_mode;
+        a.y_type = y_type;
+        a.wait_ns = kWaitNs;
+        return done(fn, fxk::launch_i8_linear(a, static_cast<cudaStream_t>(stream)));
     });
 }
 

@@ -395,9 +395,9 @@ fx_status fx_accum_finalize(const float* dev_acc, int64_t dz, int64_t dy, int64_
                             const float* dev_wz, const float* dev_wy, const float* dev_wx, float* dev_prob,
                             uint8_t* dev_u8, void* stream);
 
-/* ---- token rows: norm, 4-bit linear layers (device pointers) ----
+/* ---- token rows: norms, 4-bit and 8-bit linear layers (device pointers) ----
  * A token model's step between two attention or mixing layers: normalise the rows (with the residual's
- * addition, to 8 bits with scales or to 16 / 32), multiply them by a linear layer held in 4 bits. No
+ * addition, to 8 bits with scales or to 16 / 32), multiply them by a linear layer held in 4 or 8 bits. No
  * reference counterpart (its token models run through libtorch, src/ml/nets/dinovol.hpp).
  * Common to these calls: matrices are row-major with their rows `*_stride` elements apart (at least the
  * row's length; 0: packed) and their elements at least element-aligned. Every pointer of a call is device
@@ -405,8 +405,8 @@ fx_status fx_accum_finalize(const float* dev_acc, int64_t dz, int64_t dy, int64_
  * belongs to that device. The calls enqueue one kernel (a few in a row for extents past 65535), allocate
  * nothing, keep nothing between calls and do not synchronise, so any number may run at once and be captured
  * into graphs. Extents and strides are below 2^30. No row (rows or n = 0) is not an error: nothing is done. */
-typedef enum fx_dtype { FX_F32 = 0, FX_F16 = 1, FX_BF16 = 2, FX_E4M3 = 3 } fx_dtype;
-/* Scale of 8-bit rows (value = e4m3 * scale): none, one for the tensor, or one per row. */
+typedef enum fx_dtype { FX_F32 = 0, FX_F16 = 1, FX_BF16 = 2, FX_E4M3 = 3, FX_I8 = 4 } fx_dtype;
+/* Scale of 8-bit rows (value = e4m3 or int8 * scale): none, one for the tensor, or one per row. */
 typedef enum fx_scale { FX_SCALE_NONE = 0, FX_SCALE_TENSOR = 1, FX_SCALE_ROW = 2 } fx_scale;
 
 /* Root-mean-square norm of rows, with the residual's addition before it and quantisation after it:
@@ -468,6 +468,71 @@ fx_status fx_w4_quantize(const void* dev_w, fx_dtype w_type, int64_t n, int64_t 
 fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_dtype scale_type,
                            const uint8_t* dev_zeros, int64_t n, int64_t k, int64_t group, void* dev_w,
                            fx_dtype w_type, int64_t w_stride, void* stream);
+
+/* Layer norm of rows, with the residual's addition before it and quantisation after it:
+ *   h = x + residual,  v = (h - mean(h)) / sqrt(var(h) + eps) * weight + bias,  var = mean((h - mean(h))^2)
+ * per row of `cols` values, in f32. Types, strides, dev_sum, scales, in-place forms, limits and rows that are not finite
+ * are fx_rms_norm's; besides,
+ *   - dev_bias may be NULL (zeros) and has weight_type, as dev_weight, which may be NULL (ones);
+ *   - dev_mean and dev_rstd, f32 [rows] each, may be NULL, else receive mean(h) and 1 / sqrt(var(h) + eps), of the
+ *     unrounded h, for fx_layer_norm_backward;
+ *   - y_type may be i8: y = v / scale rounded to nearest, ties to even, and saturated to +-127, with
+ *       FX_SCALE_ROW     scale[row] = max(max |v|, 1e-30) / 127, written to dev_scale [rows]
+ *       FX_SCALE_TENSOR  scale = dev_scale[0], read
+ *     A row that holds a NaN or infinity gets zeros under a row scale that is NaN; under a tensor scale its NaN become zero.
+ * The mean is right to half a step of f32 of its own size, or 2^-48 of the largest |h| where that is more, so that rows
+ * far from zero keep their differences. */
+fx_status fx_layer_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                        const void* dev_residual, fx_dtype residual_type, int64_t residual_stride, void* dev_sum,
+                        int64_t sum_stride, const void* dev_weight, const void* dev_bias, fx_dtype weight_type, float eps,
+                        void* dev_y, fx_dtype y_type, int64_t y_stride, float* dev_mean, float* dev_rstd, float* dev_scale,
+                        fx_scale scale_mode, void* stream);
+
+/* Bytes of workspace that fx_layer_norm_backward needs for dev_dweight or dev_dbias (the same on every device); 0 where
+ * the extents are out of range. */
+uint64_t fx_layer_norm_backward_workspace(int64_t rows, int64_t cols);
+
+/* The layer norm's backward pass, from the gradient dy of v: with z = (h - mean) * rstd and g = dy * weight,
+ *   dx = (g - mean(g) - z * mean(g * z)) * rstd + dsum,   dweight = sum over rows of dy * z,   dbias = the same of dy
+ * in f32, where mean(.) is a row's. dev_h holds the values that were normalised (fx_layer_norm's dev_sum, or its x without
+ * a residual), dev_mean and dev_rstd what fx_layer_norm wrote for them. dev_dsum (may be NULL: zeros) is the gradient that
+ * reaches h beside the norm, of dx_type, as dx. dx is the gradient of x and of residual alike. dy, h, weight and dx are f32, f16 or
+ * bf16 each; dev_weight may be NULL (ones). dev_dweight and dev_dbias, f32 [cols], are overwritten, or added to where
+ * `accumulate` is not 0; they are sums of every row whatever `rows`, so without a row they are zeros (or left as they
+ * are). dx, dweight and dbias may each be NULL, not all three. Every sum repeats exactly on GPUs of one kind.
+ * dev_work: 16-byte aligned, at least fx_layer_norm_backward_workspace bytes, read by nothing else until this call's
+ * kernels are done (so calls that may run at once, captured ones included, have one each); NULL where dweight and dbias are.
+ * In place: dev_dx may be dev_dy, dev_h or dev_dsum at equal types and strides; no other overlap.
+ * 1 <= cols <= 32768. */
+fx_status fx_layer_norm_backward(const void* dev_dy, fx_dtype dy_type, int64_t rows, int64_t cols, int64_t dy_stride,
+                                 const void* dev_h, fx_dtype h_type, int64_t h_stride, const float* dev_mean,
+                                 const float* dev_rstd, const void* dev_weight, fx_dtype weight_type, const void* dev_dsum,
+                                 int64_t dsum_stride, void* dev_dx, fx_dtype dx_type, int64_t dx_stride, float* dev_dweight,
+                                 float* dev_dbias, int accumulate, void* dev_work, uint64_t work_bytes, void* stream);
+
+/* The 8-bit form of rows [rows][cols] (f32, f16, bf16): weights by output channel, activations by token.
+ *   FX_SCALE_ROW     scale[row] = max(max |x|, 1e-30) / 127 of the row's numbers, written to dev_scales [rows]
+ *   FX_SCALE_TENSOR  scale = dev_scales[0], read
+ *   code = clamp(round(x / scale), -127, 127), the f32 quotient rounded to nearest, ties to even
+ * A row that holds a NaN or infinity gets a scale that is not finite, so that what is computed from it is not either; the
+ * codes of its NaN are zeros, and under a tensor scale NaN are zeros and infinities +-127. cols is any number below 2^30. */
+fx_status fx_i8_quantize(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                         int8_t* dev_codes, int64_t codes_stride, float* dev_scales, fx_scale scale_mode, void* stream);
+/* The values such rows stand for: y = scale * code in f32, rounded to y_type (f32, f16, bf16). */
+fx_status fx_i8_dequantize(const int8_t* dev_codes, int64_t codes_stride, const float* dev_scales, fx_scale scale_mode,
+                           int64_t rows, int64_t cols, void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream);
+
+/* Linear layer of 8-bit integers: for `rows` rows of k values and n outputs
+ *   y[r][o] = (sum over i of x[r][i] * codes[o][i]) * x_scale[r] * scales[o] + bias[o]
+ * with int8 x and codes (any values, -128 among them), x_scale f32 (FX_SCALE_TENSOR one value, FX_SCALE_ROW [rows]), scales
+ * f32 [n], bias f32 [n] or NULL. The sum is exact, in 32-bit integers; the products with the scales and the addition are
+ * f32's, one rounding each, and y (f32, f16, bf16) is rounded once more. 1 <= k <= 131071; rows and n are any numbers.
+ * x_scale_mode FX_SCALE_NONE is refused. y overlaps no input. Results repeat exactly, and a row's do not depend on the
+ * other rows of its call. Rows of x and of codes that begin at multiples of 16 bytes (address and stride) are brought by
+ * TMA and multiplied on tcgen05; others take a slower way. fx_i8_quantize and fx_layer_norm write either. */
+fx_status fx_i8_linear(const int8_t* dev_x, int64_t rows, int64_t x_stride, const float* dev_x_scale, fx_scale x_scale_mode,
+                       const int8_t* dev_codes, int64_t codes_stride, const float* dev_scales, int64_t n, int64_t k,
+                       const float* dev_bias, void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream);
 
 /* ---- .fxvol archives and the chunk codec ---------------------------------------------------
  * A 64^3 chunk is one tile of 4^3 DCT-16 blocks whose magnitude categories share up to 8 clustered
