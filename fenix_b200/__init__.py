@@ -214,6 +214,8 @@ def lib():
     _sig(L, "fx_i8_quantize", i32, [vp, i32, i64, i64, i64, vp, i64, vp, i32, vp])
     _sig(L, "fx_i8_dequantize", i32, [vp, i64, vp, i32, i64, i64, vp, i32, i64, vp])
     _sig(L, "fx_i8_linear", i32, [vp, i64, i64, vp, i32, vp, i64, vp, i64, i64, vp, vp, i32, i64, vp])
+    _sig(L, "fx_i8_device_status", i32, [i32])
+    _sig(L, "fx_selftest_i8_wait_timeout", i32, [i32, i32, C.c_uint64])
     _sig(L, "fx_w4_device_status", i32, [i32])
     _sig(L, "fx_selftest_w4_wait_timeout", i32, [i32, i32, i32, C.c_uint64])
     _sig(L, "fx_w4_quantize", i32, [vp, i32, i64, i64, i64, i64, vp, vp, i32, vp, vp])
@@ -420,6 +422,11 @@ def i8_linear_dev(x_ptr: int, y_ptr: int, rows: int, n: int, k: int, codes_ptr: 
     (f32). Codes and scales are i8_quantize_dev's or layer_norm_dev's."""
     check(lib().fx_i8_linear(x_ptr, rows, x_stride, x_scale_ptr, SCALE_MODES[x_scale_mode], codes_ptr, codes_stride,
                              scales_ptr, n, k, bias_ptr, y_ptr, DTYPES[y_type], y_stride, stream))
+
+
+def i8_device_status(device: int = 0) -> None:
+    """fx_i8_device_status: raise if a bounded wait inside an 8-bit linear kernel gave up."""
+    check(lib().fx_i8_device_status(device))
 
 
 # ---- nets ----------------------------------------------------------------------------------

@@ -91,6 +91,25 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const v
     }
 }
 
+// Bounded wait for a phase. Gives up after limit_ns, or when another role of the block has. The clock is read only
+// after many tries (each may sleep for a while in hardware): an ordinary wait costs no more than itself.
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile int* abort, uint64_t limit_ns) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 0;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (it % 64 == 63) {
+            if (abort && *abort) return false;
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > limit_ns) return false;
+        }
+    }
+}
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // ---- bulk async copy global -> shared (1-D, no tensor map) ----------------------------------
 // dst/src 16-byte aligned, bytes a multiple of 16; completion is signalled as tx bytes on bar.
 __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -132,6 +151,15 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Same with 8-bit integers (kind::i8, s8 x s8, s32 accumulate).
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
@@ -290,6 +318,12 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
     return d;                             // base offset 0, lbo mode 0, layout type 0 (no swizzle)
 }
 
+// K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 |
+           static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+
 // Instruction descriptor: f32 accumulate, K-major A and B, dense.
 //   kind::f16      : a/b format 0 = f16, 1 = bf16
 //   kind::f8f6f4   : a/b format 0 = e4m3
@@ -299,6 +333,11 @@ __host__ __device__ constexpr uint32_t instr_desc(int M, int N, int optype) {
            | ((optype == kOpBF16 ? 1u : 0u) << 10)                    // B format
            | (static_cast<uint32_t>(N >> 3) << 17)                    // N / 8
            | (static_cast<uint32_t>(M >> 4) << 24);                   // M / 16
+}
+
+// The same of kind::i8: s32 accumulate, s8 A and B.
+__host__ __device__ constexpr uint32_t instr_desc_i8(int M, int N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
 // ---- small numeric helpers ---------------------------------------------------------------------

@@ -21,7 +21,7 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder() {
     return fn;
 }
 
-// Rows of 16-bit (elem = 2) or 8-byte (elem = 8) elements: `cols` of them in a row of `pitch` bytes (a multiple of
+// Rows of bytes (elem = 1), 16-bit (elem = 2) or 8-byte (elem = 8) elements: `cols` of them in a row of `pitch` bytes (a multiple of
 // 16, as the base is), boxes of box_cols x box_rows with 128 bytes in a box row, 128-byte swizzled in shared memory
 // (16-byte cell c of row r lies at cell c ^ (r % 8)). Out of range reads as zero.
 inline cudaError_t tmap_rows(CUtensorMap* map, const void* base, int elem, int64_t cols, int64_t rows, int64_t pitch,
@@ -31,7 +31,9 @@ inline cudaError_t tmap_rows(CUtensorMap* map, const void* base, int elem, int64
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
     const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / elem), static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t steps[2] = {1, 1};
-    const CUtensorMapDataType type = elem == 8 ? CU_TENSOR_MAP_DATA_TYPE_INT64 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    const CUtensorMapDataType type = elem == 8   ? CU_TENSOR_MAP_DATA_TYPE_INT64
+                                     : elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                                 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
     return tmap_encoder()(map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS

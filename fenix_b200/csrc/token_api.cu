@@ -2,6 +2,7 @@
 // call's pointers, the launch. Every check of sizes, types and nulls comes before the first CUDA call, so
 // refusals answer the same on a machine without a GPU.
 #include "fenix_b200.h"
+#include "i8_linear.cuh"
 #include "token.cuh"
 #include "w4.cuh"
 
@@ -584,6 +585,74 @@ fx_status fx_i8_linear(const int8_t* dev_x, int64_t rows, int64_t x_stride, cons
         a.y_type = y_type;
         a.wait_ns = kWaitNs;
         return done(fn, fxk::launch_i8_linear(a, static_cast<cudaStream_t>(stream)));
+    });
+}
+
+fx_status fx_i8_device_status(int device) {
+    static const char* const fn = "fx_i8_device_status";
+    return guarded([&]() -> fx_status {
+        int count = 0, cur = 0;
+        if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
+            cudaGetLastError();
+            return bad(fn, "no such device");
+        }
+        cudaGetDevice(&cur);
+        if (cudaError_t e = cudaSetDevice(device); e != cudaSuccess) return done(fn, e);
+        uint32_t stream = 0;
+        cudaError_t e = cudaDeviceSynchronize();
+        if (e == cudaSuccess) e = fxk::i8_stream_status(&stream);
+        cudaSetDevice(cur);
+        if (e != cudaSuccess) return done(fn, e);
+        if (stream)
+            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(stream));
+        return FX_OK;
+    });
+}
+
+fx_status fx_selftest_i8_wait_timeout(int device, int rows, uint64_t wait_ns) {
+    static const char* const fn = "fx_selftest_i8_wait_timeout";
+    return guarded([&]() -> fx_status {
+        int count = 0;
+        if (rows < 1 || rows > 4096 || wait_ns == 0) return bad(fn, "rows must be 1..4096 and the limit positive");
+        if (cudaGetDeviceCount(&count) != cudaSuccess || device < 0 || device >= count) {
+            cudaGetLastError();
+            return bad(fn, "no such device");
+        }
+        constexpr int kOut = 1024, kIn = 4096;
+        struct Scratch {  // zeros: the layer's operands and results
+            int back = -1;
+            void* p = nullptr;
+            ~Scratch() {
+                cudaFree(p);
+                if (back >= 0) cudaSetDevice(back);
+            }
+        } sc;
+        cudaGetDevice(&sc.back);
+        const size_t codes = size_t{kOut} * kIn, x = size_t(rows) * kIn, y = size_t(rows) * kOut * 2, scales = kOut * 4,
+                     all = codes + x + y + scales + 256;
+        cudaError_t e = cudaSetDevice(device);
+        if (e == cudaSuccess) e = cudaMalloc(&sc.p, all);
+        if (e == cudaSuccess) e = cudaMemset(sc.p, 0, all);
+        if (e != cudaSuccess) return done(fn, e);
+        int8_t* const at = static_cast<int8_t*>(sc.p);
+        fxk::I8LinearArgs a{};
+        a.codes = at;
+        a.x = at + codes;
+        a.y = at + codes + x;
+        a.scales = reinterpret_cast<const float*>(at + codes + x + y);
+        a.x_scale = a.scales;
+        a.x_scale_mode = FX_SCALE_TENSOR;
+        a.x_stride = a.codes_stride = kIn;
+        a.y_stride = kOut;
+        a.rows = rows;
+        a.n = kOut;
+        a.k = kIn;
+        a.y_type = FX_BF16;
+        a.hold_codes = true;
+        a.wait_ns = wait_ns;
+        e = fxk::launch_i8_linear(a, nullptr);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+        return done(fn, e);
     });
 }
 

@@ -44,21 +44,6 @@ cudaError_t w4_many_f16_status(uint32_t* code);
 static __device__ uint32_t g_w4_status;
 __device__ __forceinline__ void set_w4_status(uint32_t code) { set_status(&g_w4_status, code); }
 
-// Bounded wait for a phase. Gives up after limit_ns, or when another role of the block has. The clock is read only
-// after many tries (each may sleep for a while in hardware): an ordinary wait costs no more than itself.
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, const volatile int* abort, uint64_t limit_ns) {
-    uint64_t t0 = 0;
-    for (uint32_t it = 0;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (it % 64 == 63) {
-            if (abort && *abort) return false;
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > limit_ns) return false;
-        }
-    }
-}
-
 // (w & mask) | bits
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
     uint32_t r;

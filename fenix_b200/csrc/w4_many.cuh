@@ -30,12 +30,6 @@
 namespace fxk {
 namespace {
 
-// K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | static_cast<uint64_t>(1) << 16 |
-           static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
-}
-
 // D[tmem] (+)= A[tmem] * B[smem desc]^T, 16-bit inputs, f32 accumulate: every lane runs the code, on warp-uniform
 // operands, and the lane with issue != 0 executes it.
 __device__ __forceinline__ void mma_f16_ta_if(uint32_t issue, uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc,
@@ -54,9 +48,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
 }
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // Four f32 of a block of the cluster, at a shared-memory address of this one.
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {
     float4 v;

@@ -534,6 +534,15 @@ fx_status fx_i8_linear(const int8_t* dev_x, int64_t rows, int64_t x_stride, cons
                        const int8_t* dev_codes, int64_t codes_stride, const float* dev_scales, int64_t n, int64_t k,
                        const float* dev_bias, void* dev_y, fx_dtype y_type, int64_t y_stride, void* stream);
 
+/* FX_OK, or FX_INTERNAL when a wait inside an fx_i8_linear kernel on `device` gave up since the last call (every wait is
+ * bounded; such a kernel ends by itself and its outputs are undefined). Synchronises the device. */
+fx_status fx_i8_device_status(int device);
+
+/* Failure self-test of those waits: one layer of 1024 outputs and 4096 inputs over `rows` rows on `device` whose codes are
+ * never brought, with a limit of wait_ns a wait. FX_OK once the launch has ended by itself; fx_i8_device_status then reports
+ * the wait that gave up, and the context stays usable. Synchronises. */
+fx_status fx_selftest_i8_wait_timeout(int device, int rows, uint64_t wait_ns);
+
 /* ---- .fxvol archives and the chunk codec ---------------------------------------------------
  * A 64^3 chunk is one tile of 4^3 DCT-16 blocks whose magnitude categories share up to 8 clustered
  * rANS tables. Payloads and files are bit-compatible with the reference's codec and container. */
