@@ -136,8 +136,8 @@ cudaError_t launch_any(const I8LinearArgs& a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_i8_linear(const I8LinearArgs& a, cudaStream_t s) {
-    if (tma_rows(a.x, a.x_stride, a.rows) && tma_rows(a.codes, a.codes_stride, a.n) && a.rows <= 65535 * 256) return launch_i8_stream(a, s);
-    return launch_any(a, s);
+    if (!tma_rows(a.x, a.x_stride, a.rows) || !tma_rows(a.codes, a.codes_stride, a.n)) return launch_any(a, s);
+    return a.rows <= 256 ? launch_i8_stream(a, s) : launch_i8_pair(a, s);
 }
 
 }  // namespace fxk

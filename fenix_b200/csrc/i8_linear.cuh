@@ -15,8 +15,10 @@ inline bool tma_rows(const void* p, int64_t stride, int64_t rows) {
 }
 
 cudaError_t launch_i8_stream(const I8LinearArgs& a, cudaStream_t s);
+cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s);
 // The status words of the files' kernels, cleared.
 cudaError_t i8_stream_status(uint32_t* code);
+cudaError_t i8_pair_status(uint32_t* code);
 
 #ifdef __CUDACC__
 // Set by a kernel of this file's includer whose bounded wait gave up; read and cleared by take_i8_status.

@@ -598,13 +598,15 @@ fx_status fx_i8_device_status(int device) {
         }
         cudaGetDevice(&cur);
         if (cudaError_t e = cudaSetDevice(device); e != cudaSuccess) return done(fn, e);
-        uint32_t stream = 0;
+        uint32_t stream = 0, pair = 0;
         cudaError_t e = cudaDeviceSynchronize();
         if (e == cudaSuccess) e = fxk::i8_stream_status(&stream);
+        if (e == cudaSuccess) e = fxk::i8_pair_status(&pair);
         cudaSetDevice(cur);
         if (e != cudaSuccess) return done(fn, e);
-        if (stream)
-            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " + std::to_string(stream));
+        if (stream || pair)
+            return fxh::abi_error(FX_INTERNAL, std::string(fn) + ": a bounded wait gave up, code " +
+                                                   std::to_string(stream ? stream : pair));
         return FX_OK;
     });
 }
