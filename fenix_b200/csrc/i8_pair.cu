@@ -242,11 +242,13 @@ cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     Plan p{};
     p.tiles_m = (a.rows + kRows - 1) / kRows;
-    // outputs of a tile: the number whose turns over the pairs cost least
+    // Outputs of a tile: the number whose turns over the pairs cost least. A step of 32 inputs moves 256 + n lines of 32 bytes
+    // through an SM's shared memory, in and out, which takes as long as the products of 256 outputs and longer than those of
+    // fewer.
     const int pairs = sm_count() / 2;
     int64_t least = INT64_MAX;
     for (int n = kMaxOutputs; n >= 128; n -= 32) {
-        const int64_t tiles = static_cast<int64_t>(p.tiles_m) * ((a.n + n - 1) / n), cost = (tiles + pairs - 1) / pairs * n;
+        const int64_t tiles = static_cast<int64_t>(p.tiles_m) * ((a.n + n - 1) / n), cost = (tiles + pairs - 1) / pairs * (kRows + n);
         if (cost < least) least = cost, p.tile_n = n;
     }
     p.tiles_n = (a.n + p.tile_n - 1) / p.tile_n;

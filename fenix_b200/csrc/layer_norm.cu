@@ -2,7 +2,8 @@
 //
 // Bound by memory, as the RMS norm: x, residual, sum and y pass once, a row stays in the registers of its team of threads
 // between the looks at it (its mean, its squares about it, its largest magnitude where it gets a scale, its output), blocks
-// stay and walk over many rows with the next row on its way.
+// stay and walk over many rows with the next row on its way. What a value then costs are instructions: pairs of values share
+// one (add, multiply, multiply-add of two f32).
 // The variance is the mean square about the mean, not a difference of two sums, so that rows far from zero keep theirs:
 // t = h - mean is exact or rounded once, and the sum of the t, taken with that of their squares, gives what the mean
 // itself was off by.
@@ -14,6 +15,8 @@
 namespace fxk {
 namespace {
 
+constexpr float kSmaller = 8.2718061e-25f;  // 2^-80
+
 struct Red {  // of a block that is one team: a row's sums, one of each look
     float2 pair[2][32];
     float sum[2][32];
@@ -21,103 +24,135 @@ struct Red {  // of a block that is one team: a row's sums, one of each look
 };
 
 // From a row's h on; cols 0: no row, nothing is stored. red: no thread of the team still reads it.
-template <int TEAM, int TURNS, bool VEC>
+// TYPE: of x, residual, weight and bias alike, or -1: any.
+template <int TEAM, int TURNS, bool VEC, int TYPE>
 __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, int me, int cols, float (&h)[TURNS][kVec],
                                            Red& red) {
-    const float n = static_cast<float>(a.cols);
-    float mean, off, var, pre = 1.f;
-    bool past;
-    auto look = [&](int turn) {
-        float s = 0.f;
+    const float inv_n = 1.f / static_cast<float>(a.cols);
+    auto inside = [&](int u, int j) { return column<TEAM, VEC>(u, j, me) < a.cols; };  // with VEC of all eight alike
+    auto scaled = [&](float by) {
 #pragma unroll
         for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) s += h[u][j];  // columns past the row are 0
-        s = team_sum<TEAM>(s, red.sum[turn]);
-        mean = s / n;
-        float2 q = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int u = 0; u < TURNS; ++u)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const float t = column<TEAM, VEC>(u, VEC ? 0 : j, me) < a.cols ? h[u][j] - mean : 0.f;
-                q.x += t;
-                q.y = fmaf(t, t, q.y);
-            }
-        q = team_sum2<TEAM>(q, red.pair[turn]);
-        off = q.x / n;
-        var = fmaxf(q.y / n - off * off, 0.f);  // a NaN is found in past
-        past = !(fabsf(s) < 3.0e38f && q.y + a.eps < 3.0e38f);
-        if (q.y != q.y) var = q.y;
+            for (int j = 0; j < kVec; ++j) h[u][j] *= by;
     };
-    look(0);
-    // sums past f32's range, or a NaN or infinity, which stays one: sum smaller ones
-    if (TEAM < 32 ? __any_sync(0xffffffffu, past) : past) {
-        if (past) pre = 8.2718061e-25f;  // 2^-80
+    auto total = [&](float* to) {
+        float2 s = make_float2(0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) h[u][j] *= pre;
-        look(1);
+            for (int i = 0; i < kVec / 2; ++i) s = add2(s, pair_of(h[u], i));  // columns past the row are 0
+        return team_sum1<TEAM>(s.x + s.y, to);
+    };
+    float pre = 1.f;
+    float s = total(red.sum[0]);
+    // a sum past f32's range, or a NaN or infinity, which stays one: sum smaller values
+    const bool past = !(fabsf(s) < 3.0e38f);
+    if (TEAM < 32 ? __any_sync(0xffffffffu, past) : past) {
+        if (past) pre = kSmaller;
+        scaled(pre);
+        s = total(red.sum[1]);
     }
-    // (2^-160 eps may be nothing: a row of one large value is then zeros and not 0 / 0)
-    float v = var + a.eps * pre * pre;
-    if (v < 1.1754944e-38f && pre != 1.f) v = 1.1754944e-38f;
-    const float r = rsqrtf(v);
+    float mean = s * inv_n;  // what this and the sum are off by, off has
+    // t = h - mean in h's place; their sum and that of their squares
+    auto squares = [&](float less, float2* to) {
+        float2 e = make_float2(0.f, 0.f), q = e;
+        const float2 m = make_float2(-less, -less);
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            if (VEC && !inside(u, 0)) continue;
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) {
+                float2 t = add2(pair_of(h[u], i), m);
+                if (!VEC) t = make_float2(inside(u, 2 * i) ? t.x : 0.f, inside(u, 2 * i + 1) ? t.y : 0.f);
+                put_pair(h[u], i, t);
+                e = add2(e, t);
+                q = fma2(t, t, q);
+            }
+        }
+        return team_sum2<TEAM>(make_float2(e.x + e.y, q.x + q.y), to);
+    };
+    float2 q = squares(mean, red.pair[0]);
+    const bool wide = !(q.y + a.eps < 3.0e38f) && pre == 1.f;  // squares past f32's range
+    if (TEAM < 32 ? __any_sync(0xffffffffu, wide) : wide) {
+        const float by = wide ? kSmaller : 1.f;
+        pre *= by;
+        mean *= by;
+        scaled(by);
+        q = squares(0.f, red.pair[1]);
+    }
+    const float off = q.x * inv_n;
+    float var = fmaxf(q.y * inv_n - off * off, 0.f) + a.eps * pre * pre;
+    // 2^-160 eps may be nothing: a row of one large value is then zeros and not 0 / 0
+    if (var < 1.1754944e-38f && pre != 1.f) var = 1.1754944e-38f;
+    if (q.y != q.y) var = q.y;
+    const float r = rsqrtf(var);
     if (me == 0 && cols) {
         if (a.mean) a.mean[row] = (mean + off) / pre;
         if (a.rstd) a.rstd[row] = r * pre;
     }
+    const float2 r2 = make_float2(r, r), off2 = make_float2(-off * r, -off * r);
+    const bool by_row = a.scale_mode == kScaleRow;
     float top = 0.f;
 #pragma unroll
     for (int u = 0; u < TURNS; ++u) {
+        if (VEC && !inside(u, 0)) continue;
+        float w[kVec], b[kVec];
+        if (a.weight) load8<TEAM, VEC, true>(a.weight, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, w);
+        if (a.bias) load8<TEAM, VEC, true>(a.bias, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, b);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) h[u][j] = ((h[u][j] - mean) - off) * r;
-        if (a.weight) {
-            float w[kVec];
-            load8<TEAM, VEC, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) h[u][j] *= w[j];
+        for (int i = 0; i < kVec / 2; ++i) {
+            float2 v = fma2(pair_of(h[u], i), r2, off2);
+            if (a.weight && a.bias)
+                v = fma2(v, pair_of(w, i), pair_of(b, i));
+            else if (a.weight)
+                v = mul2(v, pair_of(w, i));
+            else if (a.bias)
+                v = add2(v, pair_of(b, i));
+            put_pair(h[u], i, v);
         }
-        if (a.bias) {
-            float b[kVec];
-            load8<TEAM, VEC, true>(a.bias, 0, a.weight_type, u, me, a.cols, b);
+        if (by_row) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) h[u][j] += b[j];
+            for (int i = 0; i < kVec / 2; ++i) {
+                const float2 v = pair_of(h[u], i);
+                top = max_abs(top, VEC ? v : make_float2(inside(u, 2 * i) ? v.x : 0.f, inside(u, 2 * i + 1) ? v.y : 0.f));
+            }
         }
-#pragma unroll
-        for (int j = 0; j < kVec; ++j)
-            if (column<TEAM, VEC>(u, VEC ? 0 : j, me) < a.cols) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(h[u][j])));
     }
+    float scale = 1.f, times = 1.f;
     if (a.scale_mode != kScaleNone) {
-        float scale;
-        if (a.scale_mode == kScaleRow) {
+        if (by_row) {
             // as bits a NaN is above every number
-            const uint32_t most = team_max<TEAM>(__float_as_uint(top) & 0x7fffffffu, red.top);
-            scale = __uint_as_float(max(most, __float_as_uint(1e-30f))) * (a.y_type == kTokI8 ? 1.f / 127.f : 1.f / 448.f);
+            scale = __uint_as_float(max(team_max<TEAM>(__float_as_uint(top), red.top), __float_as_uint(1e-30f))) * (a.y_type == kTokI8 ? 1.f / 127.f : 1.f / 448.f);
             if (me == 0 && cols) a.scale[row] = scale;
         } else {
             scale = a.scale[0];
         }
-        const float times = 1.f / scale;
-        if (fabsf(times) < INFINITY) {
-#pragma unroll
-            for (int u = 0; u < TURNS; ++u)
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) h[u][j] *= times;
-        } else {  // a scale near zero
+        times = 1.f / scale;
+        if (!(fabsf(times) < INFINITY)) {  // a scale near zero
 #pragma unroll
             for (int u = 0; u < TURNS; ++u)
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) h[u][j] = __fdiv_rn(h[u][j], scale);
+            times = 1.f;
         }
     }
-    if (a.y_type == kTokI8) {
+    // (a row's own scale leaves no value above 127)
+    const bool plain = by_row && scale < INFINITY;
 #pragma unroll
-        for (int u = 0; u < TURNS; ++u) store8_i8<TEAM, VEC>(a.y, row * a.y_stride, u, me, cols, h[u]);
-    } else {
+    for (int u = 0; u < TURNS; ++u) {
+        if (a.scale_mode != kScaleNone) {
 #pragma unroll
-        for (int u = 0; u < TURNS; ++u) store8<TEAM, VEC>(a.y, row * a.y_stride, a.y_type, u, me, cols, h[u]);
+            for (int i = 0; i < kVec / 2; ++i) {
+                put_pair(h[u], i, mul2(pair_of(h[u], i), make_float2(times, times)));
+            }
+        }
+        if (a.y_type != kTokI8)
+            store8<TEAM, VEC>(a.y, row * a.y_stride, a.y_type, u, me, cols, h[u]);
+        else if (VEC && plain)
+            store8_i8_within<TEAM>(a.y, row * a.y_stride, u, me, cols, h[u]);
+        else
+            store8_i8<TEAM, VEC>(a.y, row * a.y_stride, u, me, cols, h[u]);
     }
 }
 
@@ -144,12 +179,12 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) layer_norm_kernel(con
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) store8<TEAM, VEC>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
     }
-    finish_row<TEAM, TURNS, VEC>(a, row, me, a.cols, h, red);
+    finish_row<TEAM, TURNS, VEC, -1>(a, row, me, a.cols, h, red);
 }
 
 // Many rows of 16-bit x (and residual): the blocks stay and walk over the rows, a row's values on their way while the row
 // before it is worked on, so that memory does not wait for the reductions.
-template <int TEAM, int TURNS, bool RES>
+template <int TEAM, int TURNS, bool RES, int TYPE>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_stream_kernel(const __grid_constant__ LayerNormArgs a) {
     __shared__ Red red[2];
     const int me = threadIdx.x % TEAM, per = TEAM <= 32 ? 128 / TEAM : 1;
@@ -172,12 +207,12 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_stream_ker
         float h[TURNS][kVec];
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
-            unpack8(x[u], a.x_type, h[u]);
+            unpack8(x[u], TYPE < 0 ? a.x_type : TYPE, h[u]);
             if (RES) {
                 float f[kVec];
-                unpack8(r[u], a.residual_type, f);
+                unpack8(r[u], TYPE < 0 ? a.residual_type : TYPE, f);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) h[u][j] += f[j];
+                for (int i = 0; i < kVec / 2; ++i) put_pair(h[u], i, add2(pair_of(h[u], i), pair_of(f, i)));
             }
             if (row >= a.rows || column<TEAM, true>(u, 0, me) >= a.cols) {
 #pragma unroll
@@ -190,7 +225,59 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_stream_ker
 #pragma unroll
             for (int u = 0; u < TURNS; ++u) store8<TEAM, true>(a.sum, row * a.sum_stride, a.residual_type, u, me, cols, h[u]);
         }
-        finish_row<TEAM, TURNS, true>(a, row, me, cols, h, red[turn]);  // a row's barriers lie between two uses of a half of red
+        finish_row<TEAM, TURNS, true, TYPE>(a, row, me, cols, h, red[turn]);  // a row's barriers lie between two uses of a half of red
+    }
+}
+
+// The same with the next rows' values on their way to shared memory: rows so long that a block's registers would hold the
+// values on their way of no second block (8192 x 8192 bf16 with residual 97 us, 110 with them in registers; but 16384 x 4096 91
+// for 85, 16384 x 1024 31 for 27: a copy and a read more a value).
+constexpr int kAhead = 3;  // rows in shared memory
+template <int TEAM, int TURNS, bool RES>
+constexpr int kRingBytes = kAhead * (RES ? 2 : 1) * TURNS * TEAM * 16;
+
+template <int TEAM, int TURNS, bool RES, int TYPE>
+__global__ void __launch_bounds__(TEAM) layer_norm_ring_kernel(const __grid_constant__ LayerNormArgs a) {
+    __shared__ Red red[2];
+    extern __shared__ __align__(16) uint4 ring[];  // [row][x, residual][turn][thread]
+    const int me = threadIdx.x;
+    const int64_t step = gridDim.x;
+    auto slot = [&](int at, int which, int u) { return ring + ((at * (RES ? 2 : 1) + which) * TURNS + u) * TEAM + me; };
+    auto fetch = [&](int64_t row, int at) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            const int c = column<TEAM, true>(u, 0, me);
+            if (row >= a.rows || c >= a.cols) continue;
+            copy16(slot(at, 0, u), static_cast<const uint16_t*>(a.x) + row * a.x_stride + c);
+            if (RES) copy16(slot(at, 1, u), static_cast<const uint16_t*>(a.residual) + row * a.residual_stride + c);
+        }
+        copies_end_row();
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead - 1; ++i) fetch(blockIdx.x + i * step, i);
+    int64_t row = blockIdx.x;
+    for (int turn = 0, at = 0; row < a.rows; row += step, turn ^= 1) {
+        fetch(row + (kAhead - 1) * step, at == 0 ? kAhead - 1 : at - 1);
+        copies_wait<kAhead - 1>();
+        float h[TURNS][kVec];
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            if (column<TEAM, true>(u, 0, me) >= a.cols) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) h[u][j] = 0.f;
+                continue;
+            }
+            unpack8(*slot(at, 0, u), TYPE < 0 ? a.x_type : TYPE, h[u]);
+            if (RES) {
+                float f[kVec];
+                unpack8(*slot(at, 1, u), TYPE < 0 ? a.residual_type : TYPE, f);
+#pragma unroll
+                for (int i = 0; i < kVec / 2; ++i) put_pair(h[u], i, add2(pair_of(h[u], i), pair_of(f, i)));
+            }
+            if (a.sum) store8<TEAM, true>(a.sum, row * a.sum_stride, a.residual_type, u, me, a.cols, h[u]);
+        }
+        if (++at == kAhead) at = 0;
+        finish_row<TEAM, TURNS, true, TYPE>(a, row, me, a.cols, h, red[turn]);  // a row's barriers lie between two uses of a half of red
     }
 }
 
@@ -206,21 +293,37 @@ cudaError_t launch(const LayerNormArgs& a, bool vec, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-template <int TEAM, int TURNS, bool RES>
+template <int TEAM, int TURNS, bool RES, int TYPE>
 cudaError_t launch_stream(const LayerNormArgs& a, cudaStream_t s) {
-    auto* kern = layer_norm_stream_kernel<TEAM, TURNS, RES>;
-    constexpr int threads = TEAM <= 32 ? 128 : TEAM, per = threads / TEAM;
+    constexpr bool kRing = TEAM >= 512;
+    constexpr int threads = TEAM <= 32 ? 128 : TEAM, per = threads / TEAM, bytes = kRing ? kRingBytes<TEAM, TURNS, RES> : 0;
+    void (*kern)(LayerNormArgs);
+    if constexpr (kRing)
+        kern = layer_norm_ring_kernel<TEAM, TURNS, RES, TYPE>;
+    else
+        kern = layer_norm_stream_kernel<TEAM, TURNS, RES, TYPE>;
     static std::atomic<int> known;  // blocks that are resident at once on an SM; the same on every sm_100
+    if (bytes) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+    }
     int resident = known.load(std::memory_order_relaxed);
     if (!resident) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, 0);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, bytes);
         if (e != cudaSuccess) return e;
         known.store(resident, std::memory_order_relaxed);
     }
     const int64_t need = (static_cast<int64_t>(a.rows) + per - 1) / per, fit = static_cast<int64_t>(sm_count()) * resident;
     count_launch();
-    kern<<<static_cast<unsigned>(need < fit ? need : fit), threads, 0, s>>>(a);
+    kern<<<static_cast<unsigned>(need < fit ? need : fit), threads, bytes, s>>>(a);
     return cudaGetLastError();
+}
+template <int TEAM, int TURNS, bool RES>
+cudaError_t launch_stream(const LayerNormArgs& a, cudaStream_t s) {
+    const int t = a.x_type;
+    const bool one = (!a.residual || a.residual_type == t) && ((!a.weight && !a.bias) || a.weight_type == t);
+    if (!one) return launch_stream<TEAM, TURNS, RES, -1>(a, s);
+    return t == kTokF16 ? launch_stream<TEAM, TURNS, RES, kTokF16>(a, s) : launch_stream<TEAM, TURNS, RES, kTokBF16>(a, s);
 }
 template <int TEAM, int TURNS>
 cudaError_t launch_stream(const LayerNormArgs& a, cudaStream_t s) {

@@ -18,13 +18,59 @@ namespace fxk {
 namespace {
 
 constexpr int kFusedCols = 8192;
+constexpr int kJoinedCols = 512;       // of rows that share a block
+constexpr int kPlainSmem = 40 * 1024;  // dynamic shared memory that needs no asking for, beside a kernel's own
+
+// A block's sums over its rows leave as its line of the workspace.
+template <int TEAM, int TURNS, bool VEC>
+__device__ __forceinline__ void leave_sums(const LayerNormBackwardArgs& a, int me, float (&dw)[TURNS][kVec], float (&db)[TURNS][kVec]) {
+    constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
+    extern __shared__ __align__(16) uint4 dynamic[];
+    float* const joined = reinterpret_cast<float*>(dynamic);  // [2][cols]: the sums of a block of several teams
+    if (!a.work) return;
+    float* const mine = a.work + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+    if constexpr (kPer == 1) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            store8<TEAM, VEC>(mine, 0, kTokF32, u, me, a.cols, dw[u]);
+            store8<TEAM, VEC>(mine, a.cols, kTokF32, u, me, a.cols, db[u]);
+        }
+    } else {
+        // the teams of a warp by shuffles, then warp after warp
+        __syncthreads();  // over the ring, which no team reads any more
+#pragma unroll
+        for (int o = TEAM; o < 32; o <<= 1)
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    dw[u][j] += __shfl_xor_sync(0xffffffffu, dw[u][j], o);
+                    db[u][j] += __shfl_xor_sync(0xffffffffu, db[u][j], o);
+                }
+        for (int w = 0; w < kThreads / 32; ++w) {
+            if (threadIdx.x / 32 == w && threadIdx.x % 32 < TEAM) {
+#pragma unroll
+                for (int u = 0; u < TURNS; ++u)
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j) {
+                        const int c = column<TEAM, VEC>(u, VEC ? 0 : j, me) + (VEC ? j : 0);
+                        if (c < a.cols) {
+                            joined[c] = w ? joined[c] + dw[u][j] : dw[u][j];
+                            joined[a.cols + c] = w ? joined[a.cols + c] + db[u][j] : db[u][j];
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < 2 * a.cols; c += kThreads) mine[c] = joined[c];
+    }
+}
 
 // TEAM threads a row, TURNS times eight columns each.
 template <int TEAM, int TURNS, bool VEC>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
     constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
     __shared__ float2 red[2][32];
-    extern __shared__ float joined[];  // [2][cols]: the sums of a block of several teams
     const int me = threadIdx.x % TEAM;
     const float inv_n = 1.f / static_cast<float>(a.cols);
     float dw[TURNS][kVec] = {}, db[TURNS][kVec] = {};
@@ -71,42 +117,88 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_k
             store8<TEAM, VEC>(a.dx, row * a.dx_stride, a.dx_type, u, me, cols, g[u]);
         }
     }
-    if (!a.work) return;
-    float* const mine = a.work + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
-    if constexpr (kPer == 1) {
+    leave_sums<TEAM, TURNS, VEC>(a, me, dw, db);
+}
+
+// Many rows of 16-bit values: the next rows' dy, h and dsum are on their way to shared memory while a row is worked on. Pairs of
+// values share an instruction. TYPE: of dy, h, weight and dx alike, or -1: any.
+constexpr int kAhead = 3;  // rows of a team in shared memory
+template <int TEAM, int TURNS>
+constexpr int kRingBytes = kAhead * 3 * TURNS * (TEAM <= 32 ? 128 : TEAM) * 16;
+
+template <int TEAM, int TURNS, int TYPE>
+__global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_stream_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
+    __shared__ float2 red[2][32];
+    extern __shared__ __align__(16) uint4 dynamic[];
+    uint4* const ring = dynamic;  // [row][dy, h, dsum][turn][thread]
+    const int me = threadIdx.x % TEAM;
+    const float inv_n = 1.f / static_cast<float>(a.cols);
+    float dw[TURNS][kVec] = {}, db[TURNS][kVec] = {};
+    auto slot = [&](int at, int which, int u) { return ring + ((at * 3 + which) * TURNS + u) * kThreads + threadIdx.x; };
+    auto fetch = [&](int64_t row, int at) {
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
-            store8<TEAM, VEC>(mine, 0, kTokF32, u, me, a.cols, dw[u]);
-            store8<TEAM, VEC>(mine, a.cols, kTokF32, u, me, a.cols, db[u]);
+            const int c = column<TEAM, true>(u, 0, me);
+            if (row >= a.rows || c >= a.cols) continue;
+            copy16(slot(at, 0, u), static_cast<const uint16_t*>(a.dy) + row * a.dy_stride + c);
+            copy16(slot(at, 1, u), static_cast<const uint16_t*>(a.h) + row * a.h_stride + c);
+            if (a.dsum) copy16(slot(at, 2, u), static_cast<const uint16_t*>(a.dsum) + row * a.dsum_stride + c);
         }
-    } else {
-        // the teams of a warp by shuffles, then warp after warp
+        copies_end_row();
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kPer, mine = threadIdx.x / TEAM;
+    int64_t lead = static_cast<int64_t>(blockIdx.x) * kPer;
+    float mean = 0.f, rstd = 0.f;
+    if (lead + mine < a.rows) mean = a.mean[lead + mine], rstd = a.rstd[lead + mine];
 #pragma unroll
-        for (int o = TEAM; o < 32; o <<= 1)
+    for (int i = 0; i < kAhead - 1; ++i) fetch(lead + i * step + mine, i);
+    for (int turn = 0, at = 0; lead < a.rows; lead += step, turn ^= 1) {
+        const int64_t row = lead + mine;
+        const int cols = row < a.rows ? a.cols : 0;  // lanes of no row run along: the sums are the warp's
+        fetch(row + (kAhead - 1) * step, at == 0 ? kAhead - 1 : at - 1);
+        copies_wait<kAhead - 1>();
+        float g[TURNS][kVec], z[TURNS][kVec];
+        const float2 m2 = make_float2(-mean, -mean), r2 = make_float2(rstd, rstd);
+        if (row + step < a.rows) mean = a.mean[row + step], rstd = a.rstd[row + step];
+        float2 s1 = make_float2(0.f, 0.f), s2 = s1;
 #pragma unroll
-            for (int u = 0; u < TURNS; ++u)
+        for (int u = 0; u < TURNS; ++u) {
+            if (column<TEAM, true>(u, 0, me) >= cols) continue;
+            float w[kVec];
+            unpack8(*slot(at, 0, u), TYPE < 0 ? a.dy_type : TYPE, g[u]);
+            unpack8(*slot(at, 1, u), TYPE < 0 ? a.h_type : TYPE, z[u]);
+            if (a.weight) load8<TEAM, true, true>(a.weight, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, w);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    dw[u][j] += __shfl_xor_sync(0xffffffffu, dw[u][j], o);
-                    db[u][j] += __shfl_xor_sync(0xffffffffu, db[u][j], o);
-                }
-        for (int w = 0; w < kThreads / 32; ++w) {
-            if (threadIdx.x / 32 == w && threadIdx.x % 32 < TEAM) {
-#pragma unroll
-                for (int u = 0; u < TURNS; ++u)
-#pragma unroll
-                    for (int j = 0; j < kVec; ++j) {
-                        const int c = column<TEAM, VEC>(u, VEC ? 0 : j, me) + (VEC ? j : 0);
-                        if (c < a.cols) {
-                            joined[c] = w ? joined[c] + dw[u][j] : dw[u][j];
-                            joined[a.cols + c] = w ? joined[a.cols + c] + db[u][j] : db[u][j];
-                        }
-                    }
+            for (int i = 0; i < kVec / 2; ++i) {
+                float2 gi = pair_of(g[u], i);
+                const float2 zi = mul2(add2(pair_of(z[u], i), m2), r2);
+                put_pair(dw[u], i, fma2(gi, zi, pair_of(dw[u], i)));
+                put_pair(db[u], i, add2(pair_of(db[u], i), gi));
+                if (a.weight) gi = mul2(gi, pair_of(w, i));
+                s1 = add2(s1, gi);
+                s2 = fma2(gi, zi, s2);
+                put_pair(g[u], i, gi);
+                put_pair(z[u], i, zi);
             }
-            __syncthreads();
         }
-        for (int c = threadIdx.x; c < 2 * a.cols; c += kThreads) mine[c] = joined[c];
+        const float2 sums = team_sum2<TEAM>(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn]);
+        const float2 a1 = make_float2(-sums.x * inv_n, -sums.x * inv_n), a2 = make_float2(-sums.y * inv_n, -sums.y * inv_n);
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            if (column<TEAM, true>(u, 0, me) >= cols) continue;
+            float add[kVec];
+            if (a.dsum) unpack8(*slot(at, 2, u), TYPE < 0 ? a.dx_type : TYPE, add);
+#pragma unroll
+            for (int i = 0; i < kVec / 2; ++i) {
+                const float2 v = add2(pair_of(g[u], i), fma2(pair_of(z[u], i), a2, a1));
+                put_pair(g[u], i, a.dsum ? fma2(v, r2, pair_of(add, i)) : mul2(v, r2));
+            }
+            store8<TEAM, true>(a.dx, row * a.dx_stride, TYPE < 0 ? a.dx_type : TYPE, u, me, cols, g[u]);
+        }
+        if (++at == kAhead) at = 0;
     }
+    leave_sums<TEAM, TURNS, true>(a, me, dw, db);
 }
 
 // A block a row, of any length: its values are read twice.
@@ -178,27 +270,41 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __res
     if (out) out[o] = accumulate ? out[o] + s : s;
 }
 
-template <int TEAM, int TURNS, bool VEC>
-cudaError_t launch(const LayerNormBackwardArgs& a, int& lines, cudaStream_t s) {
-    auto* kern = layer_norm_backward_kernel<TEAM, TURNS, VEC>;
+template <int TEAM, class Kernel>
+cudaError_t launch(const LayerNormBackwardArgs& a, Kernel* kern, int ring, std::atomic<int>& known, int& lines, cudaStream_t s) {
     constexpr int threads = TEAM <= 32 ? 128 : TEAM, per = threads / TEAM;
-    const size_t joined = per > 1 ? size_t{8} * a.cols : 0;  // at most 8 KB
-    static std::atomic<int> known;
+    const int bytes = std::max(per > 1 ? 8 * kJoinedCols : 0, ring);
+    if (bytes > kPlainSmem) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+    }
     int resident = known.load(std::memory_order_relaxed);
     if (!resident) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, per > 1 ? 8192 : 0);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kern, threads, bytes);
         if (e != cudaSuccess) return e;
         known.store(resident, std::memory_order_relaxed);
     }
     const int64_t need = (static_cast<int64_t>(a.rows) + per - 1) / per, fit = static_cast<int64_t>(sm_count()) * resident;
     lines = static_cast<int>(std::min({need, fit, layer_norm_backward_blocks(a.rows, a.cols)}));
     count_launch();
-    kern<<<static_cast<unsigned>(lines), threads, joined, s>>>(a);
+    kern<<<static_cast<unsigned>(lines), threads, bytes, s>>>(a);
     return cudaGetLastError();
 }
 template <int TEAM, int TURNS>
 cudaError_t launch(const LayerNormBackwardArgs& a, bool vec, int& lines, cudaStream_t s) {
-    return vec ? launch<TEAM, TURNS, true>(a, lines, s) : launch<TEAM, TURNS, false>(a, lines, s);
+    static std::atomic<int> known[2];  // blocks that are resident at once on an SM; the same on every sm_100
+    return vec ? launch<TEAM>(a, layer_norm_backward_kernel<TEAM, TURNS, true>, 0, known[1], lines, s)
+               : launch<TEAM>(a, layer_norm_backward_kernel<TEAM, TURNS, false>, 0, known[0], lines, s);
+}
+template <int TEAM, int TURNS>
+cudaError_t launch_stream(const LayerNormBackwardArgs& a, int& lines, cudaStream_t s) {
+    static std::atomic<int> known[3];
+    constexpr int ring = kRingBytes<TEAM, TURNS>;
+    const int t = a.dy_type;
+    if (a.h_type != t || a.dx_type != t || (a.weight && a.weight_type != t))
+        return launch<TEAM>(a, layer_norm_backward_stream_kernel<TEAM, TURNS, -1>, ring, known[0], lines, s);
+    return t == kTokF16 ? launch<TEAM>(a, layer_norm_backward_stream_kernel<TEAM, TURNS, kTokF16>, ring, known[1], lines, s)
+                        : launch<TEAM>(a, layer_norm_backward_stream_kernel<TEAM, TURNS, kTokBF16>, ring, known[2], lines, s);
 }
 
 }  // namespace
@@ -232,7 +338,19 @@ cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStrea
         const bool vec = a.cols % kVec == 0 && rows_of_eights(a.dy, a.dy_stride, a.dy_type) &&
                          rows_of_eights(a.h, a.h_stride, a.h_type) && rows_of_eights(a.weight, 0, a.weight_type) &&
                          rows_of_eights(a.dsum, a.dsum_stride, a.dx_type) && rows_of_eights(a.dx, a.dx_stride, a.dx_type);
-        if (a.cols <= 64)
+        const bool stream = vec && a.dy_type != kTokF32 && a.h_type != kTokF32 && (!a.dsum || a.dx_type != kTokF32);
+        if (stream)
+            e = a.cols <= 64     ? launch_stream<8, 1>(a, lines, s)
+                : a.cols <= 128  ? launch_stream<16, 1>(a, lines, s)
+                : a.cols <= 256  ? launch_stream<32, 1>(a, lines, s)
+                : a.cols <= 512  ? launch_stream<32, 2>(a, lines, s)
+                : a.cols <= 1024 ? launch_stream<128, 1>(a, lines, s)
+                : a.cols <= 2048 ? launch_stream<128, 2>(a, lines, s)
+                : a.cols <= 4096 ? launch_stream<256, 2>(a, lines, s)
+                : a.cols <= 5120 ? launch_stream<320, 2>(a, lines, s)
+                : a.cols <= 6144 ? launch_stream<384, 2>(a, lines, s)
+                                 : launch_stream<512, 2>(a, lines, s);
+        else if (a.cols <= 64)
             e = launch<8, 1>(a, vec, lines, s);
         else if (a.cols <= 256)
             e = launch<32, 1>(a, vec, lines, s);

@@ -159,27 +159,83 @@ __device__ __forceinline__ uint32_t team_max(uint32_t v, uint32_t* red) {
     return v;
 }
 
-// Two sums at once.
+// Rows on their way to shared memory, a thread's own 16 bytes a turn (eight 16-bit values), several rows ahead: no registers are
+// held for them and no thread waits for another's. slot: a thread's 16 bytes of one row and tensor.
+__device__ __forceinline__ void copy16(uint4* slot, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot))), "l"(from)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_end_row() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>  // waits for this thread's copies of all rows but the last LATER
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory");
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 pair_of(const float* f, int i) { return make_float2(f[2 * i], f[2 * i + 1]); }
+__device__ __forceinline__ void put_pair(float* f, int i, const float2& v) {
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+}
+__device__ __forceinline__ uint64_t bits_of(const float2& v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair_of(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ float2 add2(const float2& a, const float2& b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 mul2(const float2& a, const float2& b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ float2 fma2(const float2& a, const float2& b, const float2& c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+    return pair_of(r);
+}
+
+// Two sums at once. The warps' sums are read by every thread and added in their order, which takes fewer turns than shuffles.
 template <int TEAM>
 __device__ __forceinline__ float2 team_sum2(float2 v, float2* red) {
 #pragma unroll
-    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o; o >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-    }
+    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o; o >>= 1)
+        v = add2(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
     if constexpr (TEAM > 32) {
         if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
         __syncthreads();
-        v = threadIdx.x % 32 < TEAM / 32 ? red[threadIdx.x % 32] : make_float2(0.f, 0.f);
+        v = red[0];
 #pragma unroll
-        for (int o = TEAM > 512 ? 16 : TEAM > 256 ? 8 : TEAM / 64; o; o >>= 1) {
-            v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-            v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-        }
-        v.x = __shfl_sync(0xffffffffu, v.x, 0);
-        v.y = __shfl_sync(0xffffffffu, v.y, 0);
+        for (int w = 1; w < TEAM / 32; ++w) v = add2(v, red[w]);
     }
     return v;
+}
+// One, the same way.
+template <int TEAM>
+__device__ __forceinline__ float team_sum1(float v, float* red) {
+#pragma unroll
+    for (int o = (TEAM < 32 ? TEAM : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (TEAM > 32) {
+        if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int w = 1; w < TEAM / 32; ++w) v += red[w];
+    }
+    return v;
+}
+// The larger of top and both magnitudes; a NaN stays one.
+__device__ __forceinline__ float max_abs(float top, const float2& v) {
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(v.x), "f"(v.y));
+    return top;
 }
 
 // v rounded to nearest, ties to even, and saturated to +-127; a NaN is 0.
@@ -203,6 +259,25 @@ __device__ __forceinline__ void store8_i8(void* p, int64_t row, int u, int me, i
             if (c < cols) q[c] = static_cast<int8_t>(i8_code(f[j]));
         }
     }
+}
+
+// The same of numbers that round to no more than 127: 1.5 * 2^23 added, a code is the low byte of the sum.
+template <int TEAM>
+__device__ __forceinline__ void store8_i8_within(void* p, int64_t row, int u, int me, int cols, const float (&f)[kVec]) {
+    const int c = column<TEAM, true>(u, 0, me);
+    if (c >= cols) return;
+    uint32_t w[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) {
+        const float2 v = add2(pair_of(f, i), make_float2(12582912.f, 12582912.f));
+        w[2 * i] = __float_as_uint(v.x);
+        w[2 * i + 1] = __float_as_uint(v.y);
+    }
+    uint32_t out[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        out[i] = __byte_perm(__byte_perm(w[4 * i], w[4 * i + 1], 0x0040), __byte_perm(w[4 * i + 2], w[4 * i + 3], 0x0040), 0x5410);
+    *reinterpret_cast<uint2*>(static_cast<int8_t*>(p) + row + c) = make_uint2(out[0], out[1]);
 }
 
 // Rows that a team reads or writes eight values at a time: 16-byte aligned (8-byte of 8-bit types). A null is.

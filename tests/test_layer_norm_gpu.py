@@ -133,6 +133,10 @@ def test_norm_teams_that_walk(cuda_torch, cols, residual):
     rows = max(2400, 10_000_000 // cols) + 3
     run_norm(cuda_torch, rows, cols, "f16" if cols % 3 else "bf16", "e4m3", mode="row", residual=residual, keep_sum=residual, seed=cols)
     run_norm(cuda_torch, rows, cols, "bf16", "bf16", residual=residual, keep_sum=residual, seed=cols)
+    if not residual:  # h is x, and is stored all the same, in any type
+        for rt in ("f32", "f16", "bf16"):
+            run_norm(cuda_torch, rows, cols, "bf16", "i8", rt, "bf16", "row", residual=False, keep_sum=True, seed=cols)
+            run_norm(cuda_torch, rows, cols, "f16", "f32", rt, "f32", residual=False, keep_sum=True, bias=False, seed=cols)
 
 
 @pytest.mark.parametrize("xt,yt,rt", list(itertools.product(["f32", "f16", "bf16"], ["f32", "f16", "bf16", "e4m3", "i8"],
