@@ -31,10 +31,13 @@ static inline cudaError_t take_i8_status(uint32_t* code) {
     return e;
 }
 
-// A result from its exact sum: the same in every kernel, so that it does not depend on the way taken. Without a bias, bias
+// A result from its exact sum, rounded to f32: the same in every kernel, so that it does not depend on the way taken. Without a bias, bias
 // is -0, which changes nothing.
+__device__ __forceinline__ float i8_value(float sum, float x_scale, float scale, float bias) {
+    return __fadd_rn(__fmul_rn(__fmul_rn(sum, x_scale), scale), bias);
+}
 __device__ __forceinline__ float i8_value(int sum, float x_scale, float scale, float bias) {
-    return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(sum), x_scale), scale), bias);
+    return i8_value(__int2float_rn(sum), x_scale, scale, bias);
 }
 // Four results to consecutive outputs; vec: all four are there and aligned.
 __device__ __forceinline__ void i8_store4(void* y, int64_t at, int type, const float (&f)[4], bool vec, int there) {

@@ -17,17 +17,18 @@ namespace {
 
 constexpr int kRows = 256;       // of a tile; each SM of the pair has half
 constexpr int kMaxOutputs = 256;  // of a tile; each SM brings half of the weights
-constexpr int kThreads = 192;    // warps: 0 TMA, 1 TMEM and MMA, 2..5 epilogue
+constexpr int kThreads = 320;    // warps: 0 TMA, 1 TMEM and MMA, 2..9 epilogue
 constexpr int kGroup = 16;       // row tiles that are walked over before the next tile of outputs
-constexpr int kPitch = 36;       // words of a staged row of 32 sums
+constexpr int kPitch = 17;       // words of a staged row of 16 results
+constexpr int kScaleBytes = 2 * 2 * kMaxOutputs * 4, kStageBytes = 8 * 32 * kPitch * 4;
 
 struct Plan {
     int tile_n;  // outputs of a tile: a multiple of 32, at most 256
     int slots;
     int tiles_m, tiles_n;
-    int stage;  // offset of the epilogue's buffers in shared memory
+    int scales, stage;  // offsets of the epilogue's buffers in shared memory
     int bytes;
-    bool y_vec;  // results aligned to four outputs
+    int y_align;  // bytes that 16 results begin at a multiple of: 32, 16, or 0 for less
 };
 
 // Loads of both SMs count their bytes on the first SM's barrier, at `bar` of the cluster's shared memory.
@@ -37,18 +38,22 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
         "l"(map), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
-__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// Every lane of the issuing warp runs these, on warp-uniform operands, and the one with issue != 0 executes them.
+__device__ __forceinline__ void mma_i8_pair_if(uint32_t issue, uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
         : "memory");
 }
 // Arrives on the barrier at this offset in both SMs once the MMAs issued so far are done.
-__device__ __forceinline__ void commit_pair(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                 "h"(static_cast<uint16_t>(3))
-                 : "memory");
+__device__ __forceinline__ void commit_pair_if(uint32_t issue, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3)), "r"(issue)
+        : "memory");
 }
 __device__ __forceinline__ uint32_t of_first(uint32_t addr) {  // the same place in the first SM's shared memory
     uint32_t r;
@@ -57,6 +62,46 @@ __device__ __forceinline__ uint32_t of_first(uint32_t addr) {  // the same place
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// 32 bytes to one address of a multiple of 32 (or 16, wide false).
+__device__ __forceinline__ void st32(void* p, const uint32_t (&w)[8], bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
+// Sixteen results to consecutive outputs.
+__device__ __forceinline__ void store16(uint8_t* to, int type, const float (&f)[16], bool wide) {
+    uint32_t w[8];
+    if (type == kTokF32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[8 * h + i]);
+            st32(to + 32 * h, w, wide);
+        }
+        return;
+    }
+    if (type == kTokF16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = reinterpret_cast<const uint32_t&>(p);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = reinterpret_cast<const uint32_t&>(p);
+        }
+    }
+    st32(to, w, wide);
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -78,10 +123,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         set_status(&g_i8_status, code);
     };
     auto tile_at = [&](int64_t t, int& m, int& n) {
-        const int64_t per = static_cast<int64_t>(kGroup) * plan.tiles_n, g = t / per, in = t - g * per;
+        const int64_t per = static_cast<int64_t>(kGroup) * plan.tiles_n, g = tiles <= per ? 0 : t / per;
         const int tall = min(kGroup, plan.tiles_m - static_cast<int>(g) * kGroup);
-        n = static_cast<int>(in / tall);
-        m = static_cast<int>(g) * kGroup + static_cast<int>(in % tall);
+        const uint32_t in = static_cast<uint32_t>(t - g * per);  // below 16 * 2^23
+        n = static_cast<int>(in / static_cast<uint32_t>(tall));
+        m = static_cast<int>(g) * kGroup + static_cast<int>(in % static_cast<uint32_t>(tall));
     };
     if (threadIdx.x == 0) {
         for (int i = 0; i < kI8MaxSlots; ++i) {
@@ -90,10 +136,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + 8 * i, 1);
-            mbar_init(acc_empty + 8 * i, 8);  // the epilogue's warps of both SMs
+            mbar_init(acc_empty + 8 * i, 16);  // the epilogue's warps of both SMs
         }
         abort_flag = 0;
         fence_mbar_init();
+    }
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&w_map) : "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_at)) : "memory");
@@ -131,25 +181,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {
+        if (rank == 0) {
             const uint32_t idesc = instr_desc_i8(kRows, 0) | static_cast<uint32_t>(tile_n >> 3) << 17;
+            // All of TMEM is this block's, so its first column is 0, a constant that the issuing loop has at no cost; it keeps
+            // to warp-uniform values throughout (and leaves at no other place than its end): a step takes the MMAs 512 cycles, and
+            // one thread's own code took the loop 690 (4096 x 4096 -> 14336 165 us).
+            if (tmem != 0) gave_up(kStatusBadTmem);
+            const uint32_t issue = elect_one();
             int at = 0, acc = 0;
             uint32_t ph = 0, acc_ph = 0;
-            for (int64_t t = pair; t < tiles && !abort_flag; t += pairs) {
+            for (int64_t t = pair; t < tiles; t += pairs) {
                 if (!wait_phase(acc_empty + 8 * acc, acc_ph ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAccFree);
-                tc_fence_after();
-                const uint32_t d = tmem + acc * kMaxOutputs;
                 for (int step = 0; step < steps; ++step) {
                     if (!wait_phase(full + 8 * at, ph, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
-                    if (abort_flag) break;
                     tc_fence_after();
-                    const uint64_t ad = desc_sw128(base + at * slot_bytes), bd = desc_sw128(base + at * slot_bytes + kRows / 2 * kI8Step);
+                    const uint64_t ad = desc_sw128(base + at * slot_bytes), bd = ad + (kRows / 2 * kI8Step >> 4);
 #pragma unroll
-                    for (int i = 0; i < kI8Step / 32; ++i) mma_i8_pair(d, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
-                    commit_pair(empty + 8 * at);
+                    for (int i = 0; i < kI8Step / 32; ++i)
+                        mma_i8_pair_if(issue, acc * kMaxOutputs, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
+                    commit_pair_if(issue, empty + 8 * at);
                     if (++at == plan.slots) at = 0, ph ^= 1;
                 }
-                commit_pair(acc_full + 8 * acc);
+                commit_pair_if(issue, acc_full + 8 * acc);
                 if (++acc == 2) acc = 0, acc_ph ^= 1;
             }
             // the last MMAs end before the blocks do
@@ -157,63 +210,79 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else {
-        // 32 columns at a time: a thread reads its row's sums, which change places in shared memory, so that a store is four
-        // outputs (or one) of neighbours
-        const int quad = warp % 4;
-        int* const stage = reinterpret_cast<int*>(smem + plan.stage) + quad * 32 * kPitch;
+        // Two warps share a quarter's rows, by halves of the columns; a thread has a row. Scales and bias of the tile's outputs come
+        // to shared memory while the MMAs run. (No role leaves this loop early: its warps meet once a tile.)
+        const int quad = warp % 4, half = (warp - 2) / 4, width = tile_n / 2;
+        float* const scales = reinterpret_cast<float*>(smem + plan.scales);  // [tile % 2][scale, bias][output]
+        float* const stage = reinterpret_cast<float*>(smem + plan.stage) + (warp - 2) * 32 * kPitch;
         const uint32_t release = of_first(acc_empty);
+        const int size = a.y_type == kTokF32 ? 4 : 2, me = threadIdx.x - 64;
         int acc = 0;
         uint32_t ph = 0;
         for (int64_t t = pair; t < tiles; t += pairs) {
             int m, n;
             tile_at(t, m, n);
-            const int r0 = m * kRows + rank * (kRows / 2) + quad * 32;
-            const float xs = r0 + lane < a.rows ? a.x_scale[a.x_scale_mode == kScaleRow ? r0 + lane : 0] : 0.f;
-            const int rows = min(32, a.rows - r0);  // of this warp; none or fewer where the tile is ragged
+            const int64_t row = static_cast<int64_t>(m) * kRows + rank * (kRows / 2) + quad * 32 + lane;
+            const float xs = row < a.rows ? a.x_scale[a.x_scale_mode == kScaleRow ? row : 0] : 0.f;
+            float* const of_tile = scales + acc * 2 * kMaxOutputs;
+            if (me < tile_n) {
+                const int o = n * tile_n + me;
+                of_tile[me] = o < a.n ? a.scales[o] : 0.f;
+                of_tile[kMaxOutputs + me] = o < a.n && a.bias ? a.bias[o] : -0.f;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
             if (!wait_phase(acc_full + 8 * acc, ph, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAcc);
-            if (__any_sync(0xffffffffu, abort_flag)) break;
+            __syncwarp();
             tc_fence_after();
-            const uint32_t from = tmem + acc * kMaxOutputs + (static_cast<uint32_t>(quad * 32) << 16);
-            for (int c = 0; c < tile_n; c += 32) {
-                uint32_t v[2][16];
-                tmem_ld16_nowait(from + c, v[0]);
-                tmem_ld16_nowait(from + c + 16, v[1]);
+            const uint32_t from = tmem + acc * kMaxOutputs + half * width + (static_cast<uint32_t>(quad * 32) << 16);
+            uint32_t next[16];
+            tmem_ld16_nowait(from, next);
+            for (int c = 0; c < width; c += 16) {
                 tmem_wait();
-                tmem_regs_ready(v[0]);
-                tmem_regs_ready(v[1]);
-                __syncwarp();  // the columns before these have left the buffer
+                tmem_regs_ready(next);
+                float f[16];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    *reinterpret_cast<uint4*>(stage + lane * kPitch + 4 * i) =
-                        make_uint4(v[i / 4][4 * (i % 4)], v[i / 4][4 * (i % 4) + 1], v[i / 4][4 * (i % 4) + 2], v[i / 4][4 * (i % 4) + 3]);
+                for (int i = 0; i < 16; ++i) f[i] = __int2float_rn(static_cast<int>(next[i]));
+                if (c + 16 < width) tmem_ld16_nowait(from + c + 16, next);  // on its way during these columns' arithmetic
+                const float* const s_at = of_tile + half * width + c;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float4 sc = *reinterpret_cast<const float4*>(s_at + 4 * i);
+                    const float4 b = *reinterpret_cast<const float4*>(s_at + kMaxOutputs + 4 * i);
+                    f[4 * i] = i8_value(f[4 * i], xs, sc.x, b.x);
+                    f[4 * i + 1] = i8_value(f[4 * i + 1], xs, sc.y, b.y);
+                    f[4 * i + 2] = i8_value(f[4 * i + 2], xs, sc.z, b.z);
+                    f[4 * i + 3] = i8_value(f[4 * i + 3], xs, sc.w, b.w);
+                }
+                const int o0 = n * tile_n + half * width + c;
+                if (plan.y_align && o0 + 16 <= a.n) {
+                    if (row < a.rows) store16(static_cast<uint8_t*>(a.y) + (row * a.y_stride + o0) * size, a.y_type, f, plan.y_align == 32);
+                    continue;
+                }
+                // unaligned: results change places in shared memory, so that half a warp stores neighbours of a row
                 __syncwarp();
-                const int o0 = n * tile_n + c;
-                if (plan.y_vec && o0 + 32 <= a.n) {
-                    const int o = o0 + lane % 8 * 4;
-                    float sc[4], b[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[e] = __ldg(a.scales + o + e);
-                        b[e] = a.bias ? __ldg(a.bias + o + e) : -0.f;
-                    }
+                for (int i = 0; i < 16; ++i) stage[lane * kPitch + i] = f[i];
+                __syncwarp();
+                const int o = o0 + lane % 16, r = lane / 16;
+                const int64_t r0 = row - lane + r;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = i * 4 + lane / 8;
-                        const float x = __shfl_sync(0xffffffffu, xs, r);
-                        const int4 s = *reinterpret_cast<const int4*>(stage + r * kPitch + lane % 8 * 4);
-                        const float f[4] = {i8_value(s.x, x, sc[0], b[0]), i8_value(s.y, x, sc[1], b[1]),
-                                            i8_value(s.z, x, sc[2], b[2]), i8_value(s.w, x, sc[3], b[3])};
-                        if (r < rows) i8_store4(a.y, static_cast<int64_t>(r0 + r) * a.y_stride + o, a.y_type, f, true, 4);
-                    }
-                } else {
-                    const int o = o0 + lane;
-                    const float sc = o < a.n ? __ldg(a.scales + o) : 0.f, b = o < a.n && a.bias ? __ldg(a.bias + o) : -0.f;
-#pragma unroll 8
-                    for (int r = 0; r < 32; ++r) {
-                        const float x = __shfl_sync(0xffffffffu, xs, r);
-                        if (r < rows && o < a.n)
-                            tok_store(a.y, static_cast<int64_t>(r0 + r) * a.y_stride + o, a.y_type, i8_value(stage[r * kPitch + lane], x, sc, b));
-                    }
+                for (int i = 0; i < 16; ++i) f[i] = stage[(2 * i + r) * kPitch + lane % 16];
+                if (o < a.n) {
+                    const int there = static_cast<int>(min(static_cast<int64_t>(32), a.rows - r0));
+                    const int64_t at = r0 * a.y_stride + o;
+                    auto each = [&](auto* y, auto&& make) {
+                        y += at;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (2 * i < there) y[2 * i * a.y_stride] = make(f[i]);
+                    };
+                    if (a.y_type == kTokF32)
+                        each(static_cast<float*>(a.y), [](float v) { return v; });
+                    else if (a.y_type == kTokF16)
+                        each(static_cast<__half*>(a.y), [](float v) { return __float2half_rn(v); });
+                    else
+                        each(static_cast<__nv_bfloat16*>(a.y), [](float v) { return __float2bfloat16_rn(v); });
                 }
             }
             tc_fence_before();
@@ -225,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
     __syncthreads();
-    cluster_sync();  // neither SM's shared memory or TMEM ends while the other may still signal or read it
+    cluster_sync_relaxed();  // neither SM's shared memory or TMEM ends while the other may still signal or read it
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -252,12 +321,13 @@ cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
         if (cost < least) least = cost, p.tile_n = n;
     }
     p.tiles_n = (a.n + p.tile_n - 1) / p.tile_n;
-    const int slot = (kRows / 2 + p.tile_n / 2) * kI8Step, stage = 4 * 32 * kPitch * 4;
-    p.slots = std::min((kSmem - stage) / slot, kI8MaxSlots);
-    p.stage = p.slots * slot;
-    p.bytes = p.stage + stage;
-    const int64_t unit = a.y_type == kTokF32 ? 16 : 8;
-    p.y_vec = reinterpret_cast<uintptr_t>(a.y) % unit == 0 && a.y_stride % 4 == 0;
+    const int slot = (kRows / 2 + p.tile_n / 2) * kI8Step;
+    p.slots = std::min((kSmem - kScaleBytes - kStageBytes) / slot, kI8MaxSlots);
+    p.scales = p.slots * slot;
+    p.stage = p.scales + kScaleBytes;
+    p.bytes = p.stage + kStageBytes;
+    const uint64_t where = reinterpret_cast<uintptr_t>(a.y) | static_cast<uint64_t>(a.y_stride) * (a.y_type == kTokF32 ? 4 : 2);
+    p.y_align = where % 32 == 0 ? 32 : where % 16 == 0 ? 16 : 0;
     auto pitch = [](int64_t stride) { return (stride + 15) / 16 * 16; };  // of one row, which has none
     CUtensorMap x, w;
     e = tmap_rows(&x, a.x, 1, a.k, a.rows, pitch(a.x_stride), kRows / 2);

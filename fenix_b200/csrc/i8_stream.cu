@@ -96,23 +96,21 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = instr_desc_i8(kTileM, 0) | static_cast<uint32_t>(tile_n >> 3) << 17;
-            int at = 0;
-            uint32_t ph = 0;
-            for (int step = 0; step < steps; ++step) {
-                if (!wait_phase(full + 8 * at, ph, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
-                if (abort_flag) break;
-                tc_fence_after();
-                const uint64_t ad = desc_sw128(base + at * slot_bytes), bd = desc_sw128(base + at * slot_bytes + kTileM * kI8Step);
+        // the warp as one, on uniform values: issuing from one thread's own code takes longer than short steps' MMAs
+        const uint32_t idesc = instr_desc_i8(kTileM, 0) | static_cast<uint32_t>(tile_n >> 3) << 17, issue = elect_one();
+        int at = 0;
+        uint32_t ph = 0;
+        for (int step = 0; step < steps; ++step) {
+            if (!wait_phase(full + 8 * at, ph, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutFull);
+            tc_fence_after();
+            const uint64_t ad = desc_sw128(base + at * slot_bytes), bd = ad + (kTileM * kI8Step >> 4);
 #pragma unroll
-                for (int i = 0; i < kI8Step / 32; ++i) mma_i8(tmem, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
-                mma_commit(empty + 8 * at);
-                if (++at == plan.slots) at = 0, ph ^= 1;
-            }
-            mma_commit(done);
-            wait_phase(done, 0, nullptr, a.wait_ns);  // the epilogue may have given up: no MMA outlives its TMEM
+            for (int i = 0; i < kI8Step / 32; ++i) mma_i8_if(issue, tmem, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
+            mma_commit_if(issue, empty + 8 * at);
+            if (++at == plan.slots) at = 0, ph ^= 1;
         }
+        mma_commit_if(issue, done);
+        wait_phase(done, 0, nullptr, a.wait_ns);  // the epilogue may have given up: no MMA outlives its TMEM
         __syncwarp();
     } else {
         const int quad = warp % 4, row = quad * 32 + lane, out = o0 + row;
