@@ -1,6 +1,7 @@
 // i8_linear.cuh — what the kernels of the 8-bit linear layer share.
 #pragma once
 
+#include "pairs.cuh"
 #include "ptx.cuh"
 #include "token.cuh"
 
@@ -35,6 +36,10 @@ static inline cudaError_t take_i8_status(uint32_t* code) {
 // is -0, which changes nothing.
 __device__ __forceinline__ float i8_value(float sum, float x_scale, float scale, float bias) {
     return __fadd_rn(__fmul_rn(__fmul_rn(sum, x_scale), scale), bias);
+}
+__device__ __forceinline__ float2 i8_value(const float2& sum, float x_scale, const float2& scale, const float2& bias) {
+    const float2 v = mul2(mul2(sum, make_float2(x_scale, x_scale)), scale);
+    return make_float2(__fadd_rn(v.x, bias.x), __fadd_rn(v.y, bias.y));  // (a pair's sum may be fused with the product before it)
 }
 __device__ __forceinline__ float i8_value(int sum, float x_scale, float scale, float bias) {
     return i8_value(__int2float_rn(sum), x_scale, scale, bias);

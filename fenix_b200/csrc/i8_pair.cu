@@ -19,8 +19,9 @@ constexpr int kRows = 256;       // of a tile; each SM of the pair has half
 constexpr int kMaxOutputs = 256;  // of a tile; each SM brings half of the weights
 constexpr int kThreads = 320;    // warps: 0 TMA, 1 TMEM and MMA, 2..9 epilogue
 constexpr int kGroup = 16;       // row tiles that are walked over before the next tile of outputs
-constexpr int kPitch = 17;       // words of a staged row of 16 results
-constexpr int kScaleBytes = 2 * 2 * kMaxOutputs * 4, kStageBytes = 8 * 32 * kPitch * 4;
+constexpr int kLine = 256;       // bytes of results of a row that are staged where rows are not aligned
+constexpr int kPitch = kLine + 16;  // with room for a line to lie as its place in memory does to a multiple of 16
+constexpr int kScaleBytes = 2 * 2 * kMaxOutputs * 4, kStageBytes = 8 * 32 * kPitch;
 
 struct Plan {
     int tile_n;  // outputs of a tile: a multiple of 32, at most 256
@@ -76,6 +77,20 @@ __device__ __forceinline__ void st32(void* p, const uint32_t (&w)[8], bool wide)
     }
 }
 
+// Sixteen results one by one, the first `there` of them.
+__device__ __forceinline__ void put16(uint8_t* to, int type, const float (&f)[16], int there = 16) {
+    auto each = [&](auto* y, auto&& make) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < there) y[i] = make(f[i]);
+    };
+    if (type == kTokF32)
+        each(reinterpret_cast<float*>(to), [](float v) { return v; });
+    else if (type == kTokF16)
+        each(reinterpret_cast<__half*>(to), [](float v) { return __float2half_rn(v); });
+    else
+        each(reinterpret_cast<__nv_bfloat16*>(to), [](float v) { return __float2bfloat16_rn(v); });
+}
 // Sixteen results to consecutive outputs.
 __device__ __forceinline__ void store16(uint8_t* to, int type, const float (&f)[16], bool wide) {
     uint32_t w[8];
@@ -214,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // to shared memory while the MMAs run. (No role leaves this loop early: its warps meet once a tile.)
         const int quad = warp % 4, half = (warp - 2) / 4, width = tile_n / 2;
         float* const scales = reinterpret_cast<float*>(smem + plan.scales);  // [tile % 2][scale, bias][output]
-        float* const stage = reinterpret_cast<float*>(smem + plan.stage) + (warp - 2) * 32 * kPitch;
+        uint8_t* const stage = smem + plan.stage + (warp - 2) * 32 * kPitch;
         const uint32_t release = of_first(acc_empty);
         const int size = a.y_type == kTokF32 ? 4 : 2, me = threadIdx.x - 64;
         int acc = 0;
@@ -249,41 +264,59 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < 4; ++i) {
                     const float4 sc = *reinterpret_cast<const float4*>(s_at + 4 * i);
                     const float4 b = *reinterpret_cast<const float4*>(s_at + kMaxOutputs + 4 * i);
-                    f[4 * i] = i8_value(f[4 * i], xs, sc.x, b.x);
-                    f[4 * i + 1] = i8_value(f[4 * i + 1], xs, sc.y, b.y);
-                    f[4 * i + 2] = i8_value(f[4 * i + 2], xs, sc.z, b.z);
-                    f[4 * i + 3] = i8_value(f[4 * i + 3], xs, sc.w, b.w);
+                    put_pair(f, 2 * i, i8_value(pair_of(f, 2 * i), xs, make_float2(sc.x, sc.y), make_float2(b.x, b.y)));
+                    put_pair(f, 2 * i + 1, i8_value(pair_of(f, 2 * i + 1), xs, make_float2(sc.z, sc.w), make_float2(b.z, b.w)));
                 }
                 const int o0 = n * tile_n + half * width + c;
-                if (plan.y_align && o0 + 16 <= a.n) {
-                    if (row < a.rows) store16(static_cast<uint8_t*>(a.y) + (row * a.y_stride + o0) * size, a.y_type, f, plan.y_align == 32);
+                if (plan.y_align) {
+                    uint8_t* const to = static_cast<uint8_t*>(a.y) + (row * a.y_stride + o0) * size;
+                    if (row < a.rows && o0 + 16 <= a.n)
+                        store16(to, a.y_type, f, plan.y_align == 32);
+                    else if (row < a.rows)
+                        put16(to, a.y_type, f, a.n - o0);
                     continue;
                 }
-                // unaligned: results change places in shared memory, so that half a warp stores neighbours of a row
+                // Rows that are not aligned: up to a line of results waits in shared memory, as far behind a multiple of 16 as its
+                // place in memory, and leaves in pieces of 16 bytes, which are whole but at its ends.
+                const int per_line = kLine / size, first = o0 - c % per_line;  // the line's first output
+                uint8_t* const begin = static_cast<uint8_t*>(a.y) + ((row - lane) * a.y_stride + first) * size;  // of the warp's first row
+                const uint32_t low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(begin)), pitch = static_cast<uint32_t>(a.y_stride) * size;
+                auto behind = [&](int r) { return static_cast<int>((low + r * pitch) % 16); };
+                put16(stage + lane * kPitch + behind(lane) + c % per_line * size, a.y_type, f);
+                if ((c + 16) % per_line != 0 && c + 16 < width) continue;
                 __syncwarp();
+                const int bytes = min(c % per_line + 16, a.n - first) * size, rows = static_cast<int>(min(static_cast<int64_t>(32), a.rows - (row - lane)));
+                // half a warp a row: a whole piece a lane, and a value of the ends a lane (before the first piece, behind the last)
+                for (int r0 = lane / 16; r0 < 32; r0 += 8) {
+                    uint4 piece[4];
+                    uint32_t edge[4];
+                    int piece_at[4], edge_at[4];  // in the staged row, or -1
 #pragma unroll
-                for (int i = 0; i < 16; ++i) stage[lane * kPitch + i] = f[i];
-                __syncwarp();
-                const int o = o0 + lane % 16, r = lane / 16;
-                const int64_t r0 = row - lane + r;
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = r0 + 2 * i, off = behind(r), end = r < rows ? off + max(bytes, 0) : off;
+                        const int head = min((off + 15) / 16 * 16, end), tail = max(end / 16 * 16, head), l = lane % 16;
+                        piece_at[i] = (off + 15) / 16 * 16 + 16 * l;
+                        if (piece_at[i] + 16 > end) piece_at[i] = -1;
+                        edge_at[i] = l < 8 ? off + l * size : tail + (l - 8) * size;
+                        if (edge_at[i] >= (l < 8 ? head : end)) edge_at[i] = -1;
+                        const uint8_t* const from_row = stage + r * kPitch;
+                        if (piece_at[i] >= 0) piece[i] = *reinterpret_cast<const uint4*>(from_row + piece_at[i]);
+                        if (edge_at[i] >= 0)
+                            edge[i] = size == 2 ? *reinterpret_cast<const uint16_t*>(from_row + edge_at[i])
+                                                : *reinterpret_cast<const uint32_t*>(from_row + edge_at[i]);
+                    }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) f[i] = stage[(2 * i + r) * kPitch + lane % 16];
-                if (o < a.n) {
-                    const int there = static_cast<int>(min(static_cast<int64_t>(32), a.rows - r0));
-                    const int64_t at = r0 * a.y_stride + o;
-                    auto each = [&](auto* y, auto&& make) {
-                        y += at;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (2 * i < there) y[2 * i * a.y_stride] = make(f[i]);
-                    };
-                    if (a.y_type == kTokF32)
-                        each(static_cast<float*>(a.y), [](float v) { return v; });
-                    else if (a.y_type == kTokF16)
-                        each(static_cast<__half*>(a.y), [](float v) { return __float2half_rn(v); });
-                    else
-                        each(static_cast<__nv_bfloat16*>(a.y), [](float v) { return __float2bfloat16_rn(v); });
+                    for (int i = 0; i < 4; ++i) {
+                        uint8_t* const to = begin + static_cast<int64_t>(r0 + 2 * i) * a.y_stride * size - behind(r0 + 2 * i);
+                        if (piece_at[i] >= 0) *reinterpret_cast<uint4*>(to + piece_at[i]) = piece[i];
+                        if (edge_at[i] < 0) continue;
+                        if (size == 2)
+                            *reinterpret_cast<uint16_t*>(to + edge_at[i]) = static_cast<uint16_t>(edge[i]);
+                        else
+                            *reinterpret_cast<uint32_t*>(to + edge_at[i]) = edge[i];
+                    }
                 }
+                __syncwarp();
             }
             tc_fence_before();
             __syncwarp();
@@ -322,12 +355,13 @@ cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
     }
     p.tiles_n = (a.n + p.tile_n - 1) / p.tile_n;
     const int slot = (kRows / 2 + p.tile_n / 2) * kI8Step;
-    p.slots = std::min((kSmem - kScaleBytes - kStageBytes) / slot, kI8MaxSlots);
-    p.scales = p.slots * slot;
-    p.stage = p.scales + kScaleBytes;
-    p.bytes = p.stage + kStageBytes;
     const uint64_t where = reinterpret_cast<uintptr_t>(a.y) | static_cast<uint64_t>(a.y_stride) * (a.y_type == kTokF32 ? 4 : 2);
     p.y_align = where % 32 == 0 ? 32 : where % 16 == 0 ? 16 : 0;
+    const int stage = p.y_align ? 0 : kStageBytes;
+    p.slots = std::min((kSmem - kScaleBytes - stage) / slot, kI8MaxSlots);
+    p.scales = p.slots * slot;
+    p.stage = p.scales + kScaleBytes;
+    p.bytes = p.stage + stage;
     auto pitch = [](int64_t stride) { return (stride + 15) / 16 * 16; };  // of one row, which has none
     CUtensorMap x, w;
     e = tmap_rows(&x, a.x, 1, a.k, a.rows, pitch(a.x_stride), kRows / 2);
