@@ -25,6 +25,9 @@ constexpr int kScaleBytes = 2 * 2 * kMaxOutputs * 4, kStageBytes = 8 * 32 * kPit
 
 struct Plan {
     int tile_n;  // outputs of a tile: a multiple of 32, at most 256
+    int split;   // pairs of a cluster that share a tile, each with a range of the inputs; such a cluster has one tile
+    int steps_each;  // steps of a pair
+    int box_m;   // rows that an SM brings: 128, or fewer where there are no more
     int slots;
     int tiles_m, tiles_n;
     int scales, stage;  // offsets of the epilogue's buffers in shared memory
@@ -48,18 +51,23 @@ __device__ __forceinline__ void mma_i8_pair_if(uint32_t issue, uint32_t d, uint6
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
         : "memory");
 }
-// Arrives on the barrier at this offset in both SMs once the MMAs issued so far are done.
-__device__ __forceinline__ void commit_pair_if(uint32_t issue, uint32_t bar) {
+// Arrives on the barrier at this offset in the cluster's blocks of the mask once the MMAs issued so far are done.
+__device__ __forceinline__ void commit_pair_if(uint32_t issue, uint32_t bar, uint16_t blocks) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
         "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
-        "h"(static_cast<uint16_t>(3)), "r"(issue)
+        "h"(blocks), "r"(issue)
         : "memory");
 }
-__device__ __forceinline__ uint32_t of_first(uint32_t addr) {  // the same place in the first SM's shared memory
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, int block) {  // the same place in another block's shared memory
     uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(block));
     return r;
+}
+__device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -119,6 +127,8 @@ __device__ __forceinline__ void store16(uint8_t* to, int type, const float (&f)[
     st32(to, w, wide);
 }
 
+// SPLIT: the pairs of a cluster share a tile.
+template <bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     i8_pair_kernel(const __grid_constant__ I8LinearArgs a, const __grid_constant__ Plan plan,
                    const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
@@ -127,8 +137,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint32_t tmem_at;
     __shared__ volatile int abort_flag;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int rank = blockIdx.x % 2, pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    const int tile_n = plan.tile_n, steps = (a.k + kI8Step - 1) / kI8Step;
+    const int split = SPLIT ? plan.split : 1, rank = blockIdx.x % 2, part = SPLIT ? static_cast<int>(blockIdx.x) / 2 % split : 0;
+    const int pair = blockIdx.x / static_cast<uint32_t>(2 * split), pairs = gridDim.x / static_cast<uint32_t>(2 * split);  // or clusters of pairs
+    const int tile_n = plan.tile_n, k_begin = part * plan.steps_each * kI8Step;
+    const int steps = (min(a.k - k_begin, plan.steps_each * kI8Step) + kI8Step - 1) / kI8Step;  // at least one: the planner's split
+    const uint16_t both = static_cast<uint16_t>(3 << (2 * part));  // this pair's blocks
     const int64_t tiles = static_cast<int64_t>(plan.tiles_m) * plan.tiles_n;
     const int slot_bytes = (kRows / 2 + tile_n / 2) * kI8Step;
     const uint32_t base = smem_u32(smem), bar = smem_u32(bars);
@@ -170,22 +183,101 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_at;
 
+    // the epilogue's warps
+    const int quad = warp % 4, half = (warp - 2) / 4, me = static_cast<int>(threadIdx.x) - 64, size = a.y_type == kTokF32 ? 4 : 2;
+    const int per_line = kLine / size;  // a power of two
+    float* const scales = reinterpret_cast<float*>(smem + plan.scales);  // [tile % 2][scale, bias][output]
+    uint8_t* const stage = smem + plan.stage + (warp - 2) * 32 * kPitch;
+    int* const partial = reinterpret_cast<int*>(smem);  // [output][row of this SM]: a cluster's sums
+    const uint32_t release = in_block(acc_empty, 2 * part);
+    auto row_of = [&](int m) { return static_cast<int64_t>(m) * kRows + rank * (kRows / 2) + quad * 32 + lane; };
+    auto columns = [&](int first, int count, int& c_begin, int& c_end) {  // this warp's, of `count`, a multiple of 16
+        const int low = (count / 16 + 1) / 2 * 16;
+        c_begin = first + half * low;
+        c_end = half ? first + count : first + low;
+    };
+    // Sixteen sums of a thread's row, from column c of the tile on, to results; c_begin and c_end: of all columns of the warp.
+    auto finish16 = [&](int64_t row, int n, float xs, const float* of_tile, int c, int c_begin, int c_end, float (&f)[16]) {
+        const float* const s_at = of_tile + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 sc = *reinterpret_cast<const float4*>(s_at + 4 * i);
+            const float4 b = *reinterpret_cast<const float4*>(s_at + kMaxOutputs + 4 * i);
+            put_pair(f, 2 * i, i8_value(pair_of(f, 2 * i), xs, make_float2(sc.x, sc.y), make_float2(b.x, b.y)));
+            put_pair(f, 2 * i + 1, i8_value(pair_of(f, 2 * i + 1), xs, make_float2(sc.z, sc.w), make_float2(b.z, b.w)));
+        }
+        const int o0 = n * tile_n + c;
+        if (plan.y_align) {
+            uint8_t* const to = static_cast<uint8_t*>(a.y) + (row * a.y_stride + o0) * size;
+            if (row < a.rows && o0 + 16 <= a.n)
+                store16(to, a.y_type, f, plan.y_align == 32);
+            else if (row < a.rows)
+                put16(to, a.y_type, f, a.n - o0);
+            return;
+        }
+        // Rows that are not aligned: up to a line of results waits in shared memory, as far behind a multiple of 16 as its
+        // place in memory, and leaves in pieces of 16 bytes, which are whole but at its ends.
+        const int in = (c - c_begin) & (per_line - 1), first = o0 - in;  // the line's first output
+        uint8_t* const begin = static_cast<uint8_t*>(a.y) + ((row - lane) * a.y_stride + first) * size;  // of the warp's first row
+        const uint32_t low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(begin)), pitch = static_cast<uint32_t>(a.y_stride) * size;
+        auto behind = [&](int r) { return static_cast<int>((low + r * pitch) % 16); };
+        put16(stage + lane * kPitch + behind(lane) + in * size, a.y_type, f);
+        if (in + 16 != per_line && c + 16 < c_end) return;
+        __syncwarp();
+        const int bytes = min(in + 16, a.n - first) * size, rows = static_cast<int>(min(static_cast<int64_t>(32), a.rows - (row - lane)));
+        // half a warp a row: a whole piece a lane, and a value of the ends a lane (before the first piece, behind the last)
+        for (int r0 = lane / 16; r0 < 32; r0 += 8) {
+            uint4 piece[4];
+            uint32_t edge[4];
+            int piece_at[4], edge_at[4];  // in the staged row, or -1
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + 2 * i, off = behind(r), end = r < rows ? off + max(bytes, 0) : off;
+                const int head = min((off + 15) / 16 * 16, end), tail = max(end / 16 * 16, head), l = lane % 16;
+                piece_at[i] = (off + 15) / 16 * 16 + 16 * l;
+                if (piece_at[i] + 16 > end) piece_at[i] = -1;
+                edge_at[i] = l < 8 ? off + l * size : tail + (l - 8) * size;
+                if (edge_at[i] >= (l < 8 ? head : end)) edge_at[i] = -1;
+                const uint8_t* const from_row = stage + r * kPitch;
+                if (piece_at[i] >= 0) piece[i] = *reinterpret_cast<const uint4*>(from_row + piece_at[i]);
+                if (edge_at[i] >= 0)
+                    edge[i] = size == 2 ? *reinterpret_cast<const uint16_t*>(from_row + edge_at[i])
+                                        : *reinterpret_cast<const uint32_t*>(from_row + edge_at[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint8_t* const to = begin + static_cast<int64_t>(r0 + 2 * i) * a.y_stride * size - behind(r0 + 2 * i);
+                if (piece_at[i] >= 0) *reinterpret_cast<uint4*>(to + piece_at[i]) = piece[i];
+                if (edge_at[i] < 0) continue;
+                if (size == 2)
+                    *reinterpret_cast<uint16_t*>(to + edge_at[i]) = static_cast<uint16_t>(edge[i]);
+                else
+                    *reinterpret_cast<uint32_t*>(to + edge_at[i]) = edge[i];
+            }
+        }
+        __syncwarp();
+    };
+
     if (warp == 0) {
         if (lane == 0) {
             int at = 0;
             uint32_t ph = 0;
-            const uint32_t signal = of_first(full);
+            const uint32_t signal = in_block(full, 2 * part);
             for (int64_t t = pair; t < tiles && !abort_flag; t += pairs) {
                 int m, n;
                 tile_at(t, m, n);
+                // an SM without rows brings none (what its lanes then sum up is stored nowhere)
+                const int r0 = m * kRows + rank * (kRows / 2), with_rows = m * kRows + kRows / 2 < a.rows ? 2 : 1;
+                const int bytes = (with_rows * plan.box_m + tile_n) * kI8Step;
                 for (int step = 0; step < steps; ++step) {
                     if (!wait_phase(empty + 8 * at, ph ^ 1, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutEmpty);
                     if (abort_flag) break;
                     const uint32_t to = base + at * slot_bytes;
-                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * at, 2 * slot_bytes);
-                    tma_load_2d_pair(to, &x_map, step * kI8Step, m * kRows + rank * (kRows / 2), signal + 8 * at);
+                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * at, bytes);
+                    if (r0 < a.rows) tma_load_2d_pair(to, &x_map, k_begin + step * kI8Step, r0, signal + 8 * at);
                     if (!a.hold_codes)
-                        tma_load_2d_pair(to + kRows / 2 * kI8Step, &w_map, step * kI8Step, n * tile_n + rank * (tile_n / 2), signal + 8 * at);
+                        tma_load_2d_pair(to + kRows / 2 * kI8Step, &w_map, k_begin + step * kI8Step, n * tile_n + rank * (tile_n / 2),
+                                         signal + 8 * at);
                     if (++at == plan.slots) at = 0, ph ^= 1;
                 }
             }
@@ -214,10 +306,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < kI8Step / 32; ++i)
                         mma_i8_pair_if(issue, acc * kMaxOutputs, ad + 2 * i, bd + 2 * i, idesc, step > 0 || i > 0);
-                    commit_pair_if(issue, empty + 8 * at);
+                    commit_pair_if(issue, empty + 8 * at, both);
                     if (++at == plan.slots) at = 0, ph ^= 1;
                 }
-                commit_pair_if(issue, acc_full + 8 * acc);
+                commit_pair_if(issue, acc_full + 8 * acc, both);
                 if (++acc == 2) acc = 0, acc_ph ^= 1;
             }
             // the last MMAs end before the blocks do
@@ -225,98 +317,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else {
-        // Two warps share a quarter's rows, by halves of the columns; a thread has a row. Scales and bias of the tile's outputs come
-        // to shared memory while the MMAs run. (No role leaves this loop early: its warps meet once a tile.)
-        const int quad = warp % 4, half = (warp - 2) / 4, width = tile_n / 2;
-        float* const scales = reinterpret_cast<float*>(smem + plan.scales);  // [tile % 2][scale, bias][output]
-        uint8_t* const stage = smem + plan.stage + (warp - 2) * 32 * kPitch;
-        const uint32_t release = of_first(acc_empty);
-        const int size = a.y_type == kTokF32 ? 4 : 2, me = threadIdx.x - 64;
+        // A thread has a row, and the two warps of a quarter's rows half of the columns each. Scales and bias of the tile's outputs
+        // come to shared memory while the MMAs run. (No role leaves this loop early: its warps meet once a tile.)
         int acc = 0;
         uint32_t ph = 0;
         for (int64_t t = pair; t < tiles; t += pairs) {
             int m, n;
             tile_at(t, m, n);
-            const int64_t row = static_cast<int64_t>(m) * kRows + rank * (kRows / 2) + quad * 32 + lane;
-            const float xs = row < a.rows ? a.x_scale[a.x_scale_mode == kScaleRow ? row : 0] : 0.f;
             float* const of_tile = scales + acc * 2 * kMaxOutputs;
             if (me < tile_n) {
                 const int o = n * tile_n + me;
                 of_tile[me] = o < a.n ? a.scales[o] : 0.f;
                 of_tile[kMaxOutputs + me] = o < a.n && a.bias ? a.bias[o] : -0.f;
             }
+            const int64_t row = row_of(m);
+            const float xs = row < a.rows ? a.x_scale[a.x_scale_mode == kScaleRow ? row : 0] : 0.f;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             if (!wait_phase(acc_full + 8 * acc, ph, &abort_flag, a.wait_ns)) gave_up(kStatusTimeoutAcc);
             __syncwarp();
             tc_fence_after();
-            const uint32_t from = tmem + acc * kMaxOutputs + half * width + (static_cast<uint32_t>(quad * 32) << 16);
+            int c_begin, c_end;
+            columns(0, tile_n, c_begin, c_end);
+            const uint32_t from = tmem + acc * kMaxOutputs + (static_cast<uint32_t>(quad * 32) << 16);
             uint32_t next[16];
-            tmem_ld16_nowait(from, next);
-            for (int c = 0; c < width; c += 16) {
+            tmem_ld16_nowait(from + c_begin, next);
+            for (int c = c_begin; c < c_end; c += 16) {
                 tmem_wait();
                 tmem_regs_ready(next);
                 float f[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) f[i] = __int2float_rn(static_cast<int>(next[i]));
-                if (c + 16 < width) tmem_ld16_nowait(from + c + 16, next);  // on its way during these columns' arithmetic
-                const float* const s_at = of_tile + half * width + c;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 sc = *reinterpret_cast<const float4*>(s_at + 4 * i);
-                    const float4 b = *reinterpret_cast<const float4*>(s_at + kMaxOutputs + 4 * i);
-                    put_pair(f, 2 * i, i8_value(pair_of(f, 2 * i), xs, make_float2(sc.x, sc.y), make_float2(b.x, b.y)));
-                    put_pair(f, 2 * i + 1, i8_value(pair_of(f, 2 * i + 1), xs, make_float2(sc.z, sc.w), make_float2(b.z, b.w)));
+                for (int i = 0; i < 16; ++i) {
+                    if (SPLIT)
+                        partial[(c + i) * (kRows / 2) + quad * 32 + lane] = static_cast<int>(next[i]);
+                    else
+                        f[i] = __int2float_rn(static_cast<int>(next[i]));
                 }
-                const int o0 = n * tile_n + half * width + c;
-                if (plan.y_align) {
-                    uint8_t* const to = static_cast<uint8_t*>(a.y) + (row * a.y_stride + o0) * size;
-                    if (row < a.rows && o0 + 16 <= a.n)
-                        store16(to, a.y_type, f, plan.y_align == 32);
-                    else if (row < a.rows)
-                        put16(to, a.y_type, f, a.n - o0);
-                    continue;
-                }
-                // Rows that are not aligned: up to a line of results waits in shared memory, as far behind a multiple of 16 as its
-                // place in memory, and leaves in pieces of 16 bytes, which are whole but at its ends.
-                const int per_line = kLine / size, first = o0 - c % per_line;  // the line's first output
-                uint8_t* const begin = static_cast<uint8_t*>(a.y) + ((row - lane) * a.y_stride + first) * size;  // of the warp's first row
-                const uint32_t low = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(begin)), pitch = static_cast<uint32_t>(a.y_stride) * size;
-                auto behind = [&](int r) { return static_cast<int>((low + r * pitch) % 16); };
-                put16(stage + lane * kPitch + behind(lane) + c % per_line * size, a.y_type, f);
-                if ((c + 16) % per_line != 0 && c + 16 < width) continue;
-                __syncwarp();
-                const int bytes = min(c % per_line + 16, a.n - first) * size, rows = static_cast<int>(min(static_cast<int64_t>(32), a.rows - (row - lane)));
-                // half a warp a row: a whole piece a lane, and a value of the ends a lane (before the first piece, behind the last)
-                for (int r0 = lane / 16; r0 < 32; r0 += 8) {
-                    uint4 piece[4];
-                    uint32_t edge[4];
-                    int piece_at[4], edge_at[4];  // in the staged row, or -1
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = r0 + 2 * i, off = behind(r), end = r < rows ? off + max(bytes, 0) : off;
-                        const int head = min((off + 15) / 16 * 16, end), tail = max(end / 16 * 16, head), l = lane % 16;
-                        piece_at[i] = (off + 15) / 16 * 16 + 16 * l;
-                        if (piece_at[i] + 16 > end) piece_at[i] = -1;
-                        edge_at[i] = l < 8 ? off + l * size : tail + (l - 8) * size;
-                        if (edge_at[i] >= (l < 8 ? head : end)) edge_at[i] = -1;
-                        const uint8_t* const from_row = stage + r * kPitch;
-                        if (piece_at[i] >= 0) piece[i] = *reinterpret_cast<const uint4*>(from_row + piece_at[i]);
-                        if (edge_at[i] >= 0)
-                            edge[i] = size == 2 ? *reinterpret_cast<const uint16_t*>(from_row + edge_at[i])
-                                                : *reinterpret_cast<const uint32_t*>(from_row + edge_at[i]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint8_t* const to = begin + static_cast<int64_t>(r0 + 2 * i) * a.y_stride * size - behind(r0 + 2 * i);
-                        if (piece_at[i] >= 0) *reinterpret_cast<uint4*>(to + piece_at[i]) = piece[i];
-                        if (edge_at[i] < 0) continue;
-                        if (size == 2)
-                            *reinterpret_cast<uint16_t*>(to + edge_at[i]) = static_cast<uint16_t>(edge[i]);
-                        else
-                            *reinterpret_cast<uint32_t*>(to + edge_at[i]) = edge[i];
-                    }
-                }
-                __syncwarp();
+                if (c + 16 < c_end) tmem_ld16_nowait(from + c + 16, next);  // on its way during these columns' arithmetic
+                if (!SPLIT) finish16(row, n, xs, of_tile, c, c_begin, c_end, f);
             }
             tc_fence_before();
             __syncwarp();
@@ -324,6 +361,38 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (++acc == 2) acc = 0, ph ^= 1;
         }
         tc_fence_before();
+    }
+    if constexpr (SPLIT) {
+        // The pairs of a cluster hold their sums out in shared memory, over the ring (whose MMAs are done); each adds up a share of
+        // the tile's columns, 512 neighbouring bytes a warp at a time, in its own place for them, and makes results of it.
+        __syncwarp();
+        cluster_sync();
+        const int share = tile_n / split, first = part * share * (kRows / 2) / 4;
+        uint32_t from[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) from[p] = in_block(base, p < split ? 2 * p + rank : 0);
+#pragma unroll 4
+        for (int i = first + threadIdx.x; i < first + share * (kRows / 2) / 4; i += kThreads) {
+            int4 q[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) q[p] = p < split ? ld_cluster4(from[p] + i * 16) : make_int4(0, 0, 0, 0);
+            reinterpret_cast<int4*>(partial)[i] = make_int4(q[0].x + q[1].x + q[2].x + q[3].x, q[0].y + q[1].y + q[2].y + q[3].y,
+                                                            q[0].z + q[1].z + q[2].z + q[3].z, q[0].w + q[1].w + q[2].w + q[3].w);
+        }
+        __syncthreads();
+        if (warp >= 2) {
+            int m, n, c_begin, c_end;
+            tile_at(pair, m, n);
+            const int64_t row = row_of(m);
+            const float xs = row < a.rows ? a.x_scale[a.x_scale_mode == kScaleRow ? row : 0] : 0.f;
+            columns(part * share, share, c_begin, c_end);
+            for (int c = c_begin; c < c_end; c += 16) {
+                float f[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) f[i] = __int2float_rn(partial[(c + i) * (kRows / 2) + quad * 32 + lane]);
+                finish16(row, n, xs, scales, c, c_begin, c_end, f);
+            }
+        }
     }
     __syncwarp();
     __syncthreads();
@@ -334,53 +403,91 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+constexpr int kSmem = 226 * 1024;
+
+// Clusters of `size` blocks that the current device runs at once.
+cudaError_t clusters(int size, int* count) {
+    static std::atomic<int> known[64][9];  // by device; 0: not asked yet
+    int dev = 0;
+    cudaGetDevice(&dev);
+    *count = dev < 64 ? known[dev][size].load(std::memory_order_relaxed) : 0;
+    if (*count) return cudaSuccess;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = size;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(count, i8_pair_kernel<true>, &cfg);
+    if (e == cudaSuccess && dev < 64) known[dev][size].store(*count, std::memory_order_relaxed);
+    return e;
+}
+
 }  // namespace
 
 cudaError_t i8_pair_status(uint32_t* code) { return take_i8_status(code); }
 
 cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
-    constexpr int kSmem = 226 * 1024;
-    cudaError_t e = cudaFuncSetAttribute(i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaError_t e = cudaFuncSetAttribute(i8_pair_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(i8_pair_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     Plan p{};
     p.tiles_m = (a.rows + kRows - 1) / kRows;
-    // Outputs of a tile: the number whose turns over the pairs cost least. A step of 32 inputs moves 256 + n lines of 32 bytes
-    // through an SM's shared memory, in and out, which takes as long as the products of 256 outputs and longer than those of
-    // fewer.
-    const int pairs = sm_count() / 2;
+    // Outputs of a tile, and pairs that share one, with the fewest cycles. A step of 32 inputs moves 256 + n lines of 32 bytes through
+    // an SM's shared memory, in and out, which takes as long as the products of 256 outputs and longer than those of fewer; a
+    // cluster's sum takes some 3000 cycles.
+    const int pairs = sm_count() / 2, steps = (a.k + kI8Step - 1) / kI8Step;
     int64_t least = INT64_MAX;
-    for (int n = kMaxOutputs; n >= 128; n -= 32) {
-        const int64_t tiles = static_cast<int64_t>(p.tiles_m) * ((a.n + n - 1) / n), cost = (tiles + pairs - 1) / pairs * (kRows + n);
-        if (cost < least) least = cost, p.tile_n = n;
+    for (int split = 1; split <= 4; ++split) {
+        int at_once = pairs;
+        if (split > 1) {
+            if (steps < 4 * split) break;
+            if (e = clusters(2 * split, &at_once); e != cudaSuccess) return e;
+        }
+        for (int n = kMaxOutputs; n >= 128; n -= 32) {
+            const int64_t tiles = static_cast<int64_t>(p.tiles_m) * ((a.n + n - 1) / n);
+            if (split > 1 && (n % (16 * split) != 0 || tiles > at_once)) continue;
+            const int64_t turns = (tiles + at_once - 1) / at_once;
+            const int64_t cost = turns * ((steps + split - 1) / split) * (kRows + n) + (split > 1 ? 3000 : 0);
+            if (cost < least) least = cost, p.tile_n = n, p.split = split;
+        }
     }
     p.tiles_n = (a.n + p.tile_n - 1) / p.tile_n;
+    p.steps_each = (steps + p.split - 1) / p.split;
+    while (p.split > 1 && (p.split - 1) * p.steps_each >= steps) --p.split;  // no pair without a step
+    if (p.tile_n % (16 * p.split) != 0) p.split = 1, p.steps_each = steps;
+    p.box_m = std::min((a.rows + 15) / 16 * 16, kRows / 2);
     const int slot = (kRows / 2 + p.tile_n / 2) * kI8Step;
     const uint64_t where = reinterpret_cast<uintptr_t>(a.y) | static_cast<uint64_t>(a.y_stride) * (a.y_type == kTokF32 ? 4 : 2);
     p.y_align = where % 32 == 0 ? 32 : where % 16 == 0 ? 16 : 0;
     const int stage = p.y_align ? 0 : kStageBytes;
     p.slots = std::min((kSmem - kScaleBytes - stage) / slot, kI8MaxSlots);
-    p.scales = p.slots * slot;
+    p.scales = std::max(p.slots * slot, p.split > 1 ? kRows / 2 * p.tile_n * 4 : 0);  // a cluster's sums lie over the ring
     p.stage = p.scales + kScaleBytes;
     p.bytes = p.stage + stage;
     auto pitch = [](int64_t stride) { return (stride + 15) / 16 * 16; };  // of one row, which has none
     CUtensorMap x, w;
-    e = tmap_rows(&x, a.x, 1, a.k, a.rows, pitch(a.x_stride), kRows / 2);
+    e = tmap_rows(&x, a.x, 1, a.k, a.rows, pitch(a.x_stride), p.box_m);
     if (e == cudaSuccess) e = tmap_rows(&w, a.codes, 1, a.k, a.n, pitch(a.codes_stride), p.tile_n / 2);
     if (e != cudaSuccess) return e;
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(tiles, pairs)));
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * p.split * (p.split > 1 ? tiles : std::min<int64_t>(tiles, pairs))));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.x = 2 * p.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
     count_launch();
-    e = cudaLaunchKernelEx(&cfg, i8_pair_kernel, a, p, x, w);
+    e = cudaLaunchKernelEx(&cfg, p.split > 1 ? i8_pair_kernel<true> : i8_pair_kernel<false>, a, p, x, w);
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
