@@ -2,8 +2,7 @@
 //
 // Bound by memory: a value passes once (4 or 2 bytes in, one out). A team of threads holds a row in registers between its
 // largest magnitude and its codes; rows past 16384 values are read twice, the second time mostly from the caches.
-// Codes are those of f32's correctly rounded quotients: a product with the scale's reciprocal stands for the quotient
-// unless it lies so near a half that the two might round differently; then the quotient is taken.
+// Codes are those of f32's correctly rounded quotients.
 #include "counters.hpp"
 #include "token_rows.cuh"
 
@@ -13,9 +12,10 @@ namespace {
 // Code of x / scale. The product t = x inv is off from the rounded quotient by less than 2^-22 |t| <= 2^-14 while |t| < 256 (the
 // reciprocal, the product and the quotient are rounded once each, 2^-24), so rounding it gives the quotient's code if it is
 // further than 2^-13 from a half.
+constexpr float kNearHalf = 0.5f - 1.220703125e-4f;
 __device__ __forceinline__ float code_near(float x, float scale, float inv) {
     const float t = x * inv, r = rintf(t);
-    if (!(fabsf(t - r) < 0.5f - 1.220703125e-4f) || !(fabsf(t) < 256.f)) return __fdiv_rn(x, scale);
+    if (!(fabsf(t - r) < kNearHalf) || !(fabsf(t) < 256.f)) return __fdiv_rn(x, scale);
     return r;
 }
 
@@ -27,8 +27,29 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
     return __fdiv_rn(__uint_as_float(max(top, __float_as_uint(1e-30f))), 127.f);
 }
 
+// Eight codes of a row under its own scale, from whose quotients none is past 127. The quotient is a product with the scale's
+// correctly rounded reciprocal, made good by its remainder (x - t scale, exact in a multiply-add) times the same: correctly
+// rounded by Markstein's theorem (1990), while no term falls below f32's normal numbers.
+__device__ __forceinline__ bool has_codes8(float scale) { return scale > 1e-28f && scale < 1e37f; }
+__device__ __forceinline__ uint2 codes8(const float (&x)[kVec], float scale, float inv) {
+    const float2 inv2 = make_float2(inv, inv), less2 = make_float2(-scale, -scale);
+    uint32_t w[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) {
+        const float2 v = pair_of(x, i), t = mul2(v, inv2), q = fma2(fma2(t, less2, v), inv2, t);
+        const float2 m = add2(q, make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's low byte is the code
+        w[2 * i] = __float_as_uint(m.x);
+        w[2 * i + 1] = __float_as_uint(m.y);
+    }
+    uint32_t out[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        out[i] = __byte_perm(__byte_perm(w[4 * i], w[4 * i + 1], 0x0040), __byte_perm(w[4 * i + 2], w[4 * i + 3], 0x0040), 0x5410);
+    return make_uint2(out[0], out[1]);
+}
+
 template <int TEAM, int TURNS, bool VEC>
-__global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) i8_quantize_kernel(const __grid_constant__ I8RowsArgs a) {
+__global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM <= 32 ? 1 : 2048 / TEAM) i8_quantize_kernel(const __grid_constant__ I8RowsArgs a) {
     __shared__ uint32_t red[32];
     constexpr int kPer = TEAM <= 32 ? 128 / TEAM : 1;
     const int me = threadIdx.x % TEAM;
@@ -39,19 +60,25 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) i8_quantize_kernel(co
     for (int u = 0; u < TURNS; ++u) load8<TEAM, VEC, false>(a.x, row * a.stride, a.type, u, me, cols, f[u]);
     float scale;
     if (a.scale_mode == kScaleRow) {
-        uint32_t top = 0;
+        float top = 0.f;
 #pragma unroll
         for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) top = max(top, __float_as_uint(f[u][j]) & 0x7fffffffu);
-        scale = row_scale(team_max<TEAM>(top, red));
+            for (int i = 0; i < kVec / 2; ++i) top = max_abs(top, pair_of(f[u], i));
+        scale = row_scale(team_max<TEAM>(__float_as_uint(top), red));
         if (me == 0 && cols) a.scale[row] = scale;
     } else {
         scale = a.scale[0];
     }
     const float inv = inverse(scale);
+    const bool plain = VEC && a.scale_mode == kScaleRow && has_codes8(scale);
 #pragma unroll
     for (int u = 0; u < TURNS; ++u) {
+        if (plain) {
+            const int c = column<TEAM, true>(u, 0, me);
+            if (c < cols) *reinterpret_cast<uint2*>(a.codes + row * a.codes_stride + c) = codes8(f[u], scale, inv);
+            continue;
+        }
 #pragma unroll
         for (int j = 0; j < kVec; ++j) f[u][j] = code_near(f[u][j], scale, inv);
         store8_i8<TEAM, VEC>(a.codes, row * a.codes_stride, u, me, cols, f[u]);
@@ -67,46 +94,83 @@ __global__ void __launch_bounds__(kWide) i8_quantize_wide_kernel(const __grid_co
     const int turns = (a.cols + kWide * kVec - 1) / (kWide * kVec);
     float scale;
     if (a.scale_mode == kScaleRow) {
-        uint32_t top = 0;
+        float top = 0.f;
+#pragma unroll 2
         for (int u = 0; u < turns; ++u) {
             float f[kVec];
             load8<kWide, VEC, false>(a.x, row * a.stride, a.type, u, threadIdx.x, a.cols, f);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
+            for (int i = 0; i < kVec / 2; ++i) top = max_abs(top, pair_of(f, i));
         }
-        scale = row_scale(team_max<kWide>(top, red));
+        scale = row_scale(team_max<kWide>(__float_as_uint(top), red));
         if (threadIdx.x == 0) a.scale[row] = scale;
     } else {
         scale = a.scale[0];
     }
     const float inv = inverse(scale);
+    const bool plain = VEC && a.scale_mode == kScaleRow && has_codes8(scale);
+#pragma unroll 2
     for (int u = 0; u < turns; ++u) {
         float f[kVec];
         load8<kWide, VEC, false>(a.x, row * a.stride, a.type, u, threadIdx.x, a.cols, f);
+        if (plain) {
+            const int c = column<kWide, true>(u, 0, threadIdx.x);
+            if (c < a.cols) *reinterpret_cast<uint2*>(a.codes + row * a.codes_stride + c) = codes8(f, scale, inv);
+            continue;
+        }
 #pragma unroll
         for (int j = 0; j < kVec; ++j) f[j] = code_near(f[j], scale, inv);
         store8_i8<kWide, VEC>(a.codes, row * a.codes_stride, u, threadIdx.x, a.cols, f);
     }
 }
 
-// A thread takes eight codes (VEC) or one, in rows of blockIdx.y, ...
-template <bool VEC>
+// A thread takes N codes (eight for 16-bit values, four for f32, so that a warp's store is whole lines; or one, of rows that
+// are not aligned) of four rows at a time.
+constexpr int kBackRows = 4;
+template <int N>
 __global__ void __launch_bounds__(256) i8_dequantize_kernel(const __grid_constant__ I8RowsArgs a) {
-    constexpr int kEach = VEC ? kVec : 1;
-    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * kEach;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N;
     if (c >= a.cols) return;
-    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const float scale = a.scale[a.scale_mode == kScaleRow ? row : 0];
-        const int8_t* const q = a.codes + row * a.codes_stride + c;
-        const int64_t o = row * a.stride + c;
-        if constexpr (VEC) {
-            const uint2 w = *reinterpret_cast<const uint2*>(q);
-            float f[kVec];
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * kBackRows; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.y) * kBackRows) {
+        uint32_t w[kBackRows][2];
+        float scale[kBackRows];
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) f[j] = scale * static_cast<float>(static_cast<int8_t>((j < 4 ? w.x : w.y) >> (8 * (j % 4))));
-            store8<1, true>(a.y, o, a.type, 0, 0, kVec, f);
-        } else {
-            tok_store(a.y, o, a.type, scale * static_cast<float>(*q));
+        for (int i = 0; i < kBackRows; ++i) {
+            const int64_t row = row0 + i;
+            if (row >= a.rows) break;
+            scale[i] = a.scale[a.scale_mode == kScaleRow ? row : 0];
+            const int8_t* const q = a.codes + row * a.codes_stride + c;
+            if constexpr (N == 8) {
+                const uint2 v = *reinterpret_cast<const uint2*>(q);
+                w[i][0] = v.x, w[i][1] = v.y;
+            } else if constexpr (N == 4) {
+                w[i][0] = *reinterpret_cast<const uint32_t*>(q);
+            } else {
+                w[i][0] = static_cast<uint8_t>(*q);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBackRows; ++i) {
+            const int64_t row = row0 + i, o = row * a.stride + c;
+            if (row >= a.rows) break;
+            if constexpr (N > 1) {
+                float f[N];
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) {
+                    // code + 128 under the exponent of 2^23, less that and 128
+                    const uint32_t v = w[i][j / 2] ^ 0x80808080u;
+                    const float2 t = add2(make_float2(__uint_as_float(__byte_perm(v, 0x4b000000u, 0x7650 + 2 * j % 4)),
+                                                      __uint_as_float(__byte_perm(v, 0x4b000000u, 0x7650 + 2 * j % 4 + 1))),
+                                          make_float2(-8388736.f, -8388736.f));
+                    put_pair(f, j, mul2(t, make_float2(scale[i], scale[i])));
+                }
+                if constexpr (N == 4)
+                    *reinterpret_cast<float4*>(static_cast<float*>(a.y) + o) = make_float4(f[0], f[1], f[2], f[3]);
+                else
+                    store8<1, true>(a.y, o, a.type, 0, 0, kVec, f);
+            } else {
+                tok_store(a.y, o, a.type, scale[i] * static_cast<float>(static_cast<int8_t>(w[i][0])));
+            }
         }
     }
 }
@@ -148,14 +212,12 @@ cudaError_t launch_i8_quantize(const I8RowsArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_i8_dequantize(const I8RowsArgs& a, cudaStream_t s) {
-    const bool vec = both_aligned(a, a.y);
-    const unsigned across = static_cast<unsigned>((a.cols + 256 * (vec ? kVec : 1) - 1) / (256 * (vec ? kVec : 1)));
-    const dim3 grid(across, a.rows < 65535 ? a.rows : 65535);
+    const int n = !both_aligned(a, a.y) ? 1 : a.type == kTokF32 ? 4 : 8;
+    const int tall = (a.rows + kBackRows - 1) / kBackRows;
+    const dim3 grid(static_cast<unsigned>((a.cols + 256 * n - 1) / (256 * n)), tall < 65535 ? tall : 65535);
+    auto* kern = n == 8 ? i8_dequantize_kernel<8> : n == 4 ? i8_dequantize_kernel<4> : i8_dequantize_kernel<1>;
     count_launch();
-    if (vec)
-        i8_dequantize_kernel<true><<<grid, 256, 0, s>>>(a);
-    else
-        i8_dequantize_kernel<false><<<grid, 256, 0, s>>>(a);
+    kern<<<grid, 256, 0, s>>>(a);
     return cudaGetLastError();
 }
 
