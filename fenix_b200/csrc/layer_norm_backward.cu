@@ -68,7 +68,7 @@ __device__ __forceinline__ void leave_sums(const LayerNormBackwardArgs& a, int m
 
 // TEAM threads a row, TURNS times eight columns each.
 template <int TEAM, int TURNS, bool VEC>
-__global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+__global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM == 256 || TEAM == 512 ? 1024 / TEAM : 1) layer_norm_backward_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
     constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
     __shared__ float2 red[2][32];
     const int me = threadIdx.x % TEAM;
@@ -120,18 +120,24 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_k
     leave_sums<TEAM, TURNS, VEC>(a, me, dw, db);
 }
 
-// Many rows of 16-bit values: the next rows' dy, h and dsum are on their way to shared memory while a row is worked on. Pairs of
-// values share an instruction. TYPE: of dy, h, weight and dx alike, or -1: any.
+// Many rows of 16-bit values: the next rows' dy, h and dsum are on their way to shared memory while a row is worked on. TYPE: of
+// dy, h, weight and dx alike, or -1: any. Where it says what the weights are, they are brought once a block and not once a row.
+// Narrow rows take two values an instruction and hold the weights in shared memory, wide ones one value and registers, which
+// leaves more of a row's work independent (bf16, us, the first and the second: 100000 x 320 59 and 75, 30000 x 1024 59 and 66,
+// 8192 x 4096 62 and 59, 4000 x 8192 64 and 55).
 constexpr int kAhead = 3;  // rows of a team in shared memory
+template <int TEAM>
+constexpr bool kNarrow = TEAM <= 128;
 template <int TEAM, int TURNS>
-constexpr int kRingBytes = kAhead * 3 * TURNS * (TEAM <= 32 ? 128 : TEAM) * 16;
+constexpr int kRingBytes = (kAhead * 3 * (TEAM <= 32 ? 128 : TEAM) + (kNarrow<TEAM> ? TEAM : 0)) * TURNS * 16;  // and the weights
 
 template <int TEAM, int TURNS, int TYPE>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_stream_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
     constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
     __shared__ float2 red[2][32];
     extern __shared__ __align__(16) uint4 dynamic[];
-    uint4* const ring = dynamic;  // [row][dy, h, dsum][turn][thread]
+    uint4* const shared_held = dynamic;  // [turn][thread of a team]: narrow rows' weights
+    uint4* const ring = dynamic + (kNarrow<TEAM> ? TURNS * TEAM : 0);  // [row][dy, h, dsum][turn][thread]
     const int me = threadIdx.x % TEAM;
     const float inv_n = 1.f / static_cast<float>(a.cols);
     float dw[TURNS][kVec] = {}, db[TURNS][kVec] = {};
@@ -147,6 +153,21 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
         }
         copies_end_row();
     };
+    auto add = [](const float2& x, const float2& y) { return kNarrow<TEAM> ? add2(x, y) : make_float2(x.x + y.x, x.y + y.y); };
+    auto mul = [](const float2& x, const float2& y) { return kNarrow<TEAM> ? mul2(x, y) : make_float2(x.x * y.x, x.y * y.y); };
+    auto mul_add = [](const float2& x, const float2& y, const float2& z) {
+        return kNarrow<TEAM> ? fma2(x, y, z) : make_float2(fmaf(x.x, y.x, z.x), fmaf(x.y, y.y, z.y));
+    };
+    uint4 held[TURNS];
+    if (TYPE >= 0 && a.weight) {
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            const int c = column<TEAM, true>(u, 0, me);
+            held[u] = c < a.cols ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c)) : make_uint4(0, 0, 0, 0);
+            if (kNarrow<TEAM> && threadIdx.x < TEAM) shared_held[u * TEAM + me] = held[u];
+        }
+        if (kNarrow<TEAM>) __syncthreads();
+    }
     const int64_t step = static_cast<int64_t>(gridDim.x) * kPer, mine = threadIdx.x / TEAM;
     int64_t lead = static_cast<int64_t>(blockIdx.x) * kPer;
     float mean = 0.f, rstd = 0.f;
@@ -168,16 +189,19 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
             float w[kVec];
             unpack8(*slot(at, 0, u), TYPE < 0 ? a.dy_type : TYPE, g[u]);
             unpack8(*slot(at, 1, u), TYPE < 0 ? a.h_type : TYPE, z[u]);
-            if (a.weight) load8<TEAM, true, true>(a.weight, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, w);
+            if (a.weight && TYPE >= 0)
+                unpack8(kNarrow<TEAM> ? shared_held[u * TEAM + me] : held[u], TYPE, w);
+            else if (a.weight)
+                load8<TEAM, true, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
 #pragma unroll
             for (int i = 0; i < kVec / 2; ++i) {
                 float2 gi = pair_of(g[u], i);
-                const float2 zi = mul2(add2(pair_of(z[u], i), m2), r2);
-                put_pair(dw[u], i, fma2(gi, zi, pair_of(dw[u], i)));
-                put_pair(db[u], i, add2(pair_of(db[u], i), gi));
-                if (a.weight) gi = mul2(gi, pair_of(w, i));
-                s1 = add2(s1, gi);
-                s2 = fma2(gi, zi, s2);
+                const float2 zi = mul(add(pair_of(z[u], i), m2), r2);
+                put_pair(dw[u], i, mul_add(gi, zi, pair_of(dw[u], i)));
+                put_pair(db[u], i, add(pair_of(db[u], i), gi));
+                if (a.weight) gi = mul(gi, pair_of(w, i));
+                s1 = add(s1, gi);
+                s2 = mul_add(gi, zi, s2);
                 put_pair(g[u], i, gi);
                 put_pair(z[u], i, zi);
             }
@@ -187,12 +211,12 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
             if (column<TEAM, true>(u, 0, me) >= cols) continue;
-            float add[kVec];
-            if (a.dsum) unpack8(*slot(at, 2, u), TYPE < 0 ? a.dx_type : TYPE, add);
+            float more[kVec];
+            if (a.dsum) unpack8(*slot(at, 2, u), TYPE < 0 ? a.dx_type : TYPE, more);
 #pragma unroll
             for (int i = 0; i < kVec / 2; ++i) {
-                const float2 v = add2(pair_of(g[u], i), fma2(pair_of(z[u], i), a2, a1));
-                put_pair(g[u], i, a.dsum ? fma2(v, r2, pair_of(add, i)) : mul2(v, r2));
+                const float2 v = add(pair_of(g[u], i), mul_add(pair_of(z[u], i), a2, a1));
+                put_pair(g[u], i, a.dsum ? mul_add(v, r2, pair_of(more, i)) : mul(v, r2));
             }
             store8<TEAM, true>(a.dx, row * a.dx_stride, TYPE < 0 ? a.dx_type : TYPE, u, me, cols, g[u]);
         }
