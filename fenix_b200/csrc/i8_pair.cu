@@ -357,7 +357,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_cluster(release + 8 * acc);
+            // only where a later tile waits for it: no signal is on its way to a block that may have ended
+            if (lane == 0 && t + 2 * static_cast<int64_t>(pairs) < tiles) arrive_cluster(release + 8 * acc);
             if (++acc == 2) acc = 0, ph ^= 1;
         }
         tc_fence_before();
@@ -396,6 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
     __syncthreads();
+    if (abort_flag) asm volatile("fence.acq_rel.cluster;" ::: "memory");  // signals that no one waited for
+    __syncwarp();
     cluster_sync_relaxed();  // neither SM's shared memory or TMEM ends while the other may still signal or read it
     if (warp == 1) {
         tc_fence_after();

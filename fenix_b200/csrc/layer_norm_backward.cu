@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __res
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;  // of dweight and dbias in a row
     const int warp = threadIdx.x / 32;
     float s = 0.f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the kernel before has ended
     if (c < 2 * cols)
 #pragma unroll 8
         for (int i = warp; i < lines; i += 8) s += work[static_cast<int64_t>(i) * 2 * cols + c];
@@ -394,9 +395,19 @@ cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStrea
             e = launch<1024, 1>(a, vec, lines, s);
     }
     if (e != cudaSuccess || !a.work) return e;
+    // launched while the kernel before it ends, which hides the launch
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((2 * a.cols + 31) / 32);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
     count_launch();
-    layer_norm_join_kernel<<<(2 * a.cols + 31) / 32, 256, 0, s>>>(a.work, lines, a.cols, a.dweight, a.dbias, a.accumulate);
-    return cudaGetLastError();
+    e = cudaLaunchKernelEx(&cfg, layer_norm_join_kernel, const_cast<const float*>(a.work), lines, a.cols, a.dweight, a.dbias, a.accumulate);
+    return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 }  // namespace fxk

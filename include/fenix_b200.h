@@ -471,17 +471,17 @@ fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_
 
 /* Layer norm of rows, with the residual's addition before it and quantisation after it:
  *   h = x + residual,  v = (h - mean(h)) / sqrt(var(h) + eps) * weight + bias,  var = mean((h - mean(h))^2)
- * per row of `cols` values, in f32. Types, strides, dev_sum, scales, in-place forms, limits and rows that are not finite
- * are fx_rms_norm's; besides,
+ * per row of `cols` values, in f32. Types, strides, dev_sum, e4m3 scales, in-place forms and limits are fx_rms_norm's;
+ * besides,
  *   - dev_bias may be NULL (zeros) and has weight_type, as dev_weight, which may be NULL (ones);
  *   - dev_mean and dev_rstd, f32 [rows] each, may be NULL, else receive mean(h) and 1 / sqrt(var(h) + eps), of the
  *     unrounded h, for fx_layer_norm_backward;
  *   - y_type may be i8: y = v / scale rounded to nearest, ties to even, and saturated to +-127, with
  *       FX_SCALE_ROW     scale[row] = max(max |v|, 1e-30) / 127, written to dev_scale [rows]
  *       FX_SCALE_TENSOR  scale = dev_scale[0], read
- *     A row that holds a NaN or infinity gets zeros under a row scale that is NaN; under a tensor scale its NaN become zero.
- * The mean is right to half a step of f32 of its own size, or 2^-48 of the largest |h| where that is more, so that rows
- * far from zero keep their differences. */
+ * The mean is made good by the sum of the differences from it, so that rows far from zero keep theirs.
+ * A row that holds a NaN or infinity, or a difference h - mean past f32's range, comes out NaN: its values, its rstd and its row
+ * scale (its mean NaN or infinite). In i8 its values are zeros, which under a tensor scale nothing tells from others. */
 fx_status fx_layer_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
                         const void* dev_residual, fx_dtype residual_type, int64_t residual_stride, void* dev_sum,
                         int64_t sum_stride, const void* dev_weight, const void* dev_bias, fx_dtype weight_type, float eps,
