@@ -227,34 +227,108 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
 
 // A block a row, of any length: its values are read twice.
 constexpr int kWideThreads = 512;
+template <bool VEC>
 __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
     __shared__ float2 red[32];
     const int64_t row = blockIdx.x;
+    const int me = threadIdx.x, turns = (a.cols + kWideThreads * kVec - 1) / (kWideThreads * kVec);
     const float mean = a.mean[row], rstd = a.rstd[row], inv_n = 1.f / static_cast<float>(a.cols);
-    auto at = [&](int c, float& g, float& z) {
-        g = tok_load(a.dy, row * a.dy_stride + c, a.dy_type);
-        if (a.weight) g *= tok_load(a.weight, c, a.weight_type);
-        z = (tok_load(a.h, row * a.h_stride + c, a.h_type) - mean) * rstd;
+    auto at = [&](int u, float (&g)[kVec], float (&z)[kVec]) {  // columns past the row are 0 in g
+        load8<kWideThreads, VEC, false>(a.dy, row * a.dy_stride, a.dy_type, u, me, a.cols, g);
+        load8<kWideThreads, VEC, false>(a.h, row * a.h_stride, a.h_type, u, me, a.cols, z);
+        if (a.weight) {
+            float w[kVec];
+            load8<kWideThreads, VEC, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) g[j] *= w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) z[j] = (z[j] - mean) * rstd;
     };
     float2 sums = make_float2(0.f, 0.f);
-#pragma unroll 8
-    for (int c = threadIdx.x; c < a.cols; c += kWideThreads) {
-        float g, z;
-        at(c, g, z);
-        sums.x += g;
-        sums.y = fmaf(g, z, sums.y);
+#pragma unroll 2
+    for (int u = 0; u < turns; ++u) {
+        float g[kVec], z[kVec];
+        at(u, g, z);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            const bool inside = column<kWideThreads, VEC>(u, VEC ? 0 : j, me) < a.cols;
+            sums.x += g[j];
+            if (inside) sums.y = fmaf(g[j], z[j], sums.y);
+        }
     }
     sums = team_sum2<kWideThreads>(sums, red);
     sums.x *= inv_n;
     sums.y *= inv_n;
-#pragma unroll 8
-    for (int c = threadIdx.x; c < a.cols; c += kWideThreads) {
-        float g, z;
-        at(c, g, z);
-        g = (g - fmaf(z, sums.y, sums.x)) * rstd;
-        if (a.dsum) g += tok_load(a.dsum, row * a.dsum_stride + c, a.dx_type);
-        tok_store(a.dx, row * a.dx_stride + c, a.dx_type, g);
+#pragma unroll 2
+    for (int u = 0; u < turns; ++u) {
+        float g[kVec], z[kVec];
+        at(u, g, z);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) g[j] = (g[j] - fmaf(z[j], sums.y, sums.x)) * rstd;
+        if (a.dsum) {
+            load8<kWideThreads, VEC, false>(a.dsum, row * a.dsum_stride, a.dx_type, u, me, a.cols, z);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) g[j] += z[j];
+        }
+        store8<kWideThreads, VEC>(a.dx, row * a.dx_stride, a.dx_type, u, me, a.cols, g);
     }
+}
+
+// The same of 16-bit rows up to 16384 columns, as they lie in memory in registers between the two looks at them.
+constexpr int kHeldTurns = 4;
+__global__ void __launch_bounds__(kWideThreads, 2) layer_norm_backward_held_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    __shared__ float2 red[32];
+    const int64_t row = blockIdx.x;
+    const int me = threadIdx.x;
+    uint4 dy[kHeldTurns], h[kHeldTurns];
+#pragma unroll
+    for (int u = 0; u < kHeldTurns; ++u) {
+        const int c = column<kWideThreads, true>(u, 0, me);
+        if (c >= a.cols) continue;
+        dy[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dy) + row * a.dy_stride + c);
+        h[u] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.h) + row * a.h_stride + c);
+    }
+    const float mean = a.mean[row], rstd = a.rstd[row], inv_n = 1.f / static_cast<float>(a.cols);
+    float2 sums = make_float2(0.f, 0.f);
+    auto each = [&](auto&& then) {
+#pragma unroll
+        for (int u = 0; u < kHeldTurns; ++u) {
+            if (column<kWideThreads, true>(u, 0, me) >= a.cols) continue;
+            float g[kVec], z[kVec];
+            unpack8(dy[u], a.dy_type, g);
+            unpack8(h[u], a.h_type, z);
+            if (a.weight) {
+                float w[kVec];
+                load8<kWideThreads, true, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) g[j] *= w[j];
+            }
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) z[j] = (z[j] - mean) * rstd;
+            then(u, g, z);
+        }
+    };
+    each([&](int, float (&g)[kVec], float (&z)[kVec]) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            sums.x += g[j];
+            sums.y = fmaf(g[j], z[j], sums.y);
+        }
+    });
+    sums = team_sum2<kWideThreads>(sums, red);
+    sums.x *= inv_n;
+    sums.y *= inv_n;
+    each([&](int u, float (&g)[kVec], float (&z)[kVec]) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) g[j] = (g[j] - fmaf(z[j], sums.y, sums.x)) * rstd;
+        if (a.dsum) {
+            load8<kWideThreads, true, false>(a.dsum, row * a.dsum_stride, a.dx_type, u, me, a.cols, z);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) g[j] += z[j];
+        }
+        store8<kWideThreads, true>(a.dx, row * a.dx_stride, a.dx_type, u, me, a.cols, g);
+    });
 }
 
 // Sums over rows alone: a block takes 256 columns and every gridDim.y-th row.
@@ -271,6 +345,71 @@ __global__ void __launch_bounds__(256) layer_norm_sums_kernel(const __grid_const
     float* const mine = a.work + static_cast<int64_t>(blockIdx.y) * 2 * a.cols;
     mine[c] = dw;
     mine[a.cols + c] = db;
+}
+
+// The same of rows aligned to eights: a warp takes 256 columns and every eighth of the block's rows. ALL16: of 16-bit values,
+// four rows on their way at a time.
+template <bool ALL16>
+__global__ void __launch_bounds__(256) layer_norm_sums8_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    constexpr int kRows = 4;
+    __shared__ float part[8][32 * kVec + 4];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c0 = blockIdx.x * (32 * kVec);
+    const int cols = min(32 * kVec, a.cols - c0);
+    float dw[kVec] = {}, db[kVec] = {};
+    const int64_t step = static_cast<int64_t>(gridDim.y) * 8;
+    auto take = [&](float (&g)[kVec], float (&z)[kVec], float mean, float rstd) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            dw[j] = fmaf(g[j], (z[j] - mean) * rstd, dw[j]);
+            db[j] += g[j];
+        }
+    };
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * 8 + warp; row0 < a.rows; row0 += kRows * step) {
+        if (ALL16) {
+            uint4 dy[kRows], h[kRows];
+            float mean[kRows], rstd[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int64_t row = row0 + i * step;
+                if (row >= a.rows || lane * kVec >= cols) break;
+                dy[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.dy) + row * a.dy_stride + c0 + lane * kVec);
+                h[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.h) + row * a.h_stride + c0 + lane * kVec);
+                mean[i] = a.mean[row], rstd[i] = a.rstd[row];
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                if (row0 + i * step >= a.rows || lane * kVec >= cols) break;
+                float g[kVec], z[kVec];
+                unpack8(dy[i], a.dy_type, g);
+                unpack8(h[i], a.h_type, z);
+                take(g, z, mean[i], rstd[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int64_t row = row0 + i * step;
+                if (row >= a.rows) break;
+                float g[kVec], z[kVec];
+                load8<32, true, false>(a.dy, row * a.dy_stride + c0, a.dy_type, 0, lane, cols, g);
+                load8<32, true, false>(a.h, row * a.h_stride + c0, a.h_type, 0, lane, cols, z);
+                take(g, z, a.mean[row], a.rstd[row]);
+            }
+        }
+    }
+    float* const mine = a.work + static_cast<int64_t>(blockIdx.y) * 2 * a.cols + c0;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) part[warp][lane * kVec + j] = which ? db[j] : dw[j];
+        __syncthreads();
+        if (static_cast<int>(threadIdx.x) < cols) {
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) sum += part[w][threadIdx.x];
+            mine[which * a.cols + threadIdx.x] = sum;
+        }
+    }
 }
 
 // The lines of the workspace added up: 32 columns a block, eight warps that take every eighth line.
@@ -347,23 +486,33 @@ cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStrea
         return e;
     }
     int lines = 0;
+    const bool vec_in = a.cols % kVec == 0 && rows_of_eights(a.dy, a.dy_stride, a.dy_type) && rows_of_eights(a.h, a.h_stride, a.h_type);
+    const bool vec = vec_in && rows_of_eights(a.weight, 0, a.weight_type) && rows_of_eights(a.dsum, a.dsum_stride, a.dx_type) &&
+                     rows_of_eights(a.dx, a.dx_stride, a.dx_type);
+    const bool stream = vec && a.dy_type != kTokF32 && a.h_type != kTokF32 && (!a.dsum || a.dx_type != kTokF32);
     if (a.cols > kFusedCols || !a.dx) {
         if (a.work) {
-            lines = static_cast<int>(std::min<int64_t>(layer_norm_backward_blocks(a.rows, a.cols), (a.rows + 7) / 8));
+            // enough blocks to fill the GPU several times (3004 x 9984 bf16: 182 us in all with a value a thread in both kernels)
+            const int64_t across = (a.cols + 255) / 256, most = layer_norm_backward_blocks(a.rows, a.cols);
+            lines = static_cast<int>(std::min({most, (static_cast<int64_t>(a.rows) + 7) / 8,
+                                               vec_in ? std::max<int64_t>(8 * sm_count() / across, 1) : most}));
             count_launch();
-            layer_norm_sums_kernel<<<dim3((a.cols + 255) / 256, lines), 256, 0, s>>>(a);
+            auto* kern = !vec_in                                              ? layer_norm_sums_kernel
+                         : a.dy_type != kTokF32 && a.h_type != kTokF32 ? layer_norm_sums8_kernel<true>
+                                                                       : layer_norm_sums8_kernel<false>;
+            kern<<<dim3(static_cast<unsigned>(across), lines), 256, 0, s>>>(a);
             e = cudaGetLastError();
         }
         if (a.dx && e == cudaSuccess) {  // after the sums: dx may take its place over dy or h
+            const bool held = vec && a.cols <= kHeldTurns * kWideThreads * kVec && a.dy_type != kTokF32 && a.h_type != kTokF32;
+            auto* kern = held ? layer_norm_backward_held_kernel
+                         : vec ? layer_norm_backward_wide_kernel<true>
+                               : layer_norm_backward_wide_kernel<false>;
             count_launch();
-            layer_norm_backward_wide_kernel<<<a.rows, kWideThreads, 0, s>>>(a);
+            kern<<<a.rows, kWideThreads, 0, s>>>(a);
             e = cudaGetLastError();
         }
     } else {
-        const bool vec = a.cols % kVec == 0 && rows_of_eights(a.dy, a.dy_stride, a.dy_type) &&
-                         rows_of_eights(a.h, a.h_stride, a.h_type) && rows_of_eights(a.weight, 0, a.weight_type) &&
-                         rows_of_eights(a.dsum, a.dsum_stride, a.dx_type) && rows_of_eights(a.dx, a.dx_stride, a.dx_type);
-        const bool stream = vec && a.dy_type != kTokF32 && a.h_type != kTokF32 && (!a.dsum || a.dx_type != kTokF32);
         if (stream)
             e = a.cols <= 64     ? launch_stream<8, 1>(a, lines, s)
                 : a.cols <= 128  ? launch_stream<16, 1>(a, lines, s)
