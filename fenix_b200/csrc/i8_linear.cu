@@ -10,97 +10,99 @@ namespace fxk {
 namespace {
 
 // ---- rows of any alignment -------------------------------------------------------------------------------------------
-// A tile of 64 rows by 64 outputs, 64 inputs a step, on m16n8k32 MMAs: four warps of 32 by 32 each. The next step's bytes
-// wait in registers while the warps multiply this one's.
-constexpr int kTile = 64, kStep = 64, kPitch = kStep + 16;
+// A tile of 128 rows by 128 outputs, 64 inputs a step, on m16n8k32 MMAs: eight warps of 64 by 32 each. The next step's bytes
+// wait in registers while the warps multiply this one's. Bound by the bytes' way through registers (1003 x 4705 -> 5003 in
+// packed rows: 283 us, 422 with a piece after the other).
+constexpr int kTile = 128, kStep = 64, kPitch = kStep + 16, kPieces = kTile * kStep / 16 / 256;
 
-// 16 bytes of a row from input k0 on, zeros past its end. Of unaligned ones the five words around them are read where all
-// five lie inside the row.
+// 16 bytes of a row from input k0 on, zeros past its end, one by one.
 __device__ __forceinline__ uint4 bytes16(const int8_t* row, int k0, int k) {
-    const int8_t* const p = row + k0;
-    uint32_t w[4];
-    if (k0 + 16 <= k) {
-        const uint32_t off = reinterpret_cast<uintptr_t>(p) & 3;
-        if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) return __ldg(reinterpret_cast<const uint4*>(p));
-        if (off == 0) {
+    uint32_t w[4] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if (k0 >= 4 && k0 + 20 <= k) {
-            const uint32_t* const q = reinterpret_cast<const uint32_t*>(p - off);
-            uint32_t v = __ldg(q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t next = __ldg(q + i + 1);
-                w[i] = __funnelshift_r(v, next, off * 8);
-                v = next;
-            }
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k0 + 4 * i + j < k) w[i] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(p + 4 * i + j))) << (8 * j);
-    }
+    for (int i = 0; i < 16; ++i)
+        if (k0 + i < k) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(row + k0 + i))) << (8 * (i % 4));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__global__ void __launch_bounds__(128) i8_any_kernel(const __grid_constant__ I8LinearArgs a) {
+// Four 8 x 16-byte matrices, a row's address a lane.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const uint8_t* at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(at))
+                 : "memory");
+}
+
+__global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8LinearArgs a) {
     __shared__ __align__(16) uint8_t xs[kTile * kPitch], ws[kTile * kPitch];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kTile;
     const int64_t o0 = static_cast<int64_t>(blockIdx.x) * kTile;
-    const int rm = warp / 2 * 32, om = warp % 2 * 32;  // the warp's corner in the tile
-    uint4 xv[2], wv[2];
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = threadIdx.x / 4 + i * 32, at = k0 + threadIdx.x % 4 * 16;
-            xv[i] = wv[i] = make_uint4(0, 0, 0, 0);
-            if (at < a.k && r0 + row < a.rows) xv[i] = bytes16(a.x + (r0 + row) * a.x_stride, at, a.k);
-            if (at < a.k && o0 + row < a.n) wv[i] = bytes16(a.codes + (o0 + row) * a.codes_stride, at, a.k);
-        }
+    const int rm = warp / 4 * 64, om = warp % 4 * 32;  // the warp's corner in the tile
+    // a piece's 16 bytes are in the five words around them; at the ends of the rows they are put together, in the first four
+    uint32_t raw[2][kPieces][5];
+    bool inside = false;
+    auto piece = [&](int i, int k0, int which) {  // its address, or null where there is no such row
+        const int64_t row = threadIdx.x / 4 + i * 64;
+        if (which ? o0 + row >= a.n : r0 + row >= a.rows) return static_cast<const int8_t*>(nullptr);
+        return (which ? a.codes + (o0 + row) * a.codes_stride : a.x + (r0 + row) * a.x_stride) + k0 + threadIdx.x % 4 * 16;
     };
-    int acc[2][4][4] = {};
+    auto fetch = [&](int k0) {
+        inside = k0 >= 4 && k0 + kStep + 4 <= a.k;
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int8_t* const p = piece(i, k0, which);
+                const int at = k0 + threadIdx.x % 4 * 16;
+                if (!p) {
+#pragma unroll
+                    for (int e = 0; e < 5; ++e) raw[which][i][e] = 0;
+                } else if (inside) {
+                    const uint32_t* const q = reinterpret_cast<const uint32_t*>(p - (reinterpret_cast<uintptr_t>(p) & 3));
+#pragma unroll
+                    for (int e = 0; e < 5; ++e) raw[which][i][e] = __ldg(q + e);
+                } else {
+                    const uint4 v = at < a.k ? bytes16(p - at, at, a.k) : make_uint4(0, 0, 0, 0);
+                    raw[which][i][0] = v.x, raw[which][i][1] = v.y, raw[which][i][2] = v.z, raw[which][i][3] = v.w, raw[which][i][4] = 0;
+                }
+            }
+    };
+    int acc[4][4][4] = {};
     fetch(0);
     for (int k0 = 0; k0 < a.k; k0 += kStep) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int to = (threadIdx.x / 4 + i * 32) * kPitch + threadIdx.x % 4 * 16;
-            *reinterpret_cast<uint4*>(xs + to) = xv[i];
-            *reinterpret_cast<uint4*>(ws + to) = wv[i];
-        }
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const uint32_t shift = inside ? static_cast<uint32_t>(reinterpret_cast<uintptr_t>(piece(i, k0, which)) & 3) * 8 : 0;
+                const uint32_t* const w = raw[which][i];
+                *reinterpret_cast<uint4*>((which ? ws : xs) + (threadIdx.x / 4 + i * 64) * kPitch + threadIdx.x % 4 * 16) =
+                    make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift), __funnelshift_r(w[2], w[3], shift),
+                               __funnelshift_r(w[3], w[4], shift));
+            }
         __syncthreads();
         if (k0 + kStep < a.k) fetch(k0 + kStep);
 #pragma unroll
         for (int kk = 0; kk < kStep; kk += 32) {
-            uint32_t af[2][4], bf[4][2];
+            uint32_t af[4][4], bf[2][4];
+            // lanes 0..7 address rows 0..7 of the first matrix, and so on: rows 0..7 and 8..15, then both 16 inputs on
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 4; ++m) ldmatrix4(af[m], xs + (rm + m * 16 + lane % 16) * kPitch + kk + lane / 16 * 16);
+            // outputs 0..7 and their inputs 16 on, then outputs 8..15
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    af[m][i] = *reinterpret_cast<const uint32_t*>(xs + (rm + m * 16 + g + i % 2 * 8) * kPitch + kk + i / 2 * 16 + t * 4);
+            for (int n = 0; n < 2; ++n) ldmatrix4(bf[n], ws + (om + n * 16 + lane / 16 * 8 + lane % 8) * kPitch + kk + lane / 8 % 2 * 16);
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    bf[n][i] = *reinterpret_cast<const uint32_t*>(ws + (om + n * 8 + g) * kPitch + kk + i * 16 + t * 4);
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
                     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                         : "+r"(acc[m][n][0]), "+r"(acc[m][n][1]), "+r"(acc[m][n][2]), "+r"(acc[m][n][3])
-                        : "r"(af[m][0]), "r"(af[m][1]), "r"(af[m][2]), "r"(af[m][3]), "r"(bf[n][0]), "r"(bf[n][1]));
+                        : "r"(af[m][0]), "r"(af[m][1]), "r"(af[m][2]), "r"(af[m][3]), "r"(bf[n / 2][n % 2 * 2]), "r"(bf[n / 2][n % 2 * 2 + 1]));
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int64_t row = r0 + rm + m * 16 + i * 8 + g;
@@ -127,7 +129,7 @@ cudaError_t launch_any(const I8LinearArgs& a, cudaStream_t s) {
         if (a.x_scale_mode == kScaleRow) part.x_scale = a.x_scale + row;
         part.y = static_cast<uint8_t*>(a.y) + row * a.y_stride * (a.y_type == kTokF32 ? 4 : 2);
         count_launch();
-        i8_any_kernel<<<dim3((a.n + kTile - 1) / kTile, (part.rows + kTile - 1) / kTile), 128, 0, s>>>(part);
+        i8_any_kernel<<<dim3((a.n + kTile - 1) / kTile, (part.rows + kTile - 1) / kTile), 256, 0, s>>>(part);
         if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
     }
     return cudaSuccess;
