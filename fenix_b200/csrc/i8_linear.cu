@@ -139,11 +139,11 @@ cudaError_t launch_any(const I8LinearArgs& a, cudaStream_t s) {
 
 cudaError_t launch_i8_linear(const I8LinearArgs& a, cudaStream_t s) {
     if (!tma_rows(a.x, a.x_stride, a.rows) || !tma_rows(a.codes, a.codes_stride, a.n)) return launch_any(a, s);
-    // Few rows stream weights past them, more share tiles of 256 rows and up to 256 outputs between two SMs. The stream's blocks
+    // Few rows have the weights stream past them, more share tiles of 256 rows and up to 256 outputs between two SMs. The stream's blocks
     // bring every row with 128 outputs, which costs more than the pairs' fixed time once they are many (us, stream and pairs:
     // 32 x 4096 -> 14336 15.9 and 16.2, 64 rows 19.4 and 16.6; 64 x 8192 -> 8192 19.4 and 21.7, 128 rows 20.7 and 22.4, 192 rows
     // 25.8 and 22; 128 x 4096 -> 28672 45 and 29).
-    const bool stream = a.rows <= 32 || (a.rows <= 128 && a.n <= sm_count() / 2 * 128);
+    const bool stream = a.rows <= 32 || (a.rows <= kI8StreamRows && a.n <= sm_count() / 2 * 128);
     return stream ? launch_i8_stream(a, s) : launch_i8_pair(a, s);
 }
 

@@ -9,6 +9,7 @@ namespace fxk {
 
 constexpr int kI8Step = 128;  // inputs of a step: a swizzled line of shared memory a row
 constexpr int kI8MaxSlots = 8;
+constexpr int kI8StreamRows = 128;  // at most
 
 // Rows of bytes that TMA brings: every row begins at a multiple of 16 bytes (one row alone has no stride).
 inline bool tma_rows(const void* p, int64_t stride, int64_t rows) {

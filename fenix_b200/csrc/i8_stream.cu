@@ -1,8 +1,9 @@
 // i8_stream.cu — linear layer of 8-bit integers, few rows: weights stream through tcgen05.
 //
-// Outputs are the MMA's M, 128 a tile, and the rows of x its N, up to 256 a tile, so that a weight is read once whatever the
-// number of rows (to 256), and a single row costs no more than its weights: bound by memory. TMA brings 128 inputs of both at
-// a time, one thread issues the MMAs, sums are held in TMEM. Few tiles are shared by a cluster each, by ranges of the inputs;
+// Outputs are the MMA's M, 128 a tile, and the rows of x its N, so that a weight is read once whatever the number of rows (to
+// 128) and a single row costs no more than its weights: bound by memory (8 x 8192 -> 28672: 41.5 us, 5.7 TB/s, 87% of the copy;
+// with few bytes by the launch, the first copies and a cluster's sum: 1 x 4096 -> 4096 7.6 us). TMA brings 128 inputs of both at
+// a time, one warp issues the MMAs, sums are held in TMEM. Few tiles are shared by a cluster each, by ranges of the inputs;
 // its blocks add up over the cluster's shared memory. Whole numbers add up to the same in any order.
 #include "counters.hpp"
 #include "i8_linear.cuh"
@@ -21,7 +22,7 @@ constexpr int kThreads = 192;  // warps: 0 TMA, 1 TMEM and MMA, 2..5 epilogue
 constexpr int kSmemTwo = 112 * 1024, kSmemOne = 224 * 1024, kSmemLeast = 80 * 1024;
 
 struct Plan {
-    int tile_n;      // rows of a tile: a multiple of 16, at most 256
+    int tile_n;      // rows, rounded up to a multiple of 16: at most kI8StreamRows
     int split;       // blocks of a cluster that share a tile
     int steps_each;  // steps of a block
     int slots;
@@ -49,8 +50,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int tile_n = plan.tile_n, split = plan.split, rank = split > 1 ? static_cast<int>(blockIdx.x) % split : 0;
     const int o0 = static_cast<int>(blockIdx.x) / split * kTileM;
-    const int r0 = static_cast<int>(blockIdx.y) * tile_n;
-    const int rows = min(a.rows - r0, tile_n);
+    const int rows = a.rows;
     const int k_begin = rank * plan.steps_each * kI8Step;
     const int steps = (min(a.k - k_begin, plan.steps_each * kI8Step) + kI8Step - 1) / kI8Step;  // at least one: the planner's split
     const int slot_bytes = (kTileM + tile_n) * kI8Step;
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const uint32_t to = base + at * slot_bytes;
                 mbar_arrive_expect_tx(full + 8 * at, slot_bytes);
                 tma_load_2d(to, &w_map, k_begin + step * kI8Step, o0, full + 8 * at);
-                tma_load_2d(to + kTileM * kI8Step, &x_map, k_begin + step * kI8Step, r0, full + 8 * at);
+                tma_load_2d(to + kTileM * kI8Step, &x_map, k_begin + step * kI8Step, 0, full + 8 * at);
                 if (++at == plan.slots) at = 0, ph ^= 1;
             }
             // copies still on their way, which roles that give up, now or later, no longer wait for
@@ -135,12 +135,12 @@ __global__ void __launch_bounds__(kThreads, 2)
                 continue;
             }
             const int r = c + lane % 16;
-            const float xs = r < rows ? a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0] : 0.f;
+            const float xs = r < rows ? a.x_scale[a.x_scale_mode == kScaleRow ? r : 0] : 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float xi = __shfl_sync(0xffffffffu, xs, i);
                 if (c + i < rows && out < a.n)
-                    tok_store(a.y, static_cast<int64_t>(r0 + c + i) * a.y_stride + out, a.y_type,
+                    tok_store(a.y, static_cast<int64_t>(c + i) * a.y_stride + out, a.y_type,
                               i8_value(static_cast<int>(v[i]), xi, scale, bias));
             }
         }
@@ -162,12 +162,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
             for (int p = 0; p < 8; ++p)
                 if (p < split) s[0] += v[p].x, s[1] += v[p].y, s[2] += v[p].z, s[3] += v[p].w;
-            const float xs = a.x_scale[a.x_scale_mode == kScaleRow ? r0 + r : 0];
+            const float xs = a.x_scale[a.x_scale_mode == kScaleRow ? r : 0];
             float f[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 f[e] = o + e < a.n ? i8_value(s[e], xs, a.scales[o + e], a.bias ? a.bias[o + e] : -0.f) : 0.f;
-            i8_store4(a.y, static_cast<int64_t>(r0 + r) * a.y_stride + o, a.y_type, f, plan.y_vec && o + 4 <= a.n, a.n - o);
+            i8_store4(a.y, static_cast<int64_t>(r) * a.y_stride + o, a.y_type, f, plan.y_vec && o + 4 <= a.n, a.n - o);
         }
         cluster_sync();  // no block's shared memory ends while another reads it
     }
@@ -208,12 +208,12 @@ cudaError_t launch_i8_stream(const I8LinearArgs& a, cudaStream_t s) {
     cudaError_t e = cudaFuncSetAttribute(i8_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemOne);
     if (e != cudaSuccess) return e;
     Plan p{};
-    const int row_tiles = (a.rows + 255) / 256;
-    p.tile_n = (a.rows + row_tiles * 16 - 1) / (row_tiles * 16) * 16;
-    const int tiles = (a.n + kTileM - 1) / kTileM * row_tiles, all_steps = (a.k + kI8Step - 1) / kI8Step;
+    if (a.rows > kI8StreamRows) return cudaErrorInvalidValue;
+    p.tile_n = (a.rows + 15) / 16 * 16;
+    const int tiles = (a.n + kTileM - 1) / kTileM, all_steps = (a.k + kI8Step - 1) / kI8Step;
     const int slot = (kTileM + p.tile_n) * kI8Step;
     // Up to 64 rows two blocks share an SM, so that one's copies go on while the other begins or ends; more rows need the shared
-    // memory for copies on their way (192 x 8192 -> 8192 26 us, 35 with two; 64 x 4096 -> 4096 9.5 us, 9.9 with one).
+    // memory for copies on their way (128 x 4096 -> 4096 11 us, 12.1 with two; 64 rows 9.5 us, 9.9 with one).
     const bool two = p.tile_n <= 64;
     int split = 1;
     for (int c = 8; c > 1 && split == 1; --c) {
@@ -237,7 +237,7 @@ cudaError_t launch_i8_stream(const I8LinearArgs& a, cudaStream_t s) {
     if (e == cudaSuccess) e = tmap_rows(&x, a.x, 1, a.k, a.rows, pitch(a.x_stride), p.tile_n);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((a.n + kTileM - 1) / kTileM * p.split, row_tiles);
+    cfg.gridDim = dim3(tiles * p.split);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;

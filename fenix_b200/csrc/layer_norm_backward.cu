@@ -5,9 +5,11 @@
 //   dx = (g - sum(g) / n - z sum(g z) / n) rstd + dsum,   dweight = sum over rows of dy z,   dbias = sum over rows of dy
 // Bound by memory: dy, h, dsum and dx pass once. Blocks stay and walk over the rows; a thread holds the same columns of every
 // row, so the sums over rows stay in its registers until its block's last row, and leave as one line of the workspace a
-// block, which a second kernel adds up in a fixed order.
-// Rows past 8192 columns would not leave room for those sums in registers: there the rows' gradient is a kernel of its own,
-// which reads a row twice (the second time from the caches), and the sums over rows another.
+// block, which a second kernel adds up in a fixed order (4 us of the whole). Those sums take the registers of a third of the
+// threads an SM could run, and what is left waits for its own results: 8192 x 4096 bf16 59 us, 4.5 TB/s, 69% of the copy;
+// 100000 x 320 59 us; f32 8192 x 4096 120 us. Rows that are not aligned, a value at a time: 1031 x 5119 f16 26 us.
+// Rows past 8192 columns would not leave room for the sums in registers: there the rows' gradient is a kernel of its own, and
+// the sums over rows another, so dy and h pass twice (3004 x 9984 bf16 78 us).
 #include "counters.hpp"
 #include "token_rows.cuh"
 
