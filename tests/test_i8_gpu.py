@@ -227,6 +227,49 @@ def test_linear_tiles_that_fill_the_gpu(cuda_torch, rows, n):
     run_linear(cuda_torch, rows, n, 999, "f16", ys=n + 5)
 
 
+@pytest.mark.parametrize("rows", [33, 48, 100, 127, 128])
+def test_linear_few_rows_of_wide_layers(cuda_torch, rows):
+    """Fewer rows than half a pair's tile, past more outputs than the stream takes."""
+    run_linear(cuda_torch, rows, 10000, 272, bias=True)
+    run_linear(cuda_torch, rows, 9479, 1000, "f16", "tensor")
+    run_linear(cuda_torch, rows, 9601, 130, "f32", y_offset=1)
+
+
+@pytest.mark.parametrize("rows", [129, 200, 256, 300, 512, 600])
+@pytest.mark.parametrize("n,k", [(256, 16384), (1000, 8192), (77, 5000), (4096, 4096), (5003, 2000), (2500, 3000), (640, 9300)])
+def test_linear_clusters_of_pairs(cuda_torch, rows, n, k):
+    """Few tiles of many inputs, which two to four pairs share; the last range may be a part, results aligned or not."""
+    run_linear(cuda_torch, rows, n, k)
+    run_linear(cuda_torch, rows, n, k, "f32", bias=True)
+    run_linear(cuda_torch, rows, n, k, "f16", "tensor", ys=n + 5, y_offset=3)
+
+
+def test_linear_kernels_of_all_kinds_at_once(cuda_torch):
+    """Calls that take different kernels, with and without tensor memory of their own, on streams of their own at once."""
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(4)
+    calls = []
+    for rows, n, k, pitch in ((1, 4096, 2048, 2048), (60, 2000, 4096, 4096), (100, 1500, 1024, 1024), (100, 12000, 512, 512),
+                              (300, 700, 8192, 8192), (1000, 2100, 1024, 1024), (70, 300, 999, 999)):
+        x = torch.randint(-127, 128, (rows, pitch), generator=g, device="cuda", dtype=torch.int8)
+        w = torch.randint(-127, 128, (n, pitch), generator=g, device="cuda", dtype=torch.int8)
+        xs, ws = torch.rand(rows, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda")
+        y = torch.empty(rows, n, device="cuda")
+        calls.append((torch.cuda.Stream(), y, linear_want(torch, x[:, :k], xs, w[:, :k], ws, None, "f32"),
+                      lambda x=x, w=w, xs=xs, ws=ws, y=y, rows=rows, n=n, k=k: fx.i8_linear_dev(
+                          ptr(x), ptr(y), rows, n, k, ptr(w), ptr(ws), ptr(xs), "f32", stream=stream(torch))))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for on, y, _, call in calls:
+            with torch.cuda.stream(on):
+                y.fill_(-1.0)
+                call()
+    torch.cuda.synchronize()
+    for _, y, want, _ in calls:
+        assert torch.equal(y, want)
+    fx.i8_device_status(0)
+
+
 def test_linear_many_rows(cuda_torch):
     run_linear(cuda_torch, 300001, 24, 64)
     run_linear(cuda_torch, 70001, 130, 33, "f16", xs=33, ws=33)

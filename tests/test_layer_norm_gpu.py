@@ -360,8 +360,9 @@ def test_backward_strides_and_offsets(cuda_torch, strides, offset):
 
 @pytest.mark.parametrize("where", ["dy", "h", "dsum"])
 def test_backward_in_place(cuda_torch, where):
-    for rows, cols in ((11, 40), (11, 77), (700, 4096), (60, 9001), (20000, 64)):
+    for rows, cols in ((11, 40), (11, 77), (700, 4096), (60, 9001), (20000, 64), (300, 9008), (300, 16384), (200, 20000)):
         run_backward(cuda_torch, rows, cols, in_place=where)
+        run_backward(cuda_torch, rows, cols, "f32", "f32", "f32", "f32", in_place=where)
 
 
 def test_backward_past_32_bits(cuda_torch):
