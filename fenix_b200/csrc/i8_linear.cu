@@ -32,11 +32,15 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const uint8_t* at) {
                  : "memory");
 }
 
-__global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8LinearArgs a) {
+// The blocks of a cluster share a tile, steps_each steps of the inputs each; alone with split 1.
+__global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8LinearArgs a, int split, int steps_each) {
+    extern __shared__ __align__(16) int partial[];  // [row][output]: a cluster's sums
     __shared__ __align__(16) uint8_t xs[kTile * kPitch], ws[kTile * kPitch];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * kTile;
-    const int64_t o0 = static_cast<int64_t>(blockIdx.x) * kTile;
+    const int rank = split > 1 ? static_cast<int>(blockIdx.x) % split : 0;
+    const int64_t o0 = static_cast<int64_t>(blockIdx.x) / split * kTile;
+    const int k_begin = rank * steps_each * kStep, k_end = min(a.k, k_begin + steps_each * kStep);  // not empty: the launcher's split
     const int rm = warp / 4 * 64, om = warp % 4 * 32;  // the warp's corner in the tile
     // a piece's 16 bytes are in the five words around them; at the ends of the rows they are put together, in the first four
     uint32_t raw[2][kPieces][5];
@@ -68,8 +72,8 @@ __global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8L
             }
     };
     int acc[4][4][4] = {};
-    fetch(0);
-    for (int k0 = 0; k0 < a.k; k0 += kStep) {
+    fetch(k_begin);
+    for (int k0 = k_begin; k0 < k_end; k0 += kStep) {
 #pragma unroll
         for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -81,7 +85,7 @@ __global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8L
                                __funnelshift_r(w[3], w[4], shift));
             }
         __syncthreads();
-        if (k0 + kStep < a.k) fetch(k0 + kStep);
+        if (k0 + kStep < k_end) fetch(k0 + kStep);
 #pragma unroll
         for (int kk = 0; kk < kStep; kk += 32) {
             uint32_t af[4][4], bf[2][4];
@@ -100,6 +104,34 @@ __global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8L
                         : "r"(af[m][0]), "r"(af[m][1]), "r"(af[m][2]), "r"(af[m][3]), "r"(bf[n / 2][n % 2 * 2]), "r"(bf[n / 2][n % 2 * 2 + 1]));
         }
         __syncthreads();
+    }
+    if (split > 1) {  // each block adds up a share of the tile over the cluster
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    *reinterpret_cast<int2*>(partial + (rm + m * 16 + i * 8 + g) * kTile + om + n * 8 + t * 2) =
+                        make_int2(acc[m][n][2 * i], acc[m][n][2 * i + 1]);
+        cluster_sync();
+        const int rows = static_cast<int>(min(static_cast<int64_t>(kTile), a.rows - r0)), all = rows * (kTile / 4);
+        const int share = (all + split - 1) / split, end = min(all, (rank + 1) * share);
+        for (int i = rank * share + threadIdx.x; i < end; i += 256) {
+            int sum[4] = {};
+            for (int p = 0; p < split; ++p) {
+                const int4 v = ld_cluster_s32x4(smem_u32(partial) + i * 16, p);
+                sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+            }
+            const int64_t row = r0 + i / (kTile / 4), o = o0 + i % (kTile / 4) * 4;
+            const float scale = a.x_scale[a.x_scale_mode == kScaleRow ? row : 0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (o + e < a.n)
+                    tok_store(a.y, row * a.y_stride + o + e, a.y_type, i8_value(sum[e], scale, a.scales[o + e], a.bias ? a.bias[o + e] : -0.f));
+        }
+        cluster_sync();  // no block's shared memory ends while another reads it
+        return;
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m)
@@ -122,15 +154,36 @@ __global__ void __launch_bounds__(256) i8_any_kernel(const __grid_constant__ I8L
 
 cudaError_t launch_any(const I8LinearArgs& a, cudaStream_t s) {
     constexpr int64_t kRows = int64_t{65535} * kTile;  // of a launch
+    constexpr int kBytes = kTile * kTile * 4;
+    cudaError_t e = cudaFuncSetAttribute(i8_any_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return e;
     for (int64_t row = 0; row < a.rows; row += kRows) {
         I8LinearArgs part = a;
         part.rows = static_cast<int>(std::min<int64_t>(kRows, a.rows - row));
         part.x = a.x + row * a.x_stride;
         if (a.x_scale_mode == kScaleRow) part.x_scale = a.x_scale + row;
         part.y = static_cast<uint8_t*>(a.y) + row * a.y_stride * (a.y_type == kTokF32 ? 4 : 2);
+        // few tiles: clusters of as many blocks as fill the GPU once share one (1 x 4097 -> 4096 81 us without)
+        const int64_t across = (a.n + kTile - 1) / kTile, down = (part.rows + kTile - 1) / kTile;
+        const int steps = (a.k + kStep - 1) / kStep;
+        int split = static_cast<int>(std::max<int64_t>(std::min<int64_t>({sm_count() / (across * down), 8, steps / 2}), 1));
+        const int steps_each = (steps + split - 1) / split;
+        split = (steps + steps_each - 1) / steps_each;  // no block without a step
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(across * split), static_cast<unsigned>(down));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = split > 1 ? kBytes : 0;
+        cfg.stream = s;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = split;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = split > 1 ? 1 : 0;
         count_launch();
-        i8_any_kernel<<<dim3((a.n + kTile - 1) / kTile, (part.rows + kTile - 1) / kTile), 256, 0, s>>>(part);
-        if (const cudaError_t e = cudaGetLastError(); e != cudaSuccess) return e;
+        e = cudaLaunchKernelEx(&cfg, i8_any_kernel, part, split, steps_each);
+        if (e == cudaSuccess) e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
 }

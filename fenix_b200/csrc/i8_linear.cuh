@@ -33,6 +33,15 @@ static inline cudaError_t take_i8_status(uint32_t* code) {
     return e;
 }
 
+// Four s32 of a block of the cluster, at a shared-memory address of this one.
+__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr, int rank) {
+    int4 v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\tld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [r];\n\t}"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr), "r"(rank));
+    return v;
+}
+
 // A result from its exact sum, rounded to f32: the same in every kernel, so that it does not depend on the way taken. Without a bias, bias
 // is -0, which changes nothing.
 __device__ __forceinline__ float i8_value(float sum, float x_scale, float scale, float bias) {

@@ -31,15 +31,6 @@ struct Plan {
     bool y_vec;      // results aligned to four outputs
 };
 
-// Four s32 of a block of the cluster, at a shared-memory address of this one.
-__device__ __forceinline__ int4 ld_cluster_s32x4(uint32_t addr, int rank) {
-    int4 v;
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %4, %5;\n\tld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [r];\n\t}"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "r"(addr), "r"(rank));
-    return v;
-}
-
 __global__ void __launch_bounds__(kThreads, 2)
     i8_stream_kernel(const __grid_constant__ I8LinearArgs a, const __grid_constant__ Plan plan,
                      const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map) {
