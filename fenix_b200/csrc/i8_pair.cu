@@ -186,6 +186,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();  // the other SM's barriers are there too
     tc_fence_after();
     const uint32_t tmem = tmem_at;
+    // TMEM is there in every block that comes here: a later kernel's blocks, which begin after all of them have, keep none from it
+    let_later_begin();
+    wait_for_earlier();
 
     // the epilogue's warps
     const int quad = warp % 4, half = (warp - 2) / 4, me = static_cast<int>(threadIdx.x) - 64, size = a.y_type == kTokF32 ? 4 : 2;
@@ -487,12 +490,14 @@ cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2 * p.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     count_launch();
     e = cudaLaunchKernelEx(&cfg, p.split > 1 ? i8_pair_kernel<true> : i8_pair_kernel<false>, a, p, x, w);
     return e == cudaSuccess ? cudaGetLastError() : e;

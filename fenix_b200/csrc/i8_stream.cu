@@ -60,6 +60,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         abort_flag = 0;
         fence_mbar_init();
     }
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&w_map) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
+    }
     if (warp == 1) {
         tmem_alloc(smem_u32(&tmem_at), plan.cols);
         tmem_relinquish();
@@ -68,6 +72,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_at;
+    // TMEM is there in every block that comes here: a later kernel's blocks, which begin after all of them have, keep none from it
+    let_later_begin();
+    wait_for_earlier();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -232,12 +239,14 @@ cudaError_t launch_i8_stream(const I8LinearArgs& a, cudaStream_t s) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = p.bytes;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = p.split;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = p.split > 1 ? 1 : 0;
+    cfg.numAttrs = 2;
     count_launch();
     e = cudaLaunchKernelEx(&cfg, i8_stream_kernel, a, p, w, x);
     return e == cudaSuccess ? cudaGetLastError() : e;
