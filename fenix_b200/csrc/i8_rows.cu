@@ -51,6 +51,8 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[kVec], float scale, flo
 
 template <int TEAM, int TURNS, bool VEC>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM <= 32 ? 1 : 2048 / TEAM) i8_quantize_kernel(const __grid_constant__ I8RowsArgs a) {
+    let_later_begin();
+    wait_for_earlier();
     __shared__ uint32_t red[32];
     constexpr int kPer = TEAM <= 32 ? 128 / TEAM : 1;
     const int me = threadIdx.x % TEAM;
@@ -90,6 +92,8 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM <= 32 ? 1 : 2048
 constexpr int kWide = 1024;
 template <bool VEC>
 __global__ void __launch_bounds__(kWide) i8_quantize_wide_kernel(const __grid_constant__ I8RowsArgs a) {
+    let_later_begin();
+    wait_for_earlier();
     __shared__ uint32_t red[32];
     const int64_t row = blockIdx.x;
     const int turns = (a.cols + kWide * kVec - 1) / (kWide * kVec);
@@ -130,6 +134,8 @@ __global__ void __launch_bounds__(kWide) i8_quantize_wide_kernel(const __grid_co
 constexpr int kBackRows = 4;
 template <int N>
 __global__ void __launch_bounds__(256) i8_dequantize_kernel(const __grid_constant__ I8RowsArgs a) {
+    let_later_begin();
+    wait_for_earlier();
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N;
     if (c >= a.cols) return;
     for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * kBackRows; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.y) * kBackRows) {
@@ -181,11 +187,7 @@ cudaError_t quantize(const I8RowsArgs& a, bool vec, cudaStream_t s) {
     constexpr int threads = TEAM <= 32 ? 128 : TEAM, per = threads / TEAM;
     const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + per - 1) / per);
     count_launch();
-    if (vec)
-        i8_quantize_kernel<TEAM, TURNS, true><<<grid, threads, 0, s>>>(a);
-    else
-        i8_quantize_kernel<TEAM, TURNS, false><<<grid, threads, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(vec ? i8_quantize_kernel<TEAM, TURNS, true> : i8_quantize_kernel<TEAM, TURNS, false>, dim3(grid), threads, 0, s, a);
 }
 
 bool both_aligned(const I8RowsArgs& a, const void* values) {
@@ -205,11 +207,7 @@ cudaError_t launch_i8_quantize(const I8RowsArgs& a, cudaStream_t s) {
     if (a.cols <= 8192) return quantize<512, 2>(a, vec, s);
     if (a.cols <= 16384) return quantize<1024, 2>(a, vec, s);
     count_launch();
-    if (vec)
-        i8_quantize_wide_kernel<true><<<a.rows, kWide, 0, s>>>(a);
-    else
-        i8_quantize_wide_kernel<false><<<a.rows, kWide, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(vec ? i8_quantize_wide_kernel<true> : i8_quantize_wide_kernel<false>, dim3(a.rows), kWide, 0, s, a);
 }
 
 cudaError_t launch_i8_dequantize(const I8RowsArgs& a, cudaStream_t s) {
@@ -218,8 +216,7 @@ cudaError_t launch_i8_dequantize(const I8RowsArgs& a, cudaStream_t s) {
     const dim3 grid(static_cast<unsigned>((a.cols + 256 * n - 1) / (256 * n)), tall < 65535 ? tall : 65535);
     auto* kern = n == 8 ? i8_dequantize_kernel<8> : n == 4 ? i8_dequantize_kernel<4> : i8_dequantize_kernel<1>;
     count_launch();
-    kern<<<grid, 256, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(kern, grid, 256, 0, s, a);
 }
 
 }  // namespace fxk

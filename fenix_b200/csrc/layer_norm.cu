@@ -100,8 +100,8 @@ __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, 
     for (int u = 0; u < TURNS; ++u) {
         if (VEC && !inside(u, 0)) continue;
         float w[kVec], b[kVec];
-        if (a.weight) load8<TEAM, VEC, true>(a.weight, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, w);
-        if (a.bias) load8<TEAM, VEC, true>(a.bias, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, b);
+        if (a.weight) load8<TEAM, VEC, false>(a.weight, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, w);
+        if (a.bias) load8<TEAM, VEC, false>(a.bias, 0, TYPE < 0 ? a.weight_type : TYPE, u, me, a.cols, b);
 #pragma unroll
         for (int i = 0; i < kVec / 2; ++i) {
             float2 v = fma2(pair_of(h[u], i), r2, off2);
@@ -161,6 +161,8 @@ __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, 
 // TEAM threads a row, TURNS times eight values each.
 template <int TEAM, int TURNS, bool VEC>
 __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) layer_norm_kernel(const __grid_constant__ LayerNormArgs a) {
+    let_later_begin();
+    wait_for_earlier();
     __shared__ Red red;
     const int me = threadIdx.x % TEAM;
     const int64_t row = TEAM == 32 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
@@ -188,6 +190,7 @@ __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) layer_norm_kernel(con
 // before it is worked on, so that memory does not wait for the reductions.
 template <int TEAM, int TURNS, bool RES, int TYPE>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_stream_kernel(const __grid_constant__ LayerNormArgs a) {
+    wait_for_earlier();
     __shared__ Red red[2];
     const int me = threadIdx.x % TEAM, per = TEAM <= 32 ? 128 / TEAM : 1;
     const int64_t step = static_cast<int64_t>(gridDim.x) * per;
@@ -240,6 +243,7 @@ constexpr int kRingBytes = kAhead * (RES ? 2 : 1) * TURNS * TEAM * 16;
 
 template <int TEAM, int TURNS, bool RES, int TYPE>
 __global__ void __launch_bounds__(TEAM) layer_norm_ring_kernel(const __grid_constant__ LayerNormArgs a) {
+    wait_for_earlier();
     __shared__ Red red[2];
     extern __shared__ __align__(16) uint4 ring[];  // [row][x, residual][turn][thread]
     const int me = threadIdx.x;
@@ -288,11 +292,7 @@ cudaError_t launch(const LayerNormArgs& a, bool vec, cudaStream_t s) {
     const int threads = TEAM == 32 ? 128 : TEAM, per = threads / TEAM;
     const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + per - 1) / per);
     count_launch();
-    if (vec)
-        layer_norm_kernel<TEAM, TURNS, true><<<grid, threads, 0, s>>>(a);
-    else
-        layer_norm_kernel<TEAM, TURNS, false><<<grid, threads, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(vec ? layer_norm_kernel<TEAM, TURNS, true> : layer_norm_kernel<TEAM, TURNS, false>, dim3(grid), threads, 0, s, a);
 }
 
 template <int TEAM, int TURNS, bool RES, int TYPE>
@@ -317,8 +317,7 @@ cudaError_t launch_stream(const LayerNormArgs& a, cudaStream_t s) {
     }
     const int64_t need = (static_cast<int64_t>(a.rows) + per - 1) / per, fit = static_cast<int64_t>(sm_count()) * resident;
     count_launch();
-    kern<<<static_cast<unsigned>(need < fit ? need : fit), threads, bytes, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(kern, dim3(static_cast<unsigned>(need < fit ? need : fit)), threads, bytes, s, a);
 }
 template <int TEAM, int TURNS, bool RES>
 cudaError_t launch_stream(const LayerNormArgs& a, cudaStream_t s) {

@@ -71,6 +71,7 @@ __device__ __forceinline__ void leave_sums(const LayerNormBackwardArgs& a, int m
 // TEAM threads a row, TURNS times eight columns each.
 template <int TEAM, int TURNS, bool VEC>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM == 256 || TEAM == 512 ? 1024 / TEAM : 1) layer_norm_backward_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    wait_for_earlier();
     constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
     __shared__ float2 red[2][32];
     const int me = threadIdx.x % TEAM;
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM == 256 || TEAM =
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
             float w[kVec];
-            if (a.weight) load8<TEAM, VEC, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+            if (a.weight) load8<TEAM, VEC, false>(a.weight, 0, a.weight_type, u, me, a.cols, w);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) {
                 z[u][j] = column<TEAM, VEC>(u, VEC ? 0 : j, me) < cols ? (z[u][j] - mean) * rstd : 0.f;
@@ -135,6 +136,7 @@ constexpr int kRingBytes = (kAhead * 3 * (TEAM <= 32 ? 128 : TEAM) + (kNarrow<TE
 
 template <int TEAM, int TURNS, int TYPE>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_stream_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    wait_for_earlier();
     constexpr int kThreads = TEAM <= 32 ? 128 : TEAM, kPer = kThreads / TEAM;
     __shared__ float2 red[2][32];
     extern __shared__ __align__(16) uint4 dynamic[];
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
 #pragma unroll
         for (int u = 0; u < TURNS; ++u) {
             const int c = column<TEAM, true>(u, 0, me);
-            held[u] = c < a.cols ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c)) : make_uint4(0, 0, 0, 0);
+            held[u] = c < a.cols ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.weight) + c) : make_uint4(0, 0, 0, 0);
             if (kNarrow<TEAM> && threadIdx.x < TEAM) shared_held[u * TEAM + me] = held[u];
         }
         if (kNarrow<TEAM>) __syncthreads();
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
             if (a.weight && TYPE >= 0)
                 unpack8(kNarrow<TEAM> ? shared_held[u * TEAM + me] : held[u], TYPE, w);
             else if (a.weight)
-                load8<TEAM, true, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+                load8<TEAM, true, false>(a.weight, 0, a.weight_type, u, me, a.cols, w);
 #pragma unroll
             for (int i = 0; i < kVec / 2; ++i) {
                 float2 gi = pair_of(g[u], i);
@@ -231,6 +233,7 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM) layer_norm_backward_s
 constexpr int kWideThreads = 512;
 template <bool VEC>
 __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    wait_for_earlier();
     __shared__ float2 red[32];
     const int64_t row = blockIdx.x;
     const int me = threadIdx.x, turns = (a.cols + kWideThreads * kVec - 1) / (kWideThreads * kVec);
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(
         load8<kWideThreads, VEC, false>(a.h, row * a.h_stride, a.h_type, u, me, a.cols, z);
         if (a.weight) {
             float w[kVec];
-            load8<kWideThreads, VEC, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+            load8<kWideThreads, VEC, false>(a.weight, 0, a.weight_type, u, me, a.cols, w);
 #pragma unroll
             for (int j = 0; j < kVec; ++j) g[j] *= w[j];
         }
@@ -280,6 +283,7 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_backward_wide_kernel(
 // The same of 16-bit rows up to 16384 columns, as they lie in memory in registers between the two looks at them.
 constexpr int kHeldTurns = 4;
 __global__ void __launch_bounds__(kWideThreads, 2) layer_norm_backward_held_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    wait_for_earlier();
     __shared__ float2 red[32];
     const int64_t row = blockIdx.x;
     const int me = threadIdx.x;
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) layer_norm_backward_held_kern
             unpack8(h[u], a.h_type, z);
             if (a.weight) {
                 float w[kVec];
-                load8<kWideThreads, true, true>(a.weight, 0, a.weight_type, u, me, a.cols, w);
+                load8<kWideThreads, true, false>(a.weight, 0, a.weight_type, u, me, a.cols, w);
 #pragma unroll
                 for (int j = 0; j < kVec; ++j) g[j] *= w[j];
             }
@@ -335,6 +339,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) layer_norm_backward_held_kern
 
 // Sums over rows alone: a block takes 256 columns and every gridDim.y-th row.
 __global__ void __launch_bounds__(256) layer_norm_sums_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    wait_for_earlier();
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= a.cols) return;
     float dw = 0.f, db = 0.f;
@@ -353,6 +358,7 @@ __global__ void __launch_bounds__(256) layer_norm_sums_kernel(const __grid_const
 // four rows on their way at a time.
 template <bool ALL16>
 __global__ void __launch_bounds__(256) layer_norm_sums8_kernel(const __grid_constant__ LayerNormBackwardArgs a) {
+    wait_for_earlier();
     constexpr int kRows = 4;
     __shared__ float part[8][32 * kVec + 4];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c0 = blockIdx.x * (32 * kVec);
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __res
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;  // of dweight and dbias in a row
     const int warp = threadIdx.x / 32;
     float s = 0.f;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the kernel before has ended
+    wait_for_earlier();
     if (c < 2 * cols)
 #pragma unroll 8
         for (int i = warp; i < lines; i += 8) s += work[static_cast<int64_t>(i) * 2 * cols + c];
@@ -453,8 +459,7 @@ cudaError_t launch(const LayerNormBackwardArgs& a, Kernel* kern, int ring, std::
     const int64_t need = (static_cast<int64_t>(a.rows) + per - 1) / per, fit = static_cast<int64_t>(sm_count()) * resident;
     lines = static_cast<int>(std::min({need, fit, layer_norm_backward_blocks(a.rows, a.cols)}));
     count_launch();
-    kern<<<static_cast<unsigned>(lines), threads, bytes, s>>>(a);
-    return cudaGetLastError();
+    return launch_early(kern, dim3(static_cast<unsigned>(lines)), threads, bytes, s, a);
 }
 template <int TEAM, int TURNS>
 cudaError_t launch(const LayerNormBackwardArgs& a, bool vec, int& lines, cudaStream_t s) {
@@ -502,8 +507,7 @@ cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStrea
             auto* kern = !vec_in                                              ? layer_norm_sums_kernel
                          : a.dy_type != kTokF32 && a.h_type != kTokF32 ? layer_norm_sums8_kernel<true>
                                                                        : layer_norm_sums8_kernel<false>;
-            kern<<<dim3(static_cast<unsigned>(across), lines), 256, 0, s>>>(a);
-            e = cudaGetLastError();
+            e = launch_early(kern, dim3(static_cast<unsigned>(across), lines), 256, 0, s, a);
         }
         if (a.dx && e == cudaSuccess) {  // after the sums: dx may take its place over dy or h
             const bool held = vec && a.cols <= kHeldTurns * kWideThreads * kVec && a.dy_type != kTokF32 && a.h_type != kTokF32;
@@ -511,8 +515,7 @@ cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStrea
                          : vec ? layer_norm_backward_wide_kernel<true>
                                : layer_norm_backward_wide_kernel<false>;
             count_launch();
-            kern<<<a.rows, kWideThreads, 0, s>>>(a);
-            e = cudaGetLastError();
+            e = launch_early(kern, dim3(a.rows), kWideThreads, 0, s, a);
         }
     } else {
         if (stream)
@@ -546,19 +549,9 @@ cudaError_t launch_layer_norm_backward(const LayerNormBackwardArgs& a, cudaStrea
             e = launch<1024, 1>(a, vec, lines, s);
     }
     if (e != cudaSuccess || !a.work) return e;
-    // launched while the kernel before it ends, which hides the launch
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((2 * a.cols + 31) / 32);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
     count_launch();
-    e = cudaLaunchKernelEx(&cfg, layer_norm_join_kernel, const_cast<const float*>(a.work), lines, a.cols, a.dweight, a.dbias, a.accumulate);
-    return e == cudaSuccess ? cudaGetLastError() : e;
+    return launch_early(layer_norm_join_kernel, dim3((2 * a.cols + 31) / 32), 256, 0, s, a.work, lines, a.cols, a.dweight, a.dbias,
+                        a.accumulate);
 }
 
 }  // namespace fxk

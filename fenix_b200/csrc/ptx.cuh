@@ -10,6 +10,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "later.cuh"
 #include "optype.cuh"
 
 namespace fxk {
@@ -114,12 +115,6 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void cluster_sync_relaxed() {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-
-// ---- kernels that begin while the one before them in the stream ends ---------------------------
-// Waits until that kernel is done and what it wrote is there: nothing in global memory is read or written before.
-__device__ __forceinline__ void wait_for_earlier() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// From here on a later kernel of that kind may begin, once every block of this one has come here.
-__device__ __forceinline__ void let_later_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- bulk async copy global -> shared (1-D, no tensor map) ----------------------------------
 // dst/src 16-byte aligned, bytes a multiple of 16; completion is signalled as tx bytes on bar.

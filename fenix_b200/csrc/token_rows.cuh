@@ -3,6 +3,7 @@
 // sums and maxima.
 #pragma once
 
+#include "later.cuh"
 #include "pairs.cuh"
 #include "token.cuh"
 
