@@ -12,7 +12,7 @@ namespace {
 // ---- rows of any alignment -------------------------------------------------------------------------------------------
 // A tile of 128 rows by 128 outputs, 64 inputs a step, on m16n8k32 MMAs: eight warps of 64 by 32 each. The next step's bytes
 // wait in registers while the warps multiply this one's. Bound by the bytes' way through registers (1003 x 4705 -> 5003 in
-// packed rows: 283 us, 422 with a piece after the other).
+// packed rows: 280 us, 422 with a piece after the other).
 constexpr int kTile = 128, kStep = 64, kPitch = kStep + 16, kPieces = kTile * kStep / 16 / 256;
 
 // 16 bytes of a row from input k0 on, zeros past its end, one by one.

@@ -7,8 +7,8 @@
 // again. The accumulators are two, of 256 columns of TMEM each: the epilogue empties one while the MMAs fill the other. Pairs
 // stay and walk over the tiles, rows first within groups of 16 row tiles, so that what runs at once reads the same weights.
 // Few tiles of many inputs are shared by a cluster of pairs each, by ranges of the inputs (256 x 14336 -> 4096 21.5 us, 35
-// without); the sum over the cluster, some 4 us, and the weights' way from memory bound those (192 x 8192 -> 8192 22 us).
-// Ragged calls are bound by whole tiles: 1003 x 4705 -> 5003 has 128 tiles of 256 x 160 for 74 pairs, two turns (36 us).
+// without); the sum over the cluster, some 4 us, and the weights' way from memory bound those (192 x 8192 -> 8192 21 us).
+// Ragged calls are bound by whole tiles: 1003 x 4705 -> 5003 has 128 tiles of 256 x 160 for 74 pairs, two turns (35 us).
 #include "counters.hpp"
 #include "i8_linear.cuh"
 #include "tmap.hpp"

@@ -5,7 +5,7 @@
 // stay and walk over many rows with the next row on its way. What a value then costs are instructions: pairs of values share
 // one (add, multiply, multiply-add of two f32), and a kernel has one type (16384 x 4096 bf16 with residual to bf16 85 us, 6.3
 // TB/s, 96% of the copy, 107 before that; to e4m3 or i8 88 us; without a residual 61 us, 4.4 TB/s, bound by a row's three
-// reductions' way through a block; 1 x 4096 3.3 us). Rows that are not aligned, read a value at a time: 1031 x 5119 22 us.
+// reductions' way through a block; 1 x 4096 3.0 us). Rows that are not aligned, read a value at a time: 1031 x 5119 22 us.
 // The variance is the mean square about the mean, not a difference of two sums, so that rows far from zero keep theirs:
 // t = h - mean is exact or rounded once, and the sum of the t, taken with that of their squares, gives what the mean
 // itself was off by.
