@@ -460,3 +460,55 @@ def test_other_device(cuda_torch):
         assert torch.cuda.current_device() == 0
     torch.cuda.synchronize(1)
     assert torch.equal(y, linear_want(torch, x, xs, w, ws, None, "f32"))
+
+
+@pytest.mark.parametrize("rows", [3, 200, 700])
+def test_captured_with_branches(cuda_torch, rows):
+    """A graph whose calls follow calls of two streams, a copy and a fill: each sees what all of them wrote, eagerly and replayed."""
+    torch = cuda_torch
+    k, n = 1024, 1536
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    h = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    w = torch.randn(n, k, generator=g, device="cuda")
+    q, qs = torch.zeros(rows, k, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    codes, scales = torch.zeros(n, k, dtype=torch.int8, device="cuda"), torch.zeros(n, device="cuda")
+    y, z, back = torch.zeros(rows, n, device="cuda"), torch.zeros(rows, n, device="cuda"), torch.zeros(n, k, device="cuda")
+    side = torch.cuda.Stream()
+
+    def step():
+        here = torch.cuda.current_stream()
+        q.zero_()
+        codes.zero_()
+        side.wait_stream(here)
+        fx.layer_norm_dev(ptr(h), ptr(q), rows, k, "bf16", "i8", scale_ptr=ptr(qs), scale_mode="row", stream=stream(torch))
+        with torch.cuda.stream(side):
+            fx.i8_quantize_dev(ptr(w), n, k, ptr(codes), ptr(scales), "f32", stream=stream(torch))
+        here.wait_stream(side)
+        fx.i8_linear_dev(ptr(q), ptr(y), rows, n, k, ptr(codes), ptr(scales), ptr(qs), "f32", stream=stream(torch))
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            fx.i8_dequantize_dev(ptr(codes), ptr(scales), n, k, ptr(back), "f32", stream=stream(torch))
+        z.copy_(y)
+        y.fill_(-1.0)
+        fx.i8_linear_dev(ptr(q), ptr(y), rows, n, k, ptr(codes), ptr(scales), ptr(qs), "f32", stream=stream(torch))
+        here.wait_stream(side)
+
+    def check():
+        torch.cuda.synchronize()
+        want_codes, sc = quantize_want(torch, w)
+        assert torch.equal(codes, want_codes) and torch.equal(back, want_codes.float() * sc)
+        want = linear_want(torch, q, qs, codes, scales, None, "f32")
+        assert bool(q.any()) and torch.equal(y, want) and torch.equal(z, want)
+
+    for _ in range(3):
+        step()
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(3):
+        h.copy_(torch.randn(rows, k, generator=g, device="cuda") * (i + 1))
+        w.copy_(torch.randn(n, k, generator=g, device="cuda"))
+        for _ in range(4):
+            graph.replay()
+        check()
