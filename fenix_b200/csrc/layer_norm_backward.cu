@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(256) layer_norm_sums8_kernel(const __grid_cons
 }
 
 // The lines of the workspace added up: 32 columns a block, eight warps that take every eighth line.
-__global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __restrict__ work, int lines, int cols, float* dweight,
-                                                             float* dbias, bool accumulate) {
+__global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* work, int lines, int cols, float* dweight, float* dbias,
+                                                             bool accumulate) {
     __shared__ float part[8][33];
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x % 32;  // of dweight and dbias in a row
     const int warp = threadIdx.x / 32;
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __res
     wait_for_earlier();
     if (c < 2 * cols)
 #pragma unroll 8
-        for (int i = warp; i < lines; i += 8) s += work[static_cast<int64_t>(i) * 2 * cols + c];
+        for (int i = warp; i < lines; i += 8) s += __ldcg(work + static_cast<int64_t>(i) * 2 * cols + c);  // written while this kernel began
     part[warp][threadIdx.x % 32] = s;
     __syncthreads();
     if (warp || c >= 2 * cols) return;

@@ -492,3 +492,42 @@ def test_forward_and_backward_captured_side_by_side(cuda_torch):
         torch.cuda.synchronize()
         for st, was in zip(steps, first):
             assert all(torch.equal(p, q) for p, q in zip(st.outputs(), was))
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 256), (700, 1024), (3000, 4096), (500, 9000), (60, 1001)])
+def test_one_workspace_call_after_call(cuda_torch, rows, cols):
+    """Calls that follow one another on a stream share a workspace, an input that each call overwrites, and accumulated sums."""
+    torch = cuda_torch
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    xs = [torch.randn(rows, cols, generator=g, device="cuda").bfloat16() * (i + 1) for i in range(12)]
+    work = torch.empty(fx.layer_norm_backward_workspace(rows, cols), dtype=torch.uint8, device="cuda")
+    s, y, dx = torch.empty_like(xs[0]), torch.empty_like(xs[0]), torch.empty_like(xs[0])
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    total = torch.zeros(2, cols, device="cuda")
+
+    def run(x, dw, db, accumulate, together):
+        st = stream(torch)
+        fx.layer_norm_dev(ptr(x), ptr(y), rows, cols, residual_ptr=ptr(x), sum_ptr=ptr(s), mean_ptr=ptr(mean), rstd_ptr=ptr(rstd), stream=st)
+        if not together:
+            torch.cuda.synchronize()
+        fx.layer_norm_backward_dev(ptr(y), ptr(s), ptr(mean), ptr(rstd), rows, cols, dx_ptr=ptr(dx), dweight_ptr=ptr(dw), dbias_ptr=ptr(db),
+                                   accumulate=accumulate, work_ptr=ptr(work), work_bytes=work.numel(), stream=st)
+        if not together:
+            torch.cuda.synchronize()
+
+    apart = [torch.empty(2, cols, device="cuda") for _ in xs]
+    for x, out in zip(xs, apart):
+        run(x, out[0], out[1], False, False)
+    for _ in range(5):
+        close = [torch.empty(2, cols, device="cuda") for _ in xs]
+        total.zero_()
+        torch.cuda.synchronize()
+        for x, out in zip(xs, close):
+            run(x, out[0], out[1], False, True)
+            run(x, total[0], total[1], True, True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(apart, close))
+        want = torch.zeros_like(total)
+        for out in apart:
+            want += out
+        assert torch.equal(total, want)
