@@ -28,16 +28,15 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
     return __fdiv_rn(__uint_as_float(max(top, __float_as_uint(1e-30f))), 127.f);
 }
 
-// Eight codes of a row under its own scale, from whose quotients none is past 127. The quotient is a product with the scale's
-// correctly rounded reciprocal, made good by its remainder (x - t scale, exact in a multiply-add) times the same: correctly
-// rounded by Markstein's theorem (1990), while no term falls below f32's normal numbers.
+// Eight codes of a row under its own scale, from whose quotients none is past 127, where no term of quotient2 falls below f32's
+// normal numbers.
 __device__ __forceinline__ bool has_codes8(float scale) { return scale > 1e-28f && scale < 1e37f; }
 __device__ __forceinline__ uint2 codes8(const float (&x)[kVec], float scale, float inv) {
     const float2 inv2 = make_float2(inv, inv), less2 = make_float2(-scale, -scale);
     uint32_t w[kVec];
 #pragma unroll
     for (int i = 0; i < kVec / 2; ++i) {
-        const float2 v = pair_of(x, i), t = mul2(v, inv2), q = fma2(fma2(t, less2, v), inv2, t);
+        const float2 q = quotient2(pair_of(x, i), inv2, less2);
         const float2 m = add2(q, make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's low byte is the code
         w[2 * i] = __float_as_uint(m.x);
         w[2 * i + 1] = __float_as_uint(m.y);

@@ -4,7 +4,7 @@
 // between the looks at it (its mean, its squares about it, its largest magnitude where it gets a scale, its output), blocks
 // stay and walk over many rows with the next row on its way. What a value then costs are instructions: pairs of values share
 // one (add, multiply, multiply-add of two f32), and a kernel has one type (16384 x 4096 bf16 with residual to bf16 85 us, 6.3
-// TB/s, 96% of the copy, 107 before that; to e4m3 or i8 88 us; without a residual 61 us, 4.4 TB/s, bound by a row's three
+// TB/s, 96% of the copy, 107 before that; to e4m3 or i8 94 us; without a residual 61 us, 4.4 TB/s, bound by a row's three
 // reductions' way through a block; 1 x 4096 3.0 us). Rows that are not aligned, read a value at a time: 1031 x 5119 22 us.
 // The variance is the mean square about the mean, not a difference of two sums, so that rows far from zero keep theirs:
 // t = h - mean is exact or rounded once, and the sum of the t, taken with that of their squares, gives what the mean
@@ -24,6 +24,13 @@ struct Red {  // of a block that is one team: a row's sums, one of each look
     float sum[2][32];
     uint32_t top[32];
 };
+
+// Scale of a row from its largest magnitude: a quotient by 127 or 448, correctly rounded (the product with the reciprocal, made good by its
+// remainder: of every f32 from 1e-30 on). Infinity and NaN stay.
+__device__ __forceinline__ float row_scale(float top, int y_type) {
+    const float by = y_type == kTokI8 ? 127.f : 448.f, inv = y_type == kTokI8 ? 1.f / 127.f : 1.f / 448.f, t = top * inv;
+    return t < INFINITY ? fmaf(fmaf(t, -by, top), inv, t) : t;
+}
 
 // From a row's h on; cols 0: no row, nothing is stored. red: no thread of the team still reads it.
 // TYPE: of x, residual, weight and bias alike, or -1: any.
@@ -121,34 +128,44 @@ __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, 
             }
         }
     }
-    float scale = 1.f, times = 1.f;
+    float scale = 1.f;
     if (a.scale_mode != kScaleNone) {
+        bool zeros = false;
         if (by_row) {
-            // as bits a NaN is above every number
-            scale = __uint_as_float(max(team_max<TEAM>(__float_as_uint(top), red.top), __float_as_uint(1e-30f))) * (a.y_type == kTokI8 ? 1.f / 127.f : 1.f / 448.f);
+            const uint32_t most = team_max<TEAM>(__float_as_uint(top), red.top);  // as bits a NaN is above every number
+            zeros = most == 0;
+            scale = row_scale(__uint_as_float(max(most, __float_as_uint(1e-30f))), a.y_type);
             if (me == 0 && cols) a.scale[row] = scale;
         } else {
             scale = a.scale[0];
         }
-        times = 1.f / scale;
-        if (!(fabsf(times) < INFINITY)) {  // a scale near zero
+        // v / scale rounded to f32, as the quantiser has it, so that a row's codes are those of its f32 values (16384 x 4096 bf16 to
+        // e4m3 or i8 94 us, 88 by a product with the reciprocal alone). Below 1e-20 and from 1e37 on terms of quotient2 could leave
+        // f32's normal numbers, but for rows of zeros.
+        const bool within = (fabsf(scale) > 1e-20f && fabsf(scale) < 1e37f) || zeros;
+        const float inv = 1.f / scale;
+        const float2 inv2 = make_float2(inv, inv), less2 = make_float2(-scale, -scale);
+        auto divided = [&](auto&& by) {
 #pragma unroll
             for (int u = 0; u < TURNS; ++u)
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) h[u][j] = __fdiv_rn(h[u][j], scale);
-            times = 1.f;
+                for (int i = 0; i < kVec / 2; ++i) put_pair(h[u], i, by(pair_of(h[u], i)));
+        };
+        if (within && by_row) {  // no quotient is past 448
+            divided([&](const float2& v) { return quotient2(v, inv2, less2); });
+        } else if (within) {  // those far above saturate as they are
+            divided([&](const float2& v) {
+                const float2 t = mul2(v, inv2), q = quotient2(v, inv2, less2);
+                return make_float2(fabsf(t.x) < 512.f ? q.x : t.x, fabsf(t.y) < 512.f ? q.y : t.y);
+            });
+        } else {
+            divided([&](const float2& v) { return make_float2(__fdiv_rn(v.x, scale), __fdiv_rn(v.y, scale)); });
         }
     }
     // (a row's own scale leaves no value above 127)
     const bool plain = by_row && scale < INFINITY;
 #pragma unroll
     for (int u = 0; u < TURNS; ++u) {
-        if (a.scale_mode != kScaleNone) {
-#pragma unroll
-            for (int i = 0; i < kVec / 2; ++i) {
-                put_pair(h[u], i, mul2(pair_of(h[u], i), make_float2(times, times)));
-            }
-        }
         if (a.y_type != kTokI8)
             store8<TEAM, VEC>(a.y, row * a.y_stride, a.y_type, u, me, cols, h[u]);
         else if (VEC && plain)

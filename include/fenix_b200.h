@@ -479,6 +479,8 @@ fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_
  *   - y_type may be i8: y = v / scale rounded to nearest, ties to even, and saturated to +-127, with
  *       FX_SCALE_ROW     scale[row] = max(max |v|, 1e-30) / 127, written to dev_scale [rows]
  *       FX_SCALE_TENSOR  scale = dev_scale[0], read
+ *   - scales and quotients v / scale, of both 8-bit types, are f32's, correctly rounded: i8 rows are bit for bit what
+ *     fx_i8_quantize makes of the f32 y.
  * The mean is made good by the sum of the differences from it, so that rows far from zero keep theirs.
  * A row that holds a NaN or infinity, or a difference h - mean past f32's range, comes out NaN: its values, its rstd and its row
  * scale (its mean NaN or infinite). In i8 its values are zeros, which under a tensor scale nothing tells from others. */
