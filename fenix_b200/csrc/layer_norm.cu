@@ -94,7 +94,7 @@ __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, 
     float var = fmaxf(q.y * inv_n - off * off, 0.f) + a.eps * pre * pre;
     // 2^-160 eps may be nothing: a row of one large value is then zeros and not 0 / 0
     if (var < 1.1754944e-38f && pre != 1.f) var = 1.1754944e-38f;
-    if (q.y != q.y) var = q.y;
+    if (!(q.y < INFINITY)) var = q.y - q.y;  // a value or a difference that is not finite: NaN
     const float r = rsqrtf(var);
     if (me == 0 && cols) {
         if (a.mean) a.mean[row] = (mean + off) / pre;
