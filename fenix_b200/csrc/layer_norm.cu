@@ -4,11 +4,11 @@
 // between the looks at it (its mean, its squares about it, its largest magnitude where it gets a scale, its output), blocks
 // stay and walk over many rows with the next row on its way. What a value then costs are instructions: pairs of values share
 // one (add, multiply, multiply-add of two f32), and a kernel has one type (16384 x 4096 bf16 with residual to bf16 85 us, 6.3
-// TB/s, 96% of the copy, 107 before that; to e4m3 or i8 94 us; without a residual 61 us, 4.4 TB/s, bound by a row's three
+// TB/s, 96% of the copy, 107 before that; to e4m3 or i8 96 us; without a residual 63 us, 4.2 TB/s, bound by a row's three
 // reductions' way through a block; 1 x 4096 3.0 us). Rows that are not aligned, read a value at a time: 1031 x 5119 22 us.
 // The variance is the mean square about the mean, not a difference of two sums, so that rows far from zero keep theirs:
 // t = h - mean is exact or rounded once, and the sum of the t, taken with that of their squares, gives what the mean
-// itself was off by.
+// itself was off by. Where that is more than the values are spread, both sums are taken again.
 #include "counters.hpp"
 #include "token_rows.cuh"
 
@@ -18,6 +18,7 @@ namespace fxk {
 namespace {
 
 constexpr float kSmaller = 8.2718061e-25f;  // 2^-80
+constexpr int kAgain = 13;  // times that squares are summed again, at most: each takes 17 bits or more (80 roundings) off what the mean is off by
 
 struct Red {  // of a block that is one team: a row's sums, one of each look
     float2 pair[2][32];
@@ -82,23 +83,31 @@ __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, 
         return team_sum2<TEAM>(make_float2(e.x + e.y, q.x + q.y), to);
     };
     float2 q = squares(mean, red.pair[0]);
-    const bool wide = !(q.y + a.eps < 3.0e38f) && pre == 1.f;  // squares past f32's range
-    if (TEAM < 32 ? __any_sync(0xffffffffu, wide) : wide) {
-        const float by = wide ? kSmaller : 1.f;
-        pre *= by;
-        mean *= by;
-        scaled(by);
-        q = squares(0.f, red.pair[1]);
+    float off = q.x * inv_n, var = fmaxf(q.y * inv_n - off * off, 0.f) + a.eps * pre * pre;
+    // Squares past f32's range; or a mean further off than the values are spread (rows nearly or all alike, far from zero), which leaves of
+    // the squares mostly their rounding: they are summed again, of smaller values, or about the better mean.
+    const bool again = !(off * off <= var && q.y + a.eps < 3.0e38f);
+    if (__builtin_expect(TEAM < 32 ? __any_sync(0xffffffffu, again) : again, 0)) {
+        for (int i = 0; i < kAgain; ++i) {
+            const bool wide = !(q.y + a.eps < 3.0e38f) && pre == 1.f, far = !wide && off * off > var;
+            if (!(TEAM < 32 ? __any_sync(0xffffffffu, wide || far) : wide || far)) break;
+            const float by = wide ? kSmaller : 1.f, less = far ? off : 0.f;
+            pre *= by;
+            mean = mean * by + less;
+            scaled(by);
+            q = squares(less, red.pair[(i + 1) % 2]);  // not the half that slower threads may still read
+            off = q.x * inv_n;
+            var = fmaxf(q.y * inv_n - off * off, 0.f) + a.eps * pre * pre;
+        }
     }
-    const float off = q.x * inv_n;
-    float var = fmaxf(q.y * inv_n - off * off, 0.f) + a.eps * pre * pre;
-    // 2^-160 eps may be nothing: a row of one large value is then zeros and not 0 / 0
-    if (var < 1.1754944e-38f && pre != 1.f) var = 1.1754944e-38f;
+    float undo = pre;
+    // 2^-160 eps may be nothing: what is left then are values all alike
+    if (var < 1.1754944e-38f && pre != 1.f) var = a.eps, undo = 1.f;
     if (!(q.y < INFINITY)) var = q.y - q.y;  // a value or a difference that is not finite: NaN
     const float r = rsqrtf(var);
     if (me == 0 && cols) {
         if (a.mean) a.mean[row] = (mean + off) / pre;
-        if (a.rstd) a.rstd[row] = r * pre;
+        if (a.rstd) a.rstd[row] = r * undo;
     }
     const float2 r2 = make_float2(r, r), off2 = make_float2(-off * r, -off * r);
     const bool by_row = a.scale_mode == kScaleRow;
