@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&w_map) : "memory");
     }
+    wait_for_earlier();  // before TMEM is taken, which the earlier kernel, of whatever library, may still ask for
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_at)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -186,9 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     cluster_sync();  // the other SM's barriers are there too
     tc_fence_after();
     const uint32_t tmem = tmem_at;
-    // TMEM is there in every block that comes here: a later kernel's blocks, which begin after all of them have, keep none from it
-    let_later_begin();
-    wait_for_earlier();
+    let_later_begin();  // TMEM is there in every block that comes here: a later kernel's blocks keep none from it
 
     // the epilogue's warps
     const int quad = warp % 4, half = (warp - 2) / 4, me = static_cast<int>(threadIdx.x) - 64, size = a.y_type == kTokF32 ? 4 : 2;

@@ -50,8 +50,8 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[kVec], float scale, flo
 
 template <int TEAM, int TURNS, bool VEC>
 __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM <= 32 ? 1 : 2048 / TEAM) i8_quantize_kernel(const __grid_constant__ I8RowsArgs a) {
-    let_later_begin();
     wait_for_earlier();
+    let_later_begin();
     __shared__ uint32_t red[32];
     constexpr int kPer = TEAM <= 32 ? 128 / TEAM : 1;
     const int me = threadIdx.x % TEAM;
@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(TEAM <= 32 ? 128 : TEAM, TEAM <= 32 ? 1 : 2048
 constexpr int kWide = 1024;
 template <bool VEC>
 __global__ void __launch_bounds__(kWide) i8_quantize_wide_kernel(const __grid_constant__ I8RowsArgs a) {
-    let_later_begin();
     wait_for_earlier();
+    let_later_begin();
     __shared__ uint32_t red[32];
     const int64_t row = blockIdx.x;
     const int turns = (a.cols + kWide * kVec - 1) / (kWide * kVec);
@@ -133,8 +133,8 @@ __global__ void __launch_bounds__(kWide) i8_quantize_wide_kernel(const __grid_co
 constexpr int kBackRows = 4;
 template <int N>
 __global__ void __launch_bounds__(256) i8_dequantize_kernel(const __grid_constant__ I8RowsArgs a) {
-    let_later_begin();
     wait_for_earlier();
+    let_later_begin();
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * N;
     if (c >= a.cols) return;
     for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * kBackRows; row0 < a.rows; row0 += static_cast<int64_t>(gridDim.y) * kBackRows) {

@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         asm volatile("prefetch.tensormap [%0];" ::"l"(&w_map) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&x_map) : "memory");
     }
+    wait_for_earlier();  // before TMEM is taken, which the earlier kernel, of whatever library, may still ask for
     if (warp == 1) {
         tmem_alloc(smem_u32(&tmem_at), plan.cols);
         tmem_relinquish();
@@ -72,9 +73,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_at;
-    // TMEM is there in every block that comes here: a later kernel's blocks, which begin after all of them have, keep none from it
-    let_later_begin();
-    wait_for_earlier();
+    let_later_begin();  // TMEM is there in every block that comes here: a later kernel's blocks keep none from it
 
     if (warp == 0) {
         if (lane == 0) {

@@ -187,8 +187,8 @@ __device__ __forceinline__ void finish_row(const LayerNormArgs& a, int64_t row, 
 // TEAM threads a row, TURNS times eight values each.
 template <int TEAM, int TURNS, bool VEC>
 __global__ void __launch_bounds__(TEAM == 32 ? 128 : TEAM) layer_norm_kernel(const __grid_constant__ LayerNormArgs a) {
-    let_later_begin();
     wait_for_earlier();
+    let_later_begin();
     __shared__ Red red;
     const int me = threadIdx.x % TEAM;
     const int64_t row = TEAM == 32 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
