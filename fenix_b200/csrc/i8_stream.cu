@@ -17,8 +17,7 @@ namespace {
 
 constexpr int kTileM = 128;
 constexpr int kThreads = 192;  // warps: 0 TMA, 1 TMEM and MMA, 2..5 epilogue
-// Two blocks share an SM, and never more: each has at most 256 columns of TMEM, so that a block never waits for TMEM held by
-// a block that waits for the first one's cluster.
+// Two blocks share an SM, and never more: each has at most 256 columns of TMEM, so that none waits for another's.
 constexpr int kSmemTwo = 112 * 1024, kSmemOne = 224 * 1024, kSmemLeast = 80 * 1024;
 
 struct Plan {
@@ -143,6 +142,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         tc_fence_before();
     }
+    // TMEM goes before the blocks of a cluster wait for one another: none holds it while it waits for one that may still ask for it
+    __syncwarp();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, plan.cols);
+    }
     if (split > 1) {  // each block adds up a share of the tile over the cluster
         __syncwarp();
         cluster_sync();
@@ -167,11 +173,6 @@ __global__ void __launch_bounds__(kThreads, 2)
             i8_store4(a.y, static_cast<int64_t>(r) * a.y_stride + o, a.y_type, f, plan.y_vec && o + 4 <= a.n, a.n - o);
         }
         cluster_sync();  // no block's shared memory ends while another reads it
-    }
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem, plan.cols);
     }
 }
 

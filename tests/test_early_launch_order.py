@@ -47,3 +47,9 @@ def test_launches_that_may_begin_early(root, file):
     """A launch that allows it is of a kernel that waits."""
     text = (root / "fenix_b200" / "csrc" / file).read_text()
     assert "programmaticStreamSerializationAllowed = 1" in text and "wait_for_earlier();" in text
+
+
+def test_tensor_memory_goes_before_the_cluster_waits(root):
+    """A block of a cluster that held tensor memory while it waits for the others could keep it from one of them."""
+    body = next(b for f, _, b in kernels(root) if f == "i8_stream.cu")
+    assert 0 < body.find("tmem_dealloc(") < body.find("cluster_sync();")
