@@ -454,7 +454,7 @@ cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
     for (int split = 1; split <= 4; ++split) {
         int at_once = pairs;
         if (split > 1) {
-            if (steps < 4 * split) break;
+            if (steps < 4 * split) break;  // with four steps a pair and at most four pairs, rounding up leaves none without a step
             if (e = clusters(2 * split, &at_once); e != cudaSuccess) return e;
         }
         for (int n = kMaxOutputs; n >= 128; n -= 32) {
@@ -467,8 +467,6 @@ cudaError_t launch_i8_pair(const I8LinearArgs& a, cudaStream_t s) {
     }
     p.tiles_n = (a.n + p.tile_n - 1) / p.tile_n;
     p.steps_each = (steps + p.split - 1) / p.split;
-    while (p.split > 1 && (p.split - 1) * p.steps_each >= steps) --p.split;  // no pair without a step
-    if (p.tile_n % (16 * p.split) != 0) p.split = 1, p.steps_each = steps;
     p.box_m = std::min((a.rows + 15) / 16 * 16, kRows / 2);
     const int slot = (kRows / 2 + p.tile_n / 2) * kI8Step;
     const uint64_t where = reinterpret_cast<uintptr_t>(a.y) | static_cast<uint64_t>(a.y_stride) * (a.y_type == kTokF32 ? 4 : 2);
