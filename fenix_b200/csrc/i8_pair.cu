@@ -1,13 +1,13 @@
 // i8_pair.cu — linear layer of 8-bit integers, many rows: tcgen05 on pairs of SMs.
 //
 // Bound by the tensor cores under the power limit (4096 x 4096 -> 14336 bf16: 158 to 165 us, 2.9 to 3.0 Pop/s at 1.64 GHz, 81% of
-// the tensor pipe's cycles; 132 us, 3.6 Pop/s, on zeros, which take no power; 8192 x 8192 -> 8192 332 us, 3.3 Pop/s). Two SMs share a tile of 256 rows by up to 256 outputs (cta_group::2): each brings its 128 rows and
+// the tensor pipe's cycles; 132 us, 3.6 Pop/s, on zeros, which take no power; 8192 x 8192 -> 8192 330 to 350 us, 3.1 to 3.3 Pop/s). Two SMs share a tile of 256 rows by up to 256 outputs (cta_group::2): each brings its 128 rows and
 // half of the outputs' weights by TMA, so that an MMA of a pair reads 8 KB of each SM's shared memory in the 128 cycles that its
 // 256 x 256 x 32 products take, and as much is written: what shared memory can do, where one SM alone would need half as much
 // again. The accumulators are two, of 256 columns of TMEM each: the epilogue empties one while the MMAs fill the other. Pairs
 // stay and walk over the tiles, rows first within groups of 16 row tiles, so that what runs at once reads the same weights.
 // Few tiles of many inputs are shared by a cluster of pairs each, by ranges of the inputs (256 x 14336 -> 4096 21.5 us, 35
-// without); the sum over the cluster, some 4 us, and the weights' way from memory bound those (192 x 8192 -> 8192 21 us).
+// without); the sum over the cluster, some 4 us, and the weights' way from memory bound those (192 x 8192 -> 8192 21.6 us).
 // Ragged calls are bound by whole tiles: 1003 x 4705 -> 5003 has 128 tiles of 256 x 160 for 74 pairs, two turns (35 us).
 #include "counters.hpp"
 #include "i8_linear.cuh"

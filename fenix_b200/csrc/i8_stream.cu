@@ -2,7 +2,7 @@
 //
 // Outputs are the MMA's M, 128 a tile, and the rows of x its N, so that a weight is read once whatever the number of rows (to
 // 128) and a single row costs no more than its weights: bound by memory (8 x 8192 -> 28672: 40 us, 5.9 TB/s, 90% of the copy;
-// with few bytes by the launch, the first copies and a cluster's sum: 1 x 4096 -> 4096 6.8 us). TMA brings 128 inputs of both at
+// with few bytes by the launch, the first copies and a cluster's sum: 1 x 4096 -> 4096 7.2 us). TMA brings 128 inputs of both at
 // a time, one warp issues the MMAs, sums are held in TMEM. Few tiles are shared by a cluster each, by ranges of the inputs;
 // its blocks add up over the cluster's shared memory. Whole numbers add up to the same in any order.
 #include "counters.hpp"

@@ -402,9 +402,10 @@ fx_status fx_accum_finalize(const float* dev_acc, int64_t dz, int64_t dy, int64_
  * Common to these calls: matrices are row-major with their rows `*_stride` elements apart (at least the
  * row's length; 0: packed) and their elements at least element-aligned. Every pointer of a call is device
  * memory of one device, which need not be the current one; `stream` (NULL: that device's default stream)
- * belongs to that device. The calls enqueue one kernel (a few in a row for extents past 65535), allocate
- * nothing, keep nothing between calls and do not synchronise, so any number may run at once and be captured
- * into graphs. Extents and strides are below 2^30. No row (rows or n = 0) is not an error: nothing is done. */
+ * belongs to that device. The calls enqueue one kernel (a few in a row for extents past 65535; the layer norm's
+ * backward pass up to three, or two fills where there is no row), allocate nothing, keep nothing between calls and
+ * do not synchronise, so any number may run at once and be captured into graphs. Extents and strides are below 2^30.
+ * No row (rows or n = 0) is not an error: nothing is done. */
 typedef enum fx_dtype { FX_F32 = 0, FX_F16 = 1, FX_BF16 = 2, FX_E4M3 = 3, FX_I8 = 4 } fx_dtype;
 /* Scale of 8-bit rows (value = e4m3 or int8 * scale): none, one for the tensor, or one per row. */
 typedef enum fx_scale { FX_SCALE_NONE = 0, FX_SCALE_TENSOR = 1, FX_SCALE_ROW = 2 } fx_scale;
@@ -481,7 +482,8 @@ fx_status fx_w4_dequantize(const uint8_t* dev_codes, const void* dev_scales, fx_
  *       FX_SCALE_TENSOR  scale = dev_scale[0], read
  *   - scales and quotients v / scale, of both 8-bit types, are f32's, correctly rounded: i8 rows are bit for bit what
  *     fx_i8_quantize makes of the f32 y.
- * The mean is made good by the sum of the differences from it, so that rows far from zero keep theirs.
+ * The mean is made good by the sum of the differences from it, as often as it takes, so that rows far from zero keep theirs
+ * and their variance, rows all alike that of nothing.
  * A row that holds a NaN or infinity, or a difference h - mean past f32's range, comes out NaN: its values, its rstd and its row
  * scale (its mean NaN or infinite). In i8 its values are zeros, which under a tensor scale nothing tells from others. */
 fx_status fx_layer_norm(const void* dev_x, fx_dtype x_type, int64_t rows, int64_t cols, int64_t x_stride,
@@ -501,7 +503,9 @@ uint64_t fx_layer_norm_backward_workspace(int64_t rows, int64_t cols);
  * reaches h beside the norm, of dx_type, as dx. dx is the gradient of x and of residual alike. dy, h, weight and dx are f32, f16 or
  * bf16 each; dev_weight may be NULL (ones). dev_dweight and dev_dbias, f32 [cols], are overwritten, or added to where
  * `accumulate` is not 0; they are sums of every row whatever `rows`, so without a row they are zeros (or left as they
- * are). dx, dweight and dbias may each be NULL, not all three. Every sum repeats exactly on GPUs of one kind.
+ * are). dx, dweight and dbias may each be NULL, not all three. Every sum repeats exactly on GPUs of one kind. A row that holds a
+ * NaN or infinity, or a difference h - mean past f32's range, comes out not finite, as do the sums over rows that take such a
+ * value in.
  * dev_work: 16-byte aligned, at least fx_layer_norm_backward_workspace bytes, read by nothing else until this call's
  * kernels are done (so calls that may run at once, captured ones included, have one each); NULL where dweight and dbias are.
  * In place: dev_dx may be dev_dy, dev_h or dev_dsum at equal types and strides; no other overlap.
